@@ -613,6 +613,96 @@ int noise_update_gradients(const noise_update_param_t *params, int nparams, int6
                            int64_t threads, const float *buffer, void *workspace, int64_t workspace_bytes,
                            noise_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Training and serving operators on [batch, token, head, dim] tensors
+ * ---------------------------------------------------------------------------------------------- */
+
+/* A [batch, tokens, heads, dim] tensor: element (b, t, h, d) at ptr + b*s_b + t*s_t + h*s_h + d (strides in elements).
+ * Rows of 16 B: ptr 16 B aligned, strides multiples of 16 B. */
+typedef struct {
+    void *ptr;
+    int64_t s_b, s_t, s_h, heads;
+} noise_heads_t;
+
+#define NOISE_BF16 0
+#define NOISE_FP32 1
+
+/* Norm of every head's queries and keys with the rotation in the same pass (utils/model.py:46-47, 55-58, 88-94 with learned
+ * weights and positions as options): for the tensors x[0] (queries) and x[1] (keys) of type `type` (NOISE_BF16 or
+ * NOISE_FP32), head_dim D 64 or 128, the row of token t of sequence b stands at position p = start[b] + t (start NULL:
+ * p = t) and
+ *   u = w * x * rsqrt(mean(x^2) + eps),   y = [u1 c + u2 s, u2 c - u1 s]
+ * with u1, u2 the row's halves, c, s row p of the fp32 tables rope_cos, rope_sin [table_rows][D/2], and w fp32 [D] (NULL:
+ * ones). The sums are in fp32 and y is rounded once. A token whose position lies outside the tables gets zeros.
+ * start: [batch] int32, or int64 with start_wide.
+ * With a cache (capacity > 0), y[1] and v_out are [batch, capacity, heads, D] tensors: the key of position p is written to
+ * their token p, and so is the row of v (any values, copied). A token whose position lies outside the tables or the
+ * cache then gets zeros in y[0] and is not written. Slots of other positions are left as they are.
+ * capacity 0: y[1] is [batch, tokens, heads, D], v and v_out are NULL. */
+int noise_qk_norm_rotary(const noise_heads_t x[2], const noise_heads_t y[2], const float *const w[2],
+                         const noise_heads_t *v, const noise_heads_t *v_out, const float *rope_cos,
+                         const float *rope_sin, int64_t table_rows, const void *start, int start_wide, int64_t batch,
+                         int64_t tokens, int64_t capacity, int64_t head_dim, int type, float eps,
+                         noise_stream_t stream);
+
+/* Its gradients: dx[i] (type `type`) from dy[i] and the x[i] of the forward call, and dw[i], fp32 [D], for the weights that
+ * are given (w[i] non-NULL), summed over all rows in a fixed order through a workspace of
+ * noise_qk_norm_rotary_bwd_workspace_bytes bytes (16 B aligned; not needed without weights). */
+int64_t noise_qk_norm_rotary_bwd_workspace_bytes(int64_t head_dim);
+int noise_qk_norm_rotary_bwd(const noise_heads_t x[2], const noise_heads_t dy[2], const noise_heads_t dx[2],
+                             const float *const w[2], float *const dw[2], const float *rope_cos, const float *rope_sin,
+                             int64_t table_rows, const void *start, int start_wide, int64_t batch, int64_t tokens,
+                             int64_t head_dim, int type, float eps, void *workspace, int64_t workspace_bytes,
+                             noise_stream_t stream);
+
+/* Causal attention with a left window and `sinks` first tokens that stay visible: query i sees the keys j <= i with
+ * i - j <= window or j < sinks (sinks 0: the mask of utils/model.py:17-21). o = softmax(scale q k^T) v in bf16 with fp32
+ * scores and sums. q, o have H heads and k, v Hk, H a multiple of Hk (query head h reads key head h / (H / Hk)); head_dim
+ * 64 or 128. lengths (NULL: tokens): [batch] int32, or int64 with lengths_wide; keys from lengths[b] on are seen by no
+ * query and queries from there on get zeros (rows there may hold anything). lse: NULL, or fp32 [batch][H][tokens], the log2 of each row's sum
+ * of exponentials, which the backward pass reads (rows past the length are not written). */
+int noise_sink_attention_fwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
+                             const noise_heads_t *o, float *lse, const void *lengths, int lengths_wide, int64_t batch,
+                             int64_t tokens, int64_t head_dim, int64_t window, int64_t sinks, float scale,
+                             noise_stream_t stream);
+
+/* Its gradients dq, dk, dv (zeros past each length) from d_o and the forward call's tensors and lse. No atomics: the sums
+ * run in a fixed order. workspace: noise_sink_attention_bwd_workspace_bytes (16 B aligned). */
+int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t window, int64_t sinks);
+int noise_sink_attention_bwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
+                             const noise_heads_t *o, const noise_heads_t *d_o, const float *lse,
+                             const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
+                             const void *lengths, int lengths_wide, int64_t batch, int64_t tokens, int64_t head_dim,
+                             int64_t window, int64_t sinks, float scale, void *workspace, int64_t workspace_bytes,
+                             noise_stream_t stream);
+
+/* The same attention of a few new tokens against a cache: q, o [batch, tokens, H, D] (tokens 1 .. 16), k, v [batch, capacity,
+ * Hk, D]. Token t of sequence b stands at position i = start[b] + t and sees the slots j <= i, j < capacity of the mask
+ * above; with no such slot (a negative position) it gets zeros. Slots that no token of its sequence sees may hold anything.
+ * workspace: noise_sink_decode_workspace_bytes (16 B aligned; may be 0). */
+int64_t noise_sink_decode_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                          int64_t capacity, int64_t head_dim, int64_t window, int64_t sinks);
+int noise_sink_decode(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v, const noise_heads_t *o,
+                      const void *start, int start_wide, int64_t batch, int64_t tokens, int64_t capacity,
+                      int64_t head_dim, int64_t window, int64_t sinks, float scale, void *workspace,
+                      int64_t workspace_bytes, noise_stream_t stream);
+
+/* Distillation from a teacher's top logits: for each of `rows` rows of logits x (type `type`, `vocab` of `stride` elements)
+ * and the teacher's `entries` logits t (type `teacher_type`) at indices i (int32, or int64 with index_wide), both [rows]
+ * [entries] contiguous,
+ *   z = cap(x) / temperature,  cap(x) = softcap tanh(x / softcap) (softcap 0: x),  p = softmax(t / temperature),
+ *   loss = temperature^2 sum_k p_k (log p_k - log softmax(z)[i_k]),
+ * the softmax p over the entries in use: those with an index in 0 .. vocab - 1 and t above -inf. A row without any has loss
+ * 0 and gradient 0. An index may stand in several entries. loss: fp32 [rows].
+ * grad (NULL: the loss alone): [rows] rows of grad_stride elements of x's type, the gradient of sum_r weight[r] loss[r] with
+ * respect to x (weight fp32 [rows], NULL: ones); its columns vocab .. width - 1 are set to zero. One pass: loss and
+ * gradient from one reading of the rows where they fit the registers. */
+int noise_distill(const void *x, int type, int64_t rows, int64_t vocab, int64_t stride, const void *teacher,
+                  int teacher_type, const void *index, int index_wide, int64_t entries, const float *weight,
+                  float temperature, float softcap, float *loss, void *grad, int64_t width, int64_t grad_stride,
+                  noise_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,8 @@ import torch
 
 from .abi import (SIGNATURES, LINEAR_AUTOCAST, ROUNDING_FUSED, ROUNDING_EAGER, ATTN_V_TRANSPOSED,  # noqa: F401
                   ATTN_QK_NORMED, ATTN_OUT_FP32, ATTN_Q_FP32, CastHeads, View, Rank1, Population, UpdateParam, SliceGroups, SLICE_GROUPS_MAX, BlockJitter,
-                  RandintSet, RANDINT_SETS_MAX, Weight, WEIGHTS_MAX, WEIGHT_BF16, WEIGHT_FP32, WEIGHT_FP32_ROUNDED, bind)
+                  RandintSet, RANDINT_SETS_MAX, Weight, WEIGHTS_MAX, WEIGHT_BF16, WEIGHT_FP32, WEIGHT_FP32_ROUNDED, Heads,
+                  TYPE_BF16, TYPE_FP32, bind)
 
 # the in-tree build (noise_amd/build.py); no other library is ever loaded
 LIB_PATH = Path(__file__).resolve().with_name('libnoise_amd.so')

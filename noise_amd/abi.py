@@ -76,10 +76,22 @@ SIGNATURES = {
     'noise_update_weights': [_p, _i64, _i64, _p, _p],
     'noise_update_workspace_bytes': [_p, _i32, _i64, _i64],
     'noise_update_gradients': [_p, _i32, _i64, _p, _f32, _i64, _i64, _u64, _u64, _i64, _p, _p, _i64, _p],
+    'noise_qk_norm_rotary': [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i32, _i64, _i64, _i64, _i64, _i32, _f32, _p],
+    'noise_qk_norm_rotary_bwd_workspace_bytes': [_i64],
+    'noise_qk_norm_rotary_bwd': [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i32, _i64, _i64, _i64, _i32, _f32, _p, _i64, _p],
+    'noise_sink_attention_fwd': [_p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p],
+    'noise_sink_attention_bwd_workspace_bytes': [_i64, _i64, _i64, _i64, _i64, _i64, _i64],
+    'noise_sink_attention_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p,
+                                 _i64, _p],
+    'noise_sink_decode_workspace_bytes': [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
+    'noise_sink_decode': [_p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p],
+    'noise_distill': [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _i32, _i64, _p, _f32, _f32, _p, _p, _i64, _i64, _p],
 }
 _RESTYPES = {'noise_last_error': ctypes.c_char_p, 'noise_update_workspace_bytes': ctypes.c_int64,
              'noise_head_ce_workspace_bytes': ctypes.c_int64, 'noise_block_split_workspace_bytes': ctypes.c_int64,
-             'noise_dust_block_workspace_bytes': ctypes.c_int64, 'noise_dust_block_static_max_bytes': ctypes.c_int64}
+             'noise_dust_block_workspace_bytes': ctypes.c_int64, 'noise_dust_block_static_max_bytes': ctypes.c_int64,
+             'noise_qk_norm_rotary_bwd_workspace_bytes': ctypes.c_int64,
+             'noise_sink_attention_bwd_workspace_bytes': ctypes.c_int64, 'noise_sink_decode_workspace_bytes': ctypes.c_int64}
 
 # y_fp32 of noise_pop_linear / noise_rank1_expand: fp32 output in autocast's form (bf16 product and dot)
 LINEAR_AUTOCAST = 2
@@ -87,6 +99,9 @@ LINEAR_AUTOCAST = 2
 # noise_population_t.rounding (include/noise_amd.h)
 ROUNDING_FUSED = 0
 ROUNDING_EAGER = 1
+
+# element types of the training and serving operators (include/noise_amd.h)
+TYPE_BF16, TYPE_FP32 = 0, 1
 
 # noise_attention_fwd flags (include/noise_amd.h)
 ATTN_V_TRANSPOSED = 1
@@ -110,6 +125,12 @@ class Population(ctypes.Structure):
     """noise_population_t (rounding: ROUNDING_FUSED, the default, or ROUNDING_EAGER)."""
     _fields_ = [('members', ctypes.c_int64), ('tokens', ctypes.c_int64), ('sign', ctypes.c_void_p),
                 ('dir_div', ctypes.c_int64), ('rounding', ctypes.c_int64)]
+
+
+class Heads(ctypes.Structure):
+    """noise_heads_t: a [batch, tokens, heads, dim] tensor with unit inner stride."""
+    _fields_ = [('ptr', ctypes.c_void_p), ('s_b', ctypes.c_int64), ('s_t', ctypes.c_int64), ('s_h', ctypes.c_int64),
+                ('heads', ctypes.c_int64)]
 
 
 SLICE_GROUPS_MAX = 64  # NOISE_SLICE_GROUPS_MAX

@@ -18,13 +18,15 @@ a 1-D parameter (the mixing scalars' eps) in noise_a and None in noise_b; block_
 the list (q, k, v, gate or None, proj, fc, out). The reference-signature wrappers that pack them are
 noise_amd.eggroll.population_loss and noise_amd.dust.head_loss / block_forward / coordinate_differences.
 """
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 from torch.library import custom_op
 
+from . import distill as _distill
 from . import dust, eggroll, model
+from . import sinks as _sinks
 
 BLOCK_WEIGHTS = ('q', 'k', 'v', 'gate', 'proj', 'fc', 'out')
 
@@ -113,3 +115,142 @@ def coordinate_differences(raw: Tensor, y: Tensor, sigma: float) -> Tensor:
 @coordinate_differences.register_fake
 def _coordinate_differences_fake(raw, y, sigma):
     return raw.new_empty(raw.shape, dtype=torch.float32)
+
+
+# --- operators with gradients ---
+# (an absent gradient of an optional tensor leaves the backward operators as an empty tensor)
+
+
+@custom_op('noise_amd::qk_norm_rotary', mutates_args=())
+def qk_norm_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, q_weight: Optional[Tensor],
+                   k_weight: Optional[Tensor], start: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor]:
+    return _sinks.norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps)
+
+
+@qk_norm_rotary.register_fake
+def _qk_norm_rotary_fake(q, k, cos, sin, q_weight, k_weight, start, eps):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@custom_op('noise_amd::qk_norm_rotary_backward', mutates_args=())
+def qk_norm_rotary_backward(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor,
+                            q_weight: Optional[Tensor], k_weight: Optional[Tensor], start: Optional[Tensor],
+                            eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    grads = _sinks.norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, eps)
+    return tuple(q.new_empty(0) if g is None else g for g in grads)
+
+
+@qk_norm_rotary_backward.register_fake
+def _qk_norm_rotary_backward_fake(dq, dk, q, k, cos, sin, q_weight, k_weight, start, eps):
+    return (q.new_empty(q.shape), k.new_empty(k.shape),
+            *(q.new_empty(0) if w is None else w.new_empty(w.shape) for w in (q_weight, k_weight)))
+
+
+def _qk_norm_rotary_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:7])
+    ctx.eps = inputs[7]
+
+
+def _qk_norm_rotary_backward(ctx, dq, dk):
+    q, k, cos, sin, qw, kw, start = ctx.saved_tensors
+    dq, dk, dqw, dkw = torch.ops.noise_amd.qk_norm_rotary_backward(dq, dk, q, k, cos, sin, qw, kw, start, ctx.eps)
+    return dq, dk, None, None, None if qw is None else dqw, None if kw is None else dkw, None, None
+
+
+qk_norm_rotary.register_autograd(_qk_norm_rotary_backward, setup_context=_qk_norm_rotary_setup)
+
+
+@custom_op('noise_amd::qk_norm_rotary_append', mutates_args=('k_cache', 'v_cache'))
+def qk_norm_rotary_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, k_cache: Tensor, v_cache: Tensor,
+                          start: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], eps: float) -> Tensor:
+    return _sinks.qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight, k_weight, eps)
+
+
+@qk_norm_rotary_append.register_fake
+def _qk_norm_rotary_append_fake(q, k, v, cos, sin, k_cache, v_cache, start, q_weight, k_weight, eps):
+    return q.new_empty(q.shape)
+
+
+@custom_op('noise_amd::sink_attention', mutates_args=())
+def sink_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int,
+                   lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    return _sinks.attend_forward(q, k, v, window, sinks, lengths, True)
+
+
+@sink_attention.register_fake
+def _sink_attention_fake(q, k, v, window, sinks, lengths):
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+@custom_op('noise_amd::sink_attention_backward', mutates_args=())
+def sink_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, window: int,
+                            sinks: int, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    return tuple(_sinks.attend_backward(dout, q, k, v, out, lse, window, sinks, lengths))
+
+
+@sink_attention_backward.register_fake
+def _sink_attention_backward_fake(dout, q, k, v, out, lse, window, sinks, lengths):
+    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+
+
+def _sink_attention_setup(ctx, inputs, output):
+    q, k, v, ctx.window, ctx.sinks, lengths = inputs
+    out, lse = output
+    ctx.mark_non_differentiable(lse)
+    ctx.save_for_backward(q, k, v, out, lse, lengths)
+
+
+def _sink_attention_backward(ctx, dout, _):
+    q, k, v, out, lse, lengths = ctx.saved_tensors
+    return (*torch.ops.noise_amd.sink_attention_backward(dout, q, k, v, out, lse, ctx.window, ctx.sinks, lengths),
+            None, None, None)
+
+
+sink_attention.register_autograd(_sink_attention_backward, setup_context=_sink_attention_setup)
+
+
+@custom_op('noise_amd::sink_attention_decode', mutates_args=())
+def sink_attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, start: Tensor, window: int,
+                          sinks: int) -> Tensor:
+    return _sinks.sink_attention_decode(q, k_cache, v_cache, start, window, sinks)
+
+
+@sink_attention_decode.register_fake
+def _sink_attention_decode_fake(q, k_cache, v_cache, start, window, sinks):
+    return q.new_empty(q.shape)
+
+
+@custom_op('noise_amd::distill_loss', mutates_args=())
+def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_index: Tensor, vocab: int, temperature: float,
+                 softcap: Optional[float]) -> Tensor:
+    return _distill.distill('distill_loss', logits, teacher_logits, teacher_index, None, vocab, temperature, softcap,
+                           False)[0]
+
+
+@distill_loss.register_fake
+def _distill_loss_fake(logits, teacher_logits, teacher_index, vocab, temperature, softcap):
+    return logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+
+
+@custom_op('noise_amd::distill_loss_grad', mutates_args=())
+def distill_loss_grad(logits: Tensor, teacher_logits: Tensor, teacher_index: Tensor, weight: Optional[Tensor],
+                      vocab: int, temperature: float, softcap: Optional[float]) -> Tuple[Tensor, Tensor]:
+    return _distill.distill('distill_loss_grad', logits, teacher_logits, teacher_index, weight, vocab, temperature,
+                           softcap, True)
+
+
+@distill_loss_grad.register_fake
+def _distill_loss_grad_fake(logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap):
+    return logits.new_empty(logits.shape[:-1], dtype=torch.float32), logits.new_empty(logits.shape)
+
+
+def _distill_loss_setup(ctx, inputs, output):
+    logits, teacher_logits, teacher_index, *ctx.more = inputs
+    ctx.save_for_backward(logits, teacher_logits, teacher_index)
+
+
+def _distill_loss_backward(ctx, weight):
+    return (torch.ops.noise_amd.distill_loss_grad(*ctx.saved_tensors, weight, *ctx.more)[1], None, None, None, None, None)
+
+
+distill_loss.register_autograd(_distill_loss_backward, setup_context=_distill_loss_setup)

@@ -1,0 +1,309 @@
+"""Attention layers of a model trained with exact gradients and served past its window.
+
+  qk_norm_rotary(q, k, cos, sin, ...)          norm of every head's queries and keys, rotated, in one pass; differentiable
+  qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, ...)   the same for new tokens, into a cache
+  sink_attention(q, k, v, window, sinks, lengths)   a sliding window and first tokens that stay visible; differentiable
+  sink_attention_decode(q, k_cache, v_cache, start, window, sinks)         a few new tokens against a cache
+
+Tensors are [batch, token, head, dim] with dim 64 or 128, as in utils/model.py; the queries' heads are a multiple of the
+keys' (query head h reads key head h // (H // Hk)). The norm and rotation are those of utils/model.py:46-47, 55-58 and
+88-94 (rotated halves; without learned weights the rotation and the norm commute), the mask that of utils/model.py:17-21
+with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators for compiled callers.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import Heads
+
+BF16, F32 = torch.bfloat16, torch.float32
+EPS = torch.finfo(F32).eps   # utils/model.py:46-47 under fp32 statistics
+TYPES = {BF16: _lib.TYPE_BF16, F32: _lib.TYPE_FP32}
+FAR = 2 ** 62                # windows from here on are all the same, whatever the cache
+MAX_NEW = 16                 # new tokens per sequence of one sink_attention_decode call
+
+
+def _check(fn, q, k, *others):
+    """[B, T, H, D] and [B, T', Hk, D] of one device, type and head dim."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f'{fn}: q and k must be [batch, token, head, dim] of one batch and dim, got '
+                         f'{tuple(q.shape)} and {tuple(k.shape)}')
+    if q.shape[3] not in (64, 128):
+        raise ValueError(f'{fn}: head dim must be 64 or 128, got {q.shape[3]}')
+    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f'{fn}: {q.shape[2]} query heads are no multiple of {k.shape[2]} key heads')
+    for t in (k, *others):
+        if t is not None and (t.device != q.device):
+            raise ValueError(f'{fn}: tensors on {q.device} and {t.device}')
+
+
+def _rows(t):
+    """t with unit inner stride and rows of whole 16 B at 16 B addresses (copied if it has not)."""
+    s, unit = t.stride(), 16 // t.element_size()
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % unit or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _heads(t):
+    s = t.stride()
+    return Heads(t.data_ptr(), s[0], s[1], s[2], t.shape[2])
+
+
+def _ref(t):
+    return None if t is None else ctypes.byref(_heads(t))
+
+
+def _call(name, device, *args):
+    """The entry point on `device`'s current stream (made the current device for the launch)."""
+    if device.type != 'cuda':
+        raise ValueError(f'{name}: tensors must be on a GPU, got {device}')
+    if torch.cuda.current_device() == device.index:
+        return _lib.call(name, *args, _lib.stream_ptr(device))
+    with torch.cuda.device(device):
+        return _lib.call(name, *args, _lib.stream_ptr(device))
+
+
+def _ints(fn, name, t, batch, device):
+    """[batch] int32 or int64 on the device, contiguous, and whether it is int64."""
+    if t.dtype not in (torch.int32, torch.int64) or t.shape != (batch,) or t.device != device:
+        raise ValueError(f'{fn}: {name} must be int32 or int64 of shape [{batch}] on {device}, got {t.dtype} '
+                         f'{tuple(t.shape)} on {t.device}')
+    return t.contiguous(), int(t.dtype == torch.int64)
+
+
+# --- norm and rotation ---
+
+
+def _tables(fn, cos, sin, D, device):
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D // 2 or cos.shape[0] == 0:
+        raise ValueError(f'{fn}: cos and sin must be [positions, {D // 2}], got {tuple(cos.shape)} and {tuple(sin.shape)}')
+    out = []
+    for t in (cos, sin):
+        if t.device != device:
+            raise ValueError(f'{fn}: rotation tables on {t.device}, tensors on {device}')
+        t = t.to(F32).contiguous()
+        out.append(t.clone() if t.data_ptr() % 16 else t)
+    return out
+
+
+def _weight(fn, w, D, device):
+    if w is None:
+        return None
+    if w.shape != (D,) or w.device != device:
+        raise ValueError(f'{fn}: weights must be [{D}] on {device}, got {tuple(w.shape)} on {w.device}')
+    w = w.detach().to(F32).contiguous()
+    return w.clone() if w.data_ptr() % 16 else w
+
+
+def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
+    _check(fn, q, k)
+    if q.shape[1] != k.shape[1] or q.dtype != k.dtype:
+        raise ValueError(f'{fn}: q and k must have one length and type, got {tuple(q.shape)} {q.dtype} and '
+                         f'{tuple(k.shape)} {k.dtype}')
+    if q.dtype not in TYPES:
+        raise ValueError(f'{fn}: bfloat16 or float32 tensors, got {q.dtype}')
+    B, T, _, D = q.shape
+    cos, sin = _tables(fn, cos, sin, D, q.device)
+    if start is not None:
+        start, wide = _ints(fn, 'start', start, B, q.device)
+    else:
+        wide = 0
+        if T > cos.shape[0]:
+            raise ValueError(f'{fn}: {T} tokens but rotation tables of {cos.shape[0]} positions')
+    return cos, sin, _weight(fn, q_weight, D, q.device), _weight(fn, k_weight, D, q.device), start, wide
+
+
+def norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps):
+    fn = 'qk_norm_rotary'
+    cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
+    B, T, H, D = q.shape
+    x = [_rows(q), _rows(k)]
+    y = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    _call('noise_qk_norm_rotary', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(*map(_heads, y)),
+          (ctypes.c_void_p * 2)(_lib.ptr(qw), _lib.ptr(kw)), None, None, cos.data_ptr(), sin.data_ptr(),
+          cos.shape[0], _lib.ptr(start), wide, B, T, 0, D, TYPES[q.dtype], eps)
+    return y[0], y[1]
+
+
+def norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, eps):
+    """Gradients of q, k and (in their types; None for absent ones) of the weights."""
+    fn = 'qk_norm_rotary'
+    cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
+    B, T, H, D = q.shape
+    x = [_rows(q), _rows(k)]
+    dy = [_rows(dq.to(q.dtype)), _rows(dk.to(q.dtype))]
+    dx = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    dw = [None if w is None else torch.empty(D, dtype=F32, device=q.device) for w in (qw, kw)]
+    need, work = 0, None
+    if qw is not None or kw is not None:
+        need = _lib.lib().noise_qk_norm_rotary_bwd_workspace_bytes(D)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    vp = ctypes.c_void_p * 2
+    _call('noise_qk_norm_rotary_bwd', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(*map(_heads, dy)),
+          (Heads * 2)(*map(_heads, dx)), vp(_lib.ptr(qw), _lib.ptr(kw)), vp(*map(_lib.ptr, dw)), cos.data_ptr(),
+          sin.data_ptr(), cos.shape[0], _lib.ptr(start), wide, B, T, D, TYPES[q.dtype], eps, _lib.ptr(work), need)
+    return (dx[0], dx[1], *(None if g is None else g.to(w.dtype) for g, w in zip(dw, (q_weight, k_weight))))
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, q_weight, k_weight, start, eps):
+        ctx.save_for_backward(q, k, cos, sin, q_weight, k_weight, start)
+        ctx.eps = eps
+        return norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, cos, sin, q_weight, k_weight, start = ctx.saved_tensors
+        dq, dk, dqw, dkw = norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, ctx.eps)
+        return dq, dk, None, None, dqw, dkw, None, None
+
+
+def qk_norm_rotary(q, k, cos, sin, q_weight=None, k_weight=None, start=None, eps=EPS):
+    """(q', k'): every row of q [B, T, H, D] and k [B, T, Hk, D] normed to RMS 1 over D (fp32 statistics), times its
+    weight [D] if there is one, and rotated for its position: t, or start[b] + t with start [B] (int32 or int64). cos and
+    sin are tables [positions, D / 2] over absolute positions (used in fp32); a token whose position lies outside them
+    gets zeros (and has no gradient). q and k are bfloat16 or float32, and so are q' and k' (contiguous), rounded once.
+    Differentiable in q, k and the weights (once); the weights' gradients are summed in fp32 in a fixed order."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
+        return _Norm.apply(q, k, cos, sin, q_weight, k_weight, start, float(eps))
+    return norm_forward(q, k, cos, sin, q_weight, k_weight, start, float(eps))
+
+
+@torch.no_grad()
+def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=None, k_weight=None, eps=EPS):
+    """q' of qk_norm_rotary for new tokens at positions start[b] + t, with k' and v [B, T, Hk, D] written to those slots of
+    k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
+    cache or the tables gets zeros in q' and leaves the cache as it is, so an idle sequence has a start of -T; no other
+    slot is touched. Not differentiable (it writes in place)."""
+    fn = 'qk_norm_rotary_append'
+    cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
+    B, T, H, D = q.shape
+    if start is None:
+        raise ValueError(f'{fn}: start is required')
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"{fn}: v must have k's shape, type and device, got {tuple(v.shape)} {v.dtype} on {v.device}")
+    S = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    for c in (k_cache, v_cache):
+        if c.shape != (B, S, k.shape[2], D) or c.dtype != k.dtype or c.device != k.device or S == 0:
+            raise ValueError(f'{fn}: caches must be [{B}, capacity, {k.shape[2]}, {D}] {k.dtype} on {k.device}, got '
+                             f'{tuple(c.shape)} {c.dtype} on {c.device}')
+        unit = 16 // c.element_size()
+        if c.stride(3) != 1 or any(s % unit for s in c.stride()[:3]) or c.data_ptr() % 16:
+            raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
+    x, v = [_rows(q), _rows(k)], _rows(v)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _call('noise_qk_norm_rotary', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(_heads(out), _heads(k_cache)),
+          (ctypes.c_void_p * 2)(_lib.ptr(qw), _lib.ptr(kw)), _ref(v), _ref(v_cache), cos.data_ptr(),
+          sin.data_ptr(), cos.shape[0], start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
+    return out
+
+
+# --- attention ---
+
+
+def _attend_operands(fn, q, k, v, window, sinks, lengths):
+    _check(fn, q, k, v)
+    if v.shape != k.shape or q.shape[1] != k.shape[1]:
+        raise ValueError(f'{fn}: k and v must have one shape and the length of q, got {tuple(q.shape)}, '
+                         f'{tuple(k.shape)}, {tuple(v.shape)}')
+    if q.dtype != BF16 or k.dtype != BF16 or v.dtype != BF16:
+        raise ValueError(f'{fn}: bfloat16 tensors, got {q.dtype}, {k.dtype}, {v.dtype}')
+    if window < 0 or sinks < 0:
+        raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
+    return (None, 0) if lengths is None else _ints(fn, 'lengths', lengths, q.shape[0], q.device)
+
+
+def attend_forward(q, k, v, window, sinks, lengths, with_lse):
+    """(out, lse or None)"""
+    fn = 'sink_attention'
+    lengths, wide = _attend_operands(fn, q, k, v, window, sinks, lengths)
+    B, T, H, D = q.shape
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty(B, T, H, D, dtype=BF16, device=q.device)
+    lse = torch.empty(B, H, T, dtype=F32, device=q.device) if with_lse else None
+    _call('noise_sink_attention_fwd', q.device, _ref(q), _ref(k), _ref(v), _ref(out), _lib.ptr(lse),
+          _lib.ptr(lengths), wide, B, T, D, window, sinks, 1.0 / math.sqrt(D))
+    return out, lse
+
+
+def attend_backward(dout, q, k, v, out, lse, window, sinks, lengths):
+    fn = 'sink_attention'
+    lengths, wide = _attend_operands(fn, q, k, v, window, sinks, lengths)
+    B, T, H, D = q.shape
+    grads = [torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v)]
+    q, k, v, out, dout = map(_rows, (q, k, v, out, dout.to(BF16)))
+    need = _lib.lib().noise_sink_attention_bwd_workspace_bytes(B, T, H, k.shape[2], D, window, sinks)
+    work = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
+    _call('noise_sink_attention_bwd', q.device, _ref(q), _ref(k), _ref(v), _ref(out), _ref(dout),
+          lse.data_ptr(), *map(_ref, grads), _lib.ptr(lengths), wide, B, T, D, window, sinks, 1.0 / math.sqrt(D),
+          work.data_ptr(), need)
+    return grads
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, lengths):
+        out, lse = attend_forward(q, k, v, window, sinks, lengths, True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.mask = (window, sinks)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        return (*attend_backward(dout, q, k, v, out, lse, *ctx.mask, lengths), None, None, None)
+
+
+def sink_attention(q, k, v, window, sinks=0, lengths=None):
+    """Causal attention in which token i sees the tokens j <= i with i - j <= window or j < sinks, [B, T, H, D] from q
+    [B, T, H, D] and k, v [B, T, Hk, D] in bfloat16 (fp32 scores and sums; the weights and, in the backward pass, the scores'
+    gradients are rounded to bfloat16 for their products). lengths [B] (int32 or int64): the batch is padded; tokens from
+    lengths[b] on are seen by none, get zeros, have no gradient, and may hold anything. Keys of the sequence itself are
+    taken to be finite. Differentiable in q, k and v (once), with sums in a fixed order."""
+    window, sinks = min(int(window), FAR), min(int(sinks), FAR)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attend.apply(q, k, v, window, sinks, lengths)
+    return attend_forward(q, k, v, window, sinks, lengths, False)[0]
+
+
+@torch.no_grad()
+def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
+    """sink_attention of T new tokens (1 to 16) against a cache: q [B, T, H, D], k_cache and v_cache [B, capacity, Hk, D]
+    in bfloat16, whose slots hold the positions 0, 1, ...; token t of sequence b stands at position start[b] + t (its own
+    key already in the cache, as qk_norm_rotary_append leaves it) and sees the slots up to there that the window and the
+    sinks allow. A token at a negative position (an idle sequence has a start of -T) gets zeros. Slots that no token of
+    the call sees may hold anything. Not differentiable."""
+    fn = 'sink_attention_decode'
+    window, sinks = min(int(window), FAR), min(int(sinks), FAR)
+    _check(fn, q, k_cache, v_cache)
+    if v_cache.shape != k_cache.shape or k_cache.shape[1] == 0:
+        raise ValueError(f'{fn}: caches must have one shape and some capacity, got {tuple(k_cache.shape)} and '
+                         f'{tuple(v_cache.shape)}')
+    if q.dtype != BF16 or k_cache.dtype != BF16 or v_cache.dtype != BF16:
+        raise ValueError(f'{fn}: bfloat16 tensors, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}')
+    B, T, H, D = q.shape
+    if T > MAX_NEW:
+        raise ValueError(f'{fn}: at most {MAX_NEW} new tokens, got {T}')
+    if window < 0 or sinks < 0:
+        raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
+    start, wide = _ints(fn, 'start', start, B, q.device)
+    for c in (k_cache, v_cache):
+        if c.stride(3) != 1 or any(s % 8 for s in c.stride()[:3]) or c.data_ptr() % 16:
+            raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
+    q = _rows(q)
+    out = torch.empty(B, T, H, D, dtype=BF16, device=q.device)
+    S, Hk = k_cache.shape[1:3]
+    need = _lib.lib().noise_sink_decode_workspace_bytes(B, T, H, Hk, S, D, window, sinks)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    _call('noise_sink_decode', q.device, _ref(q), _ref(k_cache), _ref(v_cache), _ref(out), start.data_ptr(),
+          wide, B, T, S, D, window, sinks, 1.0 / math.sqrt(D), _lib.ptr(work), need)
+    return out

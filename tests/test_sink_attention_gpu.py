@@ -1,0 +1,202 @@
+"""sink_attention and its gradients against the 64-bit definition, element by element.
+
+Bounds (bf16's half step u = 2^-8): the weights p are rounded once for p v and the result once, so an output is off by at
+most u (sum p |v| + |o|). For the gradients oracle.sinks.attend_grads adds up the same roundings of p, of the scores'
+gradients and of the output. fp32 sums of at most some thousand terms and exponents of scores below 2^7 add less than
+2^-14 of the same sums: 2 % of u."""
+import math
+
+import pytest
+import torch
+
+from oracle import sinks as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda', 0)
+U = 2.0 ** -8
+MORE = 1.02
+TINY = 1e-30
+
+
+def inputs(B, T, H, Hk, D, seed, n=3):
+    g = torch.Generator(DEV).manual_seed(seed)
+    q, *rest = (torch.randn(B, T, H if i in (0, 3) else Hk, D, device=DEV, generator=g) for i in range(n))
+    rest[0][:, :2] *= 1.5     # first keys that draw attention
+    return [t.bfloat16() for t in (q, *rest)]
+
+
+def check(got, want, bound, what):
+    assert got.shape == want.shape and got.dtype == torch.bfloat16
+    off = (got.double() - want).abs()
+    worst = (off - MORE * bound - TINY).max().item()
+    assert worst <= 0 and bool(torch.isfinite(got).all()), f'{what}: {off.max().item()} off, {worst} past its bound'
+
+
+def check_all(q, k, v, dout, window, sinks, lengths=None):
+    from noise_amd.sinks import sink_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sink_attention(*leaves, window, sinks, lengths)
+    want, weight = oracle.attend(q, k, v, window, sinks, lengths)
+    check(out.detach(), want, U * (weight + want.abs()), 'out')
+    assert torch.equal(sink_attention(q, k, v, window, sinks, lengths), out)
+    grads = torch.autograd.grad(out, leaves, dout)
+    wants, bounds = oracle.attend_grads(q, k, v, dout, window, sinks, lengths)
+    for name, got, want, bound in zip('qkv', grads, wants, bounds):
+        check(got, want, bound, f'd{name}')
+    return out.detach(), grads
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('T', [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 513, 777])
+def test_lengths_of_the_sequence(T, D):
+    for H, Hk, window, sinks in ((1, 1, T, 0), (2, 1, 40, 3), (6, 2, 0, 1), (3, 3, 70, 100)):
+        print(T, D, H, Hk, window, sinks, flush=True)
+        check_all(*inputs(2, T, H, Hk, D, T, 4), window, sinks)
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('window', [0, 1, 31, 32, 63, 64, 65, 200, 10 ** 9])
+@pytest.mark.parametrize('sinks', [0, 1, 4, 32, 63, 64, 65, 130, 10 ** 9])
+def test_masks(window, sinks, D):
+    print(window, sinks, D, flush=True)
+    check_all(*inputs(1, 421, 2, 1, D, 7, 4), window, sinks)
+
+
+@pytest.mark.parametrize('D', [64, 128])
+def test_a_long_sequence(D):
+    check_all(*inputs(1, 2100, 4, 2, D, 1, 4), 300, 70)
+
+
+@pytest.mark.parametrize('wide', [torch.int32, torch.int64])
+@pytest.mark.parametrize('D', [64, 128])
+def test_padded_batch(D, wide):
+    """Rows past the lengths hold NaN, infinities and the type's lowest value; lengths of 0 and 1, past the tensors and
+    negative."""
+    T = 333
+    lengths = torch.tensor([T, 0, 1, 64, 200, T + 5, -3, 65], device=DEV, dtype=wide)
+    q, k, v, dout = inputs(8, T, 4, 2, D, 3, 4)
+    clean = check_all(q, k, v, dout, 50, 3, lengths)
+    bad = [math.nan, math.inf, -math.inf, torch.finfo(torch.bfloat16).min]
+    for t in (q, k, v, dout):
+        for b in range(8):
+            n = min(T, max(0, int(lengths[b])))
+            t[b, n:] = torch.tensor(bad, device=DEV).repeat(D // 4).bfloat16()
+    from noise_amd.sinks import sink_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sink_attention(*leaves, 50, 3, lengths)
+    for got, want in zip((out, *torch.autograd.grad(out, leaves, dout)), (clean[0], *clean[1])):
+        assert torch.equal(got, want)
+
+
+def test_strides_and_views():
+    B, T, H, D = 2, 150, 4, 64
+    g = torch.Generator(DEV).manual_seed(5)
+    packed = torch.randn(B, T, 3 * H + 1, D, device=DEV, generator=g).bfloat16()
+    q, k, v = packed[:, :, :H], packed[:, :, H:2 * H], packed[:, :, 2 * H:3 * H]
+    dout = torch.randn(B, H, T, D, device=DEV, generator=g).bfloat16().transpose(1, 2)
+    check_all(q, k, v, dout, 60, 5)
+    wide = torch.randn(B, T, H, D + 1, device=DEV, generator=g).bfloat16()
+    check_all(wide[..., 1:], k[:, :, :2], wide[..., :2 * 64][:, :, :2, 1:], dout, 60, 5)   # odd addresses: copied
+    check_all(q[:1].expand(B, T, H, D), k[:1].expand(B, T, H, D), v, dout, 60, 5)          # a broadcast batch
+    check_all(q, k[:, :, :1].expand(B, T, 2, D), v[:, :, :2], dout, 60, 5)                 # a broadcast head
+    check_all(q, k, v, dout[:, :1].expand(B, T, H, D), 60, 5)
+
+
+def test_gradients_of_broadcast_inputs_add_up():
+    from noise_amd.sinks import sink_attention
+    q, k, v, dout = inputs(3, 70, 4, 2, 64, 2, 4)
+    one = k[:1].clone().requires_grad_()
+    sink_attention(q, one.expand(3, 70, 2, 64), v, 30, 2).backward(dout)
+    each = k[:1].expand(3, 70, 2, 64).clone().requires_grad_()
+    sink_attention(q, each, v, 30, 2).backward(dout)
+    assert torch.allclose(one.grad.float(), each.grad.float().sum(0, keepdim=True), rtol=2 * U, atol=4 * U)
+
+
+def test_gradients_against_differences():
+    """The step's change of sum(dout * out), by the 64-bit definition, over a step along each gradient's own direction."""
+    from noise_amd.sinks import sink_attention
+    q, k, v, dout = inputs(1, 90, 4, 2, 64, 11, 4)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(sink_attention(*leaves, 25, 2), leaves, dout)
+    bounds = oracle.attend_grads(q, k, v, dout, 25, 2)[1]
+    for i in range(3):
+        d = grads[i].double()
+        at = lambda step: (oracle.attend(*[t.double() + (step * d if n == i else 0) for n, t in enumerate((q, k, v))],
+                                         25, 2)[0] * dout.double()).sum()
+        h = 1e-4 / d.abs().max()
+        slope = (at(h) - at(-h)) / (2 * h)
+        # the slope along d is d . (true gradient): off from d . d by at most |d| . bound (and the difference's h^2)
+        assert abs(slope - d.square().sum()) <= MORE * (d.abs() * bounds[i]).sum() + 1e-5 * d.square().sum()
+
+
+def test_empty():
+    from noise_amd.sinks import sink_attention
+    for shape in ((0, 5, 4, 64), (2, 0, 4, 64)):
+        q = torch.empty(shape, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        out = sink_attention(q, q[:, :, :2], q[:, :, 2:], 10, 2)
+        assert out.shape == shape
+        out.sum().backward()
+        assert q.grad.shape == shape
+
+
+def test_growing_scores():
+    """Scores far apart, and rows whose largest weight stands in the last tile or the first key."""
+    q, k, v, dout = inputs(1, 400, 2, 2, 64, 8, 4)
+    k = (k.float() * torch.linspace(0.1, 9, 400, device=DEV)[None, :, None, None]).bfloat16()
+    check_all(q, k, v, dout, 390, 0)
+    check_all(q, k.flip(1).contiguous(), v, dout, 100, 7)
+
+
+def test_repeats_and_streams():
+    from noise_amd.sinks import sink_attention
+    q, k, v, dout = inputs(2, 700, 8, 2, 128, 4, 4)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    run = lambda: (lambda o: (o, *torch.autograd.grad(o, leaves, dout)))(sink_attention(*leaves, 100, 70))
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        others = [run() for _ in range(3)]
+    here = [run() for _ in range(3)]
+    torch.cuda.synchronize()
+    for results in (*others, *here):
+        assert all(torch.equal(x, y) for x, y in zip(first, results))
+
+
+def test_captured_graphs():
+    """Forward and backward captured twice; the replays, in turn with eager calls on other inputs, give the eager bits."""
+    from noise_amd.sinks import attend_backward, attend_forward, sink_attention
+    q, k, v, dout = inputs(2, 500, 4, 2, 64, 6, 4)
+
+    def step():
+        out, lse = attend_forward(q, k, v, 90, 4, None, True)
+        return (out, *attend_backward(dout, q, k, v, out, lse, 90, 4, None))
+
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for n in range(3):
+        for t, x in zip((q, k, v, dout), inputs(2, 500, 4, 2, 64, 50 + n, 4)):
+            t.copy_(x)
+        want = step()
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+        sink_attention(q[:1], k[:1], v[:1], 3)
+
+
+def test_compiled_operator():
+    q, k, v, dout = inputs(2, 130, 4, 2, 64, 12, 4)
+    from noise_amd.sinks import sink_attention
+    results = []
+    for f in (lambda *t: torch.ops.noise_amd.sink_attention(*t, 40, 3, None)[0], lambda *t: sink_attention(*t, 40, 3)):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = f(*leaves)
+        results.append((out, *torch.autograd.grad(out, leaves, dout)))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
