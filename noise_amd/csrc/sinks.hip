@@ -258,26 +258,6 @@ int launch_units(void (*kernel)(SinkArgs), SinkArgs &a, int64_t units, hipStream
 
 using namespace noise;
 
-extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                                        const noise_heads_t *o, float *lse, const void *lengths, int lengths_wide,
-                                        int64_t batch, int64_t tokens, int64_t head_dim, int64_t window,
-                                        int64_t sinks, float scale, noise_stream_t stream) {
-    clear_error();
-    const char *fn = "noise_sink_attention_fwd";
-    NOISE_CHECK_ARG(q && k && v && o && q->heads == o->heads && k->heads == v->heads, "%s: tensors missing or of other heads", fn);
-    int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
-    if (st) return st;
-    if (batch == 0 || tokens == 0) return NOISE_OK;
-    SinkArgs a;
-    if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||
-        (st = check_heads(fn, "v", v, &a.v)) || (st = check_heads(fn, "o", o, &a.o)))
-        return st;
-    fill_args(&a, lengths, nullptr, lengths_wide, tokens, tokens, q->heads, k->heads, window, sinks, scale);
-    a.lse = lse;
-    return launch_units(head_dim == 64 ? sink_fwd_kernel<64> : sink_fwd_kernel<128>, a, batch * q->heads * tokens,
-                        (hipStream_t)stream, fn);
-}
-
 extern "C" int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads,
                                                             int64_t kv_heads, int64_t head_dim, int64_t window,
                                                             int64_t sinks) {

@@ -40,9 +40,10 @@ def _check(fn, q, k, *others):
 
 
 def _rows(t):
-    """t with unit inner stride and rows of whole 16 B at 16 B addresses (copied if it has not)."""
+    """t with unit inner stride and rows of whole 16 B at 16 B addresses, less than 2^25 elements from token to token (copied
+    if it has not)."""
     s, unit = t.stride(), 16 // t.element_size()
-    if s[3] != 1 or (s[0] | s[1] | s[2]) % unit or t.data_ptr() % 16:
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % unit or s[1] >= 1 << 25 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
