@@ -1,0 +1,523 @@
+// Backward pass of the attention with a sliding window and first tokens that stay visible, without atomics:
+//   delta_i = sum_d dO_id o_id,  p_ij = 2^(c s_ij - lse_i),  dS = p (dO V^T - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+// Two kernels recompute the scores. sink_dq_kernel walks the key tiles of 128 queries (4 waves of 32) with transposed scores, as
+// the forward pass does, and leaves delta and lse as the second kernel wants them. sink_dkv_kernel walks the query tiles of
+// 128 keys (4 waves of 32, keys and values in registers) over all query heads of the key head. In both a lane's scores and
+// their gradients are the operand of the product that adds them up, so neither passes through LDS; the tiles that walk
+// by are copied into two LDS stages and read by rows and by columns. The lists of query tiles of the first tokens' keys reach
+// to the end of the sequence, far past the window: a list is cut into parts of a fixed length, each part's sums go to the
+// workspace in fp32 and sink_join_kernel adds them in order.
+#include "sink_common.hpp"
+
+namespace noise {
+namespace {
+
+constexpr int kTileRows = 64;  // rows of the tiles that walk by
+constexpr int kOwn = 128;      // queries (dq) or keys (dk, dv) of a workgroup
+
+struct BwdArgs {
+    Rows q, k, v, o, d_o, dq, dk, dv;
+    const float *lse;
+    float *nlse, *ndelta;    // -lse / c and -delta, [batch * heads][tokens]
+    float *parts;
+    const void *lengths;
+    int64_t first;
+    int wide, tokens, heads, kv_heads, group, window, sinks, tiles;
+    int rows, xcd_rows;              // batch * heads (dq) or batch * kv_heads (dk, dv)
+    int sink_tiles, sink_parts, band_parts, part;  // key tiles with first tokens; most parts of each kind; tiles per part
+    float scale, scale_log2;
+};
+
+__device__ __forceinline__ int row_of(int u, int xcd_rows) { return xcd_rows ? (u & 7) * xcd_rows + (u >> 3) : u; }
+
+__device__ __forceinline__ int seq_len(const BwdArgs &a, int b) {
+    int len = a.tokens;
+    if (a.lengths) {
+        const int64_t n = at_wide(a.lengths, a.wide, b);
+        len = n < 0 ? 0 : n < len ? (int)n : len;
+        len = __builtin_amdgcn_readfirstlane(len);
+    }
+    return len;
+}
+
+// A tile pair's copies into a stage by 4 waves, rows past `last` taken from it
+template <int D>
+struct Copies {
+    using TL = Tile<D>;
+    static constexpr int kTile = kTileRows * TL::RB, kStage = 2 * kTile;
+    static constexpr int CPW = kTile / 1024 / 4;  // copies per wave and tensor
+    static_assert(4 * TL::RPC % 16 == 0, "uniform swizzle");
+    int r0, chunk, wave;
+    __device__ Copies(int wave_, int lane) : wave(wave_) {
+        r0 = TL::RPC * wave + lane / TL::CPR;
+        chunk = TL::swb(r0, lane % TL::CPR);
+    }
+    __device__ __forceinline__ void one(const Rows &t, const __bf16 *base, int row0, int last, unsigned st) const {
+        if (row0 + kTileRows - 1 > last) {
+#pragma unroll
+            for (int i = 0; i < CPW; ++i) {
+                const int r = i * 4 * TL::RPC + r0;
+                const unsigned rr = (unsigned)(row0 + r > last ? last - row0 : r);
+                lds_dma16_at(base + (int64_t)row0 * t.s_t, rr * (unsigned)t.s_t * 2 + chunk * 16, st + (4 * i + wave) * 1024);
+            }
+        } else {
+            const unsigned off = (unsigned)(r0 * (int)t.s_t * 2 + chunk * 16);
+#pragma unroll
+            for (int i = 0; i < CPW; ++i)
+                lds_dma16_at(base + (int64_t)(row0 + i * 4 * TL::RPC) * t.s_t, off, st + (4 * i + wave) * 1024);
+        }
+    }
+};
+
+// Fragments of a tile (a stage's half): rows in the order sigma, and columns (as a source, lane 16 g + i addresses row
+// 8 (g / 2) + i / 4 (+ 16 s, + 4), columns 16 (g % 2) + 4 (i % 4) .. + 4 (+ 32 db: offset ^ 64 db))
+template <int D>
+struct Frags {
+    using TL = Tile<D>;
+    int rows, cols;
+    __device__ Frags(int lane) {
+        const int sj = sigma(lane & 31), hf = lane >> 5, r = 8 * hf + ((lane & 15) >> 2);
+        rows = sj * TL::RB + (TL::swb(sj, hf) << 4);
+        cols = r * TL::RB + (TL::swb(r, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + 8 * (lane & 1);
+    }
+    // rows 32 blk + sigma(j), k-step s
+    __device__ __forceinline__ bf16x8 row(const char *tile, int blk, int s) const {
+        return *reinterpret_cast<const bf16x8 *>(tile + (rows ^ (32 * s)) + blk * 32 * TL::RB);
+    }
+    // columns 32 db .., rows 16 s .. of the tile (the second read's four rows differ in the chunk's lowest bit)
+    __device__ __forceinline__ bf16x8 col(const char *tile, int db, int s) const {
+        const char *p = tile + 16 * TL::RB * s;
+        return cat(lds_read_tr16(p + (cols ^ (64 * db))), lds_read_tr16(p + 4 * TL::RB + (cols ^ (64 * db) ^ 16)));
+    }
+};
+
+// a wave's 32 x D block, held as [D / 32] transposed 32 x 32 results, times mul, stored as rows of bf16 through its own LDS:
+// rows [r0, end) of the tensor, those from `zero` on as zeros
+template <int D>
+__device__ __forceinline__ void store_block(const f32x16 (&acc)[D / 32], float mul, const Rows &t, __bf16 *base, int r0,
+                                            int end, int zero, char *lds, int lane) {
+    using TL = Tile<D>;
+    constexpr int kPitch = D + 8;
+    __bf16 *stg = reinterpret_cast<__bf16 *>(lds);
+    const int j = lane & 31, hf = lane >> 5;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            bf16x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (__bf16)(r0 + j < zero ? acc[db][4 * g + e] * mul : 0.f);
+            store_bf16x4(stg + j * kPitch + 32 * db + 8 * g + 4 * hf, v);
+        }
+    wave_lds_sync();
+#pragma unroll
+    for (int it = 0; it < TL::CPR / 2; ++it) {
+        const int c = it * 64 + lane, r = c / TL::CPR, ch = c % TL::CPR;
+        if (r0 + r < end) store_bf16x8(base + (int64_t)(r0 + r) * t.s_t + ch * 8, load_bf16x8(stg + r * kPitch + ch * 8));
+    }
+    wave_lds_sync();
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
+    using TL = Tile<D>;
+    using CP = Copies<D>;
+    constexpr int KS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage];
+    const int64_t wg = a.first + blockIdx.x;
+    const int qt = a.tiles - 1 - (int)(wg / a.rows), row = row_of((int)(wg % a.rows), a.xcd_rows);
+    const int b = row / a.heads, h = row - b * a.heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j = lane & 31, hf = lane >> 5;
+    const int len = seq_len(a, b), last = len - 1, q_lo = qt * kOwn, q0w = q_lo + 32 * wave;
+    __bf16 *dqb = a.dq.ptr + b * a.dq.s_b + h * a.dq.s_h;
+    if (q_lo > last) {
+        const int n = (a.tokens - q_lo < kOwn ? a.tokens - q_lo : kOwn) * TL::CPR;
+        for (int c = tid; c < n; c += 256)
+            store_bf16x8(dqb + (int64_t)(q_lo + c / TL::CPR) * a.dq.s_t + 8 * (c % TL::CPR), zero_bf16x8());
+        return;
+    }
+    const __bf16 *Kb = a.k.ptr + b * a.k.s_b + (h / a.group) * a.k.s_h;
+    const __bf16 *Vb = a.v.ptr + b * a.v.s_b + (h / a.group) * a.v.s_h;
+    bf16x8 qf[KS], df[KS];
+    float nd = 0.f, lse;
+    {
+        const int q = q0w + j < last ? q0w + j : last;
+        const __bf16 *qp = a.q.ptr + b * a.q.s_b + h * a.q.s_h + (int64_t)q * a.q.s_t + 8 * hf;
+        const __bf16 *dp = a.d_o.ptr + b * a.d_o.s_b + h * a.d_o.s_h + (int64_t)q * a.d_o.s_t + 8 * hf;
+        const __bf16 *op = a.o.ptr + b * a.o.s_b + h * a.o.s_h + (int64_t)q * a.o.s_t + 8 * hf;
+        const int64_t li = (int64_t)row * a.tokens + q;
+        lse = a.lse[li];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            qf[s] = load_bf16x8(qp + 16 * s);
+            df[s] = load_bf16x8(dp + 16 * s);
+            const bf16x8 o = load_bf16x8(op + 16 * s);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) nd -= (float)df[s][e] * (float)o[e];
+        }
+        nd += swap_halves(nd);
+        if (hf == 0 && q0w + j <= last) {
+            a.nlse[li] = -lse / a.scale_log2;
+            a.ndelta[li] = nd;
+        }
+    }
+    vm_wait<0>();
+    const int W = a.window, n_sinks = a.sinks;
+    const int q_hi = q_lo + kOwn - 1 < last ? q_lo + kOwn - 1 : last;
+    const int band = (q_lo > W ? q_lo - W : 0) / kTileRows;
+    const int sunk = (n_sinks + kTileRows - 1) / kTileRows < band ? (n_sinks + kTileRows - 1) / kTileRows : band;
+    const int nt = sunk + q_hi / kTileRows - band + 1;
+    auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kTileRows; };
+    const CP cp(wave, lane);
+    const Frags<D> fr(lane);
+    const unsigned lb = lds_addr(lds);
+    auto issue = [&](int t) {
+        const unsigned st = lb + (t & 1) * CP::kStage;
+        cp.one(a.k, Kb, tile_k0(t), last, st);
+        cp.one(a.v, Vb, tile_k0(t), last, st + CP::kTile);
+    };
+    f32x16 dq[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
+    const int wq_lo = q0w, wq_hi = q0w > last ? -1 : q0w + 31 < last ? q0w + 31 : last;
+    const float c2 = a.scale_log2;
+    issue(0);
+#pragma unroll 1
+    for (int t = 0; t < nt; ++t) {
+        vm_wait<0>();
+        __syncthreads();   // tile t landed, and every wave is past tile t - 1
+        if (t + 1 < nt) issue(t + 1);
+        const int k0 = tile_k0(t);
+        if (k0 > wq_hi || (k0 + kTileRows - 1 < wq_lo - W && k0 >= n_sinks)) continue;
+        const char *kt = lds + (t & 1) * CP::kStage, *vt = kt + CP::kTile;
+        const bool causal_edge = k0 + kTileRows - 1 > wq_lo, window_edge = k0 < wq_hi - W;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x16 sc = f32x16{}, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dp[r] = nd;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                sc = mfma32x32x16(fr.row(kt, kb, s), qf[s], sc);
+                dp = mfma32x32x16(fr.row(vt, kb, s), df[s], dp);
+            }
+            if (causal_edge || window_edge) {
+                // as in the forward pass: key c = 16 (r / 8) + r % 8 from here
+                int d0 = q0w + j - k0 - 32 * kb - 8 * hf, ds = n_sinks - k0 - 32 * kb - 8 * hf;
+                unsigned wd = (unsigned)(d0 - W > ds ? d0 - W - ds : 0);
+                asm volatile("" : "+v"(d0), "+v"(wd), "+v"(ds));
+                if (causal_edge)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[r] = 16 * (r >> 3) + (r & 7) <= d0 ? sc[r] : -__builtin_inff();
+                if (window_edge)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        sc[r] = (unsigned)(16 * (r >> 3) + (r & 7) - ds) >= wd ? sc[r] : -__builtin_inff();
+            }
+            // the scores' gradients rounded to bf16 for the product on the matrix cores
+            bf16x8 g[2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) g[r >> 3][r & 7] = (__bf16)(exp2_fast(__builtin_fmaf(sc[r], c2, -lse)) * dp[r]);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) dq[db] = mfma32x32x16(fr.col(kt, db, 2 * kb + s), g[s], dq[db]);
+        }
+    }
+    __syncthreads();
+    static_assert(4 * 32 * (D + 8) * 2 <= 2 * CP::kStage, "staging fits");
+    store_block<D>(dq, a.scale, a.dq, dqb, q0w, a.tokens, len, lds + wave * 32 * (D + 8) * 2, lane);
+}
+
+// query tiles of key tile kt: first, and how many (of one query head)
+__device__ __forceinline__ int query_tiles(const BwdArgs &a, int kt, int len, int *first) {
+    const int k_lo = kt * kOwn, last = len - 1;
+    *first = k_lo / kTileRows;
+    if (k_lo > last) return 0;
+    const int k_hi = k_lo + kOwn - 1 + a.window;
+    const int end = k_lo < a.sinks || k_hi > last ? last : k_hi;
+    return end / kTileRows - *first + 1;
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
+    using TL = Tile<D>;
+    using CP = Copies<D>;
+    constexpr int KS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage + 2 * 2 * kTileRows * 4];
+    const int64_t wg = a.first + blockIdx.x;
+    const int item = (int)(wg / a.rows), row = row_of((int)(wg % a.rows), a.xcd_rows);
+    const int ns = a.sink_tiles * a.sink_parts;
+    const int kt = item < ns ? item / a.sink_parts : a.sink_tiles + (item - ns) / a.band_parts;
+    const int part = item < ns ? item % a.sink_parts : (item - ns) % a.band_parts;
+    const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int j = lane & 31, hf = lane >> 5;
+    const int len = seq_len(a, b), last = len - 1, k0w = kt * kOwn + 32 * wave;
+    int first;
+    const int nq = query_tiles(a, kt, len, &first), total = a.group * nq, parts = (total + a.part - 1) / a.part;
+    __bf16 *dkb = a.dk.ptr + b * a.dk.s_b + hk * a.dk.s_h, *dvb = a.dv.ptr + b * a.dv.s_b + hk * a.dv.s_h;
+    if (part >= parts) {
+        if (parts == 0 && part == 0) {
+            const int n = (a.tokens - kt * kOwn < kOwn ? a.tokens - kt * kOwn : kOwn) * TL::CPR;
+            for (int c = tid; c < n; c += 256) {
+                const int64_t t = kt * kOwn + c / TL::CPR;
+                store_bf16x8(dkb + t * a.dk.s_t + 8 * (c % TL::CPR), zero_bf16x8());
+                store_bf16x8(dvb + t * a.dv.s_t + 8 * (c % TL::CPR), zero_bf16x8());
+            }
+        }
+        return;
+    }
+    const int i0 = part * a.part, i1 = i0 + a.part < total ? i0 + a.part : total;
+    bf16x8 kf[KS], vf[KS];
+    {
+        const int key = k0w + j < last ? k0w + j : last;
+        const __bf16 *kp = a.k.ptr + b * a.k.s_b + hk * a.k.s_h + (int64_t)key * a.k.s_t + 8 * hf;
+        const __bf16 *vp = a.v.ptr + b * a.v.s_b + hk * a.v.s_h + (int64_t)key * a.v.s_t + 8 * hf;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            kf[s] = load_bf16x8(kp + 16 * s);
+            vf[s] = load_bf16x8(vp + 16 * s);
+        }
+    }
+    vm_wait<0>();
+    const CP cp(wave, lane);
+    const Frags<D> fr(lane);
+    const unsigned lb = lds_addr(lds);
+    auto issue = [&](int i) {
+        const int g = i / nq, q0 = (first + i - g * nq) * kTileRows;
+        const int h = hk * a.group + g;
+        const unsigned st = lb + (i & 1) * CP::kStage;
+        cp.one(a.q, a.q.ptr + b * a.q.s_b + h * a.q.s_h, q0, last, st);
+        cp.one(a.d_o, a.d_o.ptr + b * a.d_o.s_b + h * a.d_o.s_h, q0, last, st + CP::kTile);
+        // waves 0 and 1: -lse / c and -delta of the tile's queries
+        if (wave < 2) {
+            const float *src = (wave ? a.ndelta : a.nlse) + (int64_t)(b * a.heads + h) * a.tokens + q0;
+            lds_dma4_at(src, (unsigned)(q0 + lane > last ? last - q0 : lane) * 4,
+                        lb + 2 * CP::kStage + ((i & 1) * 2 + wave) * kTileRows * 4);
+        }
+    };
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
+    const int W = a.window, n_sinks = a.sinks;
+    // the queries that see this lane's key: key .. key + span (none: span -1)
+    const int key = k0w + j;
+    const int span = key > last ? -1 : (key < n_sinks || key + W > last ? last : key + W) - key;
+    // ... and that see all of the wave's keys, or any
+    const int all_lo = k0w + 31, all_hi = k0w + 31 > last ? -1 : k0w + W < last ? k0w + W : last;
+    const int any_hi = k0w > last ? -1 : k0w < n_sinks || k0w + 31 + W > last ? last : k0w + 31 + W;
+    const float c2 = a.scale_log2;
+    issue(i0);
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        vm_wait<0>();
+        __syncthreads();   // tile i landed, and every wave is past tile i - 1
+        if (i + 1 < i1) issue(i + 1);
+        const int q0 = (first + i % nq) * kTileRows;
+        const char *qt = lds + (i & 1) * CP::kStage, *dt = qt + CP::kTile;
+        const float *stats = reinterpret_cast<const float *>(lds + 2 * CP::kStage) + (i & 1) * 2 * kTileRows;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+            const int q = q0 + 32 * qb;
+            if (q + 31 < k0w || q > any_hi) continue;
+            // register r: query 16 (r / 8) + 8 hf + r % 8. The products accumulate onto -lse / c and -delta
+            f32x16 sc, dp;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int at = 32 * qb + 16 * (r >> 3) + 8 * hf + (r & 7);
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(stats + at);
+                const f32x4 y = *reinterpret_cast<const f32x4 *>(stats + kTileRows + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[r + e] = x[e], dp[r + e] = y[e];
+            }
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                sc = mfma32x32x16(fr.row(qt, qb, s), kf[s], sc);
+                dp = mfma32x32x16(fr.row(dt, qb, s), vf[s], dp);
+            }
+            if (q < all_lo || q + 31 > all_hi) {
+                // seen iff 0 <= query - key <= span: queries from q + 8 hf are c = 16 (r / 8) + r % 8
+                int lo = key - q - 8 * hf;
+                unsigned n = (unsigned)(span + 1);
+                asm volatile("" : "+v"(lo), "+v"(n));
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sc[r] = (unsigned)(16 * (r >> 3) + (r & 7) - lo) < n ? sc[r] : -__builtin_inff();
+            }
+            bf16x8 p[2], g[2];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = exp2_fast(sc[r] * c2);
+                p[r >> 3][r & 7] = (__bf16)e;
+                g[r >> 3][r & 7] = (__bf16)(e * dp[r]);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    dv[db] = mfma32x32x16(fr.col(dt, db, 2 * qb + s), p[s], dv[db]);
+                    dk[db] = mfma32x32x16(fr.col(qt, db, 2 * qb + s), g[s], dk[db]);
+                }
+        }
+    }
+    if (parts > 1) {
+        // [dk, dv][db][g][lane][4] of each wave: whole lines
+        float *out = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * 4 + wave) * (2 * DB * 16 * 64) + 4 * lane;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x16 &s = x ? dv[db] : dk[db];
+                    *reinterpret_cast<f32x4 *>(out + ((x * DB + db) * 4 + g) * 256) =
+                        f32x4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+                }
+        return;
+    }
+    __syncthreads();
+    char *stg = lds + wave * 32 * (D + 8) * 2;
+    store_block<D>(dk, a.scale, a.dk, dkb, k0w, a.tokens, len, stg, lane);
+    store_block<D>(dv, 1.f, a.dv, dvb, k0w, a.tokens, len, stg, lane);
+}
+
+// Adds the parts of key tiles that have several. grid: (key tiles, rows), 4 waves of 32 keys, the same registers as above
+template <int D>
+__global__ __launch_bounds__(256) void sink_join_kernel(BwdArgs a, int band) {
+    constexpr int DB = D / 32;
+    const int kt = band ? a.sink_tiles + blockIdx.x : blockIdx.x, row = blockIdx.y;
+    const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.z / DB, db = blockIdx.z % DB;
+    const int len = seq_len(a, b);
+    int first;
+    const int total = a.group * query_tiles(a, kt, len, &first), parts = (total + a.part - 1) / a.part;
+    if (parts < 2) return;
+    const int ns = a.sink_tiles * a.sink_parts;
+    const int item = kt < a.sink_tiles ? kt * a.sink_parts : ns + (kt - a.sink_tiles) * a.band_parts;
+    const int key = kt * kOwn + 32 * wave + (lane & 31);
+    if (key >= a.tokens) return;
+    const float *src = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * 4 + wave) * (2 * DB * 16 * 64) +
+                       (x * DB + db) * 1024 + 4 * lane;
+    f32x4 s[4] = {};
+    for (int p = 0; p < parts; ++p)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            s[g] += *reinterpret_cast<const f32x4 *>(src + (int64_t)p * a.rows * 4 * (2 * DB * 16 * 64) + g * 256);
+    const Rows &t = x ? a.dv : a.dk;
+    const float mul = x ? 1.f : a.scale;
+    __bf16 *out = t.ptr + b * t.s_b + hk * t.s_h + (int64_t)key * t.s_t + 32 * db + 4 * (lane >> 5);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (__bf16)(s[g][e] * mul);
+        store_bf16x4(out + 8 * g, v);
+    }
+}
+
+// How the lists of query tiles are cut: parts of `part` tiles, at most sink_parts of a key tile with first tokens and
+// band_parts of the others.
+struct Plan {
+    int64_t tiles, rows, sink_tiles, sink_parts, band_parts, part, items;
+    int64_t stats, bytes;
+};
+Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
+    Plan p;
+    const int64_t group = heads / kv_heads, q_tiles = (tokens + kTileRows - 1) / kTileRows;
+    window = window < tokens ? window : tokens;
+    sinks = sinks < tokens ? sinks : tokens;
+    p.tiles = (tokens + kOwn - 1) / kOwn;
+    p.rows = batch * kv_heads;
+    p.sink_tiles = (sinks + kOwn - 1) / kOwn;
+    const int64_t reach = (window + kOwn - 1) / kTileRows + 1;
+    const int64_t band = group * (reach < q_tiles ? reach : q_tiles);
+    p.part = band;
+    p.band_parts = p.sink_tiles < p.tiles ? 1 : 0;
+    p.sink_parts = p.sink_tiles ? (group * q_tiles + p.part - 1) / p.part : 0;
+    p.items = p.sink_tiles * p.sink_parts + (p.tiles - p.sink_tiles) * p.band_parts;
+    p.stats = (batch * heads * tokens * 4 + 15) / 16 * 16;
+    p.bytes = 2 * p.stats;
+    if (p.sink_parts > 1 || p.band_parts > 1) p.bytes += p.items * p.rows * kOwn * head_dim * 2 * 4;
+    return p;
+}
+
+}  // namespace
+}  // namespace noise
+
+using namespace noise;
+
+extern "C" int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads,
+                                                            int64_t kv_heads, int64_t head_dim, int64_t window,
+                                                            int64_t sinks) {
+    clear_error();
+    const int st = check_sizes("noise_sink_attention_bwd_workspace_bytes", batch, tokens, tokens, heads, kv_heads,
+                               head_dim, window, sinks);
+    if (st) return st;
+    if (batch == 0 || tokens == 0) return 0;
+    return plan(batch, tokens, heads, kv_heads, head_dim, window, sinks).bytes;
+}
+
+extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
+                                        const noise_heads_t *o, const noise_heads_t *d_o, const float *lse,
+                                        const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
+                                        const void *lengths, int lengths_wide, int64_t batch, int64_t tokens,
+                                        int64_t head_dim, int64_t window, int64_t sinks, float scale, void *workspace,
+                                        int64_t workspace_bytes, noise_stream_t stream) {
+    clear_error();
+    const char *fn = "noise_sink_attention_bwd";
+    NOISE_CHECK_ARG(q && k && v && o && d_o && dq && dk && dv && q->heads == o->heads && q->heads == d_o->heads &&
+                        q->heads == dq->heads && k->heads == v->heads && k->heads == dk->heads && k->heads == dv->heads,
+                    "%s: tensors missing or of other heads", fn);
+    int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
+    if (st) return st;
+    NOISE_CHECK_ARG(scale > 0.f && scale < __builtin_inff(), "%s: scale must be positive", fn);
+    if (batch == 0 || tokens == 0) return NOISE_OK;
+    NOISE_CHECK_ARG(lse && aligned(lse, 4), "%s: lse is required", fn);
+    NOISE_CHECK_ARG(!lengths || aligned(lengths, lengths_wide ? 8 : 4), "%s: lengths misaligned", fn);
+    const Plan p = plan(batch, tokens, q->heads, k->heads, head_dim, window, sinks);
+    NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes,
+                    "%s: workspace NULL, misaligned or below %lld bytes", fn, (long long)p.bytes);
+    BwdArgs a;
+    if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||
+        (st = check_heads(fn, "v", v, &a.v)) || (st = check_heads(fn, "o", o, &a.o)) ||
+        (st = check_heads(fn, "d_o", d_o, &a.d_o)) || (st = check_heads(fn, "dq", dq, &a.dq)) ||
+        (st = check_heads(fn, "dk", dk, &a.dk)) || (st = check_heads(fn, "dv", dv, &a.dv)))
+        return st;
+    for (const Rows *t : {&a.q, &a.k, &a.v, &a.d_o})
+        NOISE_CHECK_ARG(t->s_t >= 0 && t->s_t < kMaxStride, "%s: token strides of q, k, v and d_o must be below 2^25", fn);
+    NOISE_CHECK_ARG(p.rows <= 65535, "%s: at most 65535 sequences times key heads", fn);
+    a.lse = lse;
+    a.nlse = static_cast<float *>(workspace);
+    a.ndelta = a.nlse + p.stats / 4;
+    a.parts = a.ndelta + p.stats / 4;
+    a.lengths = lengths; a.wide = lengths_wide;
+    a.tokens = (int)tokens; a.heads = (int)q->heads; a.kv_heads = (int)k->heads; a.group = a.heads / a.kv_heads;
+    a.window = (int)(window < tokens ? window : tokens);
+    a.sinks = (int)(sinks < tokens ? sinks : tokens);
+    a.tiles = (int)p.tiles;
+    a.sink_tiles = (int)p.sink_tiles; a.sink_parts = (int)p.sink_parts; a.band_parts = (int)p.band_parts;
+    a.part = (int)p.part;
+    a.scale = scale; a.scale_log2 = scale * kLog2e;
+    const bool narrow = head_dim == 64;
+    auto launch = [&](void (*kernel)(BwdArgs), int64_t rows, int64_t items) {
+        a.rows = (int)rows;
+        a.xcd_rows = rows % 8 == 0 ? (int)(rows / 8) : 0;
+        for (a.first = 0; a.first < rows * items; a.first += kLaunchGroups) {
+            const int64_t n = rows * items - a.first < kLaunchGroups ? rows * items - a.first : kLaunchGroups;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
+        }
+    };
+    launch(narrow ? sink_dq_kernel<64> : sink_dq_kernel<128>, batch * q->heads, p.tiles);
+    launch(narrow ? sink_dkv_kernel<64> : sink_dkv_kernel<128>, p.rows, p.items);
+    for (int band = 0; band < 2; ++band) {
+        const int64_t n = band ? (p.band_parts > 1 ? p.tiles - p.sink_tiles : 0) : p.sink_parts > 1 ? p.sink_tiles : 0;
+        if (n)
+            hipLaunchKernelGGL(narrow ? sink_join_kernel<64> : sink_join_kernel<128>,
+                               dim3((unsigned)n, (unsigned)p.rows, (unsigned)(head_dim / 32 * 2)), dim3(256), 0,
+                               (hipStream_t)stream, a, band);
+    }
+    return launch_status(fn);
+}

@@ -40,18 +40,21 @@ __device__ __forceinline__ float wave_sum(float v) {
 // stands for row 16 (r / 8) + 8 (lane / 32) + r % 8, eight consecutive ones per operand of the next product
 __device__ __forceinline__ int sigma(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 
-// A tile of rows of D bf16 in LDS, filled by 1 KB wave-wide copies and read in two ways: `frag` reads 16 B of a lane's own
-// row (rows of 2 D bytes, 16 B chunks XOR-swizzled so that 16 rows lie on distinct banks); `frag_t` reads columns by two
-// transposing reads of four rows each, for which the four rows of each group of 16 lanes must lie on distinct banks.
-// The two want different swizzles; BOTH is a swizzle that serves both.
+// A tile of rows of D bf16 in LDS, filled by 1 KB wave-wide copies. It is read in two ways: 16 B of each lane's own row
+// (16 lanes on 16 consecutive rows must lie on distinct banks), and by columns, with transposing reads of four rows for
+// each group of 16 lanes (the four rows of two neighbouring groups must). The 16 B chunks of a row are XOR-swizzled by
+// swz for the first, swt for the second and swb for both.
 template <int D>
 struct Tile {
     static constexpr int RB = 2 * D;             // bytes per row
     static constexpr int CPR = D / 8;            // 16 B chunks per row
     static constexpr int RPC = 1024 / RB;        // rows per copy
-    // slot of chunk c in row r: rows read whole (swz) and by columns (swt)
     __device__ static int swz(int r, int c) { return D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
     __device__ static int swt(int r, int c) { return D == 64 ? c ^ (2 * (r & 3)) : c ^ (4 * (r & 3)); }
+    // bits 2 (and 3) from the row's lowest differing bits, as swt; the others from the next two, so that 16 rows differ
+    __device__ static int swb(int r, int c) {
+        return D == 64 ? c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3)) : c ^ (((r & 3) << 2) | ((r >> 2) & 3));
+    }
 };
 
 int check_heads(const char *fn, const char *name, const noise_heads_t *h, Rows *out) {

@@ -258,50 +258,6 @@ int launch_units(void (*kernel)(SinkArgs), SinkArgs &a, int64_t units, hipStream
 
 using namespace noise;
 
-extern "C" int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads,
-                                                            int64_t kv_heads, int64_t head_dim, int64_t window,
-                                                            int64_t sinks) {
-    clear_error();
-    const int st = check_sizes("noise_sink_attention_bwd_workspace_bytes", batch, tokens, tokens, heads, kv_heads,
-                               head_dim, window, sinks);
-    if (st) return st;
-    return batch * tokens * heads * 4;
-}
-
-extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                                        const noise_heads_t *o, const noise_heads_t *d_o, const float *lse,
-                                        const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
-                                        const void *lengths, int lengths_wide, int64_t batch, int64_t tokens,
-                                        int64_t head_dim, int64_t window, int64_t sinks, float scale, void *workspace,
-                                        int64_t workspace_bytes, noise_stream_t stream) {
-    clear_error();
-    const char *fn = "noise_sink_attention_bwd";
-    NOISE_CHECK_ARG(q && k && v && o && d_o && dq && dk && dv && q->heads == o->heads && q->heads == d_o->heads &&
-                        q->heads == dq->heads && k->heads == v->heads && k->heads == dk->heads && k->heads == dv->heads,
-                    "%s: tensors missing or of other heads", fn);
-    int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
-    if (st) return st;
-    if (batch == 0 || tokens == 0) return NOISE_OK;
-    NOISE_CHECK_ARG(lse && aligned(lse, 4), "%s: lse is required", fn);
-    const int64_t need = noise_sink_attention_bwd_workspace_bytes(batch, tokens, q->heads, k->heads, head_dim, window, sinks);
-    NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= need,
-                    "%s: workspace NULL, misaligned or below %lld bytes", fn, (long long)need);
-    SinkArgs a;
-    if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||
-        (st = check_heads(fn, "v", v, &a.v)) || (st = check_heads(fn, "o", o, &a.o)) ||
-        (st = check_heads(fn, "d_o", d_o, &a.d_o)) || (st = check_heads(fn, "dq", dq, &a.dq)) ||
-        (st = check_heads(fn, "dk", dk, &a.dk)) || (st = check_heads(fn, "dv", dv, &a.dv)))
-        return st;
-    fill_args(&a, lengths, nullptr, lengths_wide, tokens, tokens, q->heads, k->heads, window, sinks, scale);
-    a.lse = const_cast<float *>(lse);
-    a.delta = static_cast<float *>(workspace);
-    st = launch_units(head_dim == 64 ? sink_dq_kernel<64> : sink_dq_kernel<128>, a, batch * q->heads * tokens,
-                      (hipStream_t)stream, fn);
-    if (st) return st;
-    return launch_units(head_dim == 64 ? sink_dkv_kernel<64> : sink_dkv_kernel<128>, a, batch * k->heads * tokens,
-                        (hipStream_t)stream, fn);
-}
-
 extern "C" int64_t noise_sink_decode_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                      int64_t capacity, int64_t head_dim, int64_t window,
                                                      int64_t sinks) {
