@@ -25,17 +25,6 @@ __device__ __forceinline__ int64_t at_wide(const void *p, int wide, int64_t i) {
     return wide ? static_cast<const int64_t *>(p)[i] : (int64_t)static_cast<const int32_t *>(p)[i];
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
 // bits 2 and 3 of a row index swapped: with a block's rows read in this order, register r of a lane's 32 x 32 result
 // stands for row 16 (r / 8) + 8 (lane / 32) + r % 8, eight consecutive ones per operand of the next product
 __device__ __forceinline__ int sigma(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }

@@ -79,6 +79,10 @@ def test_huge_positions_and_masks():
     start = torch.tensor([2 ** 62, -2 ** 62, 2 ** 31, 99], device=DEV)
     for window, sinks in ((2 ** 40, 2 ** 40), (3, 2 ** 40), (2 ** 40, 1), (3, 0)):
         check_decode(q, k, v, start, window, sinks)
+    far = torch.tensor([2 ** 63 - 1, -2 ** 63, 2 ** 63 - 2, 99], device=DEV)
+    assert (check_decode(q, k, v, far.clamp(-1000, 1000), 3, 5) == check_decode(q, k, v, start, 3, 5))[[0, 3]].all()
+    from noise_amd.sinks import sink_attention_decode
+    assert torch.equal(sink_attention_decode(q, k, v, far, 3, 5), sink_attention_decode(q, k, v, start, 3, 5))
 
 
 def test_strided_caches():
