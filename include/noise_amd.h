@@ -689,7 +689,7 @@ int noise_sink_decode(const noise_heads_t *q, const noise_heads_t *k, const nois
                       int64_t workspace_bytes, noise_stream_t stream);
 
 /* Distillation from a teacher's top logits: for each of `rows` rows of logits x (type `type`, `vocab` of `stride` elements)
- * and the teacher's `entries` logits t (type `teacher_type`) at indices i (int32, or int64 with index_wide), both [rows]
+ * and the teacher's `entries` (1 .. 1024) logits t (type `teacher_type`) at indices i (int32, or int64 with index_wide), both [rows]
  * [entries] contiguous,
  *   z = cap(x) / temperature,  cap(x) = softcap tanh(x / softcap) (softcap 0: x),  p = softmax(t / temperature),
  *   loss = temperature^2 sum_k p_k (log p_k - log softmax(z)[i_k]),

@@ -11,6 +11,8 @@ import torch
 from . import _lib
 from .sinks import F32, TYPES, _call
 
+MAX_ENTRIES = 1024
+
 
 def _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, softcap):
     if logits.dtype not in TYPES or logits.dim() < 1:
@@ -26,6 +28,8 @@ def _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, sof
     if teacher_logits.shape != teacher_index.shape or teacher_logits.shape[:-1] != shape or teacher_logits.shape[-1] == 0:
         raise ValueError(f'{fn}: teacher logits and indices must be [{", ".join(map(str, shape))}, entries], got '
                          f'{tuple(teacher_logits.shape)} and {tuple(teacher_index.shape)}')
+    if teacher_index.shape[-1] > MAX_ENTRIES:
+        raise ValueError(f'{fn}: at most {MAX_ENTRIES} teacher entries per token, got {teacher_index.shape[-1]}')
     if teacher_index.dtype not in (torch.int32, torch.int64):
         raise ValueError(f'{fn}: teacher indices must be int32 or int64, got {teacher_index.dtype}')
     if teacher_logits.dtype not in TYPES:
@@ -79,7 +83,7 @@ def distill_loss(logits, teacher_logits, teacher_index, vocab=None, temperature=
         loss = temperature^2 * sum_k p_k (log p_k - log softmax(z)[index_k])
 
     with p over the entries in use: an index outside 0 .. vocab - 1 or a teacher logit of -inf leaves its entry out, and a
-    token without entries has loss and gradient 0. The same index may stand in several entries. Statistics and sums are in
+    token without entries has loss and gradient 0; at most 1024 entries. The same index may stand in several entries. Statistics and sums are in
     fp32. Differentiable in the logits (once); the teacher has no gradient."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, teacher_logits, teacher_index, vocab, float(temperature), softcap)

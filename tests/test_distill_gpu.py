@@ -54,7 +54,7 @@ def check_all(x, t, i, w, vocab, tau, cap):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize('V', [1, 2, 7, 63, 64, 65, 257, 1000, 2049, 4096, 4097, 8191, 16384, 20011, 65536, 100001])
+@pytest.mark.parametrize('V', [1, 2, 7, 63, 64, 65, 257, 1000, 2049, 4096, 4097, 8191, 16384, 20011, 65536, 100001, 200003, 250000])
 def test_vocabularies(V, dtype):
     for W, K, tau, cap in ((V, min(V, 5), 1.0, None), (V + 1, min(V, 64), 2.0, 15.0), (V + 47, 1, 0.7, None)):
         print(V, W, K, tau, cap, dtype, flush=True)

@@ -72,7 +72,7 @@ def test_distill_refusals():
     x, t, i = torch.zeros(3, 10), torch.zeros(3, 4), torch.zeros(3, 4, dtype=torch.int64)
     for args, more, words in (((x.half(), t, i), {}, 'bfloat16 or float32'), ((x, t[:2], i), {}, 'entries'),
                               ((x, t, i[:, :3]), {}, 'entries'), ((x, t[:, :0], i[:, :0]), {}, 'entries'),
-                              ((x, t, i.float()), {}, 'int32 or int64'), ((x, t.double(), i), {}, 'teacher logits'),
+                              ((x, t.repeat(1, 257), i.repeat(1, 257)), {}, 'at most 1024'), ((x, t, i.float()), {}, 'int32 or int64'), ((x, t.double(), i), {}, 'teacher logits'),
                               ((x, t, i), dict(vocab=11), 'vocab'), ((x, t, i), dict(vocab=0), 'vocab'),
                               ((x, t, i), dict(temperature=0.0), 'temperature'),
                               ((x, t, i), dict(temperature=math.nan), 'temperature'),
@@ -132,7 +132,7 @@ def test_entry_points_refuse():
     refused(nb(None, 0), 'workspace')
     dist = lambda rows=2, vocab=9, K=3, tau=1.0, cap=0.0, grad=16, width=9, gs=9, x=16: lib.noise_distill(
         x, 1, rows, vocab, 9, 16, 1, 16, 1, K, None, tau, cap, 16, grad, width, gs, None)
-    for st in (dist(vocab=0), dist(K=0), dist(tau=0.0), dist(cap=-1.0), dist(width=8), dist(gs=8), dist(x=2), dist(x=None)):
+    for st in (dist(vocab=0), dist(K=0), dist(K=1025), dist(tau=0.0), dist(cap=-1.0), dist(width=8), dist(gs=8), dist(x=2), dist(x=None)):
         assert st == -1
     assert dist(rows=0) == 0
 
