@@ -36,10 +36,10 @@ def _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, sof
         raise ValueError(f'{fn}: bfloat16 or float32 teacher logits, got {teacher_logits.dtype}')
     if teacher_logits.device != logits.device or teacher_index.device != logits.device:
         raise ValueError(f'{fn}: tensors on {logits.device}, {teacher_logits.device} and {teacher_index.device}')
-    x = logits.reshape(-1, width)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, width)
     if x.stride(1) != 1 and width > 1 or x.stride(0) < 0:
         x = x.contiguous()
-    return x, teacher_logits.contiguous(), teacher_index.contiguous(), vocab
+    return x, *(t if t.is_contiguous() else t.contiguous() for t in (teacher_logits, teacher_index)), vocab
 
 
 def distill(fn, logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap, with_grad):
@@ -50,9 +50,10 @@ def distill(fn, logits, teacher_logits, teacher_index, weight, vocab, temperatur
         if weight.shape != logits.shape[:-1] or weight.device != logits.device:
             raise ValueError(f'{fn}: weights must be {tuple(logits.shape[:-1])} on {logits.device}, got '
                              f'{tuple(weight.shape)} on {weight.device}')
-        weight = weight.detach().to(F32).contiguous()
-    loss = torch.empty(logits.shape[:-1], dtype=F32, device=x.device)
-    grad = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if with_grad else None
+        if weight.dtype != F32 or not weight.is_contiguous():
+            weight = weight.to(F32).contiguous()
+    loss = x.new_empty(logits.shape[:-1], dtype=F32)
+    grad = x.new_empty(logits.shape) if with_grad else None
     if rows:
         _call('noise_distill', x.device, x.data_ptr(), TYPES[x.dtype], rows, vocab, x.stride(0), t.data_ptr(),
               TYPES[t.dtype], i.data_ptr(), int(i.dtype == torch.int64), t.shape[-1], _lib.ptr(weight),
@@ -90,7 +91,6 @@ def distill_loss(logits, teacher_logits, teacher_index, vocab=None, temperature=
     return distill('distill_loss', logits, teacher_logits, teacher_index, None, vocab, temperature, softcap, False)[0]
 
 
-@torch.no_grad()
 def distill_loss_grad(logits, teacher_logits, teacher_index, weight=None, vocab=None, temperature=1.0, softcap=None):
     """(losses, gradient) of distill_loss in one pass over the logits, for a training step that knows its weights before
     the loss: the gradient, of the logits' shape and type, is that of sum(weight * loss), weight [...] (None: ones).

@@ -11,12 +11,11 @@ keys' (query head h reads key head h // (H // Hk)). The norm and rotation are th
 with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators for compiled callers.
 """
 import ctypes
-import math
+import functools
 
 import torch
 
 from . import _lib
-from ._lib import Heads
 
 BF16, F32 = torch.bfloat16, torch.float32
 EPS = torch.finfo(F32).eps   # utils/model.py:46-47 under fp32 statistics
@@ -35,13 +34,15 @@ def _check(fn, q, k, *others):
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError(f'{fn}: {q.shape[2]} query heads are no multiple of {k.shape[2]} key heads')
     for t in (k, *others):
-        if t is not None and (t.device != q.device):
+        if t.device != q.device:
             raise ValueError(f'{fn}: tensors on {q.device} and {t.device}')
 
 
 def _rows(t):
     """t with unit inner stride and rows of whole 16 B at 16 B addresses, less than 2^25 elements from token to token (copied
     if it has not)."""
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return t
     s, unit = t.stride(), 16 // t.element_size()
     if s[3] != 1 or (s[0] | s[1] | s[2]) % unit or s[1] >= 1 << 25 or t.data_ptr() % 16:
         t = t.contiguous()
@@ -50,21 +51,35 @@ def _rows(t):
     return t
 
 
-def _heads(t):
-    s = t.stride()
-    return Heads(t.data_ptr(), s[0], s[1], s[2], t.shape[2])
+def _cache_rows(fn, c):
+    a, b, s, unit = c.stride()
+    if unit != 1 or (a | b | s) % (16 // c.element_size()) or c.data_ptr() % 16:
+        raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
 
 
-def _ref(t):
-    return None if t is None else ctypes.byref(_heads(t))
+_ARRAYS = [ctypes.c_int64 * (5 * n) for n in range(10)]
+_HEADS = 5 * 8   # bytes of a noise_heads_t: five 64-bit numbers
+
+
+def _table(*tensors):
+    """noise_heads_t of each tensor, in a row: byref(table, i * _HEADS) is that of the i-th"""
+    flat = []
+    for t in tensors:
+        a, b, c, _ = t.stride()
+        flat += t.data_ptr(), a, b, c, t.shape[2]
+    return _ARRAYS[len(tensors)](*flat)
+
+
+_PAIR = ctypes.c_void_p * 2
 
 
 def _call(name, device, *args):
     """The entry point on `device`'s current stream (made the current device for the launch)."""
-    if device.type != 'cuda':
+    index = device.index
+    if index is None:
         raise ValueError(f'{name}: tensors must be on a GPU, got {device}')
-    if torch.cuda.current_device() == device.index:
-        return _lib.call(name, *args, _lib.stream_ptr(device))
+    if torch._C._cuda_getDevice() == index:
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
         return _lib.call(name, *args, _lib.stream_ptr(device))
 
@@ -74,7 +89,7 @@ def _ints(fn, name, t, batch, device):
     if t.dtype not in (torch.int32, torch.int64) or t.shape != (batch,) or t.device != device:
         raise ValueError(f'{fn}: {name} must be int32 or int64 of shape [{batch}] on {device}, got {t.dtype} '
                          f'{tuple(t.shape)} on {t.device}')
-    return t.contiguous(), int(t.dtype == torch.int64)
+    return t if t.is_contiguous() else t.contiguous(), int(t.dtype == torch.int64)
 
 
 # --- norm and rotation ---
@@ -83,13 +98,16 @@ def _ints(fn, name, t, batch, device):
 def _tables(fn, cos, sin, D, device):
     if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D // 2 or cos.shape[0] == 0:
         raise ValueError(f'{fn}: cos and sin must be [positions, {D // 2}], got {tuple(cos.shape)} and {tuple(sin.shape)}')
-    out = []
-    for t in (cos, sin):
-        if t.device != device:
-            raise ValueError(f'{fn}: rotation tables on {t.device}, tensors on {device}')
+    if cos.device != device or sin.device != device:
+        raise ValueError(f'{fn}: rotation tables on {cos.device} and {sin.device}, tensors on {device}')
+    return _plain(cos), _plain(sin)
+
+
+def _plain(t):
+    """t in fp32, contiguous, at a 16 B address"""
+    if t.dtype != F32 or not t.is_contiguous():
         t = t.to(F32).contiguous()
-        out.append(t.clone() if t.data_ptr() % 16 else t)
-    return out
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _weight(fn, w, D, device):
@@ -97,11 +115,11 @@ def _weight(fn, w, D, device):
         return None
     if w.shape != (D,) or w.device != device:
         raise ValueError(f'{fn}: weights must be [{D}] on {device}, got {tuple(w.shape)} on {w.device}')
-    w = w.detach().to(F32).contiguous()
-    return w.clone() if w.data_ptr() % 16 else w
+    return _plain(w.detach())
 
 
 def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
+    """(cos, sin, q_weight, k_weight, start, start is int64) as the kernels take them"""
     _check(fn, q, k)
     if q.shape[1] != k.shape[1] or q.dtype != k.dtype:
         raise ValueError(f'{fn}: q and k must have one length and type, got {tuple(q.shape)} {q.dtype} and '
@@ -110,60 +128,81 @@ def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
         raise ValueError(f'{fn}: bfloat16 or float32 tensors, got {q.dtype}')
     B, T, _, D = q.shape
     cos, sin = _tables(fn, cos, sin, D, q.device)
+    wide = 0
     if start is not None:
         start, wide = _ints(fn, 'start', start, B, q.device)
-    else:
-        wide = 0
-        if T > cos.shape[0]:
-            raise ValueError(f'{fn}: {T} tokens but rotation tables of {cos.shape[0]} positions')
+    elif T > cos.shape[0]:
+        raise ValueError(f'{fn}: {T} tokens but rotation tables of {cos.shape[0]} positions')
     return cos, sin, _weight(fn, q_weight, D, q.device), _weight(fn, k_weight, D, q.device), start, wide
 
 
+def _norm_forward(q, k, cos, sin, qw, kw, start, wide, eps):
+    """qk_norm_rotary of checked operands"""
+    B, T, _, D = q.shape
+    out = q.new_empty(q.shape), k.new_empty(k.shape)
+    x = _rows(q), _rows(k)   # (copies among them live until the launch)
+    t = _table(*x, *out)
+    _call('noise_qk_norm_rotary', q.device, t, ctypes.byref(t, 2 * _HEADS), _PAIR(_lib.ptr(qw), _lib.ptr(kw)), None, None,
+          cos.data_ptr(), sin.data_ptr(), cos.shape[0], _lib.ptr(start), wide, B, T, 0, D, TYPES[q.dtype], eps)
+    return out
+
+
+@functools.lru_cache(maxsize=None)
+def _norm_workspace(D):
+    return _lib.lib().noise_qk_norm_rotary_bwd_workspace_bytes(D)
+
+
+def _norm_backward(dq, dk, q, k, cos, sin, qw, kw, start, wide, eps):
+    """Gradients of q, k and (fp32; None for absent ones) of the weights, of checked operands"""
+    B, T, _, D = q.shape
+    dt = q.dtype
+    dx = q.new_empty(q.shape), k.new_empty(k.shape)
+    x = _rows(q), _rows(k), _rows(dq if dq.dtype == dt else dq.to(dt)), _rows(dk if dk.dtype == dt else dk.to(dt))
+    t = _table(*x, *dx)
+    need, work, dqw, dkw = 0, None, None, None
+    if qw is not None or kw is not None:
+        need = _norm_workspace(D)
+        work = q.new_empty(need, dtype=torch.uint8)
+        dqw = None if qw is None else qw.new_empty(D)
+        dkw = None if kw is None else kw.new_empty(D)
+    _call('noise_qk_norm_rotary_bwd', q.device, t, ctypes.byref(t, 2 * _HEADS), ctypes.byref(t, 4 * _HEADS),
+          _PAIR(_lib.ptr(qw), _lib.ptr(kw)), _PAIR(_lib.ptr(dqw), _lib.ptr(dkw)), cos.data_ptr(), sin.data_ptr(),
+          cos.shape[0], _lib.ptr(start), wide, B, T, D, TYPES[dt], eps, _lib.ptr(work), need)
+    return dx[0], dx[1], dqw, dkw
+
+
+def _as(grad, like):
+    return grad if grad is None or grad.dtype == like.dtype else grad.to(like.dtype)
+
+
 def norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps):
-    fn = 'qk_norm_rotary'
-    cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
-    B, T, H, D = q.shape
-    x = [_rows(q), _rows(k)]
-    y = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
-    _call('noise_qk_norm_rotary', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(*map(_heads, y)),
-          (ctypes.c_void_p * 2)(_lib.ptr(qw), _lib.ptr(kw)), None, None, cos.data_ptr(), sin.data_ptr(),
-          cos.shape[0], _lib.ptr(start), wide, B, T, 0, D, TYPES[q.dtype], eps)
-    return y[0], y[1]
+    return _norm_forward(q, k, *_norm_operands('qk_norm_rotary', q, k, cos, sin, q_weight, k_weight, start), eps)
 
 
 def norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, eps):
     """Gradients of q, k and (in their types; None for absent ones) of the weights."""
-    fn = 'qk_norm_rotary'
-    cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
-    B, T, H, D = q.shape
-    x = [_rows(q), _rows(k)]
-    dy = [_rows(dq.to(q.dtype)), _rows(dk.to(q.dtype))]
-    dx = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
-    dw = [None if w is None else torch.empty(D, dtype=F32, device=q.device) for w in (qw, kw)]
-    need, work = 0, None
-    if qw is not None or kw is not None:
-        need = _lib.lib().noise_qk_norm_rotary_bwd_workspace_bytes(D)
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    vp = ctypes.c_void_p * 2
-    _call('noise_qk_norm_rotary_bwd', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(*map(_heads, dy)),
-          (Heads * 2)(*map(_heads, dx)), vp(_lib.ptr(qw), _lib.ptr(kw)), vp(*map(_lib.ptr, dw)), cos.data_ptr(),
-          sin.data_ptr(), cos.shape[0], _lib.ptr(start), wide, B, T, D, TYPES[q.dtype], eps, _lib.ptr(work), need)
-    return (dx[0], dx[1], *(None if g is None else g.to(w.dtype) for g, w in zip(dw, (q_weight, k_weight))))
+    operands = _norm_operands('qk_norm_rotary', q, k, cos, sin, q_weight, k_weight, start)
+    dq, dk, dqw, dkw = _norm_backward(dq, dk, q, k, *operands, eps)
+    return dq, dk, _as(dqw, q_weight), _as(dkw, k_weight)
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, cos, sin, q_weight, k_weight, start, eps):
-        ctx.save_for_backward(q, k, cos, sin, q_weight, k_weight, start)
-        ctx.eps = eps
-        return norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps)
+        cos, sin, qw, kw, start, wide = _norm_operands('qk_norm_rotary', q, k, cos, sin, q_weight, k_weight, start)
+        # (what the kernels take is saved: the tensors themselves, or the fp32 copies made of them)
+        ctx.save_for_backward(q, k, cos, sin, qw, kw, start)
+        ctx.more = wide, eps
+        ctx.types = tuple(None if w is None else w.dtype for w in (q_weight, k_weight))
+        return _norm_forward(q, k, cos, sin, qw, kw, start, wide, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        q, k, cos, sin, q_weight, k_weight, start = ctx.saved_tensors
-        dq, dk, dqw, dkw = norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, ctx.eps)
-        return dq, dk, None, None, dqw, dkw, None, None
+        dq, dk, dqw, dkw = _norm_backward(dq, dk, *ctx.saved_tensors, *ctx.more)
+        a, b = ctx.types
+        return (dq, dk, None, None, dqw if a is None or a == F32 else dqw.to(a),
+                dkw if b is None or b == F32 else dkw.to(b), None, None)
 
 
 def qk_norm_rotary(q, k, cos, sin, q_weight=None, k_weight=None, start=None, eps=EPS):
@@ -178,7 +217,6 @@ def qk_norm_rotary(q, k, cos, sin, q_weight=None, k_weight=None, start=None, eps
     return norm_forward(q, k, cos, sin, q_weight, k_weight, start, float(eps))
 
 
-@torch.no_grad()
 def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=None, k_weight=None, eps=EPS):
     """q' of qk_norm_rotary for new tokens at positions start[b] + t, with k' and v [B, T, Hk, D] written to those slots of
     k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
@@ -196,14 +234,13 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
         if c.shape != (B, S, k.shape[2], D) or c.dtype != k.dtype or c.device != k.device or S == 0:
             raise ValueError(f'{fn}: caches must be [{B}, capacity, {k.shape[2]}, {D}] {k.dtype} on {k.device}, got '
                              f'{tuple(c.shape)} {c.dtype} on {c.device}')
-        unit = 16 // c.element_size()
-        if c.stride(3) != 1 or any(s % unit for s in c.stride()[:3]) or c.data_ptr() % 16:
-            raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
-    x, v = [_rows(q), _rows(k)], _rows(v)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _call('noise_qk_norm_rotary', q.device, (Heads * 2)(*map(_heads, x)), (Heads * 2)(_heads(out), _heads(k_cache)),
-          (ctypes.c_void_p * 2)(_lib.ptr(qw), _lib.ptr(kw)), _ref(v), _ref(v_cache), cos.data_ptr(),
-          sin.data_ptr(), cos.shape[0], start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
+        _cache_rows(fn, c)
+    out = q.new_empty(q.shape)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    t = _table(q, k, out, k_cache, v, v_cache)
+    _call('noise_qk_norm_rotary', q.device, t, ctypes.byref(t, 2 * _HEADS), _PAIR(_lib.ptr(qw), _lib.ptr(kw)),
+          ctypes.byref(t, 4 * _HEADS), ctypes.byref(t, 5 * _HEADS), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+          start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
     return out
 
 
@@ -222,46 +259,66 @@ def _attend_operands(fn, q, k, v, window, sinks, lengths):
     return (None, 0) if lengths is None else _ints(fn, 'lengths', lengths, q.shape[0], q.device)
 
 
-def attend_forward(q, k, v, window, sinks, lengths, with_lse):
-    """(out, lse or None)"""
-    fn = 'sink_attention'
-    lengths, wide = _attend_operands(fn, q, k, v, window, sinks, lengths)
+def _attend_forward(q, k, v, window, sinks, lengths, wide, with_lse):
+    """(out, lse or None) of checked operands"""
     B, T, H, D = q.shape
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((B, H, T), dtype=F32) if with_lse else None
     q, k, v = _rows(q), _rows(k), _rows(v)
-    out = torch.empty(B, T, H, D, dtype=BF16, device=q.device)
-    lse = torch.empty(B, H, T, dtype=F32, device=q.device) if with_lse else None
-    _call('noise_sink_attention_fwd', q.device, _ref(q), _ref(k), _ref(v), _ref(out), _lib.ptr(lse),
-          _lib.ptr(lengths), wide, B, T, D, window, sinks, 1.0 / math.sqrt(D))
+    t = _table(q, k, v, out)
+    _call('noise_sink_attention_fwd', q.device, t, *_parts(t, 1, 4), _lib.ptr(lse), _lib.ptr(lengths), wide, B, T, D, window,
+          sinks, D ** -0.5)
     return out, lse
 
 
-def attend_backward(dout, q, k, v, out, lse, window, sinks, lengths):
-    fn = 'sink_attention'
-    lengths, wide = _attend_operands(fn, q, k, v, window, sinks, lengths)
+def _parts(table, first, end):
+    return [ctypes.byref(table, i * _HEADS) for i in range(first, end)]
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(*sizes):
+    return _lib.lib().noise_sink_attention_bwd_workspace_bytes(*sizes)
+
+
+def _attend_backward(dout, q, k, v, out, lse, window, sinks, lengths, wide):
     B, T, H, D = q.shape
-    grads = [torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v)]
-    q, k, v, out, dout = map(_rows, (q, k, v, out, dout.to(BF16)))
-    need = _lib.lib().noise_sink_attention_bwd_workspace_bytes(B, T, H, k.shape[2], D, window, sinks)
-    work = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
-    _call('noise_sink_attention_bwd', q.device, _ref(q), _ref(k), _ref(v), _ref(out), _ref(dout),
-          lse.data_ptr(), *map(_ref, grads), _lib.ptr(lengths), wide, B, T, D, window, sinks, 1.0 / math.sqrt(D),
-          work.data_ptr(), need)
+    grads = [x.new_empty(x.shape) for x in (q, k, v)]
+    x = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout if dout.dtype == BF16 else dout.to(BF16))
+    t = _table(*x, *grads)
+    need = _attend_workspace(B, T, H, k.shape[2], D, window, sinks)
+    work = q.new_empty(max(need, 0), dtype=torch.uint8)
+    refs = _parts(t, 0, 8)
+    _call('noise_sink_attention_bwd', q.device, *refs[:5], lse.data_ptr(), *refs[5:], _lib.ptr(lengths), wide, B, T, D, window,
+          sinks, D ** -0.5, work.data_ptr(), need)
     return grads
+
+
+def attend_forward(q, k, v, window, sinks, lengths, with_lse):
+    """(out, lse or None)"""
+    return _attend_forward(q, k, v, window, sinks, *_attend_operands('sink_attention', q, k, v, window, sinks, lengths),
+                           with_lse)
+
+
+def attend_backward(dout, q, k, v, out, lse, window, sinks, lengths):
+    operands = _attend_operands('sink_attention', q, k, v, window, sinks, lengths)
+    return _attend_backward(dout, q, k, v, out, lse, window, sinks, *operands)
 
 
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, lengths):
-        out, lse = attend_forward(q, k, v, window, sinks, lengths, True)
+        lengths, wide = _attend_operands('sink_attention', q, k, v, window, sinks, lengths)
+        out, lse = _attend_forward(q, k, v, window, sinks, lengths, wide, True)
         ctx.save_for_backward(q, k, v, out, lse, lengths)
-        ctx.mask = (window, sinks)
+        ctx.more = window, sinks, wide
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lengths = ctx.saved_tensors
-        return (*attend_backward(dout, q, k, v, out, lse, *ctx.mask, lengths), None, None, None)
+        window, sinks, wide = ctx.more
+        return (*_attend_backward(dout, q, k, v, out, lse, window, sinks, lengths, wide), None, None, None)
 
 
 def sink_attention(q, k, v, window, sinks=0, lengths=None):
@@ -276,7 +333,11 @@ def sink_attention(q, k, v, window, sinks=0, lengths=None):
     return attend_forward(q, k, v, window, sinks, lengths, False)[0]
 
 
-@torch.no_grad()
+@functools.lru_cache(maxsize=1024)
+def _decode_workspace(*sizes):
+    return _lib.lib().noise_sink_decode_workspace_bytes(*sizes)
+
+
 def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     """sink_attention of T new tokens (1 to 16) against a cache: q [B, T, H, D], k_cache and v_cache [B, capacity, Hk, D]
     in bfloat16, whose slots hold the positions 0, 1, ...; token t of sequence b stands at position start[b] + t (its own
@@ -298,13 +359,13 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
         raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
     start, wide = _ints(fn, 'start', start, B, q.device)
     for c in (k_cache, v_cache):
-        if c.stride(3) != 1 or any(s % 8 for s in c.stride()[:3]) or c.data_ptr() % 16:
-            raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
-    q = _rows(q)
-    out = torch.empty(B, T, H, D, dtype=BF16, device=q.device)
+        _cache_rows(fn, c)
+    out = q.new_empty(q.shape)
     S, Hk = k_cache.shape[1:3]
-    need = _lib.lib().noise_sink_decode_workspace_bytes(B, T, H, Hk, S, D, window, sinks)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-    _call('noise_sink_decode', q.device, _ref(q), _ref(k_cache), _ref(v_cache), _ref(out), start.data_ptr(),
-          wide, B, T, S, D, window, sinks, 1.0 / math.sqrt(D), _lib.ptr(work), need)
+    need = _decode_workspace(B, T, H, Hk, S, D, window, sinks)
+    work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    q = _rows(q)
+    t = _table(q, k_cache, v_cache, out)
+    _call('noise_sink_decode', q.device, t, *_parts(t, 1, 4), start.data_ptr(), wide, B, T, S, D, window, sinks, D ** -0.5,
+          _lib.ptr(work), need)
     return out
