@@ -209,22 +209,25 @@ __global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(NormArgs a) {
     }
 }
 
-// dw[i] = the sum of its partial rows; one workgroup per tensor
-template <int D>
-__global__ __launch_bounds__(1024) void head_norm_dw_kernel(const float *partial, float *dw0, float *dw1, int blocks) {
-    float *out = blockIdx.x ? dw1 : dw0;
+// dw[i] = the sum of its partial rows: a workgroup per 16 columns, 64 rows at a time
+__global__ __launch_bounds__(1024) void head_norm_dw_kernel(const float *partial, float *dw0, float *dw1, int blocks, int D) {
+    float *out = blockIdx.y ? dw1 : dw0;
     if (!out) return;
-    constexpr int G = 1024 / D;
-    __shared__ float sum[G][D];
-    const int col = threadIdx.x % D, g = threadIdx.x / D;
-    const float *p = partial + (int64_t)blockIdx.x * kPartials * D + col;
+    __shared__ float sum[16][16];
+    const int col = threadIdx.x & 15, wave = threadIdx.x >> 6;
+    const float *p = partial + (int64_t)blockIdx.y * kPartials * D + 16 * blockIdx.x + col;
     float s = 0.f;
-    for (int k = g; k < blocks; k += G) s += p[(int64_t)k * D];
-    sum[g][col] = s;
+#pragma unroll 8
+    for (int k = threadIdx.x >> 4; k < blocks; k += 64) s += p[(int64_t)k * D];
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if ((threadIdx.x & 63) < 16) sum[wave][col] = s;
     __syncthreads();
-    if (g == 0) {
-        for (int k = 1; k < G; ++k) s += sum[k][col];
-        out[col] = s;
+    if (threadIdx.x < 16) {
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) s += sum[w][col];
+        out[16 * blockIdx.x + col] = s;
     }
 }
 
@@ -347,7 +350,7 @@ extern "C" int noise_qk_norm_rotary_bwd(const noise_heads_t x[2], const noise_he
         hipLaunchKernelGGL(kernel, dim3((unsigned)a.blocks, 2), dim3(kThreads), 0, (hipStream_t)stream, a);
     }
     if (weights)
-        hipLaunchKernelGGL(head_dim == 64 ? head_norm_dw_kernel<64> : head_norm_dw_kernel<128>, dim3(2), dim3(1024), 0,
-                           (hipStream_t)stream, a.partial, w[0] ? dw[0] : nullptr, w[1] ? dw[1] : nullptr, a.blocks);
+        hipLaunchKernelGGL(head_norm_dw_kernel, dim3((unsigned)(head_dim / 16), 2), dim3(1024), 0, (hipStream_t)stream,
+                           a.partial, w[0] ? dw[0] : nullptr, w[1] ? dw[1] : nullptr, a.blocks, (int)head_dim);
     return launch_status(fn);
 }

@@ -14,7 +14,7 @@ namespace noise {
 namespace {
 
 constexpr int kTileRows = 64;  // rows of the tiles that walk by
-constexpr int kOwn = 128;      // queries (dq) or keys (dk, dv) of a workgroup
+constexpr int kOwnQ = 128;     // queries of a workgroup (dq)
 
 struct BwdArgs {
     Rows q, k, v, o, d_o, dq, dk, dv;
@@ -130,10 +130,10 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
     const int b = row / a.heads, h = row - b * a.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
-    const int len = seq_len(a, b), last = len - 1, q_lo = qt * kOwn, q0w = q_lo + 32 * wave;
+    const int len = seq_len(a, b), last = len - 1, q_lo = qt * kOwnQ, q0w = q_lo + 32 * wave;
     __bf16 *dqb = a.dq.ptr + b * a.dq.s_b + h * a.dq.s_h;
     if (q_lo > last) {
-        const int n = (a.tokens - q_lo < kOwn ? a.tokens - q_lo : kOwn) * TL::CPR;
+        const int n = (a.tokens - q_lo < kOwnQ ? a.tokens - q_lo : kOwnQ) * TL::CPR;
         for (int c = tid; c < n; c += 256)
             store_bf16x8(dqb + (int64_t)(q_lo + c / TL::CPR) * a.dq.s_t + 8 * (c % TL::CPR), zero_bf16x8());
         return;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
     }
     vm_wait<0>();
     const int W = a.window, n_sinks = a.sinks;
-    const int q_hi = q_lo + kOwn - 1 < last ? q_lo + kOwn - 1 : last;
+    const int q_hi = q_lo + kOwnQ - 1 < last ? q_lo + kOwnQ - 1 : last;
     const int band = (q_lo > W ? q_lo - W : 0) / kTileRows;
     const int sunk = (n_sinks + kTileRows - 1) / kTileRows < band ? (n_sinks + kTileRows - 1) / kTileRows : band;
     const int nt = sunk + q_hi / kTileRows - band + 1;
@@ -232,20 +232,21 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
 }
 
 // query tiles of key tile kt: first, and how many (of one query head)
-__device__ __forceinline__ int query_tiles(const BwdArgs &a, int kt, int len, int *first) {
-    const int k_lo = kt * kOwn, last = len - 1;
+__device__ __forceinline__ int query_tiles(const BwdArgs &a, int kt, int own, int len, int *first) {
+    const int k_lo = kt * own, last = len - 1;
     *first = k_lo / kTileRows;
     if (k_lo > last) return 0;
-    const int k_hi = k_lo + kOwn - 1 + a.window;
+    const int k_hi = k_lo + own - 1 + a.window;
     const int end = k_lo < a.sinks || k_hi > last ? last : k_hi;
     return end / kTileRows - *first + 1;
 }
 
-template <int D>
+// KW: waves along the keys; with 2, two waves share each 32 keys, one for either half of the query tiles, and add up in LDS
+template <int D, int KW>
 __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     using TL = Tile<D>;
     using CP = Copies<D>;
-    constexpr int KS = D / 16, DB = D / 32;
+    constexpr int KS = D / 16, DB = D / 32, kOwn = 32 * KW;
     __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage + 2 * 2 * kTileRows * 4];
     const int64_t wg = a.first + blockIdx.x;
     const int item = (int)(wg / a.rows), row = row_of((int)(wg % a.rows), a.xcd_rows);
@@ -255,9 +256,10 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
-    const int len = seq_len(a, b), last = len - 1, k0w = kt * kOwn + 32 * wave;
+    const int kw = wave % KW;
+    const int len = seq_len(a, b), last = len - 1, k0w = kt * kOwn + 32 * kw;
     int first;
-    const int nq = query_tiles(a, kt, len, &first), total = a.group * nq, parts = (total + a.part - 1) / a.part;
+    const int nq = query_tiles(a, kt, kOwn, len, &first), total = a.group * nq, parts = (total + a.part - 1) / a.part;
     __bf16 *dkb = a.dk.ptr + b * a.dk.s_b + hk * a.dk.s_h, *dvb = a.dv.ptr + b * a.dv.s_b + hk * a.dv.s_h;
     if (part >= parts) {
         if (parts == 0 && part == 0) {
@@ -320,8 +322,8 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
         const char *qt = lds + (i & 1) * CP::kStage, *dt = qt + CP::kTile;
         const float *stats = reinterpret_cast<const float *>(lds + 2 * CP::kStage) + (i & 1) * 2 * kTileRows;
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) {
-            const int q = q0 + 32 * qb;
+        for (int x = 0; x < KW / 2; ++x) {
+            const int qb = KW == 4 ? x : wave / KW, q = q0 + 32 * qb;
             if (q + 31 < k0w || q > any_hi) continue;
             // register r: query 16 (r / 8) + 8 hf + r % 8. The products accumulate onto -lse / c and -delta
             f32x16 sc, dp;
@@ -363,9 +365,39 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
                 }
         }
     }
+    if constexpr (KW == 2) {
+        // the second wave's sums onto the first's, through LDS
+        __syncthreads();
+        float *x = reinterpret_cast<float *>(lds) + kw * (DB * 16 * 64) + 4 * lane;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x16 &s = half ? dv[db] : dk[db];
+                    f32x4 *at = reinterpret_cast<f32x4 *>(x + (db * 4 + g) * 256);
+                    if (wave >= KW) *at = f32x4{s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]};
+                }
+            __syncthreads();
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x16 &s = half ? dv[db] : dk[db];
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(x + (db * 4 + g) * 256);
+                    if (wave < KW) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[4 * g + e] += v[e];
+                    }
+                }
+            __syncthreads();
+        }
+        if (wave >= KW) return;
+    }
     if (parts > 1) {
         // [dk, dv][db][g][lane][4] of each wave: whole lines
-        float *out = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * 4 + wave) * (2 * DB * 16 * 64) + 4 * lane;
+        float *out = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * KW + kw) * (2 * DB * 16 * 64) + 4 * lane;
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -378,34 +410,35 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
                 }
         return;
     }
-    __syncthreads();
-    char *stg = lds + wave * 32 * (D + 8) * 2;
+    if constexpr (KW == 4) __syncthreads();
+    char *stg = lds + kw * 32 * (D + 8) * 2;
     store_block<D>(dk, a.scale, a.dk, dkb, k0w, a.tokens, len, stg, lane);
     store_block<D>(dv, 1.f, a.dv, dvb, k0w, a.tokens, len, stg, lane);
 }
 
-// Adds the parts of key tiles that have several. grid: (key tiles, rows), 4 waves of 32 keys, the same registers as above
-template <int D>
-__global__ __launch_bounds__(256) void sink_join_kernel(BwdArgs a, int band) {
-    constexpr int DB = D / 32;
+// Adds the parts of key tiles that have several, in order. grid: (key tiles, rows, blocks of 32 dims of dk, then of dv), a wave
+// per 32 keys, the same registers as above
+template <int D, int KW>
+__global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band) {
+    constexpr int DB = D / 32, kOwn = 32 * KW;
     const int kt = band ? a.sink_tiles + blockIdx.x : blockIdx.x, row = blockIdx.y;
     const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.z / DB, db = blockIdx.z % DB;
     const int len = seq_len(a, b);
     int first;
-    const int total = a.group * query_tiles(a, kt, len, &first), parts = (total + a.part - 1) / a.part;
+    const int total = a.group * query_tiles(a, kt, kOwn, len, &first), parts = (total + a.part - 1) / a.part;
     if (parts < 2) return;
     const int ns = a.sink_tiles * a.sink_parts;
     const int item = kt < a.sink_tiles ? kt * a.sink_parts : ns + (kt - a.sink_tiles) * a.band_parts;
     const int key = kt * kOwn + 32 * wave + (lane & 31);
     if (key >= a.tokens) return;
-    const float *src = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * 4 + wave) * (2 * DB * 16 * 64) +
+    const float *src = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * KW + wave) * (2 * DB * 16 * 64) +
                        (x * DB + db) * 1024 + 4 * lane;
     f32x4 s[4] = {};
     for (int p = 0; p < parts; ++p)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            s[g] += *reinterpret_cast<const f32x4 *>(src + (int64_t)p * a.rows * 4 * (2 * DB * 16 * 64) + g * 256);
+            s[g] += *reinterpret_cast<const f32x4 *>(src + (int64_t)p * a.rows * KW * (2 * DB * 16 * 64) + g * 256);
     const Rows &t = x ? a.dv : a.dk;
     const float mul = x ? 1.f : a.scale;
     __bf16 *out = t.ptr + b * t.s_b + hk * t.s_h + (int64_t)key * t.s_t + 32 * db + 4 * (lane >> 5);
@@ -421,7 +454,7 @@ __global__ __launch_bounds__(256) void sink_join_kernel(BwdArgs a, int band) {
 // How the lists of query tiles are cut: parts of `part` tiles, at most sink_parts of a key tile with first tokens and
 // band_parts of the others.
 struct Plan {
-    int64_t tiles, rows, sink_tiles, sink_parts, band_parts, part, items;
+    int64_t own, tiles, rows, sink_tiles, sink_parts, band_parts, part, items;
     int64_t stats, bytes;
 };
 Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
@@ -429,18 +462,26 @@ Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_
     const int64_t group = heads / kv_heads, q_tiles = (tokens + kTileRows - 1) / kTileRows;
     window = window < tokens ? window : tokens;
     sinks = sinks < tokens ? sinks : tokens;
-    p.tiles = (tokens + kOwn - 1) / kOwn;
     p.rows = batch * kv_heads;
-    p.sink_tiles = (sinks + kOwn - 1) / kOwn;
-    const int64_t reach = (window + kOwn - 1) / kTileRows + 1;
+    p.own = p.rows * ((tokens + 127) / 128) < 1024 ? 64 : 128;
+    p.tiles = (tokens + p.own - 1) / p.own;
+    p.sink_tiles = (sinks + p.own - 1) / p.own;
+    const int64_t reach = (window + p.own - 1) / kTileRows + 1;
     const int64_t band = group * (reach < q_tiles ? reach : q_tiles);
-    p.part = band;
-    p.band_parts = p.sink_tiles < p.tiles ? 1 : 0;
+    // the others' lists in all: whole ones, then the last tiles' shorter ones, step by step
+    const int64_t step = p.own / kTileRows, whole = q_tiles > reach ? (q_tiles - reach) / step + 1 : 0;
+    const int64_t full = whole < p.tiles ? whole : p.tiles, tail = p.tiles - full;
+    const int64_t steps = p.rows * group * (full * reach + tail * (q_tiles - full * step) - step * (tail * (tail - 1) / 2));
+    int64_t cut = 544 * band / (steps > 0 ? steps : 1);
+    cut = cut < band / 6 ? cut : band / 6;
+    cut = cut > 1 ? cut : 1;
+    p.part = (band + cut - 1) / cut;
+    p.band_parts = p.sink_tiles < p.tiles ? (band + p.part - 1) / p.part : 0;
     p.sink_parts = p.sink_tiles ? (group * q_tiles + p.part - 1) / p.part : 0;
     p.items = p.sink_tiles * p.sink_parts + (p.tiles - p.sink_tiles) * p.band_parts;
     p.stats = (batch * heads * tokens * 4 + 15) / 16 * 16;
     p.bytes = 2 * p.stats;
-    if (p.sink_parts > 1 || p.band_parts > 1) p.bytes += p.items * p.rows * kOwn * head_dim * 2 * 4;
+    if (p.sink_parts > 1 || p.band_parts > 1) p.bytes += p.items * p.rows * p.own * head_dim * 2 * 4;
     return p;
 }
 
@@ -497,7 +538,6 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     a.tokens = (int)tokens; a.heads = (int)q->heads; a.kv_heads = (int)k->heads; a.group = a.heads / a.kv_heads;
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
-    a.tiles = (int)p.tiles;
     a.sink_tiles = (int)p.sink_tiles; a.sink_parts = (int)p.sink_parts; a.band_parts = (int)p.band_parts;
     a.part = (int)p.part;
     a.scale = scale; a.scale_log2 = scale * kLog2e;
@@ -510,14 +550,18 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
             hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
         }
     };
-    launch(narrow ? sink_dq_kernel<64> : sink_dq_kernel<128>, batch * q->heads, p.tiles);
-    launch(narrow ? sink_dkv_kernel<64> : sink_dkv_kernel<128>, p.rows, p.items);
+    a.tiles = (int)((tokens + kOwnQ - 1) / kOwnQ);
+    launch(narrow ? sink_dq_kernel<64> : sink_dq_kernel<128>, batch * q->heads, a.tiles);
+    const bool small = p.own == 64;
+    launch(narrow ? (small ? sink_dkv_kernel<64, 2> : sink_dkv_kernel<64, 4>)
+                  : (small ? sink_dkv_kernel<128, 2> : sink_dkv_kernel<128, 4>), p.rows, p.items);
     for (int band = 0; band < 2; ++band) {
         const int64_t n = band ? (p.band_parts > 1 ? p.tiles - p.sink_tiles : 0) : p.sink_parts > 1 ? p.sink_tiles : 0;
         if (n)
-            hipLaunchKernelGGL(narrow ? sink_join_kernel<64> : sink_join_kernel<128>,
-                               dim3((unsigned)n, (unsigned)p.rows, (unsigned)(head_dim / 32 * 2)), dim3(256), 0,
-                               (hipStream_t)stream, a, band);
+            hipLaunchKernelGGL(narrow ? (small ? sink_join_kernel<64, 2> : sink_join_kernel<64, 4>)
+                                      : (small ? sink_join_kernel<128, 2> : sink_join_kernel<128, 4>),
+                               dim3((unsigned)n, (unsigned)p.rows, (unsigned)(head_dim / 32 * 2)),
+                               dim3(small ? 128 : 256), 0, (hipStream_t)stream, a, band);
     }
     return launch_status(fn);
 }

@@ -14,8 +14,6 @@ namespace noise {
 namespace {
 
 constexpr int kBK = 64;    // keys per tile
-constexpr int kBQ = 256;   // queries per workgroup
-constexpr int kStages = 4;
 
 struct FwdArgs {
     Rows q, k, v, o;
@@ -27,11 +25,11 @@ struct FwdArgs {
     float scale_log2;
 };
 
-template <int D>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void sink_fwd_kernel(FwdArgs a) {
     using TL = Tile<D>;
-    constexpr int RB = TL::RB, KS = D / 16, DB = D / 32, NS = kStages;
+    constexpr int RB = TL::RB, KS = D / 16, DB = D / 32, NS = NW == 8 ? 4 : 2, kBQ = 32 * NW;
     constexpr int kTile = kBK * RB, kStage = 2 * kTile;
     constexpr int CPW = kStage / 1024 / 4;   // copies per wave of group A and tile
     __shared__ __attribute__((aligned(16))) char lds[NS * kStage];
@@ -55,7 +53,7 @@ void sink_fwd_kernel(FwdArgs a) {
     if (wg_q_lo > last) {
         // queries past the length: zeros
         const int n = (a.tokens - wg_q_lo < kBQ ? a.tokens - wg_q_lo : kBQ) * TL::CPR;
-        for (int c = tid; c < n; c += 512)
+        for (int c = tid; c < n; c += 64 * NW)
             store_bf16x8(ob + (int64_t)(wg_q_lo + c / TL::CPR) * a.o.s_t + 8 * (c % TL::CPR), zero_bf16x8());
         return;
     }
@@ -80,7 +78,7 @@ void sink_fwd_kernel(FwdArgs a) {
     const int nt = sunk + wg_q_hi / kBK - band + 1;
     auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kBK; };
 
-    // copies of 1 KB: c = 4 i + wave of group A; K's first, then V's
+    // copies of 1 KB: c = 4 i + wave of group A (or of all four waves); K's first, then V's
     constexpr int KC = kTile / 1024;   // copies per K (or V) tile: 8 or 16
     const int crow = lane / TL::CPR, cslot = lane % TL::CPR;
     const bool group_a = wave < 4;
@@ -210,6 +208,26 @@ void sink_fwd_kernel(FwdArgs a) {
             }
     };
 
+    if constexpr (NW == 4) {
+        issue(tile_k0(0), lb);
+#pragma unroll 1
+        for (int t0 = 0; t0 < nt; t0 += NS) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                const int t = t0 + u;
+                if (t < nt) {
+                    vm_wait<0>();
+                    __syncthreads();  // tile t landed, and every wave is past tile t - 1
+                    if (t + 1 < nt) issue(tile_k0(t + 1), lb + ((t + 1) & (NS - 1)) * kStage);
+                    if (active(t)) {
+                        qk(t);
+                        softmax(t);
+                        pv(t);
+                    }
+                }
+            }
+        }
+    } else {
     if (group_a) {
 #pragma unroll
         for (int t = 0; t < 3; ++t)
@@ -260,11 +278,12 @@ void sink_fwd_kernel(FwdArgs a) {
             pv(nt - 1);
         }
     }
+    }
 
     // O^T through LDS (the ring, free once both groups are past their last tile), stored as whole rows; queries past the
     // length get zeros
     constexpr int kPitch = D + 8;
-    static_assert(8 * 32 * kPitch * 2 <= NS * kStage, "staging fits the ring");
+    static_assert(NW * 32 * kPitch * 2 <= NS * kStage, "staging fits the ring");
     l += swap_halves(l);
     const int q = q0w + j;
     const float inv = q <= last ? 1.0f / l : 0.f;   // (a token sees itself: l > 0)
@@ -315,15 +334,18 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.tokens = (int)tokens; a.heads = (int)q->heads; a.group = (int)(q->heads / k->heads);
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
-    a.qtiles = (int)((tokens + kBQ - 1) / kBQ);
     a.rows = (int)(batch * q->heads);
+    const int64_t wide = (tokens + 255) / 256 * a.rows;
+    const bool small = wide < 512;
+    a.qtiles = (int)((tokens + (small ? 127 : 255)) / (small ? 128 : 256));
     a.xcd_rows = a.rows % 8 == 0 ? a.rows / 8 : 0;
     a.scale_log2 = scale * kLog2e;
+    auto kernel = head_dim == 64 ? (small ? sink_fwd_kernel<64, 4> : sink_fwd_kernel<64, 8>)
+                                 : (small ? sink_fwd_kernel<128, 4> : sink_fwd_kernel<128, 8>);
     const int64_t groups = (int64_t)a.qtiles * a.rows;
     for (a.first = 0; a.first < groups; a.first += kLaunchGroups) {
         const int64_t n = groups - a.first < kLaunchGroups ? groups - a.first : kLaunchGroups;
-        hipLaunchKernelGGL(head_dim == 64 ? sink_fwd_kernel<64> : sink_fwd_kernel<128>, dim3((unsigned)n), dim3(512), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(small ? 256 : 512), 0, (hipStream_t)stream, a);
     }
     return launch_status(fn);
 }
