@@ -659,20 +659,21 @@ int noise_qk_norm_rotary_bwd(const noise_heads_t x[2], const noise_heads_t dy[2]
  * i - j <= window or j < sinks (sinks 0: the mask of utils/model.py:17-21). o = softmax(scale q k^T) v in bf16 with fp32
  * scores and sums. q, o have H heads and k, v Hk, H a multiple of Hk (query head h reads key head h / (H / Hk)); head_dim
  * 64 or 128. lengths (NULL: tokens): [batch] int32, or int64 with lengths_wide; keys from lengths[b] on are seen by no
- * query and queries from there on get zeros (rows there may hold anything). lse: NULL, or fp32 [batch][H][tokens], the log2 of each row's sum
- * of exponentials, which the backward pass reads (rows past the length are not written). */
+ * query and queries from there on get zeros (rows there may hold anything). For the backward pass (else NULL, both): lse,
+ * fp32 [batch][H][tokens], the log2 of each row's sum of exponentials (not written past the lengths), and o_rest, like o,
+ * what o's rounding to bf16 left out. */
 int noise_sink_attention_fwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                             const noise_heads_t *o, float *lse, const void *lengths, int lengths_wide, int64_t batch,
-                             int64_t tokens, int64_t head_dim, int64_t window, int64_t sinks, float scale,
-                             noise_stream_t stream);
+                             const noise_heads_t *o, const noise_heads_t *o_rest, float *lse, const void *lengths,
+                             int lengths_wide, int64_t batch, int64_t tokens, int64_t head_dim, int64_t window,
+                             int64_t sinks, float scale, noise_stream_t stream);
 
-/* Its gradients dq, dk, dv (zeros past each length) from d_o and the forward call's tensors and lse. No atomics: the sums
+/* Its gradients dq, dk, dv (zeros past each length) from d_o and the forward call's tensors. No atomics: the sums
  * run in a fixed order. workspace: noise_sink_attention_bwd_workspace_bytes (16 B aligned). */
 int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t window, int64_t sinks);
 int noise_sink_attention_bwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                             const noise_heads_t *o, const noise_heads_t *d_o, const float *lse,
-                             const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
+                             const noise_heads_t *o, const noise_heads_t *o_rest, const noise_heads_t *d_o,
+                             const float *lse, const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
                              const void *lengths, int lengths_wide, int64_t batch, int64_t tokens, int64_t head_dim,
                              int64_t window, int64_t sinks, float scale, void *workspace, int64_t workspace_bytes,
                              noise_stream_t stream);

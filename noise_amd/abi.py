@@ -79,9 +79,9 @@ SIGNATURES = {
     'noise_qk_norm_rotary': [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i32, _i64, _i64, _i64, _i64, _i32, _f32, _p],
     'noise_qk_norm_rotary_bwd_workspace_bytes': [_i64],
     'noise_qk_norm_rotary_bwd': [_p, _p, _p, _p, _p, _p, _p, _i64, _p, _i32, _i64, _i64, _i64, _i32, _f32, _p, _i64, _p],
-    'noise_sink_attention_fwd': [_p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p],
+    'noise_sink_attention_fwd': [_p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p],
     'noise_sink_attention_bwd_workspace_bytes': [_i64, _i64, _i64, _i64, _i64, _i64, _i64],
-    'noise_sink_attention_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p,
+    'noise_sink_attention_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _p,
                                  _i64, _p],
     'noise_sink_decode_workspace_bytes': [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
     'noise_sink_decode': [_p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p],

@@ -1,5 +1,5 @@
 // Backward pass of the attention with a sliding window and first tokens that stay visible, without atomics:
-//   delta_i = sum_d dO_id o_id,  p_ij = 2^(c s_ij - lse_i),  dS = p (dO V^T - delta),
+//   delta_i = sum_d dO_id (o + o_rest)_id,  p_ij = 2^(c s_ij - lse_i),  dS = p (dO V^T - delta),
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
 // Two kernels recompute the scores. sink_dq_kernel walks the key tiles of 128 queries (4 waves of 32) with transposed scores, as
 // the forward pass does, and leaves delta and lse as the second kernel wants them. sink_dkv_kernel walks the query tiles of
@@ -17,7 +17,7 @@ constexpr int kTileRows = 64;  // rows of the tiles that walk by
 constexpr int kOwnQ = 128;     // queries of a workgroup (dq)
 
 struct BwdArgs {
-    Rows q, k, v, o, d_o, dq, dk, dv;
+    Rows q, k, v, o, rest, d_o, dq, dk, dv;
     const float *lse;
     float *nlse, *ndelta;    // -lse / c and -delta, [batch * heads][tokens]
     float *parts;
@@ -147,15 +147,16 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
         const __bf16 *qp = a.q.ptr + b * a.q.s_b + h * a.q.s_h + (int64_t)q * a.q.s_t + 8 * hf;
         const __bf16 *dp = a.d_o.ptr + b * a.d_o.s_b + h * a.d_o.s_h + (int64_t)q * a.d_o.s_t + 8 * hf;
         const __bf16 *op = a.o.ptr + b * a.o.s_b + h * a.o.s_h + (int64_t)q * a.o.s_t + 8 * hf;
+        const __bf16 *rp = a.rest.ptr + b * a.rest.s_b + h * a.rest.s_h + (int64_t)q * a.rest.s_t + 8 * hf;
         const int64_t li = (int64_t)row * a.tokens + q;
         lse = a.lse[li];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             qf[s] = load_bf16x8(qp + 16 * s);
             df[s] = load_bf16x8(dp + 16 * s);
-            const bf16x8 o = load_bf16x8(op + 16 * s);
+            const bf16x8 o = load_bf16x8(op + 16 * s), rest = load_bf16x8(rp + 16 * s);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) nd -= (float)df[s][e] * (float)o[e];
+            for (int e = 0; e < 8; ++e) nd -= (float)df[s][e] * ((float)o[e] + (float)rest[e]);
         }
         nd += swap_halves(nd);
         if (hf == 0 && q0w + j <= last) {
@@ -502,14 +503,16 @@ extern "C" int64_t noise_sink_attention_bwd_workspace_bytes(int64_t batch, int64
 }
 
 extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                                        const noise_heads_t *o, const noise_heads_t *d_o, const float *lse,
+                                        const noise_heads_t *o, const noise_heads_t *o_rest, const noise_heads_t *d_o,
+                                        const float *lse,
                                         const noise_heads_t *dq, const noise_heads_t *dk, const noise_heads_t *dv,
                                         const void *lengths, int lengths_wide, int64_t batch, int64_t tokens,
                                         int64_t head_dim, int64_t window, int64_t sinks, float scale, void *workspace,
                                         int64_t workspace_bytes, noise_stream_t stream) {
     clear_error();
     const char *fn = "noise_sink_attention_bwd";
-    NOISE_CHECK_ARG(q && k && v && o && d_o && dq && dk && dv && q->heads == o->heads && q->heads == d_o->heads &&
+    NOISE_CHECK_ARG(q && k && v && o && o_rest && d_o && dq && dk && dv && q->heads == o->heads &&
+                        q->heads == o_rest->heads && q->heads == d_o->heads &&
                         q->heads == dq->heads && k->heads == v->heads && k->heads == dk->heads && k->heads == dv->heads,
                     "%s: tensors missing or of other heads", fn);
     int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
@@ -524,7 +527,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     BwdArgs a;
     if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||
         (st = check_heads(fn, "v", v, &a.v)) || (st = check_heads(fn, "o", o, &a.o)) ||
-        (st = check_heads(fn, "d_o", d_o, &a.d_o)) || (st = check_heads(fn, "dq", dq, &a.dq)) ||
+        (st = check_heads(fn, "o_rest", o_rest, &a.rest)) || (st = check_heads(fn, "d_o", d_o, &a.d_o)) || (st = check_heads(fn, "dq", dq, &a.dq)) ||
         (st = check_heads(fn, "dk", dk, &a.dk)) || (st = check_heads(fn, "dv", dv, &a.dv)))
         return st;
     for (const Rows *t : {&a.q, &a.k, &a.v, &a.d_o})

@@ -16,7 +16,7 @@ namespace {
 constexpr int kBK = 64;    // keys per tile
 
 struct FwdArgs {
-    Rows q, k, v, o;
+    Rows q, k, v, o, rest;
     float *lse;
     const void *lengths;
     int64_t first;        // this launch's first workgroup
@@ -25,7 +25,11 @@ struct FwdArgs {
     float scale_log2;
 };
 
-template <int D, int NW>
+// TRAIN: with what the backward pass needs beside o, the rows' lse and o's own rounding error. The backward pass forms
+// dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (2^-9 of o) would drown it. With o and its
+// error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is left
+// is 2^-9 of the other weights, in proportion to the difference itself.
+template <int D, int NW, bool TRAIN>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void sink_fwd_kernel(FwdArgs a) {
     using TL = Tile<D>;
@@ -170,10 +174,10 @@ void sink_fwd_kernel(FwdArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][r]);
         mx = fmaxf(mx, swap_halves(mx));
-        // the reference maximum moves only where some row's maximum passes it by more than 8 (log2 units): the weights stay
+        // the reference maximum moves (TRAIN: with every larger score) only where some row's maximum passes it by more than 8 (log2 units): the weights stay
         // below 2^8, and sums and outputs share the stale maximum, so that the rescale runs in few tiles
         const float mc = mx * c2;
-        if (__builtin_amdgcn_ballot_w64(mc > m + 8.0f)) {
+        if (__builtin_amdgcn_ballot_w64(mc > m + (TRAIN ? 0.f : 8.0f))) {
             const float m_new = fmaxf(m, mc);
             const float alpha = exp2_fast(m - m_new);
             m = m_new;
@@ -289,23 +293,30 @@ void sink_fwd_kernel(FwdArgs a) {
     const float inv = q <= last ? 1.0f / l : 0.f;   // (a token sees itself: l > 0)
     __syncthreads();
     __bf16 *stg = reinterpret_cast<__bf16 *>(lds) + wave * 32 * kPitch;
+    auto store = [&](const Rows &t, __bf16 *base, auto rounded) {
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            bf16x4 v;
+            for (int g = 0; g < 4; ++g) {
+                bf16x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (__bf16)(q <= last ? o[db][4 * g + e] * inv : 0.f);
-            store_bf16x4(stg + j * kPitch + 32 * db + 8 * g + 4 * hf, v);
+                for (int e = 0; e < 4; ++e) v[e] = rounded(q <= last ? o[db][4 * g + e] * inv : 0.f);
+                store_bf16x4(stg + j * kPitch + 32 * db + 8 * g + 4 * hf, v);
+            }
+        wave_lds_sync();
+#pragma unroll
+        for (int it = 0; it < TL::CPR / 2; ++it) {
+            const int c = it * 64 + lane, r = c / TL::CPR, ch = c % TL::CPR;
+            if (q0w + r < a.tokens)
+                store_bf16x8(base + (int64_t)(q0w + r) * t.s_t + ch * 8, load_bf16x8(stg + r * kPitch + ch * 8));
         }
-    wave_lds_sync();
-#pragma unroll
-    for (int it = 0; it < TL::CPR / 2; ++it) {
-        const int c = it * 64 + lane, r = c / TL::CPR, ch = c % TL::CPR;
-        if (q0w + r < a.tokens)
-            store_bf16x8(ob + (int64_t)(q0w + r) * a.o.s_t + ch * 8, load_bf16x8(stg + r * kPitch + ch * 8));
+    };
+    store(a.o, ob, [](float x) { return (__bf16)x; });
+    if constexpr (TRAIN) {
+        wave_lds_sync();
+        store(a.rest, a.rest.ptr + b * a.rest.s_b + h * a.rest.s_h, [](float x) { return (__bf16)(x - (float)(__bf16)x); });
+        if (hf == 0 && q <= last) a.lse[(int64_t)row * a.tokens + q] = m + __builtin_amdgcn_logf(l);
     }
-    if (a.lse && hf == 0 && q <= last) a.lse[(int64_t)row * a.tokens + q] = m + __builtin_amdgcn_logf(l);
 }
 
 }  // namespace
@@ -314,7 +325,8 @@ void sink_fwd_kernel(FwdArgs a) {
 using namespace noise;
 
 extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
-                                        const noise_heads_t *o, float *lse, const void *lengths, int lengths_wide,
+                                        const noise_heads_t *o, const noise_heads_t *o_rest, float *lse,
+                                        const void *lengths, int lengths_wide,
                                         int64_t batch, int64_t tokens, int64_t head_dim, int64_t window,
                                         int64_t sinks, float scale, noise_stream_t stream) {
     clear_error();
@@ -327,6 +339,9 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||
         (st = check_heads(fn, "v", v, &a.v)) || (st = check_heads(fn, "o", o, &a.o)))
         return st;
+    NOISE_CHECK_ARG((lse == nullptr) == (o_rest == nullptr) && aligned(lse, 4) && (!o_rest || o_rest->heads == q->heads),
+                    "%s: o_rest and lse go together", fn);
+    if (o_rest && (st = check_heads(fn, "o_rest", o_rest, &a.rest))) return st;
     NOISE_CHECK_ARG(a.k.s_t >= 0 && a.k.s_t < kMaxStride && a.v.s_t >= 0 && a.v.s_t < kMaxStride,
                     "%s: token strides of k and v must be below 2^25", fn);
     NOISE_CHECK_ARG(!lengths || aligned(lengths, lengths_wide ? 8 : 4), "%s: lengths misaligned", fn);
@@ -340,8 +355,10 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.qtiles = (int)((tokens + (small ? 127 : 255)) / (small ? 128 : 256));
     a.xcd_rows = a.rows % 8 == 0 ? a.rows / 8 : 0;
     a.scale_log2 = scale * kLog2e;
-    auto kernel = head_dim == 64 ? (small ? sink_fwd_kernel<64, 4> : sink_fwd_kernel<64, 8>)
-                                 : (small ? sink_fwd_kernel<128, 4> : sink_fwd_kernel<128, 8>);
+    auto kernel = lse ? (head_dim == 64 ? (small ? sink_fwd_kernel<64, 4, true> : sink_fwd_kernel<64, 8, true>)
+                                        : (small ? sink_fwd_kernel<128, 4, true> : sink_fwd_kernel<128, 8, true>))
+                      : (head_dim == 64 ? (small ? sink_fwd_kernel<64, 4, false> : sink_fwd_kernel<64, 8, false>)
+                                        : (small ? sink_fwd_kernel<128, 4, false> : sink_fwd_kernel<128, 8, false>));
     const int64_t groups = (int64_t)a.qtiles * a.rows;
     for (a.first = 0; a.first < groups; a.first += kLaunchGroups) {
         const int64_t n = groups - a.first < kLaunchGroups ? groups - a.first : kLaunchGroups;

@@ -173,36 +173,35 @@ def _qk_norm_rotary_append_fake(q, k, v, cos, sin, k_cache, v_cache, start, q_we
 
 @custom_op('noise_amd::sink_attention', mutates_args=())
 def sink_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int,
-                   lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+                   lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     return _sinks.attend_forward(q, k, v, window, sinks, lengths, True)
 
 
 @sink_attention.register_fake
 def _sink_attention_fake(q, k, v, window, sinks, lengths):
-    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+    return q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
 
 
 @custom_op('noise_amd::sink_attention_backward', mutates_args=())
-def sink_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, window: int,
-                            sinks: int, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
-    return tuple(_sinks.attend_backward(dout, q, k, v, out, lse, window, sinks, lengths))
+def sink_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: Tensor, lse: Tensor,
+                            window: int, sinks: int, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    return tuple(_sinks.attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths))
 
 
 @sink_attention_backward.register_fake
-def _sink_attention_backward_fake(dout, q, k, v, out, lse, window, sinks, lengths):
+def _sink_attention_backward_fake(dout, q, k, v, out, rest, lse, window, sinks, lengths):
     return tuple(t.new_empty(t.shape) for t in (q, k, v))
 
 
 def _sink_attention_setup(ctx, inputs, output):
     q, k, v, ctx.window, ctx.sinks, lengths = inputs
-    out, lse = output
-    ctx.mark_non_differentiable(lse)
-    ctx.save_for_backward(q, k, v, out, lse, lengths)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.save_for_backward(q, k, v, *output, lengths)
 
 
-def _sink_attention_backward(ctx, dout, _):
-    q, k, v, out, lse, lengths = ctx.saved_tensors
-    return (*torch.ops.noise_amd.sink_attention_backward(dout, q, k, v, out, lse, ctx.window, ctx.sinks, lengths),
+def _sink_attention_backward(ctx, dout, *_):
+    *saved, lengths = ctx.saved_tensors
+    return (*torch.ops.noise_amd.sink_attention_backward(dout, *saved, ctx.window, ctx.sinks, lengths),
             None, None, None)
 
 

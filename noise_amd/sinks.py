@@ -259,16 +259,20 @@ def _attend_operands(fn, q, k, v, window, sinks, lengths):
     return (None, 0) if lengths is None else _ints(fn, 'lengths', lengths, q.shape[0], q.device)
 
 
-def _attend_forward(q, k, v, window, sinks, lengths, wide, with_lse):
-    """(out, lse or None) of checked operands"""
+def _attend_forward(q, k, v, window, sinks, lengths, wide, training):
+    """(out, what its rounding left out or None, lse or None) of checked operands"""
     B, T, H, D = q.shape
-    out = q.new_empty(q.shape)
-    lse = q.new_empty((B, H, T), dtype=F32) if with_lse else None
+    out, rest, lse = q.new_empty(q.shape), None, None
     q, k, v = _rows(q), _rows(k), _rows(v)
-    t = _table(q, k, v, out)
-    _call('noise_sink_attention_fwd', q.device, t, *_parts(t, 1, 4), _lib.ptr(lse), _lib.ptr(lengths), wide, B, T, D, window,
-          sinks, D ** -0.5)
-    return out, lse
+    if training:
+        rest, lse = q.new_empty(out.shape), q.new_empty((B, H, T), dtype=F32)
+        t = _table(q, k, v, out, rest)
+        ref = ctypes.byref(t, 4 * _HEADS)
+    else:
+        t, ref = _table(q, k, v, out), None
+    _call('noise_sink_attention_fwd', q.device, *_parts(t, 0, 4), ref, _lib.ptr(lse), _lib.ptr(lengths), wide, B, T, D,
+          window, sinks, D ** -0.5)
+    return out, rest, lse
 
 
 def _parts(table, first, end):
@@ -280,45 +284,45 @@ def _attend_workspace(*sizes):
     return _lib.lib().noise_sink_attention_bwd_workspace_bytes(*sizes)
 
 
-def _attend_backward(dout, q, k, v, out, lse, window, sinks, lengths, wide):
+def _attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths, wide):
     B, T, H, D = q.shape
     grads = [x.new_empty(x.shape) for x in (q, k, v)]
-    x = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout if dout.dtype == BF16 else dout.to(BF16))
+    x = _rows(q), _rows(k), _rows(v), _rows(out), rest, _rows(dout if dout.dtype == BF16 else dout.to(BF16))
     t = _table(*x, *grads)
     need = _attend_workspace(B, T, H, k.shape[2], D, window, sinks)
     work = q.new_empty(max(need, 0), dtype=torch.uint8)
-    refs = _parts(t, 0, 8)
-    _call('noise_sink_attention_bwd', q.device, *refs[:5], lse.data_ptr(), *refs[5:], _lib.ptr(lengths), wide, B, T, D, window,
+    refs = _parts(t, 0, 9)
+    _call('noise_sink_attention_bwd', q.device, *refs[:6], lse.data_ptr(), *refs[6:], _lib.ptr(lengths), wide, B, T, D, window,
           sinks, D ** -0.5, work.data_ptr(), need)
     return grads
 
 
-def attend_forward(q, k, v, window, sinks, lengths, with_lse):
-    """(out, lse or None)"""
+def attend_forward(q, k, v, window, sinks, lengths, training):
+    """(out, rest, lse): with `training` what attend_backward takes beside the output, else None"""
     return _attend_forward(q, k, v, window, sinks, *_attend_operands('sink_attention', q, k, v, window, sinks, lengths),
-                           with_lse)
+                           training)
 
 
-def attend_backward(dout, q, k, v, out, lse, window, sinks, lengths):
+def attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths):
     operands = _attend_operands('sink_attention', q, k, v, window, sinks, lengths)
-    return _attend_backward(dout, q, k, v, out, lse, window, sinks, *operands)
+    return _attend_backward(dout, q, k, v, out, rest, lse, window, sinks, *operands)
 
 
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, lengths):
         lengths, wide = _attend_operands('sink_attention', q, k, v, window, sinks, lengths)
-        out, lse = _attend_forward(q, k, v, window, sinks, lengths, wide, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, rest, lse = _attend_forward(q, k, v, window, sinks, lengths, wide, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, lengths)
         ctx.more = window, sinks, wide
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, rest, lse, lengths = ctx.saved_tensors
         window, sinks, wide = ctx.more
-        return (*_attend_backward(dout, q, k, v, out, lse, window, sinks, lengths, wide), None, None, None)
+        return (*_attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths, wide), None, None, None)
 
 
 def sink_attention(q, k, v, window, sinks=0, lengths=None):

@@ -38,7 +38,7 @@ def check_all(q, k, v, dout, window, sinks, lengths=None):
     out = sink_attention(*leaves, window, sinks, lengths)
     want, weight = oracle.attend(q, k, v, window, sinks, lengths)
     check(out.detach(), want, U * (weight + want.abs()), 'out')
-    assert torch.equal(sink_attention(q, k, v, window, sinks, lengths), out)
+    check(sink_attention(q, k, v, window, sinks, lengths), want, U * (weight + want.abs()), 'out without gradients')
     grads = torch.autograd.grad(out, leaves, dout)
     wants, bounds = oracle.attend_grads(q, k, v, dout, window, sinks, lengths)
     for name, got, want, bound in zip('qkv', grads, wants, bounds):
@@ -139,6 +139,25 @@ def test_empty():
         assert q.grad.shape == shape
 
 
+@pytest.mark.parametrize('D', [64, 128])
+def test_gradients_of_weights_close_to_one(D):
+    """Rows that give nearly all their weight to one key: dP - dO . out nearly cancels there. Relative to the whole gradient, its
+    parts' roundings of 2^-9 (rms 2^-9 / sqrt 3 each: of the scores' gradients, of the weights in the output, of the
+    result) leave less than 3 2^-9; the output's own rounding in dO . out would leave several times that."""
+    q, k, v, dout = inputs(1, 300, 2, 1, D, 9, 4)
+    k[:, 0] = (q.float().mean((1, 2), keepdim=True)[:, 0] * 40).bfloat16()
+    k[:, 7] = k[:, 0]
+    for scale, window, sinks in ((0.4, 3, 1), (1.0, 3, 1), (1.0, 100, 8)):
+        keys = (k.float() * scale).bfloat16()
+        from noise_amd.sinks import sink_attention
+        leaves = [t.detach().requires_grad_() for t in (q, keys, v)]
+        grads = torch.autograd.grad(sink_attention(*leaves, window, sinks), leaves, dout)
+        for got, want in zip(grads, oracle.attend_grads(q, keys, v, dout, window, sinks)[0]):
+            rel = ((got.double() - want).norm() / want.norm()).item()
+            print(D, scale, window, sinks, rel, flush=True)
+            assert rel <= 3 * 2.0 ** -9
+
+
 def test_growing_scores():
     """Scores far apart, and rows whose largest weight stands in the last tile or the first key."""
     q, k, v, dout = inputs(1, 400, 2, 2, 64, 8, 4)
@@ -169,8 +188,8 @@ def test_captured_graphs():
     q, k, v, dout = inputs(2, 500, 4, 2, 64, 6, 4)
 
     def step():
-        out, lse = attend_forward(q, k, v, 90, 4, None, True)
-        return (out, *attend_backward(dout, q, k, v, out, lse, 90, 4, None))
+        out, *more = attend_forward(q, k, v, 90, 4, None, True)
+        return (out, *attend_backward(dout, q, k, v, out, *more, 90, 4, None))
 
     step()
     torch.cuda.synchronize()

@@ -89,8 +89,8 @@ def test_entry_points_refuse():
     rows = lambda ptr=16, s=64, heads=2: _lib.Heads(ptr, 5 * s * heads, s * heads, s, heads)
     H = lambda **more: ctypes.byref(rows(**more))
     err = lambda: lib.noise_last_error().decode()
-    fwd = lambda q=H(), k=H(), v=H(), o=H(), B=1, T=5, D=64, W=3, n=0: lib.noise_sink_attention_fwd(
-        q, k, v, o, None, None, 0, B, T, D, W, n, 0.1, None)
+    fwd = lambda q=H(), k=H(), v=H(), o=H(), rest=None, B=1, T=5, D=64, W=3, n=0: lib.noise_sink_attention_fwd(
+        q, k, v, o, rest, None, None, 0, B, T, D, W, n, 0.1, None)
     def refused(st, words):
         assert st == -1 and words in err(), (st, err())
 
@@ -102,12 +102,13 @@ def test_entry_points_refuse():
     refused(fwd(o=H(heads=3)), 'heads')
     refused(fwd(q=H(heads=3), o=H(heads=3)), 'key heads')
     refused(fwd(v=None), 'missing')
+    refused(fwd(rest=H()), 'go together')
     refused(fwd(T=-1), 'tokens')
     refused(fwd(T=1 << 40), 'tokens')
     refused(fwd(B=1 << 50, T=1 << 29), 'too many')
     assert fwd(B=0) == 0 and fwd(T=0) == 0
     h = [H() for _ in range(9)]
-    bwd = lambda ws, size: lib.noise_sink_attention_bwd(*h[:5], 16, *h[5:8], None, 0, 1, 5, 64, 3, 0, 0.1, ws, size, None)
+    bwd = lambda ws, size: lib.noise_sink_attention_bwd(*h[:6], 16, *h[6:9], None, 0, 1, 5, 64, 3, 0, 0.1, ws, size, None)
     refused(bwd(16, 8), 'workspace')
     refused(bwd(None, 1 << 40), 'workspace')
     refused(lib.noise_sink_attention_bwd_workspace_bytes(1, 5, 3, 2, 64, 3, 0), 'key heads')
@@ -140,8 +141,8 @@ def test_entry_points_refuse():
 def test_fake_shapes():
     with FakeTensorMode():
         q, k, v = qkv()
-        out, lse = torch.ops.noise_amd.sink_attention(q, k, v, 3, 1, None)
-        assert out.shape == q.shape and lse.shape == (2, 4, 5) and lse.dtype == torch.float32
+        out, rest, lse = torch.ops.noise_amd.sink_attention(q, k, v, 3, 1, None)
+        assert out.shape == rest.shape == q.shape and lse.shape == (2, 4, 5) and lse.dtype == torch.float32
         start = torch.zeros(2, dtype=torch.int64)
         assert torch.ops.noise_amd.sink_attention_decode(q[:, :1], k, v, start, 3, 1).shape == (2, 1, 4, 64)
         a, b = torch.ops.noise_amd.qk_norm_rotary(q, k, torch.zeros(5, 32), torch.zeros(5, 32), None, None, None, 1e-6)
