@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     }
     vm_wait<0>();
     const CP cp(wave, lane);
-    const Frags<D> fr(lane);
+    const Frags<D> frags(lane);
     const unsigned lb = lds_addr(lds);
     auto issue = [&](int i) {
         const int g = i / nq, q0 = (first + i - g * nq) * kTileRows;
@@ -326,6 +326,9 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
         for (int x = 0; x < KW / 2; ++x) {
             const int qb = KW == 4 ? x : wave / KW, q = q0 + 32 * qb;
             if (q + 31 < k0w || q > any_hi) continue;
+            // (the fragments' addresses are formed anew in each block: kept over the loop, they would push sums out to memory)
+            Frags<D> fr = frags;
+            asm volatile("" : "+v"(fr.rows), "+v"(fr.cols));
             // register r: query 16 (r / 8) + 8 hf + r % 8. The products accumulate onto -lse / c and -delta
             f32x16 sc, dp;
 #pragma unroll
