@@ -23,13 +23,12 @@ struct BwdArgs {
     float *parts;
     const void *lengths;
     int64_t first;
-    int wide, tokens, heads, kv_heads, group, window, sinks, tiles;
-    int rows, xcd_rows;              // batch * heads (dq) or batch * kv_heads (dk, dv)
+    int wide, tokens, heads, kv_heads, group, window, sinks;
+    int tiles;                       // of queries (dq) or keys (dk, dv)
+    int rows;                        // batch * heads (dq) or batch * kv_heads (dk, dv)
     int sink_tiles, sink_parts, band_parts, part;  // key tiles with first tokens; most parts of each kind; tiles per part
     float scale, scale_log2;
 };
-
-__device__ __forceinline__ int row_of(int u, int xcd_rows) { return xcd_rows ? (u & 7) * xcd_rows + (u >> 3) : u; }
 
 __device__ __forceinline__ int seq_len(const BwdArgs &a, int b) {
     int len = a.tokens;
@@ -126,7 +125,8 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
     constexpr int KS = D / 16, DB = D / 32;
     __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage];
     const int64_t wg = a.first + blockIdx.x;
-    const int qt = a.tiles - 1 - (int)(wg / a.rows), row = row_of((int)(wg % a.rows), a.xcd_rows);
+    const int round = (int)(wg / a.rows), qt = a.tiles - 1 - round;
+    const int row = row_of((int)(wg % a.rows), round, a.rows, a.lengths != nullptr);
     const int b = row / a.heads, h = row - b * a.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
@@ -250,10 +250,12 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     constexpr int KS = D / 16, DB = D / 32, kOwn = 32 * KW;
     __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage + 2 * 2 * kTileRows * 4];
     const int64_t wg = a.first + blockIdx.x;
-    const int item = (int)(wg / a.rows), row = row_of((int)(wg % a.rows), a.xcd_rows);
-    const int ns = a.sink_tiles * a.sink_parts;
-    const int kt = item < ns ? item / a.sink_parts : a.sink_tiles + (item - ns) / a.band_parts;
-    const int part = item < ns ? item % a.sink_parts : (item - ns) % a.band_parts;
+    const int item = (int)(wg / a.rows), row = row_of((int)(wg % a.rows), item, a.rows, a.lengths != nullptr);
+    // the first parts of all key tiles, then the second ones: the workgroups of an XCD go to its engines in turn, and one that
+    // got all long parts would hold up the ones that follow
+    const int ns = a.sink_tiles * a.sink_parts, bands = a.tiles - a.sink_tiles;
+    const int kt = item < ns ? item % a.sink_tiles : a.sink_tiles + (item - ns) % bands;
+    const int part = item < ns ? item / a.sink_tiles : (item - ns) / bands;
     const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
@@ -433,7 +435,8 @@ __global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band)
     const int total = a.group * query_tiles(a, kt, kOwn, len, &first), parts = (total + a.part - 1) / a.part;
     if (parts < 2) return;
     const int ns = a.sink_tiles * a.sink_parts;
-    const int item = kt < a.sink_tiles ? kt * a.sink_parts : ns + (kt - a.sink_tiles) * a.band_parts;
+    const int item = kt < a.sink_tiles ? kt : ns + kt - a.sink_tiles;
+    const int next = kt < a.sink_tiles ? a.sink_tiles : a.tiles - a.sink_tiles;   // items from part to part
     const int key = kt * kOwn + 32 * wave + (lane & 31);
     if (key >= a.tokens) return;
     const float *src = a.parts + ((int64_t)(item * (int64_t)a.rows + row) * KW + wave) * (2 * DB * 16 * 64) +
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band)
     for (int p = 0; p < parts; ++p)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            s[g] += *reinterpret_cast<const f32x4 *>(src + (int64_t)p * a.rows * KW * (2 * DB * 16 * 64) + g * 256);
+            s[g] += *reinterpret_cast<const f32x4 *>(src + (int64_t)p * next * a.rows * KW * (2 * DB * 16 * 64) + g * 256);
     const Rows &t = x ? a.dv : a.dk;
     const float mul = x ? 1.f : a.scale;
     __bf16 *out = t.ptr + b * t.s_b + hk * t.s_h + (int64_t)key * t.s_t + 32 * db + 4 * (lane >> 5);
@@ -550,7 +553,6 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     const bool narrow = head_dim == 64;
     auto launch = [&](void (*kernel)(BwdArgs), int64_t rows, int64_t items) {
         a.rows = (int)rows;
-        a.xcd_rows = rows % 8 == 0 ? (int)(rows / 8) : 0;
         for (a.first = 0; a.first < rows * items; a.first += kLaunchGroups) {
             const int64_t n = rows * items - a.first < kLaunchGroups ? rows * items - a.first : kLaunchGroups;
             hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
@@ -559,6 +561,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     a.tiles = (int)((tokens + kOwnQ - 1) / kOwnQ);
     launch(narrow ? sink_dq_kernel<64> : sink_dq_kernel<128>, batch * q->heads, a.tiles);
     const bool small = p.own == 64;
+    a.tiles = (int)p.tiles;
     launch(narrow ? (small ? sink_dkv_kernel<64, 2> : sink_dkv_kernel<64, 4>)
                   : (small ? sink_dkv_kernel<128, 2> : sink_dkv_kernel<128, 4>), p.rows, p.items);
     for (int band = 0; band < 2; ++band) {

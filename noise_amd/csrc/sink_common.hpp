@@ -25,6 +25,14 @@ __device__ __forceinline__ int64_t at_wide(const void *p, int wide, int64_t i) {
     return wide ? static_cast<const int64_t *>(p)[i] : (int64_t)static_cast<const int32_t *>(p)[i];
 }
 
+// Which row (of heads of sequences) workgroup u of a round of `rows` workgroups takes. Workgroups go to the 8 XCDs in turn. With
+// rows in eighths each XCD takes neighbouring rows, whose heads share keys in its L2; in padded batches that would leave the
+// XCDs of short sequences idle, so there the rounds are shifted against each other.
+__device__ __forceinline__ int row_of(int u, int round, int rows, bool padded) {
+    if (padded) return (u + round) % rows;
+    return rows % 8 ? u : (u & 7) * (rows / 8) + (u >> 3);
+}
+
 // bits 2 and 3 of a row index swapped: with a block's rows read in this order, register r of a lane's 32 x 32 result
 // stands for row 16 (r / 8) + 8 (lane / 32) + r % 8, eight consecutive ones per operand of the next product
 __device__ __forceinline__ int sigma(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }

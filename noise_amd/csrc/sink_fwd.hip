@@ -21,7 +21,6 @@ struct FwdArgs {
     const void *lengths;
     int64_t first;        // this launch's first workgroup
     int wide, tokens, heads, group, window, sinks, qtiles, rows;  // group: query heads per key head; rows: batch * heads
-    int xcd_rows;         // rows per XCD where rows divide by 8, else 0
     float scale_log2;
 };
 
@@ -38,11 +37,10 @@ void sink_fwd_kernel(FwdArgs a) {
     constexpr int CPW = kStage / 1024 / 4;   // copies per wave of group A and tile
     __shared__ __attribute__((aligned(16))) char lds[NS * kStage];
 
-    // the last query tiles (those with the most keys) of all heads first; heads in runs on one XCD (workgroups go to the
-    // XCDs in turn), so that query heads of one key head share its L2
+    // the last query tiles (those with the most keys) of all heads first
     const int64_t wg = a.first + blockIdx.x;
-    const int qt = a.qtiles - 1 - (int)(wg / a.rows), u = (int)(wg % a.rows);
-    const int row = a.xcd_rows ? (u & 7) * a.xcd_rows + (u >> 3) : u;
+    const int round = (int)(wg / a.rows), qt = a.qtiles - 1 - round;
+    const int row = row_of((int)(wg % a.rows), round, a.rows, a.lengths != nullptr);
     const int b = row / a.heads, h = row - b * a.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
@@ -353,7 +351,6 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     const int64_t wide = (tokens + 255) / 256 * a.rows;
     const bool small = wide < 512;
     a.qtiles = (int)((tokens + (small ? 127 : 255)) / (small ? 128 : 256));
-    a.xcd_rows = a.rows % 8 == 0 ? a.rows / 8 : 0;
     a.scale_log2 = scale * kLog2e;
     auto kernel = lse ? (head_dim == 64 ? (small ? sink_fwd_kernel<64, 4, true> : sink_fwd_kernel<64, 8, true>)
                                         : (small ? sink_fwd_kernel<128, 4, true> : sink_fwd_kernel<128, 8, true>))
