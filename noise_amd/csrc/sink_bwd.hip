@@ -118,23 +118,25 @@ __device__ __forceinline__ void store_block(const f32x16 (&acc)[D / 32], float m
     wave_lds_sync();
 }
 
-template <int D>
-__global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
+// SPLIT: 8 waves, every second key tile by either half, whose sums are added in LDS
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a) {
     using TL = Tile<D>;
     using CP = Copies<D>;
-    constexpr int KS = D / 16, DB = D / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * CP::kStage];
+    constexpr int KS = D / 16, DB = D / 32, HALVES = SPLIT ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) char lds[2 * HALVES * CP::kStage];
     const int64_t wg = a.first + blockIdx.x;
     const int round = (int)(wg / a.rows), qt = a.tiles - 1 - round;
     const int row = row_of((int)(wg % a.rows), round, a.rows, a.lengths != nullptr);
     const int b = row / a.heads, h = row - b * a.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
-    const int len = seq_len(a, b), last = len - 1, q_lo = qt * kOwnQ, q0w = q_lo + 32 * wave;
+    const int len = seq_len(a, b), last = len - 1, q_lo = qt * kOwnQ;
+    const int half = wave >> 2, q0w = q_lo + 32 * (wave & 3);
     __bf16 *dqb = a.dq.ptr + b * a.dq.s_b + h * a.dq.s_h;
     if (q_lo > last) {
         const int n = (a.tokens - q_lo < kOwnQ ? a.tokens - q_lo : kOwnQ) * TL::CPR;
-        for (int c = tid; c < n; c += 256)
+        for (int c = tid; c < n; c += 256 * HALVES)
             store_bf16x8(dqb + (int64_t)(q_lo + c / TL::CPR) * a.dq.s_t + 8 * (c % TL::CPR), zero_bf16x8());
         return;
     }
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
             for (int e = 0; e < 8; ++e) nd -= (float)df[s][e] * ((float)o[e] + (float)rest[e]);
         }
         nd += swap_halves(nd);
-        if (hf == 0 && q0w + j <= last) {
+        if (hf == 0 && half == 0 && q0w + j <= last) {
             a.nlse[li] = -lse / a.scale_log2;
             a.ndelta[li] = nd;
         }
@@ -171,11 +173,13 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
     const int sunk = (n_sinks + kTileRows - 1) / kTileRows < band ? (n_sinks + kTileRows - 1) / kTileRows : band;
     const int nt = sunk + q_hi / kTileRows - band + 1;
     auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kTileRows; };
-    const CP cp(wave, lane);
+    const CP cp(wave & 3, lane);
     const Frags<D> fr(lane);
     const unsigned lb = lds_addr(lds);
-    auto issue = [&](int t) {
-        const unsigned st = lb + (t & 1) * CP::kStage;
+    auto issue = [&](int i) {
+        const int t = i * HALVES + half;
+        if (t >= nt) return;
+        const unsigned st = lb + ((i & 1) * HALVES + half) * CP::kStage;
         cp.one(a.k, Kb, tile_k0(t), last, st);
         cp.one(a.v, Vb, tile_k0(t), last, st + CP::kTile);
     };
@@ -184,15 +188,18 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
     for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
     const int wq_lo = q0w, wq_hi = q0w > last ? -1 : q0w + 31 < last ? q0w + 31 : last;
     const float c2 = a.scale_log2;
+    const int rounds = (nt + HALVES - 1) / HALVES;
     issue(0);
 #pragma unroll 1
-    for (int t = 0; t < nt; ++t) {
+    for (int i = 0; i < rounds; ++i) {
         vm_wait<0>();
-        __syncthreads();   // tile t landed, and every wave is past tile t - 1
-        if (t + 1 < nt) issue(t + 1);
+        __syncthreads();   // round i's tiles landed, and every wave is past round i - 1
+        if (i + 1 < rounds) issue(i + 1);
+        const int t = i * HALVES + half;
+        if (t >= nt) continue;
         const int k0 = tile_k0(t);
         if (k0 > wq_hi || (k0 + kTileRows - 1 < wq_lo - W && k0 >= n_sinks)) continue;
-        const char *kt = lds + (t & 1) * CP::kStage, *vt = kt + CP::kTile;
+        const char *kt = lds + ((i & 1) * HALVES + half) * CP::kStage, *vt = kt + CP::kTile;
         const bool causal_edge = k0 + kTileRows - 1 > wq_lo, window_edge = k0 < wq_hi - W;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -228,8 +235,32 @@ __global__ __launch_bounds__(256, 2) void sink_dq_kernel(BwdArgs a) {
         }
     }
     __syncthreads();
-    static_assert(4 * 32 * (D + 8) * 2 <= 2 * CP::kStage, "staging fits");
-    store_block<D>(dq, a.scale, a.dq, dqb, q0w, a.tokens, len, lds + wave * 32 * (D + 8) * 2, lane);
+    constexpr int kPart = SPLIT ? DB * 16 * 64 * 4 : 32 * (D + 8) * 2;   // bytes of a wave's sums, or of its staged rows
+    static_assert(32 * (D + 8) * 2 <= kPart && 4 * kPart <= 2 * HALVES * CP::kStage, "staging fits");
+    char *mine = lds + (wave & 3) * kPart;
+    if constexpr (SPLIT) {
+        float *x = reinterpret_cast<float *>(mine) + 4 * lane;
+        if (half) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4 *>(x + (db * 4 + g) * 256) =
+                        f32x4{dq[db][4 * g], dq[db][4 * g + 1], dq[db][4 * g + 2], dq[db][4 * g + 3]};
+        }
+        __syncthreads();
+        if (half) return;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(x + (db * 4 + g) * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dq[db][4 * g + e] += v[e];
+            }
+        wave_lds_sync();
+    }
+    store_block<D>(dq, a.scale, a.dq, dqb, q0w, a.tokens, len, mine, lane);
 }
 
 // query tiles of key tile kt: first, and how many (of one query head)
@@ -551,19 +582,22 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     a.part = (int)p.part;
     a.scale = scale; a.scale_log2 = scale * kLog2e;
     const bool narrow = head_dim == 64;
-    auto launch = [&](void (*kernel)(BwdArgs), int64_t rows, int64_t items) {
+    auto launch = [&](void (*kernel)(BwdArgs), int64_t rows, int64_t items, int threads) {
         a.rows = (int)rows;
         for (a.first = 0; a.first < rows * items; a.first += kLaunchGroups) {
             const int64_t n = rows * items - a.first < kLaunchGroups ? rows * items - a.first : kLaunchGroups;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3((unsigned)threads), 0, (hipStream_t)stream, a);
         }
     };
     a.tiles = (int)((tokens + kOwnQ - 1) / kOwnQ);
-    launch(narrow ? sink_dq_kernel<64> : sink_dq_kernel<128>, batch * q->heads, a.tiles);
+    // no more workgroups than CUs: two halves of the keys for each
+    const bool split = batch * q->heads * a.tiles <= 256;
+    launch(narrow ? (split ? sink_dq_kernel<64, true> : sink_dq_kernel<64, false>)
+                  : (split ? sink_dq_kernel<128, true> : sink_dq_kernel<128, false>), batch * q->heads, a.tiles, split ? 512 : 256);
     const bool small = p.own == 64;
     a.tiles = (int)p.tiles;
     launch(narrow ? (small ? sink_dkv_kernel<64, 2> : sink_dkv_kernel<64, 4>)
-                  : (small ? sink_dkv_kernel<128, 2> : sink_dkv_kernel<128, 4>), p.rows, p.items);
+                  : (small ? sink_dkv_kernel<128, 2> : sink_dkv_kernel<128, 4>), p.rows, p.items, 256);
     for (int band = 0; band < 2; ++band) {
         const int64_t n = band ? (p.band_parts > 1 ? p.tiles - p.sink_tiles : 0) : p.sink_parts > 1 ? p.sink_tiles : 0;
         if (n)

@@ -15,6 +15,8 @@ namespace {
 
 constexpr int kBK = 64;    // keys per tile
 
+enum { kPaired, kFour, kSplit };
+
 struct FwdArgs {
     Rows q, k, v, o, rest;
     float *lse;
@@ -24,18 +26,22 @@ struct FwdArgs {
     float scale_log2;
 };
 
+// FORM: kPaired, as above, 256 queries by 8 waves; for fewer workgroups than the CUs hold at a time, kFour, 128 queries by 4
+// waves and two stages, and for no more than there are CUs, kSplit, 128 queries by 8 waves, every second tile by either half,
+// which are joined in LDS.
 // TRAIN: with what the backward pass needs beside o, the rows' lse and o's own rounding error. The backward pass forms
 // dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (2^-9 of o) would drown it. With o and its
 // error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is left
 // is 2^-9 of the other weights, in proportion to the difference itself.
-template <int D, int NW, bool TRAIN>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
+template <int D, int FORM, bool TRAIN>
+__global__ __launch_bounds__(FORM == kFour ? 256 : 512) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void sink_fwd_kernel(FwdArgs a) {
     using TL = Tile<D>;
-    constexpr int RB = TL::RB, KS = D / 16, DB = D / 32, NS = NW == 8 ? 4 : 2, kBQ = 32 * NW;
+    constexpr int RB = TL::RB, KS = D / 16, DB = D / 32, NW = FORM == kFour ? 4 : 8, NS = FORM == kPaired ? 4 : 2;
+    constexpr int kBQ = FORM == kPaired ? 256 : 128, HALVES = FORM == kSplit ? 2 : 1;
     constexpr int kTile = kBK * RB, kStage = 2 * kTile;
     constexpr int CPW = kStage / 1024 / 4;   // copies per wave of group A and tile
-    __shared__ __attribute__((aligned(16))) char lds[NS * kStage];
+    __shared__ __attribute__((aligned(16))) char lds[NS * HALVES * kStage];
 
     // the last query tiles (those with the most keys) of all heads first
     const int64_t wg = a.first + blockIdx.x;
@@ -60,7 +66,7 @@ void sink_fwd_kernel(FwdArgs a) {
         return;
     }
     const int W = a.window, n_sinks = a.sinks;
-    const int q0w = wg_q_lo + 32 * wave;
+    const int half = FORM == kSplit ? wave >> 2 : 0, q0w = wg_q_lo + 32 * (FORM == kSplit ? wave & 3 : wave);
     const __bf16 *Qb = a.q.ptr + b * a.q.s_b + h * a.q.s_h;
     const __bf16 *Kb = a.k.ptr + b * a.k.s_b + (h / a.group) * a.k.s_h;
     const __bf16 *Vb = a.v.ptr + b * a.v.s_b + (h / a.group) * a.v.s_h;
@@ -80,12 +86,12 @@ void sink_fwd_kernel(FwdArgs a) {
     const int nt = sunk + wg_q_hi / kBK - band + 1;
     auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kBK; };
 
-    // copies of 1 KB: c = 4 i + wave of group A (or of all four waves); K's first, then V's
+    // copies of 1 KB: c = 4 i + wave % 4 of group A (kPaired) or of a tile's four waves; K's first, then V's
     constexpr int KC = kTile / 1024;   // copies per K (or V) tile: 8 or 16
     const int crow = lane / TL::CPR, cslot = lane % TL::CPR;
     const bool group_a = wave < 4;
     const unsigned lb = lds_addr(lds);
-    // this lane's chunk: row R = RPC c + crow with c = 4 i + wave, whose swizzle does not depend on i (RPC 4 i is a multiple
+    // this lane's chunk: row R = RPC c + crow, whose swizzle does not depend on i (RPC 4 i is a multiple
     // of the swizzles' period of 16 rows)
     static_assert(4 * TL::RPC % 16 == 0, "uniform swizzle");
     const int r0 = TL::RPC * (wave & 3) + crow;
@@ -96,7 +102,7 @@ void sink_fwd_kernel(FwdArgs a) {
             // the tile with the last token: each lane's row is clamped
 #pragma unroll
             for (int i = 0; i < CPW; ++i) {
-                const int c = 4 * i + wave, r = (i * 4 * TL::RPC + r0) % kBK;
+                const int c = 4 * i + (wave & 3), r = (i * 4 * TL::RPC + r0) % kBK;
                 const unsigned rr = (unsigned)(k0 + r > last ? last - k0 : r);
                 if (c < KC)
                     lds_dma16_at(Kb + (int64_t)k0 * a.k.s_t, rr * (unsigned)a.k.s_t * 2 + kchunk * 16, st + c * 1024);
@@ -107,7 +113,7 @@ void sink_fwd_kernel(FwdArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < CPW; ++i) {
-            const int c = 4 * i + wave;
+            const int c = 4 * i + (wave & 3);
             if (c < KC)
                 lds_dma16_at(Kb + (int64_t)(k0 + 4 * i * TL::RPC) * a.k.s_t, koff, st + c * 1024);
             else
@@ -135,7 +141,7 @@ void sink_fwd_kernel(FwdArgs a) {
         return k0 <= wq_hi && (k0 + kBK - 1 >= wq_lo - W || k0 < n_sinks);
     };
     auto qk = [&](int t) {
-        const char *st = lds + (t & (NS - 1)) * kStage;
+        const char *st = lds + ((t / HALVES & (NS - 1)) * HALVES + half) * kStage;
         sc[0] = f32x16{};
         sc[1] = f32x16{};
 #pragma unroll
@@ -200,7 +206,7 @@ void sink_fwd_kernel(FwdArgs a) {
             for (int e = 0; e < 8; ++e) pf[s][e] = (__bf16)sc[s >> 1][8 * (s & 1) + e];
     };
     auto pv = [&](int t) {
-        const char *st = lds + (t & (NS - 1)) * kStage;
+        const char *st = lds + ((t / HALVES & (NS - 1)) * HALVES + half) * kStage;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -210,18 +216,24 @@ void sink_fwd_kernel(FwdArgs a) {
             }
     };
 
-    if constexpr (NW == 4) {
-        issue(tile_k0(0), lb);
+    if constexpr (FORM != kPaired) {
+        // round t0 works on tiles HALVES t0 + half
+        const int rounds = (nt + HALVES - 1) / HALVES;
+        auto copy = [&](int i) {
+            const int t = i * HALVES + half;
+            if (t < nt) issue(tile_k0(t), lb + ((i & (NS - 1)) * HALVES + half) * kStage);
+        };
+        copy(0);
 #pragma unroll 1
-        for (int t0 = 0; t0 < nt; t0 += NS) {
+        for (int i0 = 0; i0 < rounds; i0 += NS) {
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
-                const int t = t0 + u;
-                if (t < nt) {
+                const int i = i0 + u, t = i * HALVES + half;
+                if (i < rounds) {
                     vm_wait<0>();
-                    __syncthreads();  // tile t landed, and every wave is past tile t - 1
-                    if (t + 1 < nt) issue(tile_k0(t + 1), lb + ((t + 1) & (NS - 1)) * kStage);
-                    if (active(t)) {
+                    __syncthreads();  // round i's tiles landed, and every wave is past round i - 1
+                    if (i + 1 < rounds) copy(i + 1);
+                    if (t < nt && active(t)) {
                         qk(t);
                         softmax(t);
                         pv(t);
@@ -284,13 +296,45 @@ void sink_fwd_kernel(FwdArgs a) {
 
     // O^T through LDS (the ring, free once both groups are past their last tile), stored as whole rows; queries past the
     // length get zeros
+    if constexpr (FORM == kSplit) {
+        // the second half's maximum, sum and outputs (l and o still as the lanes hold them) onto the first's
+        constexpr int kPart = DB * 16 * 64;
+        static_assert((4 * kPart + 8 * 64) * 4 <= NS * HALVES * kStage, "one half's outputs fit");
+        float *x = reinterpret_cast<float *>(lds) + (wave & 3) * kPart + 4 * lane;
+        float *ml = reinterpret_cast<float *>(lds) + 4 * kPart + (wave & 3) * 128 + lane;
+        __syncthreads();
+        if (half) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4 *>(x + (db * 4 + g) * 256) =
+                        f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+            ml[0] = m;
+            ml[64] = l;
+        }
+        __syncthreads();
+        if (half) return;
+        const float m2 = ml[0], top = fmaxf(m, m2), f = exp2_fast(m - top), f2 = exp2_fast(m2 - top);
+        l = l * f + ml[64] * f2;
+        m = top;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(x + (db * 4 + g) * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[db][4 * g + e] = o[db][4 * g + e] * f + v[e] * f2;
+            }
+    }
     constexpr int kPitch = D + 8;
-    static_assert(NW * 32 * kPitch * 2 <= NS * kStage, "staging fits the ring");
+    static_assert(NW / HALVES * 32 * kPitch * 2 <= NS * HALVES * kStage, "staging fits the ring");
     l += swap_halves(l);
     const int q = q0w + j;
     const float inv = q <= last ? 1.0f / l : 0.f;   // (a token sees itself: l > 0)
-    __syncthreads();
-    __bf16 *stg = reinterpret_cast<__bf16 *>(lds) + wave * 32 * kPitch;
+    if constexpr (FORM != kSplit) __syncthreads();
+    else wave_lds_sync();
+    __bf16 *stg = reinterpret_cast<__bf16 *>(lds) + wave * (FORM == kSplit ? DB * 16 * 64 * 2 : 32 * kPitch);
     auto store = [&](const Rows &t, __bf16 *base, auto rounded) {
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -348,18 +392,24 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
     a.rows = (int)(batch * q->heads);
-    const int64_t wide = (tokens + 255) / 256 * a.rows;
-    const bool small = wide < 512;
-    a.qtiles = (int)((tokens + (small ? 127 : 255)) / (small ? 128 : 256));
+    const int64_t paired = (tokens + 255) / 256 * a.rows, fours = (tokens + 127) / 128 * a.rows;
+    const int form = paired >= 512 ? kPaired : fours > 256 ? kFour : kSplit;
+    a.qtiles = (int)(form == kPaired ? (tokens + 255) / 256 : (tokens + 127) / 128);
     a.scale_log2 = scale * kLog2e;
-    auto kernel = lse ? (head_dim == 64 ? (small ? sink_fwd_kernel<64, 4, true> : sink_fwd_kernel<64, 8, true>)
-                                        : (small ? sink_fwd_kernel<128, 4, true> : sink_fwd_kernel<128, 8, true>))
-                      : (head_dim == 64 ? (small ? sink_fwd_kernel<64, 4, false> : sink_fwd_kernel<64, 8, false>)
-                                        : (small ? sink_fwd_kernel<128, 4, false> : sink_fwd_kernel<128, 8, false>));
+    auto pick = [&](auto... kernels) {   // [head_dim 64, 128][form][lse]
+        void (*all[])(FwdArgs) = {kernels...};
+        return all[(head_dim == 64 ? 0 : 6) + 2 * form + (lse ? 1 : 0)];
+    };
+    auto kernel = pick(sink_fwd_kernel<64, kPaired, false>, sink_fwd_kernel<64, kPaired, true>,
+                       sink_fwd_kernel<64, kFour, false>, sink_fwd_kernel<64, kFour, true>,
+                       sink_fwd_kernel<64, kSplit, false>, sink_fwd_kernel<64, kSplit, true>,
+                       sink_fwd_kernel<128, kPaired, false>, sink_fwd_kernel<128, kPaired, true>,
+                       sink_fwd_kernel<128, kFour, false>, sink_fwd_kernel<128, kFour, true>,
+                       sink_fwd_kernel<128, kSplit, false>, sink_fwd_kernel<128, kSplit, true>);
     const int64_t groups = (int64_t)a.qtiles * a.rows;
     for (a.first = 0; a.first < groups; a.first += kLaunchGroups) {
         const int64_t n = groups - a.first < kLaunchGroups ? groups - a.first : kLaunchGroups;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(small ? 256 : 512), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(form == kFour ? 256 : 512), 0, (hipStream_t)stream, a);
     }
     return launch_status(fn);
 }
