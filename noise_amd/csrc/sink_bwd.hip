@@ -40,7 +40,7 @@ __device__ __forceinline__ int seq_len(const BwdArgs &a, int b) {
     return len;
 }
 
-// A tile pair's copies into a stage by 4 waves, rows past `last` taken from it
+// A tile's copies into its half of a stage by 4 waves; `rows` of its rows are there (1 or more), past them the last one is taken
 template <int D>
 struct Copies {
     using TL = Tile<D>;
@@ -52,19 +52,19 @@ struct Copies {
         r0 = TL::RPC * wave + lane / TL::CPR;
         chunk = TL::swb(r0, lane % TL::CPR);
     }
-    __device__ __forceinline__ void one(const Rows &t, const __bf16 *base, int row0, int last, unsigned st) const {
-        if (row0 + kTileRows - 1 > last) {
+    __device__ __forceinline__ void one(const Rows &t, const __bf16 *tile, int rows, unsigned st) const {
+        if (rows < kTileRows) {
 #pragma unroll
             for (int i = 0; i < CPW; ++i) {
                 const int r = i * 4 * TL::RPC + r0;
-                const unsigned rr = (unsigned)(row0 + r > last ? last - row0 : r);
-                lds_dma16_at(base + (int64_t)row0 * t.s_t, rr * (unsigned)t.s_t * 2 + chunk * 16, st + (4 * i + wave) * 1024);
+                lds_dma16_at(tile, (unsigned)(r < rows ? r : rows - 1) * (unsigned)t.s_t * 2 + chunk * 16,
+                             st + (4 * i + wave) * 1024);
             }
         } else {
             const unsigned off = (unsigned)(r0 * (int)t.s_t * 2 + chunk * 16);
+            const int64_t step = 4 * TL::RPC * t.s_t;
 #pragma unroll
-            for (int i = 0; i < CPW; ++i)
-                lds_dma16_at(base + (int64_t)(row0 + i * 4 * TL::RPC) * t.s_t, off, st + (4 * i + wave) * 1024);
+            for (int i = 0; i < CPW; ++i, tile += step) lds_dma16_at(tile, off, st + (4 * i + wave) * 1024);
         }
     }
 };
@@ -180,8 +180,9 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a
         const int t = i * HALVES + half;
         if (t >= nt) return;
         const unsigned st = lb + ((i & 1) * HALVES + half) * CP::kStage;
-        cp.one(a.k, Kb, tile_k0(t), last, st);
-        cp.one(a.v, Vb, tile_k0(t), last, st + CP::kTile);
+        const int k0 = tile_k0(t);
+        cp.one(a.k, Kb + k0 * a.k.s_t, len - k0, st);
+        cp.one(a.v, Vb + k0 * a.v.s_t, len - k0, st + CP::kTile);
     };
     f32x16 dq[DB];
 #pragma unroll
@@ -322,17 +323,37 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     const CP cp(wave, lane);
     const Frags<D> frags(lane);
     const unsigned lb = lds_addr(lds);
-    auto issue = [&](int i) {
-        const int g = i / nq, q0 = (first + i - g * nq) * kTileRows;
+    // the list: query tiles first .. first + nq - 1 of the first head, then of the next; the copies are one tile ahead
+    const int64_t q_step = kTileRows * a.q.s_t, d_step = kTileRows * a.d_o.s_t;
+    int head, tile, q_next;
+    const __bf16 *qp, *dop;
+    const float *sp;
+    auto seek = [&](int g, int t) {
+        head = g;
+        tile = t;
+        q_next = (first + t) * kTileRows;
         const int h = hk * a.group + g;
-        const unsigned st = lb + (i & 1) * CP::kStage;
-        cp.one(a.q, a.q.ptr + b * a.q.s_b + h * a.q.s_h, q0, last, st);
-        cp.one(a.d_o, a.d_o.ptr + b * a.d_o.s_b + h * a.d_o.s_h, q0, last, st + CP::kTile);
+        qp = a.q.ptr + b * a.q.s_b + h * a.q.s_h + (first + t) * q_step;
+        dop = a.d_o.ptr + b * a.d_o.s_b + h * a.d_o.s_h + (first + t) * d_step;
         // waves 0 and 1: -lse / c and -delta of the tile's queries
-        if (wave < 2) {
-            const float *src = (wave ? a.ndelta : a.nlse) + (int64_t)(b * a.heads + h) * a.tokens + q0;
-            lds_dma4_at(src, (unsigned)(q0 + lane > last ? last - q0 : lane) * 4,
+        sp = (wave ? a.ndelta : a.nlse) + (int64_t)(b * a.heads + h) * a.tokens + q_next;
+    };
+    auto issue = [&](int i) {
+        const unsigned st = lb + (i & 1) * CP::kStage;
+        const int rows = len - q_next;
+        cp.one(a.q, qp, rows, st);
+        cp.one(a.d_o, dop, rows, st + CP::kTile);
+        if (wave < 2)
+            lds_dma4_at(sp, (unsigned)(lane < rows ? lane : rows - 1) * 4,
                         lb + 2 * CP::kStage + ((i & 1) * 2 + wave) * kTileRows * 4);
+        if (tile + 1 == nq) {
+            seek(head + 1, 0);
+        } else {
+            ++tile;
+            q_next += kTileRows;
+            qp += q_step;
+            dop += d_step;
+            sp += kTileRows;
         }
     };
     f32x16 dk[DB], dv[DB];
@@ -346,13 +367,15 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     const int all_lo = k0w + 31, all_hi = k0w + 31 > last ? -1 : k0w + W < last ? k0w + W : last;
     const int any_hi = k0w > last ? -1 : k0w < n_sinks || k0w + 31 + W > last ? last : k0w + 31 + W;
     const float c2 = a.scale_log2;
+    seek(i0 / nq, i0 % nq);
+    int q0 = q_next;
     issue(i0);
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
         vm_wait<0>();
         __syncthreads();   // tile i landed, and every wave is past tile i - 1
+        const int q_then = q_next;
         if (i + 1 < i1) issue(i + 1);
-        const int q0 = (first + i % nq) * kTileRows;
         const char *qt = lds + (i & 1) * CP::kStage, *dt = qt + CP::kTile;
         const float *stats = reinterpret_cast<const float *>(lds + 2 * CP::kStage) + (i & 1) * 2 * kTileRows;
 #pragma unroll
@@ -401,6 +424,7 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
                     dk[db] = mfma32x32x16(fr.col(qt, db, 2 * qb + s), g[s], dk[db]);
                 }
         }
+        q0 = q_then;
     }
     if constexpr (KW == 2) {
         // the second wave's sums onto the first's, through LDS

@@ -86,8 +86,7 @@ void sink_fwd_kernel(FwdArgs a) {
     const int nt = sunk + wg_q_hi / kBK - band + 1;
     auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kBK; };
 
-    // copies of 1 KB: c = 4 i + wave % 4 of group A (kPaired) or of a tile's four waves; K's first, then V's
-    constexpr int KC = kTile / 1024;   // copies per K (or V) tile: 8 or 16
+    // copies of 1 KB: c = 4 i + wave % 4 of K's and of V's, by group A (kPaired) or a tile's four waves
     const int crow = lane / TL::CPR, cslot = lane % TL::CPR;
     const bool group_a = wave < 4;
     const unsigned lb = lds_addr(lds);
@@ -97,28 +96,25 @@ void sink_fwd_kernel(FwdArgs a) {
     const int r0 = TL::RPC * (wave & 3) + crow;
     const int kchunk = TL::swz(r0, cslot), vchunk = TL::swt(r0, cslot);
     const unsigned koff = (unsigned)(r0 * a.k.s_t * 2 + kchunk * 16), voff = (unsigned)(r0 * a.v.s_t * 2 + vchunk * 16);
+    const int64_t kstep = 4 * TL::RPC * a.k.s_t, vstep = 4 * TL::RPC * a.v.s_t;
     auto issue = [&](int k0, unsigned st) {
+        const __bf16 *kp = Kb + k0 * a.k.s_t, *vp = Vb + k0 * a.v.s_t;
+        st += (wave & 3) * 1024;
         if (k0 + kBK > len) {
             // the tile with the last token: each lane's row is clamped
 #pragma unroll
-            for (int i = 0; i < CPW; ++i) {
-                const int c = 4 * i + (wave & 3), r = (i * 4 * TL::RPC + r0) % kBK;
+            for (int i = 0; i < CPW / 2; ++i) {
+                const int r = i * 4 * TL::RPC + r0;
                 const unsigned rr = (unsigned)(k0 + r > last ? last - k0 : r);
-                if (c < KC)
-                    lds_dma16_at(Kb + (int64_t)k0 * a.k.s_t, rr * (unsigned)a.k.s_t * 2 + kchunk * 16, st + c * 1024);
-                else
-                    lds_dma16_at(Vb + (int64_t)k0 * a.v.s_t, rr * (unsigned)a.v.s_t * 2 + vchunk * 16, st + c * 1024);
+                lds_dma16_at(kp, rr * (unsigned)a.k.s_t * 2 + kchunk * 16, st + 4 * i * 1024);
+                lds_dma16_at(vp, rr * (unsigned)a.v.s_t * 2 + vchunk * 16, st + kTile + 4 * i * 1024);
             }
             return;
         }
 #pragma unroll
-        for (int i = 0; i < CPW; ++i) {
-            const int c = 4 * i + (wave & 3);
-            if (c < KC)
-                lds_dma16_at(Kb + (int64_t)(k0 + 4 * i * TL::RPC) * a.k.s_t, koff, st + c * 1024);
-            else
-                lds_dma16_at(Vb + (int64_t)(k0 + 4 * i * TL::RPC - kBK) * a.v.s_t, voff, st + c * 1024);
-        }
+        for (int i = 0; i < CPW / 2; ++i, kp += kstep) lds_dma16_at(kp, koff, st + 4 * i * 1024);
+#pragma unroll
+        for (int i = 0; i < CPW / 2; ++i, vp += vstep) lds_dma16_at(vp, voff, st + kTile + 4 * i * 1024);
     };
     // fragment offsets in a stage: K row sigma(j) (+ 32 kb), k-step s; V^T by columns: as a source, lane 16 g + i addresses key
     // 8 (g / 2) + i / 4 (+ 16 s, + 4), dims 16 (g % 2) + 4 (i % 4) .. + 4 (+ 32 db: offset ^ 64 db)
