@@ -232,14 +232,25 @@ __global__ __launch_bounds__(256) void sink_decode_join_kernel(DecodeArgs a) {
     if (at >= a.units / a.blocks * per) return;
     const int row = (int)(at % per), hk = (int)(bk % a.kv_heads);
     const float *p = a.parts + ((bk * a.blocks + row / kRows) * a.splits * kRows + row % kRows) * (D + 2);
+    const int64_t step = (int64_t)kRows * (D + 2);
+    // a lane per part (and every 64th from there): maxima and weights at once, then the sums, several parts in flight
     float top = -1e30f, weight = 0.f, s[D / 64] = {};
-    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, p[(int64_t)i * kRows * (D + 2) + D]);
-    for (int i = 0; i < a.splits; ++i) {
-        const float *x = p + (int64_t)i * kRows * (D + 2), f = exp2_fast(x[D] - top);
-        weight += x[D + 1] * f;
+    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, p[i * step + D]);
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) s[e] += x[lane + 64 * e] * f;
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    for (int i0 = 0; i0 < a.splits; i0 += 64) {
+        const int n = a.splits - i0 < 64 ? a.splits - i0 : 64;
+        const float f = lane < n ? exp2_fast(p[(i0 + lane) * step + D] - top) : 0.f;
+        weight += lane < n ? p[(i0 + lane) * step + D + 1] * f : 0.f;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float fi = __shfl(f, i, 64);
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) s[e] += p[(i0 + i) * step + lane + 64 * e] * fi;
+        }
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) weight += __shfl_xor(weight, o, 64);
     const float inv = 1.f / weight;
     __bf16 *out = a.o.ptr + b * a.o.s_b + row / a.group * a.o.s_t + (hk * a.group + row % a.group) * a.o.s_h;
 #pragma unroll

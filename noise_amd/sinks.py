@@ -24,18 +24,22 @@ FAR = 2 ** 62                # windows from here on are all the same, whatever t
 MAX_NEW = 16                 # new tokens per sequence of one sink_attention_decode call
 
 
-def _check(fn, q, k, *others):
-    """[B, T, H, D] and [B, T', Hk, D] of one device, type and head dim."""
-    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f'{fn}: q and k must be [batch, token, head, dim] of one batch and dim, got '
-                         f'{tuple(q.shape)} and {tuple(k.shape)}')
-    if q.shape[3] not in (64, 128):
-        raise ValueError(f'{fn}: head dim must be 64 or 128, got {q.shape[3]}')
-    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f'{fn}: {q.shape[2]} query heads are no multiple of {k.shape[2]} key heads')
-    for t in (k, *others):
-        if t.device != q.device:
-            raise ValueError(f'{fn}: tensors on {q.device} and {t.device}')
+def _check(fn, q, k, v=None):
+    """(B, T, H, D, T', Hk) of [B, T, H, D] and [B, T', Hk, D] of one device, type and head dim"""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[3] != ks[3]:
+        raise ValueError(f'{fn}: q and k must be [batch, token, head, dim] of one batch and dim, got {tuple(qs)} and '
+                         f'{tuple(ks)}')
+    B, T, H, D = qs
+    _, S, Hk, _ = ks
+    if D != 64 and D != 128:
+        raise ValueError(f'{fn}: head dim must be 64 or 128, got {D}')
+    if Hk == 0 or H == 0 or H % Hk:
+        raise ValueError(f'{fn}: {H} query heads are no multiple of {Hk} key heads')
+    device = q.device
+    if k.device != device or (v is not None and v.device != device):
+        raise ValueError(f'{fn}: tensors on {device}, {k.device}' + (f' and {v.device}' if v is not None else ''))
+    return B, T, H, D, S, Hk
 
 
 def _rows(t):
@@ -66,7 +70,7 @@ def _table(*tensors):
     flat = []
     for t in tensors:
         a, b, c, _ = t.stride()
-        flat += t.data_ptr(), a, b, c, t.shape[2]
+        flat += (t.data_ptr(), a, b, c, t.size(2))
     return _ARRAYS[len(tensors)](*flat)
 
 
@@ -350,22 +354,20 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     the call sees may hold anything. Not differentiable."""
     fn = 'sink_attention_decode'
     window, sinks = min(int(window), FAR), min(int(sinks), FAR)
-    _check(fn, q, k_cache, v_cache)
-    if v_cache.shape != k_cache.shape or k_cache.shape[1] == 0:
+    B, T, H, D, S, Hk = _check(fn, q, k_cache, v_cache)
+    if S == 0 or v_cache.shape != k_cache.shape:
         raise ValueError(f'{fn}: caches must have one shape and some capacity, got {tuple(k_cache.shape)} and '
                          f'{tuple(v_cache.shape)}')
     if q.dtype != BF16 or k_cache.dtype != BF16 or v_cache.dtype != BF16:
         raise ValueError(f'{fn}: bfloat16 tensors, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}')
-    B, T, H, D = q.shape
     if T > MAX_NEW:
         raise ValueError(f'{fn}: at most {MAX_NEW} new tokens, got {T}')
     if window < 0 or sinks < 0:
         raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
     start, wide = _ints(fn, 'start', start, B, q.device)
-    for c in (k_cache, v_cache):
-        _cache_rows(fn, c)
+    _cache_rows(fn, k_cache)
+    _cache_rows(fn, v_cache)
     out = q.new_empty(q.shape)
-    S, Hk = k_cache.shape[1:3]
     need = _decode_workspace(B, T, H, Hk, S, D, window, sinks)
     work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     q = _rows(q)
