@@ -8,6 +8,12 @@
 // by are copied into two LDS stages and read by rows and by columns. The lists of query tiles of the first tokens' keys reach
 // to the end of the sequence, far past the window: a list is cut into parts of a fixed length, each part's sums go to the
 // workspace in fp32 and sink_join_kernel adds them in order.
+//
+// Recomputing the scores in both kernels costs 7 products per pair of which 5 are needed; it keeps dQ out of memory and the
+// order of its sum fixed. Heads of 128 hold 254 registers, two waves per SIMD: matrix cores busy 0.6 of the time in
+// sink_dq_kernel (16384 tokens, 16 heads on 4, window 2048, 4 first tokens: 390 us, 990 TFLOP/s) and 0.45 in
+// sink_dkv_kernel (515 us, 1 PFLOP/s), which waits for its LDS reads between the products. Heads of 64 (8 x 2048 tokens, 8
+// heads, window 1024): 55 us (700 TFLOP/s) and 62 us (830), the vector work on the scores beside the products.
 #include "sink_common.hpp"
 
 namespace noise {
@@ -477,14 +483,14 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     store_block<D>(dv, 1.f, a.dv, dvb, k0w, a.tokens, len, stg, lane);
 }
 
-// Adds the parts of key tiles that have several, in order. grid: (key tiles, rows, blocks of 32 dims of dk, then of dv), a wave
-// per 32 keys, the same registers as above
+// Adds the parts of key tiles that have several, in order. grid: (key tiles times rows, blocks of 32 dims of dk, then of dv), a
+// wave per 32 keys, the same registers as above
 template <int D, int KW>
 __global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band) {
     constexpr int DB = D / 32, kOwn = 32 * KW;
-    const int kt = band ? a.sink_tiles + blockIdx.x : blockIdx.x, row = blockIdx.y;
+    const int kt = (band ? a.sink_tiles : 0) + blockIdx.x / a.rows, row = blockIdx.x % a.rows;
     const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.z / DB, db = blockIdx.z % DB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.y / DB, db = blockIdx.y % DB;
     const int len = seq_len(a, b);
     int first;
     const int total = a.group * query_tiles(a, kt, kOwn, len, &first), parts = (total + a.part - 1) / a.part;
@@ -525,6 +531,9 @@ Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_
     window = window < tokens ? window : tokens;
     sinks = sinks < tokens ? sinks : tokens;
     p.rows = batch * kv_heads;
+    // 64 keys (two waves on each 32, the queries halved between them) where 128 would leave the CUs without a second workgroup:
+    // one sequence of 8192 tokens, 8 heads of 128 on 2, 290 us against 350 for the whole pass; 8 heads of 64, 8 x 2048
+    // tokens (1024 of 128), 127 us with 128 keys, and no less with 64
     p.own = p.rows * ((tokens + 127) / 128) < 1024 ? 64 : 128;
     p.tiles = (tokens + p.own - 1) / p.own;
     p.sink_tiles = (sinks + p.own - 1) / p.own;
@@ -534,6 +543,9 @@ Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_
     const int64_t step = p.own / kTileRows, whole = q_tiles > reach ? (q_tiles - reach) / step + 1 : 0;
     const int64_t full = whole < p.tiles ? whole : p.tiles, tail = p.tiles - full;
     const int64_t steps = p.rows * group * (full * reach + tail * (q_tiles - full * step) - step * (tail * (tail - 1) / 2));
+    // as many parts as make 512 workgroups (two per CU) of them, six tiles or more each: 4096 tokens, 8 heads of 128 on 2,
+    // window 1024 (128 lists): 185 us for the whole pass uncut, 104 in four. Each part's sums are written and read once more,
+    // so lists that come near 512 (544: an odd few over do not matter) stay whole: 280 lists, 121 us whole, 135 in two
     int64_t cut = 544 * band / (steps > 0 ? steps : 1);
     cut = cut < band / 6 ? cut : band / 6;
     cut = cut > 1 ? cut : 1;
@@ -593,7 +605,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
         return st;
     for (const Rows *t : {&a.q, &a.k, &a.v, &a.d_o})
         NOISE_CHECK_ARG(t->s_t >= 0 && t->s_t < kMaxStride, "%s: token strides of q, k, v and d_o must be below 2^25", fn);
-    NOISE_CHECK_ARG(p.rows <= 65535, "%s: at most 65535 sequences times key heads", fn);
+    NOISE_CHECK_ARG(p.rows * p.items < (1 << 30), "%s: too many key tiles", fn);
     a.lse = lse;
     a.nlse = static_cast<float *>(workspace);
     a.ndelta = a.nlse + p.stats / 4;
@@ -614,7 +626,8 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
         }
     };
     a.tiles = (int)((tokens + kOwnQ - 1) / kOwnQ);
-    // no more workgroups than CUs: two halves of the keys for each
+    // no more workgroups than CUs: two halves of the keys for each (4096 tokens, 4 heads of 64, causal: the whole pass 91 us
+    // against 107)
     const bool split = batch * q->heads * a.tiles <= 256;
     launch(narrow ? (split ? sink_dq_kernel<64, true> : sink_dq_kernel<64, false>)
                   : (split ? sink_dq_kernel<128, true> : sink_dq_kernel<128, false>), batch * q->heads, a.tiles, split ? 512 : 256);
@@ -627,7 +640,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
         if (n)
             hipLaunchKernelGGL(narrow ? (small ? sink_join_kernel<64, 2> : sink_join_kernel<64, 4>)
                                       : (small ? sink_join_kernel<128, 2> : sink_join_kernel<128, 4>),
-                               dim3((unsigned)n, (unsigned)p.rows, (unsigned)(head_dim / 32 * 2)),
+                               dim3((unsigned)(n * p.rows), (unsigned)(head_dim / 32 * 2)),
                                dim3(small ? 128 : 256), 0, (hipStream_t)stream, a, band);
     }
     return launch_status(fn);

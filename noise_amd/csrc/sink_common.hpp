@@ -12,6 +12,7 @@ namespace noise {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.4028234663852886e38f;  // a running maximum before the first score
 constexpr int64_t kFar = 1ll << 62;         // sums of a position and a window stay in 64 bits
 constexpr int64_t kLaunchGroups = 1 << 22;  // a launch has fewer than 2^32 threads (a multiple of 8: XCDs do not move)
 constexpr int64_t kMaxStride = 1 << 25;     // token strides that a tile's 32-bit copy offsets span

@@ -7,6 +7,10 @@
 // products are the forward pass's, S^T = K Q^T and O^T += V^T P^T, with up to 32 rows (tokens times query heads of the
 // key head) as the columns. The waves join their sums in LDS; the parts of a list over several workgroups go to the workspace
 // in fp32 and sink_decode_join_kernel adds them up.
+//
+// 64 sequences, 32 heads of 128 on 8, 4100 visible slots each: 184 us, 5.9 TB/s (a large copy runs at 4.9 TB/s here, read and
+// write together). One sequence of 8 heads of 64, 1028 slots: 5.4 us over 72 workgroups and 4.8 us for the join, where the
+// call's host part takes 12 us.
 #include "sink_common.hpp"
 
 namespace noise {
@@ -113,7 +117,7 @@ __global__ __launch_bounds__(64 * kWaves) void sink_decode_kernel(DecodeArgs a) 
     const int kfo = sj * RB + (TL::swz(sj, hf) << 4);
     const int vnb = kTile + vnr * RB + (TL::swt(vnr, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + 8 * (lane & 1);
 
-    float m = -1e30f, l = 0.f;
+    float m = kLowest, l = 0.f;
     f32x16 o[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16{};
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(256) void sink_decode_join_kernel(DecodeArgs a) {
     const float *p = a.parts + ((bk * a.blocks + row / kRows) * a.splits * kRows + row % kRows) * (D + 2);
     const int64_t step = (int64_t)kRows * (D + 2);
     // a lane per part (and every 64th from there): maxima and weights at once, then the sums, several parts in flight
-    float top = -1e30f, weight = 0.f, s[D / 64] = {};
+    float top = kLowest, weight = 0.f, s[D / 64] = {};
     for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, p[i * step + D]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -257,7 +261,8 @@ __global__ __launch_bounds__(256) void sink_decode_join_kernel(DecodeArgs a) {
     for (int e = 0; e < D / 64; ++e) out[lane + 64 * e] = (__bf16)(weight != 0.f ? s[e] * inv : 0.f);
 }
 
-// Workgroups that share a list: enough for two on each of the 256 CUs, of four tiles (one per wave) or more
+// Workgroups that share a list: enough for two on each of the 256 CUs, of four tiles (one per wave) or more. (One workgroup
+// for each list of 1028 slots, 8 in all, took 15 us.)
 int64_t splits_of(int64_t units, int64_t tokens, int64_t slots, int64_t window, int64_t sinks) {
     int64_t most = window < slots && sinks < slots && window + sinks + tokens < slots ? window + sinks + tokens : slots;
     const int64_t useful = (most + kWaves * kKeys - 1) / (kWaves * kKeys), wanted = (512 + units - 1) / units;

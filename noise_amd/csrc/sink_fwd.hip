@@ -8,6 +8,11 @@
 // stages; V^T fragments come from transposing reads of the V tile. The waves work in two groups half a tile apart, one of each
 // on every SIMD, so that one group's softmax (VALU) runs beside the other's products (matrix cores): per barrier group A
 // does S, softmax and O of tile t, group B softmax and O of tile t - 1, then S of tile t.
+//
+// Heads of 128: bound by the matrix products (16384 tokens, 16 heads on 4, window 2048, 4 first tokens: 290 us, 890 TFLOP/s
+// of the visible pairs, 1 PFLOP/s with the tiles' edges; a large bf16 product runs at 1250 here). Heads of 64: by the
+// vector work on the scores and the products together, 58 and 31 % of the cycles (8 x 2048 tokens, 8 heads, window 1024:
+// 44 us, 590 TFLOP/s).
 #include "sink_common.hpp"
 
 namespace noise {
@@ -123,7 +128,7 @@ void sink_fwd_kernel(FwdArgs a) {
     const int vnr = 8 * hf + ((lane & 15) >> 2);
     const int vnb = kTile + vnr * RB + (TL::swt(vnr, 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + 8 * (lane & 1);
 
-    float m = -1e30f, l = 0.f;
+    float m = kLowest, l = 0.f;
     f32x16 o[DB], sc[2];
     bf16x8 pf[4];
 #pragma unroll
@@ -388,6 +393,10 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
     a.rows = (int)(batch * q->heads);
+    // 256-query workgroups where they fill the CUs twice, else smaller ones (us): 8 heads of 64, 4 x 2048 tokens, window 1024
+    // (256 of 256), kPaired 32.0, kFour 28.5; 8 heads of 128, 4096 tokens (256 of 128), kFour 33.0, kSplit 28.3; 4 heads of
+    // 64, 4096 tokens, causal (128 of 128), kPaired 76, kFour 61, kSplit 41. With 16 heads of 128 on 2 x 4096 tokens, causal
+    // (512 of 256), kPaired 143, kFour 154
     const int64_t paired = (tokens + 255) / 256 * a.rows, fours = (tokens + 127) / 128 * a.rows;
     const int form = paired >= 512 ? kPaired : fours > 256 ? kFour : kSplit;
     a.qtiles = (int)(form == kPaired ? (tokens + 255) / 256 : (tokens + 127) / 128);

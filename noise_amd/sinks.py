@@ -225,7 +225,7 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     """q' of qk_norm_rotary for new tokens at positions start[b] + t, with k' and v [B, T, Hk, D] written to those slots of
     k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
     cache or the tables gets zeros in q' and leaves the cache as it is, so an idle sequence has a start of -T; no other
-    slot is touched. Not differentiable (it writes in place)."""
+    slot is touched. k and v must not share memory with the caches. Not differentiable (it writes in place)."""
     fn = 'qk_norm_rotary_append'
     cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
     B, T, H, D = q.shape
@@ -333,8 +333,9 @@ def sink_attention(q, k, v, window, sinks=0, lengths=None):
     """Causal attention in which token i sees the tokens j <= i with i - j <= window or j < sinks, [B, T, H, D] from q
     [B, T, H, D] and k, v [B, T, Hk, D] in bfloat16 (fp32 scores and sums; the weights and, in the backward pass, the scores'
     gradients are rounded to bfloat16 for their products). lengths [B] (int32 or int64): the batch is padded; tokens from
-    lengths[b] on are seen by none, get zeros, have no gradient, and may hold anything. Keys of the sequence itself are
-    taken to be finite. Differentiable in q, k and v (once), with sums in a fixed order."""
+    lengths[b] on are seen by none, get zeros, have no gradient, and may hold anything. Tokens of the sequence itself
+    are taken to be finite, with scores (q . k / sqrt(D)) below 2^28 in size; gradients take the scores' exponents from fp32
+    sums, whose steps are 2^-7 of a weight at scores of 2^15. Differentiable in q, k and v (once), with sums in a fixed order."""
     window, sinks = min(int(window), FAR), min(int(sinks), FAR)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attend.apply(q, k, v, window, sinks, lengths)

@@ -219,3 +219,65 @@ def test_compiled_operator():
         out = f(*leaves)
         results.append((out, *torch.autograd.grad(out, leaves, dout)))
     assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_far_scores():
+    """Scores of 2^27 and their negatives (a single product of powers of two and bf16 values: exact in fp32): the key with the
+    largest, or those that tie for it, take all the weight, and nothing overflows on the way."""
+    from noise_amd.sinks import sink_attention, sink_attention_decode
+    B, T, H, D = 1, 150, 2, 64
+    g = torch.Generator(DEV).manual_seed(1)
+    v = torch.randn(B, T, H, D, device=DEV, generator=g).bfloat16()
+    q = torch.zeros(B, T, H, D, device=DEV, dtype=torch.bfloat16)
+    k = torch.zeros_like(q)
+    q[..., 0] = 2.0 ** 15
+    for sign in (1, -1):
+        k[..., 0] = (sign * 2.0 ** 15 * (1 + torch.arange(T, device=DEV)[None, :, None] / 256)).bfloat16()
+        want, weight = oracle.attend(q, k, v, 60, 3)
+        check(sink_attention(q, k, v, 60, 3), want, U * (weight + want.abs()), 'out')
+        start = torch.tensor([T - 1], device=DEV)
+        check(sink_attention_decode(q[:, -1:], k, v, start, 60, 3), want[:, -1:], (U * (weight + want.abs()))[:, -1:], 'decode')
+
+
+def test_compiled_step():
+    """The operators in a compiled function (forward and backward traced, no graph break) give the eager bits."""
+    from noise_amd.distill import distill_loss
+    from noise_amd.sinks import qk_norm_rotary, sink_attention
+    q, k, v, _ = inputs(2, 64, 4, 2, 64, 13, 4)
+    angle = torch.rand(64, 32, device=DEV)
+    cos, sin = angle.cos(), angle.sin()
+    w = torch.rand(64, device=DEV)
+    t, i = torch.randn(2, 64, 4, 3, device=DEV), torch.randint(0, 64, (2, 64, 4, 3), device=DEV)
+
+    def step(q, k, v, w):
+        q, k = torch.ops.noise_amd.qk_norm_rotary(q, k, cos, sin, w, None, None, 1e-6)
+        out = torch.ops.noise_amd.sink_attention(q, k, v, 20, 2, None)[0]
+        return torch.ops.noise_amd.distill_loss(out, t, i, 64, 1.0, 15.0)
+
+    def plain(q, k, v, w):
+        q, k = qk_norm_rotary(q, k, cos, sin, w, eps=1e-6)
+        return distill_loss(sink_attention(q, k, v, 20, 2), t, i, softcap=15.0)
+
+    results = []
+    for f in (torch.compile(step, backend='aot_eager', fullgraph=True), plain):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, w)]
+        loss = f(*leaves)
+        results.append((loss, *torch.autograd.grad(loss.sum(), leaves)))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+def test_many_sequences():
+    """More sequences than a grid's second dimension holds, each of a few tokens, with cut lists."""
+    B, T = 70000, 3
+    q, k, v, dout = inputs(B, T, 1, 1, 64, 14, 4)
+    from noise_amd.sinks import sink_attention
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sink_attention(*leaves, 1, 1)
+    grads = torch.autograd.grad(out, leaves, dout)
+    some = torch.tensor([0, 1, 65534, 65535, 65536, B - 1], device=DEV)
+    mine = [t[some].detach().requires_grad_() for t in (q, k, v)]
+    part = sink_attention(*mine, 1, 1)
+    want, weight = oracle.attend(q[some], k[some], v[some], 1, 1)
+    check(out[some].detach(), want, U * (weight + want.abs()), 'out')
+    for x, y in zip(grads, torch.autograd.grad(part, mine, dout[some])):
+        assert torch.equal(x[some], y)
