@@ -180,7 +180,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a
     const int nt = sunk + q_hi / kTileRows - band + 1;
     auto tile_k0 = [&](int t) { return (t < sunk ? t : t - sunk + band) * kTileRows; };
     const CP cp(wave & 3, lane);
-    const Frags<D> fr(lane);
+    const Frags<D> frags(lane);
     const unsigned lb = lds_addr(lds);
     auto issue = [&](int i) {
         const int t = i * HALVES + half;
@@ -210,6 +210,9 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a
         const bool causal_edge = k0 + kTileRows - 1 > wq_lo, window_edge = k0 < wq_hi - W;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
+            // (the fragments' addresses are formed anew in each block: kept over the loop, they would push registers out to memory)
+            Frags<D> fr = frags;
+            asm volatile("" : "+v"(fr.rows), "+v"(fr.cols));
             f32x16 sc = f32x16{}, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) dp[r] = nd;
@@ -231,14 +234,27 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a
                     for (int r = 0; r < 16; ++r)
                         sc[r] = (unsigned)(16 * (r >> 3) + (r & 7) - ds) >= wd ? sc[r] : -__builtin_inff();
             }
-            // the scores' gradients rounded to bf16 for the product on the matrix cores
-            bf16x8 g[2];
+            // the scores' gradients as two bf16 each, of 16 bits together: a row's add up to zero, and with keys that have much in
+            // common the roundings of a single one (2^-9 each) would outweigh the result's own (dq's error against 64 bits, 300
+            // keys and 70 first tokens: 3.1e-3 with one, 2.2e-3 with two, 1.7e-3 the rounding of the result alone; a third
+            // more products, 55 -> 67 us at 8 x 2048 tokens, 8 heads of 64)
+            bf16x8 g[2], rest[2];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) g[r >> 3][r & 7] = (__bf16)(exp2_fast(__builtin_fmaf(sc[r], c2, -lse)) * dp[r]);
+            for (int r = 0; r < 16; ++r) {
+                const float x = exp2_fast(__builtin_fmaf(sc[r], c2, -lse)) * dp[r];
+                g[r >> 3][r & 7] = (__bf16)x;
+                rest[r >> 3][r & 7] = (__bf16)(x - (float)(__bf16)x);
+            }
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int db = 0; db < DB; ++db) dq[db] = mfma32x32x16(fr.col(kt, db, 2 * kb + s), g[s], dq[db]);
+                for (int d0 = 0; d0 < DB; d0 += 2) {
+                    const bf16x8 x = fr.col(kt, d0, 2 * kb + s), y = fr.col(kt, d0 + 1, 2 * kb + s);
+                    dq[d0] = mfma32x32x16(x, g[s], dq[d0]);
+                    dq[d0 + 1] = mfma32x32x16(y, g[s], dq[d0 + 1]);
+                    dq[d0] = mfma32x32x16(x, rest[s], dq[d0]);
+                    dq[d0 + 1] = mfma32x32x16(y, rest[s], dq[d0 + 1]);
+                }
         }
     }
     __syncthreads();
@@ -388,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
         for (int x = 0; x < KW / 2; ++x) {
             const int qb = KW == 4 ? x : wave / KW, q = q0 + 32 * qb;
             if (q + 31 < k0w || q > any_hi) continue;
-            // (the fragments' addresses are formed anew in each block: kept over the loop, they would push sums out to memory)
+            // (as in sink_dq_kernel)
             Frags<D> fr = frags;
             asm volatile("" : "+v"(fr.rows), "+v"(fr.cols));
             // register r: query 16 (r / 8) + 8 hf + r % 8. The products accumulate onto -lse / c and -delta
