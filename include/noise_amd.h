@@ -693,6 +693,7 @@ int noise_sink_decode(const noise_heads_t *q, const noise_heads_t *k, const nois
  * and the teacher's `entries` (1 .. 1024) logits t (type `teacher_type`) at indices i (int32, or int64 with index_wide), both [rows]
  * [entries] contiguous,
  *   z = cap(x) / temperature,  cap(x) = softcap tanh(x / softcap) (softcap 0: x),  p = softmax(t / temperature),
+ *   (temperature and softcap 1e-6 .. 1e6)
  *   loss = temperature^2 sum_k p_k (log p_k - log softmax(z)[i_k]),
  * the softmax p over the entries in use: those with an index in 0 .. vocab - 1 and t above -inf. A row without any has loss
  * 0 and gradient 0. An index may stand in several entries. loss: fp32 [rows].

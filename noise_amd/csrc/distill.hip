@@ -6,6 +6,10 @@
 // takes the maximum, the sum, the loss and the gradient from there. Rows past 393 KB do not fit; they are read twice.
 // The teacher's entries go through LDS. Their terms reach the gradient last: an entry's thread writes the whole gradient of
 // its index over what the row's pass left there (summing the entries that share the index, so that they write the same).
+//
+// 16384 fp32 rows of 4096 soft-capped logits, 64 entries, loss and gradient: 122 us (545 MB, 4.5 TB/s, where a large copy runs at
+// 4.9); 4096 bf16 rows of 65536: 251 us (1.08 GB, 4.3 TB/s; 512 threads with twice the chunks 258; streaming stores 242, but
+// 136 us for the former). The loss alone of 100 bf16 rows of 4000: 4.9 us.
 #include "common.hpp"
 #include "mfma.hpp"
 
@@ -256,8 +260,8 @@ extern "C" int noise_distill(const void *x, int type, int64_t rows, int64_t voca
     NOISE_CHECK_ARG(teacher_type == NOISE_BF16 || teacher_type == NOISE_FP32, "%s: unknown teacher type %d", fn, teacher_type);
     NOISE_CHECK_ARG(rows >= 0 && vocab > 0 && vocab <= (1 << 30) && entries > 0 && entries <= kMaxEntries,
                     "%s: rows >= 0, vocab 1 .. 2^30 and entries 1 .. %d required", fn, kMaxEntries);
-    NOISE_CHECK_ARG(temperature > 0.f && temperature < __builtin_inff(), "%s: temperature must be positive", fn);
-    NOISE_CHECK_ARG(softcap >= 0.f && softcap < __builtin_inff(), "%s: softcap must be positive, or 0 for none", fn);
+    NOISE_CHECK_ARG(temperature >= 1e-6f && temperature <= 1e6f, "%s: temperature must be 1e-6 .. 1e6", fn);
+    NOISE_CHECK_ARG(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e6f), "%s: softcap must be 1e-6 .. 1e6, or 0 for none", fn);
     if (rows == 0) return NOISE_OK;
     NOISE_CHECK_ARG(x && teacher && index && loss, "%s: NULL pointer", fn);
     const size_t size = type == NOISE_BF16 ? 2 : 4;

@@ -32,7 +32,8 @@ struct BwdArgs {
     int wide, tokens, heads, kv_heads, group, window, sinks;
     int tiles;                       // of queries (dq) or keys (dk, dv)
     int rows;                        // batch * heads (dq) or batch * kv_heads (dk, dv)
-    int sink_tiles, sink_parts, band_parts, part;  // key tiles with first tokens; most parts of each kind; tiles per part
+    int sink_tiles, sink_parts, band_parts;  // key tiles with first tokens; most parts of each kind
+    int sink_part, part;             // query tiles per part of each kind
     float scale, scale_log2;
 };
 
@@ -309,14 +310,14 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
     // got all long parts would hold up the ones that follow
     const int ns = a.sink_tiles * a.sink_parts, bands = a.tiles - a.sink_tiles;
     const int kt = item < ns ? item % a.sink_tiles : a.sink_tiles + (item - ns) % bands;
-    const int part = item < ns ? item / a.sink_tiles : (item - ns) / bands;
+    const int part = item < ns ? item / a.sink_tiles : (item - ns) / bands, size = item < ns ? a.sink_part : a.part;
     const int b = row / a.kv_heads, hk = row - b * a.kv_heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 31, hf = lane >> 5;
     const int kw = wave % KW;
     const int len = seq_len(a, b), last = len - 1, k0w = kt * kOwn + 32 * kw;
     int first;
-    const int nq = query_tiles(a, kt, kOwn, len, &first), total = a.group * nq, parts = (total + a.part - 1) / a.part;
+    const int nq = query_tiles(a, kt, kOwn, len, &first), total = a.group * nq, parts = (total + size - 1) / size;
     __bf16 *dkb = a.dk.ptr + b * a.dk.s_b + hk * a.dk.s_h, *dvb = a.dv.ptr + b * a.dv.s_b + hk * a.dv.s_h;
     if (part >= parts) {
         if (parts == 0 && part == 0) {
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void sink_dkv_kernel(BwdArgs a) {
         }
         return;
     }
-    const int i0 = part * a.part, i1 = i0 + a.part < total ? i0 + a.part : total;
+    const int i0 = part * size, i1 = i0 + size < total ? i0 + size : total;
     bf16x8 kf[KS], vf[KS];
     {
         const int key = k0w + j < last ? k0w + j : last;
@@ -509,7 +510,8 @@ __global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.y / DB, db = blockIdx.y % DB;
     const int len = seq_len(a, b);
     int first;
-    const int total = a.group * query_tiles(a, kt, kOwn, len, &first), parts = (total + a.part - 1) / a.part;
+    const int total = a.group * query_tiles(a, kt, kOwn, len, &first), size = band ? a.part : a.sink_part;
+    const int parts = (total + size - 1) / size;
     if (parts < 2) return;
     const int ns = a.sink_tiles * a.sink_parts;
     const int item = kt < a.sink_tiles ? kt : ns + kt - a.sink_tiles;
@@ -535,10 +537,10 @@ __global__ __launch_bounds__(64 * KW) void sink_join_kernel(BwdArgs a, int band)
     }
 }
 
-// How the lists of query tiles are cut: parts of `part` tiles, at most sink_parts of a key tile with first tokens and
-// band_parts of the others.
+// How the lists of query tiles are cut: a key tile with first tokens into at most sink_parts of sink_part tiles, the others into
+// at most band_parts of `part`.
 struct Plan {
-    int64_t own, tiles, rows, sink_tiles, sink_parts, band_parts, part, items;
+    int64_t own, tiles, rows, sink_tiles, sink_parts, band_parts, sink_part, part, items;
     int64_t stats, bytes;
 };
 Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t window, int64_t sinks) {
@@ -567,11 +569,16 @@ Plan plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_
     cut = cut > 1 ? cut : 1;
     p.part = (band + cut - 1) / cut;
     p.band_parts = p.sink_tiles < p.tiles ? (band + p.part - 1) / p.part : 0;
-    p.sink_parts = p.sink_tiles ? (group * q_tiles + p.part - 1) / p.part : 0;
+    // as long as the others' parts, or longer where many first tokens would make more than 1024 of them
+    const int64_t least = (p.rows * p.sink_tiles * group * q_tiles + 1023) / 1024;
+    p.sink_part = p.part > least ? p.part : least;
+    p.sink_parts = p.sink_tiles ? (group * q_tiles + p.sink_part - 1) / p.sink_part : 0;
     p.items = p.sink_tiles * p.sink_parts + (p.tiles - p.sink_tiles) * p.band_parts;
     p.stats = (batch * heads * tokens * 4 + 15) / 16 * 16;
     p.bytes = 2 * p.stats;
-    if (p.sink_parts > 1 || p.band_parts > 1) p.bytes += p.items * p.rows * p.own * head_dim * 2 * 4;
+    // (the first tokens' items come first: whole lists after them need no room)
+    const int64_t held = p.band_parts > 1 ? p.items : p.sink_parts > 1 ? p.sink_tiles * p.sink_parts : 0;
+    p.bytes += held * p.rows * p.own * head_dim * 2 * 4;
     return p;
 }
 
@@ -631,7 +638,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
     a.sink_tiles = (int)p.sink_tiles; a.sink_parts = (int)p.sink_parts; a.band_parts = (int)p.band_parts;
-    a.part = (int)p.part;
+    a.part = (int)p.part; a.sink_part = (int)(p.sink_part < INT32_MAX / 2 ? p.sink_part : INT32_MAX / 2);
     a.scale = scale; a.scale_log2 = scale * kLog2e;
     const bool narrow = head_dim == 64;
     auto launch = [&](void (*kernel)(BwdArgs), int64_t rows, int64_t items, int threads) {

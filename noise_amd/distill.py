@@ -21,10 +21,10 @@ def _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, sof
     vocab = width if vocab is None else int(vocab)
     if not 0 < vocab <= width:
         raise ValueError(f'{fn}: vocab must be 1 .. {width}, got {vocab}')
-    if not temperature > 0:
-        raise ValueError(f'{fn}: temperature must be positive, got {temperature}')
-    if softcap is not None and not softcap > 0:
-        raise ValueError(f'{fn}: softcap must be positive (None: no cap), got {softcap}')
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f'{fn}: temperature must be 1e-6 .. 1e6, got {temperature}')
+    if softcap is not None and not 1e-6 <= softcap <= 1e6:
+        raise ValueError(f'{fn}: softcap must be 1e-6 .. 1e6 (None: no cap), got {softcap}')
     if teacher_logits.shape != teacher_index.shape or teacher_logits.shape[:-1] != shape or teacher_logits.shape[-1] == 0:
         raise ValueError(f'{fn}: teacher logits and indices must be [{", ".join(map(str, shape))}, entries], got '
                          f'{tuple(teacher_logits.shape)} and {tuple(teacher_index.shape)}')

@@ -239,6 +239,10 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
             raise ValueError(f'{fn}: caches must be [{B}, capacity, {k.shape[2]}, {D}] {k.dtype} on {k.device}, got '
                              f'{tuple(c.shape)} {c.dtype} on {c.device}')
         _cache_rows(fn, c)
+        if 0 in c.stride() and any(s == 0 and n > 1 for s, n in zip(c.stride(), c.shape)):
+            raise ValueError(f'{fn}: a broadcast cache has no slots of its own to write to')
+    if k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError(f'{fn}: k_cache and v_cache are the same memory')
     out = q.new_empty(q.shape)
     q, k, v = _rows(q), _rows(k), _rows(v)
     t = _table(q, k, out, k_cache, v, v_cache)

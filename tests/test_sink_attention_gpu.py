@@ -65,6 +65,8 @@ def test_masks(window, sinks, D):
 @pytest.mark.parametrize('D', [64, 128])
 def test_a_long_sequence(D):
     check_all(*inputs(1, 2100, 4, 2, D, 1, 4), 300, 70)
+    check_all(*inputs(1, 2100, 4, 1, D, 1, 4), 3, 1500)
+    check_all(*inputs(1, 2100, 2, 2, D, 1, 4), 10, 1)
 
 
 @pytest.mark.parametrize('wide', [torch.int32, torch.int64])

@@ -63,7 +63,9 @@ def test_norm_refusals():
                         ((q, k, v, cos, sin, cache, cache.float(), start), 'caches must be'),
                         ((q, k, v, cos, sin, odd, cache, start), 'cache rows'),
                         ((q, k, v, cos, sin, cache, cache, None), 'start is required'),
-                        ((q, k, v, cos, sin, cache, cache, start), 'on a GPU')):
+                        ((q, k, v, cos, sin, cache[:1].expand(2, 9, 2, 64), cache, start), 'broadcast'),
+                        ((q, k, v, cos, sin, cache, cache, start), 'same memory'),
+                        ((q, k, v, cos, sin, cache, cache.clone(), start), 'on a GPU')):
         with pytest.raises(ValueError, match=words):
             sinks.qk_norm_rotary_append(*args)
 
@@ -75,7 +77,7 @@ def test_distill_refusals():
                               ((x, t.repeat(1, 257), i.repeat(1, 257)), {}, 'at most 1024'), ((x, t, i.float()), {}, 'int32 or int64'), ((x, t.double(), i), {}, 'teacher logits'),
                               ((x, t, i), dict(vocab=11), 'vocab'), ((x, t, i), dict(vocab=0), 'vocab'),
                               ((x, t, i), dict(temperature=0.0), 'temperature'),
-                              ((x, t, i), dict(temperature=math.nan), 'temperature'),
+                              ((x, t, i), dict(temperature=math.nan), 'temperature'), ((x, t, i), dict(temperature=math.inf), 'temperature'),
                               ((x, t, i), dict(softcap=0.0), 'softcap'), ((x, t, i), dict(softcap=-1.0), 'softcap'),
                               ((x, t, i), {}, 'on a GPU')):
         with pytest.raises(ValueError, match=words):
@@ -112,6 +114,10 @@ def test_entry_points_refuse():
     refused(bwd(16, 8), 'workspace')
     refused(bwd(None, 1 << 40), 'workspace')
     refused(lib.noise_sink_attention_bwd_workspace_bytes(1, 5, 3, 2, 64, 3, 0), 'key heads')
+    # first tokens all over a long sequence do not cut its lists into ever more parts
+    for sinks in (0, 4, 1000, 16384):
+        assert 0 < lib.noise_sink_attention_bwd_workspace_bytes(8, 16384, 64, 64, 128, 0, sinks) < 1 << 30
+        assert 0 < lib.noise_sink_attention_bwd_workspace_bytes(1, 1 << 22, 8, 1, 64, 100, sinks) < 1 << 30
     dec = lambda T=1, start=16, S=9, ws=None: lib.noise_sink_decode(*h[:4], start, 0, 1, T, S, 64, 3, 0, 0.1, ws, 0, None)
     refused(dec(T=17), '16')
     refused(dec(start=None), 'start')
