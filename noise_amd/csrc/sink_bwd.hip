@@ -9,11 +9,11 @@
 // to the end of the sequence, far past the window: a list is cut into parts of a fixed length, each part's sums go to the
 // workspace in fp32 and sink_join_kernel adds them in order.
 //
-// Recomputing the scores in both kernels costs 7 products per pair of which 5 are needed; it keeps dQ out of memory and the
-// order of its sum fixed. Heads of 128 hold 254 registers, two waves per SIMD: matrix cores busy 0.6 of the time in
-// sink_dq_kernel (16384 tokens, 16 heads on 4, window 2048, 4 first tokens: 390 us, 990 TFLOP/s) and 0.45 in
-// sink_dkv_kernel (515 us, 1 PFLOP/s), which waits for its LDS reads between the products. Heads of 64 (8 x 2048 tokens, 8
-// heads, window 1024): 55 us (700 TFLOP/s) and 62 us (830), the vector work on the scores beside the products.
+// Recomputing the scores in both kernels costs 8 products per pair where 5 would do (dQ's takes two); it keeps dQ's partial
+// sums out of memory and their order fixed. Heads of 128 hold 250 registers, two waves per SIMD. 16384 tokens, 16 heads of 128
+// on 4, window 2048, 4 first tokens: sink_dq_kernel 510 us (1.0 PFLOP/s), sink_dkv_kernel 510 us (1.0 PFLOP/s), matrix
+// cores busy 0.45 to 0.5 of the time and the waves waiting for LDS reads between the products. 8 x 2048 tokens, 8 heads of 64,
+// window 1024: 67 us (770 TFLOP/s) and 62 us (830), with the vector work on the scores beside the products.
 #include "sink_common.hpp"
 
 namespace noise {
