@@ -9,7 +9,7 @@ torch.ops.noise_amd operators too.
 import torch
 
 from . import _lib
-from .sinks import F32, TYPES, _call
+from .sinks import F32, TYPES, _call, _new
 
 MAX_ENTRIES = 1024
 
@@ -53,7 +53,7 @@ def distill(fn, logits, teacher_logits, teacher_index, weight, vocab, temperatur
         if weight.dtype != F32 or not weight.is_contiguous():
             weight = weight.to(F32).contiguous()
     loss = x.new_empty(logits.shape[:-1], dtype=F32)
-    grad = x.new_empty(logits.shape) if with_grad else None
+    grad = _new(logits) if with_grad else None
     if rows:
         _call('noise_distill', x.device, x.data_ptr(), TYPES[x.dtype], rows, vocab, x.stride(0), t.data_ptr(),
               TYPES[t.dtype], i.data_ptr(), int(i.dtype == torch.int64), t.shape[-1], _lib.ptr(weight),

@@ -10,8 +10,8 @@ keys' (query head h reads key head h // (H // Hk)). The norm and rotation are th
 88-94 (rotated halves; without learned weights the rotation and the norm commute), the mask that of utils/model.py:17-21
 with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators for compiled callers.
 """
-import ctypes
 import functools
+from array import array
 
 import torch
 
@@ -61,20 +61,25 @@ def _cache_rows(fn, c):
         raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
 
 
-_ARRAYS = [ctypes.c_int64 * (5 * n) for n in range(10)]
 _HEADS = 5 * 8   # bytes of a noise_heads_t: five 64-bit numbers
 
 
-def _table(*tensors):
-    """noise_heads_t of each tensor, in a row: byref(table, i * _HEADS) is that of the i-th"""
+def _table(*tensors, pointers=()):
+    """noise_heads_t of each tensor, one after the other, then the tensors' or None's addresses in `pointers`; and the address of
+    the first (the array holds them for as long as it lives)"""
     flat = []
     for t in tensors:
         a, b, c, _ = t.stride()
         flat += (t.data_ptr(), a, b, c, t.size(2))
-    return _ARRAYS[len(tensors)](*flat)
+    for t in pointers:
+        flat.append(0 if t is None else t.data_ptr())
+    table = array('q', flat)
+    return table, table.buffer_info()[0]
 
 
-_PAIR = ctypes.c_void_p * 2
+def _new(t):
+    """an uninitialised contiguous tensor like t"""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _call(name, device, *args):
@@ -119,7 +124,7 @@ def _weight(fn, w, D, device):
         return None
     if w.shape != (D,) or w.device != device:
         raise ValueError(f'{fn}: weights must be [{D}] on {device}, got {tuple(w.shape)} on {w.device}')
-    return _plain(w.detach())
+    return _plain(w)
 
 
 def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
@@ -143,11 +148,11 @@ def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
 def _norm_forward(q, k, cos, sin, qw, kw, start, wide, eps):
     """qk_norm_rotary of checked operands"""
     B, T, _, D = q.shape
-    out = q.new_empty(q.shape), k.new_empty(k.shape)
-    x = _rows(q), _rows(k)   # (copies among them live until the launch)
-    t = _table(*x, *out)
-    _call('noise_qk_norm_rotary', q.device, t, ctypes.byref(t, 2 * _HEADS), _PAIR(_lib.ptr(qw), _lib.ptr(kw)), None, None,
-          cos.data_ptr(), sin.data_ptr(), cos.shape[0], _lib.ptr(start), wide, B, T, 0, D, TYPES[q.dtype], eps)
+    out = _new(q), _new(k)
+    x = _rows(q), _rows(k)   # (copies among them, and the table, live until the launch)
+    table, at = _table(*x, *out, pointers=(qw, kw))
+    _call('noise_qk_norm_rotary', q.device, at, at + 2 * _HEADS, at + 4 * _HEADS, None, None, cos.data_ptr(),
+          sin.data_ptr(), cos.size(0), None if start is None else start.data_ptr(), wide, B, T, 0, D, TYPES[q.dtype], eps)
     return out
 
 
@@ -160,18 +165,18 @@ def _norm_backward(dq, dk, q, k, cos, sin, qw, kw, start, wide, eps):
     """Gradients of q, k and (fp32; None for absent ones) of the weights, of checked operands"""
     B, T, _, D = q.shape
     dt = q.dtype
-    dx = q.new_empty(q.shape), k.new_empty(k.shape)
+    dx = _new(q), _new(k)
     x = _rows(q), _rows(k), _rows(dq if dq.dtype == dt else dq.to(dt)), _rows(dk if dk.dtype == dt else dk.to(dt))
-    t = _table(*x, *dx)
     need, work, dqw, dkw = 0, None, None, None
     if qw is not None or kw is not None:
         need = _norm_workspace(D)
         work = q.new_empty(need, dtype=torch.uint8)
-        dqw = None if qw is None else qw.new_empty(D)
-        dkw = None if kw is None else kw.new_empty(D)
-    _call('noise_qk_norm_rotary_bwd', q.device, t, ctypes.byref(t, 2 * _HEADS), ctypes.byref(t, 4 * _HEADS),
-          _PAIR(_lib.ptr(qw), _lib.ptr(kw)), _PAIR(_lib.ptr(dqw), _lib.ptr(dkw)), cos.data_ptr(), sin.data_ptr(),
-          cos.shape[0], _lib.ptr(start), wide, B, T, D, TYPES[dt], eps, _lib.ptr(work), need)
+        dqw = None if qw is None else torch.empty_like(qw)
+        dkw = None if kw is None else torch.empty_like(kw)
+    table, at = _table(*x, *dx, pointers=(qw, kw, dqw, dkw))
+    _call('noise_qk_norm_rotary_bwd', q.device, at, at + 2 * _HEADS, at + 4 * _HEADS, at + 6 * _HEADS,
+          at + 6 * _HEADS + 16, cos.data_ptr(), sin.data_ptr(), cos.size(0), None if start is None else start.data_ptr(), wide,
+          B, T, D, TYPES[dt], eps, None if work is None else work.data_ptr(), need)
     return dx[0], dx[1], dqw, dkw
 
 
@@ -197,7 +202,7 @@ class _Norm(torch.autograd.Function):
         # (what the kernels take is saved: the tensors themselves, or the fp32 copies made of them)
         ctx.save_for_backward(q, k, cos, sin, qw, kw, start)
         ctx.more = wide, eps
-        ctx.types = tuple(None if w is None else w.dtype for w in (q_weight, k_weight))
+        ctx.types = None if q_weight is None else q_weight.dtype, None if k_weight is None else k_weight.dtype
         return _norm_forward(q, k, cos, sin, qw, kw, start, wide, eps)
 
     @staticmethod
@@ -243,12 +248,11 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
             raise ValueError(f'{fn}: a broadcast cache has no slots of its own to write to')
     if k_cache.data_ptr() == v_cache.data_ptr():
         raise ValueError(f'{fn}: k_cache and v_cache are the same memory')
-    out = q.new_empty(q.shape)
+    out = _new(q)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    t = _table(q, k, out, k_cache, v, v_cache)
-    _call('noise_qk_norm_rotary', q.device, t, ctypes.byref(t, 2 * _HEADS), _PAIR(_lib.ptr(qw), _lib.ptr(kw)),
-          ctypes.byref(t, 4 * _HEADS), ctypes.byref(t, 5 * _HEADS), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-          start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
+    table, at = _table(q, k, out, k_cache, v, v_cache, pointers=(qw, kw))
+    _call('noise_qk_norm_rotary', q.device, at, at + 2 * _HEADS, at + 6 * _HEADS, at + 4 * _HEADS, at + 5 * _HEADS,
+          cos.data_ptr(), sin.data_ptr(), cos.size(0), start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
     return out
 
 
@@ -270,21 +274,15 @@ def _attend_operands(fn, q, k, v, window, sinks, lengths):
 def _attend_forward(q, k, v, window, sinks, lengths, wide, training):
     """(out, what its rounding left out or None, lse or None) of checked operands"""
     B, T, H, D = q.shape
-    out, rest, lse = q.new_empty(q.shape), None, None
+    out, rest, lse = _new(q), None, None
     q, k, v = _rows(q), _rows(k), _rows(v)
     if training:
-        rest, lse = q.new_empty(out.shape), q.new_empty((B, H, T), dtype=F32)
-        t = _table(q, k, v, out, rest)
-        ref = ctypes.byref(t, 4 * _HEADS)
-    else:
-        t, ref = _table(q, k, v, out), None
-    _call('noise_sink_attention_fwd', q.device, *_parts(t, 0, 4), ref, _lib.ptr(lse), _lib.ptr(lengths), wide, B, T, D,
-          window, sinks, D ** -0.5)
+        rest, lse = torch.empty_like(out), q.new_empty((B, H, T), dtype=F32)
+    table, at = _table(q, k, v, out, *((rest,) if training else ()))
+    _call('noise_sink_attention_fwd', q.device, at, at + _HEADS, at + 2 * _HEADS, at + 3 * _HEADS,
+          at + 4 * _HEADS if training else None, lse.data_ptr() if training else None,
+          None if lengths is None else lengths.data_ptr(), wide, B, T, D, window, sinks, D ** -0.5)
     return out, rest, lse
-
-
-def _parts(table, first, end):
-    return [ctypes.byref(table, i * _HEADS) for i in range(first, end)]
 
 
 @functools.lru_cache(maxsize=1024)
@@ -294,14 +292,14 @@ def _attend_workspace(*sizes):
 
 def _attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths, wide):
     B, T, H, D = q.shape
-    grads = [x.new_empty(x.shape) for x in (q, k, v)]
+    grads = [_new(q), _new(k), _new(v)]
     x = _rows(q), _rows(k), _rows(v), _rows(out), rest, _rows(dout if dout.dtype == BF16 else dout.to(BF16))
-    t = _table(*x, *grads)
-    need = _attend_workspace(B, T, H, k.shape[2], D, window, sinks)
+    table, at = _table(*x, *grads)
+    need = _attend_workspace(B, T, H, k.size(2), D, window, sinks)
     work = q.new_empty(max(need, 0), dtype=torch.uint8)
-    refs = _parts(t, 0, 9)
-    _call('noise_sink_attention_bwd', q.device, *refs[:6], lse.data_ptr(), *refs[6:], _lib.ptr(lengths), wide, B, T, D, window,
-          sinks, D ** -0.5, work.data_ptr(), need)
+    _call('noise_sink_attention_bwd', q.device, *range(at, at + 6 * _HEADS, _HEADS), lse.data_ptr(),
+          *range(at + 6 * _HEADS, at + 9 * _HEADS, _HEADS), None if lengths is None else lengths.data_ptr(), wide, B, T, D,
+          window, sinks, D ** -0.5, work.data_ptr(), need)
     return grads
 
 
@@ -372,11 +370,11 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     start, wide = _ints(fn, 'start', start, B, q.device)
     _cache_rows(fn, k_cache)
     _cache_rows(fn, v_cache)
-    out = q.new_empty(q.shape)
+    out = _new(q)
     need = _decode_workspace(B, T, H, Hk, S, D, window, sinks)
     work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     q = _rows(q)
-    t = _table(q, k_cache, v_cache, out)
-    _call('noise_sink_decode', q.device, t, *_parts(t, 1, 4), start.data_ptr(), wide, B, T, S, D, window, sinks, D ** -0.5,
-          _lib.ptr(work), need)
+    table, at = _table(q, k_cache, v_cache, out)
+    _call('noise_sink_decode', q.device, at, at + _HEADS, at + 2 * _HEADS, at + 3 * _HEADS, start.data_ptr(), wide, B, T, S, D,
+          window, sinks, D ** -0.5, None if work is None else work.data_ptr(), need)
     return out
