@@ -12,7 +12,7 @@
 // Heads of 128: bound by the matrix products (16384 tokens, 16 heads on 4, window 2048, 4 first tokens: 290 us, 890 TFLOP/s
 // of the visible pairs, 1 PFLOP/s with the tiles' edges; a large bf16 product runs at 1250 here). Heads of 64: by the
 // vector work on the scores and the products together, 58 and 31 % of the cycles (8 x 2048 tokens, 8 heads, window 1024:
-// 44 us, 590 TFLOP/s).
+// 43 us, 600 TFLOP/s; 47 us with what the backward pass needs).
 #include "sink_common.hpp"
 
 namespace noise {
@@ -31,9 +31,8 @@ struct FwdArgs {
     float scale_log2;
 };
 
-// FORM: kPaired, as above, 256 queries by 8 waves; for fewer workgroups than the CUs hold at a time, kFour, 128 queries by 4
-// waves and two stages, and for no more than there are CUs, kSplit, 128 queries by 8 waves, every second tile by either half,
-// which are joined in LDS.
+// FORM: kPaired, as above, 256 queries by 8 waves, for long windows; kFour, 128 queries by 4 waves and two stages; for no more
+// workgroups than there are CUs, kSplit, 128 queries by 8 waves, every second tile by either half, which are joined in LDS.
 // TRAIN: with what the backward pass needs beside o, the rows' lse and o's own rounding error. The backward pass forms
 // dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (2^-9 of o) would drown it. With o and its
 // error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is left
@@ -393,12 +392,14 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.window = (int)(window < tokens ? window : tokens);
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
     a.rows = (int)(batch * q->heads);
-    // 256-query workgroups where they fill the CUs twice, else smaller ones (us): 8 heads of 64, 4 x 2048 tokens, window 1024
-    // (256 of 256), kPaired 32.0, kFour 28.5; 8 heads of 128, 4096 tokens (256 of 128), kFour 33.0, kSplit 28.3; 4 heads of
-    // 64, 4096 tokens, causal (128 of 128), kPaired 76, kFour 61, kSplit 41. With 16 heads of 128 on 2 x 4096 tokens, causal
-    // (512 of 256), kPaired 143, kFour 154
+    // 256-query workgroups where they fill the CUs twice and their windows are long, else smaller ones, which have less to do
+    // past the window's edges (us): 16 heads of 128 on 4 x 4096 tokens, window 1024, kPaired 160, kFour 150; 8 heads of 64,
+    // 8 x 2048 tokens, window 1024, 48.4 and 46.4; 16 x 2048 tokens, causal, 99 and 104; 16 heads of 128, 2 x 4096 tokens,
+    // causal, 141 and 153. With fewer: 8 heads of 64, 4 x 2048 tokens, window 1024 (256 of 256), kPaired 32.9, kFour
+    // 28.3; 8 heads of 128, 4096 tokens (256 of 128), kFour 33.0, kSplit 28.3; 4 heads of 64, 4096 tokens, causal (128 of
+    // 128), kPaired 76, kFour 61, kSplit 41
     const int64_t paired = (tokens + 255) / 256 * a.rows, fours = (tokens + 127) / 128 * a.rows;
-    const int form = paired >= 512 ? kPaired : fours > 256 ? kFour : kSplit;
+    const int form = paired >= 512 && a.window >= 2048 ? kPaired : fours > 256 ? kFour : kSplit;
     a.qtiles = (int)(form == kPaired ? (tokens + 255) / 256 : (tokens + 127) / 128);
     a.scale_log2 = scale * kLog2e;
     auto pick = [&](auto... kernels) {   // [head_dim 64, 128][form][lse]

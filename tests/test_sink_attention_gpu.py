@@ -160,6 +160,31 @@ def test_gradients_of_weights_close_to_one(D):
             assert rel <= 3 * 2.0 ** -9
 
 
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('B,T,window,padded', [(8, 2500, 2100, False), (32, 1100, 200, False), (32, 1100, 200, True)])
+def test_enough_rows(B, T, window, padded, D):
+    """Rows enough for the larger workgroups (256 queries with a long window, 128 keys), lengths off their tiles, first tokens past
+    the window; against the 64-bit definition on some heads of some sequences."""
+    from noise_amd.sinks import sink_attention
+    q, k, v, dout = inputs(B, T, 8, 4, D, 21, 4)
+    lengths = torch.tensor([(T, 700, 0, 129)[b % 4] for b in range(B)], device=DEV) if padded else None
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sink_attention(*leaves, window, 70, lengths)
+    plain = sink_attention(q, k, v, window, 70, lengths)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for b, h in ((0, 0), (5, 3), (2, 1), (7, 2)):
+        heads = [t[b:b + 1, :, 2 * h:2 * h + 2] for t in (q, dout)]
+        kv = [t[b:b + 1, :, h:h + 1] for t in (k, v)]
+        n = None if lengths is None else lengths[b:b + 1]
+        want, weight = oracle.attend(heads[0], *kv, window, 70, n)
+        for got in (out.detach(), plain):
+            check(got[b:b + 1, :, 2 * h:2 * h + 2], want, U * (weight + want.abs()), 'out')
+        wants, bounds = oracle.attend_grads(heads[0], *kv, heads[1], window, 70, n)
+        check(grads[0][b:b + 1, :, 2 * h:2 * h + 2], wants[0], bounds[0], 'dq')
+        for i in (1, 2):
+            check(grads[i][b:b + 1, :, h:h + 1], wants[i], bounds[i], 'dk, dv')
+
+
 def test_growing_scores():
     """Scores far apart, and rows whose largest weight stands in the last tile or the first key."""
     q, k, v, dout = inputs(1, 400, 2, 2, 64, 8, 4)
