@@ -618,7 +618,8 @@ int noise_update_gradients(const noise_update_param_t *params, int nparams, int6
  * ---------------------------------------------------------------------------------------------- */
 
 /* A [batch, tokens, heads, dim] tensor: element (b, t, h, d) at ptr + b*s_b + t*s_t + h*s_h + d (strides in elements).
- * Rows of 16 B: ptr 16 B aligned, strides multiples of 16 B. */
+ * Rows of 16 B: ptr 16 B aligned, strides multiples of 16 B. Tensors that sink_attention's kernels copy tile by tile (q, k, v and d_o
+ * of the backward pass, k and v of the forward) have less than 2^25 elements from token to token; caches have no such limit. */
 typedef struct {
     void *ptr;
     int64_t s_b, s_t, s_h, heads;

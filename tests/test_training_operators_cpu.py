@@ -178,3 +178,31 @@ def test_oracles():
     loss, grad = distill_oracle.distill(x, t, i, 12, 2.0, 15.0)
     auto, = torch.autograd.grad(loss.sum(), x)
     assert torch.allclose(grad, auto, atol=1e-12) and loss[2] == 0 and (grad[2] == 0).all()
+
+
+def test_tensor_tables_match_the_header(tmp_path):
+    """noise_heads_t as a C compiler lays it out, as ctypes mirrors it and as the calls pack it: five 64-bit numbers."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    q = torch.zeros(3, 5, 7, 64, dtype=BF16)[:, :, 1:]
+    w = torch.zeros(64)
+    table, at = sinks._table(q, q[:, 2:], pointers=(None, w))
+    assert ctypes.sizeof(_lib.Heads) == sinks._HEADS == 40
+    for i, t in enumerate((q, q[:, 2:])):
+        h = _lib.Heads.from_address(at + i * sinks._HEADS)
+        assert (h.ptr, h.s_b, h.s_t, h.s_h, h.heads) == (t.data_ptr(), *t.stride()[:3], 6)
+    assert list((ctypes.c_int64 * 2).from_address(at + 2 * sinks._HEADS)) == [0, w.data_ptr()] and len(table) == 12
+    gcc = shutil.which('gcc')
+    if gcc is None:
+        pytest.skip('gcc not available')
+    fields = [n for n, _ in _lib.Heads._fields_]
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "noise_amd.h"', 'int main(void) {',
+             '    printf("%zu", sizeof(noise_heads_t));']
+    lines += [f'    printf(" %zu", offsetof(noise_heads_t, {n}));' for n in fields]
+    (tmp_path / 'layout.c').write_text('\n'.join([*lines, '    return 0;', '}']) + '\n')
+    subprocess.run([gcc, '-std=c99', '-I', str(root / 'include'), str(tmp_path / 'layout.c'), '-o', str(tmp_path / 'layout')],
+                   check=True)
+    out = subprocess.run([str(tmp_path / 'layout')], capture_output=True, text=True, check=True).stdout.split()
+    assert list(map(int, out)) == [40, *(getattr(_lib.Heads, n).offset for n in fields)]
