@@ -140,15 +140,16 @@ __global__ __launch_bounds__(NT, NT == 1024 && C == 8 ? 8 : 4) void distill_kern
             float top = t.get(0);
 #pragma unroll
             for (int e = 1; e < N; ++e) top = fmaxf(top, t.get(e));
+            // (under the cap -inf is a value like others, -softcap, and so is a maximum of it)
             if (top > m) {
-                s = m > -__builtin_inff() ? s * exp2_fast((capped(m) - capped(top)) * c) : 0.f;
+                s = CAP || m > -__builtin_inff() ? s * exp2_fast((capped(m) - capped(top)) * c) : 0.f;
                 m = top;
             }
             const float at = capped(m);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float v = t.get(e);   // (nothing but -inf and NaN so far: only the latter counts)
-                s += m > -__builtin_inff() ? exp2_fast((capped(v) - at) * c) : v != v ? v : 0.f;
+                const float v = t.get(e);   // (without it, nothing but -inf and NaN so far: only the latter counts)
+                s += CAP || m > -__builtin_inff() ? exp2_fast((capped(v) - at) * c) : v != v ? v : 0.f;
             }
         }
     }

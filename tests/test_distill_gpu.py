@@ -105,6 +105,51 @@ def test_extreme_logits():
     assert torch.isnan(loss[[3, 4]]).all() and torch.isfinite(loss[[0, 2]]).all()
 
 
+@pytest.mark.parametrize('cap', [None, 15.0])
+@pytest.mark.parametrize('dtype,V', [(torch.float32, 300), (torch.float32, 100001), (torch.bfloat16, 300),
+                                     (torch.bfloat16, 200003)])
+def test_infinities_in_rows_of_any_width(V, dtype, cap):
+    """-inf (a value of -softcap under the cap, nothing without it) over the first half of a row, everywhere but at one place
+    or the last one, and in the whole row; NaN at the end of a row that is finite elsewhere; inf under the cap.
+
+    Bounds: a sum over the vocabulary has at most V / 1024 + 16 terms in turn (a thread's) and 10 levels, so log s is off by
+    (V / 1024 + 26) 2^-24 beside the loss's 16 A 2^-24. In a gradient the cap's slope 1 - t^2 is off by less than 24 2^-24 (8
+    roundings of t, twice, and those of the product) of the parts q + p that it multiplies."""
+    from noise_amd.distill import distill_loss_grad
+    tau, K = 2.0, 10
+    x, t, i, w = make(8, V, V + 1, K, dtype, 30)
+    half = V // 2 // 64 * 64
+    x[0, :half] = -math.inf
+    x[1, :V] = -math.inf
+    x[1, half + 5] = 1.5
+    x[2, :V] = -math.inf
+    x[2, V - 1] = -2.5
+    x[3, ::2] = -math.inf
+    x[4, :V] = -math.inf
+    x[6, V - 1] = math.nan
+    where = torch.arange(half, half + 2 * K, 2, device=DEV) + 1
+    i[0], i[1], i[2], i[3] = where, half + 5, V - 1, where    # (finite logits, so that a loss without the cap is)
+    if cap:
+        i[0, :3], i[1, 1:4], i[2, 1:4] = 0, 7, 8
+        x[7, 9] = math.inf
+    loss, grad = distill_loss_grad(x, t, i, w, vocab=V, temperature=tau, softcap=cap)
+    assert torch.isnan(loss[6]) and torch.isnan(grad[6, :V]).all()
+    rows = [0, 1, 2, 3, 5, 7] + ([4] if cap else [])
+    want, want_grad = oracle.distill(x[rows], t[rows], i[rows], V, tau, cap, w[rows])
+    z = x[rows, :V].double()
+    z = z if cap is None else cap * torch.tanh(z / cap)
+    A = (z.abs().masked_fill(z == -math.inf, 0).amax(-1) + t[rows].double().abs().amax(-1)) / tau + math.log(V)
+    off = (loss[rows].double() - want).abs()
+    assert (off <= F * tau ** 2 * (16 * A + V / 1024 + 26)).all(), off
+    parts = torch.softmax(z / tau, -1).scatter_add_(1, i[rows], torch.softmax(t[rows].double() / tau, -1))
+    g = want_grad[:, :V]
+    bound = HALF[dtype] * g.abs() + F * (40 + 8 * A + V / 1024 + 26)[:, None] * tau * w[rows].double()[:, None] * parts
+    off = (grad[rows, :V].double() - g).abs()
+    assert (off <= bound + 1e-37).all(), (off - bound).amax(-1)
+    if cap is None:
+        assert torch.isnan(loss[4])     # a row of nothing but -inf has no softmax
+
+
 def test_agreement():
     """A student equal to the teacher over the whole vocabulary: no loss, no gradient (to the roundings)."""
     x, _, _, _ = make(4, 64, 64, 1, torch.float32, 3)
