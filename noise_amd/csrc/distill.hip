@@ -140,15 +140,17 @@ __global__ __launch_bounds__(NT, NT == 1024 && C == 8 ? 8 : 4) void distill_kern
             float top = t.get(0);
 #pragma unroll
             for (int e = 1; e < N; ++e) top = fmaxf(top, t.get(e));
-            // (under the cap -inf is a value like others, -softcap, and so is a maximum of it)
+            // Under the cap -inf is a value like others, -softcap, and so is a maximum of it. Without one, a thread that has met
+            // nothing but -inf and NaN holds 0 or, for good, NaN in s.
+            const bool counts = CAP || m > -__builtin_inff();
             if (top > m) {
-                s = CAP || m > -__builtin_inff() ? s * exp2_fast((capped(m) - capped(top)) * c) : 0.f;
+                if (counts) s *= exp2_fast((capped(m) - capped(top)) * c);
                 m = top;
             }
             const float at = capped(m);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float v = t.get(e);   // (without it, nothing but -inf and NaN so far: only the latter counts)
+                const float v = t.get(e);
                 s += CAP || m > -__builtin_inff() ? exp2_fast((capped(v) - at) * c) : v != v ? v : 0.f;
             }
         }

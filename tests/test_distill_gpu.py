@@ -110,7 +110,8 @@ def test_extreme_logits():
                                      (torch.bfloat16, 200003)])
 def test_infinities_in_rows_of_any_width(V, dtype, cap):
     """-inf (a value of -softcap under the cap, nothing without it) over the first half of a row, everywhere but at one place
-    or the last one, and in the whole row; NaN at the end of a row that is finite elsewhere; inf under the cap.
+    or the last one, and in the whole row; NaN beside -inf at the row's start, or at its end, in a row that is finite elsewhere;
+    inf under the cap.
 
     Bounds: a sum over the vocabulary has at most V / 1024 + 16 terms in turn (a thread's) and 10 levels, so log s is off by
     (V / 1024 + 26) 2^-24 beside the loss's 16 A 2^-24. In a gradient the cap's slope 1 - t^2 is off by less than 24 2^-24 (8
@@ -126,6 +127,8 @@ def test_infinities_in_rows_of_any_width(V, dtype, cap):
     x[2, V - 1] = -2.5
     x[3, ::2] = -math.inf
     x[4, :V] = -math.inf
+    x[5, :128] = -math.inf
+    x[5, 70] = math.nan            # (in a thread's first elements, one without any of the row's last ones)
     x[6, V - 1] = math.nan
     where = torch.arange(half, half + 2 * K, 2, device=DEV) + 1
     i[0], i[1], i[2], i[3] = where, half + 5, V - 1, where    # (finite logits, so that a loss without the cap is)
@@ -133,8 +136,8 @@ def test_infinities_in_rows_of_any_width(V, dtype, cap):
         i[0, :3], i[1, 1:4], i[2, 1:4] = 0, 7, 8
         x[7, 9] = math.inf
     loss, grad = distill_loss_grad(x, t, i, w, vocab=V, temperature=tau, softcap=cap)
-    assert torch.isnan(loss[6]) and torch.isnan(grad[6, :V]).all()
-    rows = [0, 1, 2, 3, 5, 7] + ([4] if cap else [])
+    assert torch.isnan(loss[5:7]).all() and torch.isnan(grad[5:7, :V]).all()
+    rows = [0, 1, 2, 3, 7] + ([4] if cap else [])
     want, want_grad = oracle.distill(x[rows], t[rows], i[rows], V, tau, cap, w[rows])
     z = x[rows, :V].double()
     z = z if cap is None else cap * torch.tanh(z / cap)
