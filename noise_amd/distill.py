@@ -4,12 +4,12 @@
   distill_loss_grad(logits, teacher_logits, teacher_index, weight, ...)   losses and the weighted sum's gradient in one pass
 
 The logits are the head's raw ones (utils/model.py:204-206) with its soft cap as an option. The calls are
-torch.ops.noise_amd operators too.
+torch.ops.noise_amd operators too. Derivatives are taken backwards and once, as in noise_amd.sinks.
 """
 import torch
 
 from . import _lib
-from .sinks import F32, TYPES, _call, _new
+from .sinks import F32, TYPES, _call, _new, _no_tangents
 
 MAX_ENTRIES = 1024
 
@@ -45,6 +45,7 @@ def _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, sof
 def distill(fn, logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap, with_grad):
     """(losses, gradient of sum weight * loss or None); weight None: ones"""
     x, t, i, vocab = _operands(fn, logits, teacher_logits, teacher_index, vocab, temperature, softcap)
+    _no_tangents(fn, logits, teacher_logits, weight)
     rows, width = x.shape
     if weight is not None:
         if weight.shape != logits.shape[:-1] or weight.device != logits.device:

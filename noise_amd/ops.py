@@ -22,6 +22,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.library import custom_op
 
 from . import distill as _distill
@@ -121,9 +122,17 @@ def _coordinate_differences_fake(raw, y, sigma):
 # (an absent gradient of an optional tensor leaves the backward operators as an empty tensor)
 
 
+def _backwards_only(name):
+    """Refuses an operator's call inside a forward-mode level. torch.func.jvp hands an operator plain tensors: whether they
+    carry tangents cannot be told here, and those that do would get derivatives of 0."""
+    if forward_ad._current_level >= 0:
+        raise NotImplementedError(f'torch.ops.noise_amd.{name}: forward-mode derivatives are not implemented')
+
+
 @custom_op('noise_amd::qk_norm_rotary', mutates_args=())
 def qk_norm_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, q_weight: Optional[Tensor],
                    k_weight: Optional[Tensor], start: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor]:
+    _backwards_only('qk_norm_rotary')
     return _sinks.norm_forward(q, k, cos, sin, q_weight, k_weight, start, eps)
 
 
@@ -136,6 +145,7 @@ def _qk_norm_rotary_fake(q, k, cos, sin, q_weight, k_weight, start, eps):
 def qk_norm_rotary_backward(dq: Tensor, dk: Tensor, q: Tensor, k: Tensor, cos: Tensor, sin: Tensor,
                             q_weight: Optional[Tensor], k_weight: Optional[Tensor], start: Optional[Tensor],
                             eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    _backwards_only('qk_norm_rotary_backward')
     grads = _sinks.norm_backward(dq, dk, q, k, cos, sin, q_weight, k_weight, start, eps)
     return tuple(q.new_empty(0) if g is None else g for g in grads)
 
@@ -163,6 +173,7 @@ qk_norm_rotary.register_autograd(_qk_norm_rotary_backward, setup_context=_qk_nor
 @custom_op('noise_amd::qk_norm_rotary_append', mutates_args=('k_cache', 'v_cache'))
 def qk_norm_rotary_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, k_cache: Tensor, v_cache: Tensor,
                           start: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], eps: float) -> Tensor:
+    _backwards_only('qk_norm_rotary_append')
     return _sinks.qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight, k_weight, eps)
 
 
@@ -174,6 +185,7 @@ def _qk_norm_rotary_append_fake(q, k, v, cos, sin, k_cache, v_cache, start, q_we
 @custom_op('noise_amd::sink_attention', mutates_args=())
 def sink_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int,
                    lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    _backwards_only('sink_attention')
     return _sinks.attend_forward(q, k, v, window, sinks, lengths, True)
 
 
@@ -185,6 +197,7 @@ def _sink_attention_fake(q, k, v, window, sinks, lengths):
 @custom_op('noise_amd::sink_attention_backward', mutates_args=())
 def sink_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: Tensor, lse: Tensor,
                             window: int, sinks: int, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    _backwards_only('sink_attention_backward')
     return tuple(_sinks.attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths))
 
 
@@ -211,6 +224,7 @@ sink_attention.register_autograd(_sink_attention_backward, setup_context=_sink_a
 @custom_op('noise_amd::sink_attention_decode', mutates_args=())
 def sink_attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, start: Tensor, window: int,
                           sinks: int) -> Tensor:
+    _backwards_only('sink_attention_decode')
     return _sinks.sink_attention_decode(q, k_cache, v_cache, start, window, sinks)
 
 
@@ -222,6 +236,7 @@ def _sink_attention_decode_fake(q, k_cache, v_cache, start, window, sinks):
 @custom_op('noise_amd::distill_loss', mutates_args=())
 def distill_loss(logits: Tensor, teacher_logits: Tensor, teacher_index: Tensor, vocab: int, temperature: float,
                  softcap: Optional[float]) -> Tensor:
+    _backwards_only('distill_loss')
     return _distill.distill('distill_loss', logits, teacher_logits, teacher_index, None, vocab, temperature, softcap,
                            False)[0]
 
@@ -234,6 +249,7 @@ def _distill_loss_fake(logits, teacher_logits, teacher_index, vocab, temperature
 @custom_op('noise_amd::distill_loss_grad', mutates_args=())
 def distill_loss_grad(logits: Tensor, teacher_logits: Tensor, teacher_index: Tensor, weight: Optional[Tensor],
                       vocab: int, temperature: float, softcap: Optional[float]) -> Tuple[Tensor, Tensor]:
+    _backwards_only('distill_loss_grad')
     return _distill.distill('distill_loss_grad', logits, teacher_logits, teacher_index, weight, vocab, temperature,
                            softcap, True)
 

@@ -9,11 +9,14 @@ Tensors are [batch, token, head, dim] with dim 64 or 128, as in utils/model.py; 
 keys' (query head h reads key head h // (H // Hk)). The norm and rotation are those of utils/model.py:46-47, 55-58 and
 88-94 (rotated halves; without learned weights the rotation and the norm commute), the mask that of utils/model.py:17-21
 with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators for compiled callers.
+
+Derivatives are taken backwards and once; tensors with forward-mode tangents (torch.autograd.forward_ad) are refused.
 """
 import functools
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -59,6 +62,12 @@ def _cache_rows(fn, c):
     a, b, s, unit = c.stride()
     if unit != 1 or (a | b | s) % (16 // c.element_size()) or c.data_ptr() % 16:
         raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
+
+
+def _no_tangents(fn, *tensors):
+    """Refuses tensors that carry forward-mode tangents, which would otherwise be dropped and read as derivatives of 0"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f'{fn}: forward-mode derivatives are not implemented')
 
 
 _HEADS = 5 * 8   # bytes of a noise_heads_t: five 64-bit numbers
@@ -135,6 +144,7 @@ def _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start):
                          f'{tuple(k.shape)} {k.dtype}')
     if q.dtype not in TYPES:
         raise ValueError(f'{fn}: bfloat16 or float32 tensors, got {q.dtype}')
+    _no_tangents(fn, q, k, cos, sin, q_weight, k_weight)
     B, T, _, D = q.shape
     cos, sin = _tables(fn, cos, sin, D, q.device)
     wide = 0
@@ -163,6 +173,7 @@ def _norm_workspace(D):
 
 def _norm_backward(dq, dk, q, k, cos, sin, qw, kw, start, wide, eps):
     """Gradients of q, k and (fp32; None for absent ones) of the weights, of checked operands"""
+    _no_tangents('qk_norm_rotary', dq, dk)
     B, T, _, D = q.shape
     dt = q.dtype
     dx = _new(q), _new(k)
@@ -238,6 +249,7 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
         raise ValueError(f'{fn}: start is required')
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError(f"{fn}: v must have k's shape, type and device, got {tuple(v.shape)} {v.dtype} on {v.device}")
+    _no_tangents(fn, v, k_cache, v_cache)
     S = k_cache.shape[1] if k_cache.dim() == 4 else 0
     for c in (k_cache, v_cache):
         if c.shape != (B, S, k.shape[2], D) or c.dtype != k.dtype or c.device != k.device or S == 0:
@@ -268,6 +280,7 @@ def _attend_operands(fn, q, k, v, window, sinks, lengths):
         raise ValueError(f'{fn}: bfloat16 tensors, got {q.dtype}, {k.dtype}, {v.dtype}')
     if window < 0 or sinks < 0:
         raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
+    _no_tangents(fn, q, k, v)
     return (None, 0) if lengths is None else _ints(fn, 'lengths', lengths, q.shape[0], q.device)
 
 
@@ -291,6 +304,7 @@ def _attend_workspace(*sizes):
 
 
 def _attend_backward(dout, q, k, v, out, rest, lse, window, sinks, lengths, wide):
+    _no_tangents('sink_attention', dout)
     B, T, H, D = q.shape
     grads = [_new(q), _new(k), _new(v)]
     x = _rows(q), _rows(k), _rows(v), _rows(out), rest, _rows(dout if dout.dtype == BF16 else dout.to(BF16))
@@ -367,6 +381,7 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
         raise ValueError(f'{fn}: at most {MAX_NEW} new tokens, got {T}')
     if window < 0 or sinks < 0:
         raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
+    _no_tangents(fn, q, k_cache, v_cache)
     start, wide = _ints(fn, 'start', start, B, q.device)
     _cache_rows(fn, k_cache)
     _cache_rows(fn, v_cache)

@@ -1,0 +1,104 @@
+"""What the calls of noise_amd.sinks and noise_amd.distill do around their kernels, without a GPU: the launches are left out, and
+what would have been launched is kept."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from noise_amd import distill, sinks
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The entry points' names and arguments, in order"""
+    made = []
+    for module in (sinks, distill):
+        monkeypatch.setattr(module, '_call', lambda name, device, *args: made.append((name, args)))
+    return made
+
+
+def operands(B=2, T=5, H=4, Hk=2, D=64, S=9):
+    """A call's tensors by name"""
+    t = {n: torch.randn(B, T, h, D).to(BF16) for n, h in (('q', H), ('k', Hk), ('v', Hk))}
+    t.update({n: torch.zeros(B, S, Hk, D, dtype=BF16) for n in ('k_cache', 'v_cache')}, start=torch.zeros(B, dtype=torch.int64))
+    t.update({n: torch.rand(S, D // 2) for n in ('cos', 'sin')}, q_weight=torch.rand(D), k_weight=torch.rand(D))
+    t.update(logits=torch.randn(3, 10), teacher=torch.randn(3, 4), index=torch.zeros(3, 4, dtype=torch.int64),
+             weight=torch.rand(3))
+    return t
+
+
+CALLS = {   # call -> its tensors that may be differentiated, the call, its torch.ops form
+    'qk_norm_rotary': (
+        ('q', 'k', 'q_weight', 'k_weight'),
+        lambda t: sinks.qk_norm_rotary(t['q'], t['k'], t['cos'], t['sin'], t['q_weight'], t['k_weight']),
+        lambda t: torch.ops.noise_amd.qk_norm_rotary(t['q'], t['k'], t['cos'], t['sin'], t['q_weight'], t['k_weight'], None,
+                                                     1e-6)),
+    'qk_norm_rotary_append': (
+        ('q', 'k', 'v', 'k_cache', 'v_cache', 'q_weight', 'k_weight'),
+        lambda t: sinks.qk_norm_rotary_append(t['q'], t['k'], t['v'], t['cos'], t['sin'], t['k_cache'], t['v_cache'],
+                                              t['start'], t['q_weight'], t['k_weight']),
+        lambda t: torch.ops.noise_amd.qk_norm_rotary_append(t['q'], t['k'], t['v'], t['cos'], t['sin'], t['k_cache'],
+                                                            t['v_cache'], t['start'], t['q_weight'], t['k_weight'], 1e-6)),
+    'sink_attention': (
+        ('q', 'k', 'v'), lambda t: sinks.sink_attention(t['q'], t['k'], t['v'], 3, 1),
+        lambda t: torch.ops.noise_amd.sink_attention(t['q'], t['k'], t['v'], 3, 1, None)),
+    'sink_attention_decode': (
+        ('q', 'k_cache', 'v_cache'), lambda t: sinks.sink_attention_decode(t['q'], t['k_cache'], t['v_cache'], t['start'], 3, 1),
+        lambda t: torch.ops.noise_amd.sink_attention_decode(t['q'], t['k_cache'], t['v_cache'], t['start'], 3, 1)),
+    'distill_loss': (
+        ('logits', 'teacher'), lambda t: distill.distill_loss(t['logits'], t['teacher'], t['index']),
+        lambda t: torch.ops.noise_amd.distill_loss(t['logits'], t['teacher'], t['index'], 10, 1.0, None)),
+    'distill_loss_grad': (
+        ('logits', 'teacher', 'weight'),
+        lambda t: distill.distill_loss_grad(t['logits'], t['teacher'], t['index'], t['weight']),
+        lambda t: torch.ops.noise_amd.distill_loss_grad(t['logits'], t['teacher'], t['index'], t['weight'], 10, 1.0, None)),
+}
+
+
+@pytest.mark.parametrize('name', CALLS)
+def test_forward_mode_is_refused(name, launches):
+    """A tangent on any tensor is refused with and without gradients, by the call and by the operator; without tangents the call
+    goes through inside a forward-mode level."""
+    tensors, call, operator = CALLS[name]
+    for which in tensors:
+        for also in (None, tensors[0]):
+            t = operands()
+            if also is not None and 'cache' not in which and name in ('qk_norm_rotary', 'sink_attention', 'distill_loss'):
+                t[also].requires_grad_()
+            with forward_ad.dual_level():
+                t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+                for f in (call, operator):
+                    with pytest.raises(NotImplementedError, match='forward.mode'):
+                        f(t)
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match='forward.mode'):
+                        f(t)
+            assert not launches
+    with forward_ad.dual_level():
+        call(operands())
+    assert len(launches) == 1
+
+
+@pytest.mark.parametrize('name', CALLS)
+def test_forward_mode_transforms_are_refused(name, launches):
+    """torch.func.jvp gives no derivatives of 0 either."""
+    tensors, call, operator = CALLS[name]
+    for which in tensors:
+        for f in (call, operator):
+            t = operands()
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                torch.func.jvp(lambda x: f({**t, which: x}), (t[which],), (torch.ones_like(t[which]),))
+            assert not launches
+
+
+@pytest.mark.parametrize('name,grads', [('qk_norm_rotary', 2), ('sink_attention', 1), ('distill_loss', 1)])
+def test_tangents_of_upstream_gradients_are_refused(name, grads, launches):
+    t = operands()
+    tensors, call, _ = CALLS[name]
+    out = call({**t, tensors[0]: t[tensors[0]].requires_grad_()})
+    outs = out if isinstance(out, tuple) else (out,)
+    with forward_ad.dual_level():
+        up = [forward_ad.make_dual(torch.ones_like(o), torch.ones_like(o)) for o in outs]
+        with pytest.raises(NotImplementedError, match='forward.mode'):
+            torch.autograd.grad(outs, t[tensors[0]], up)
+    assert len(outs) == grads and len(launches) == 1
