@@ -265,6 +265,7 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     table, at = _table(q, k, out, k_cache, v, v_cache, pointers=(qw, kw))
     _call('noise_qk_norm_rotary', q.device, at, at + 2 * _HEADS, at + 6 * _HEADS, at + 4 * _HEADS, at + 5 * _HEADS,
           cos.data_ptr(), sin.data_ptr(), cos.size(0), start.data_ptr(), wide, B, T, S, D, TYPES[q.dtype], float(eps))
+    torch.autograd.graph.increment_version((k_cache, v_cache))   # (a graph that holds them refuses its backward pass)
     return out
 
 

@@ -104,3 +104,20 @@ def test_tangents_of_upstream_gradients_are_refused(name, grads, launches):
         with pytest.raises(NotImplementedError, match='forward.mode'):
             torch.autograd.grad(outs, t[tensors[0]], up)
     assert len(outs) == grads and len(launches) == 1
+
+
+def test_append_raises_the_caches_versions(launches):
+    """A graph that holds a cache as it was must not run backwards on what was written over it; views of a cache count, and
+    caches made in inference mode have no version."""
+    for of in (lambda c: c, lambda c: c[:, 2:]):
+        t = operands()
+        for n in ('k_cache', 'v_cache'):
+            held = torch.ones_like(t[n], requires_grad=True) * t[n]
+            before = t[n]._version
+            CALLS['qk_norm_rotary_append'][1]({**t, 'k_cache': of(t['k_cache']), 'v_cache': of(t['v_cache'])})
+            assert t[n]._version == before + 1
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                held.float().sum().backward()
+    with torch.inference_mode():
+        CALLS['qk_norm_rotary_append'][1](operands())
+    assert len(launches) == 5
