@@ -95,5 +95,6 @@ def distill_loss(logits, teacher_logits, teacher_index, vocab=None, temperature=
 def distill_loss_grad(logits, teacher_logits, teacher_index, weight=None, vocab=None, temperature=1.0, softcap=None):
     """(losses, gradient) of distill_loss in one pass over the logits, for a training step that knows its weights before
     the loss: the gradient, of the logits' shape and type, is that of sum(weight * loss), weight [...] (None: ones).
-    Columns from `vocab` on get zeros."""
+    Columns from `vocab` on get zeros. Both results are plain tensors, for logits that require a gradient too
+    (logits.backward(gradient) goes on from there)."""
     return distill('distill_loss_grad', logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap, True)

@@ -70,6 +70,14 @@ def _no_tangents(fn, *tensors):
         raise NotImplementedError(f'{fn}: forward-mode derivatives are not implemented')
 
 
+def _no_gradients(fn, *tensors):
+    """Refuses tensors whose gradient a call without a backward pass would drop"""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f'{fn}: not differentiable, and a tensor requires a gradient: call it under torch.no_grad()')
+
+
 _HEADS = 5 * 8   # bytes of a noise_heads_t: five 64-bit numbers
 
 
@@ -241,7 +249,8 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     """q' of qk_norm_rotary for new tokens at positions start[b] + t, with k' and v [B, T, Hk, D] written to those slots of
     k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
     cache or the tables gets zeros in q' and leaves the cache as it is, so an idle sequence has a start of -T; no other
-    slot is touched. k and v must not share memory with the caches. Not differentiable (it writes in place)."""
+    slot is touched. q, k and v must not share memory with the caches. Not differentiable (it writes in place): while
+    gradients are recorded, tensors that require one are refused."""
     fn = 'qk_norm_rotary_append'
     cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
     B, T, H, D = q.shape
@@ -250,6 +259,7 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError(f"{fn}: v must have k's shape, type and device, got {tuple(v.shape)} {v.dtype} on {v.device}")
     _no_tangents(fn, v, k_cache, v_cache)
+    _no_gradients(fn, q, k, v, k_cache, v_cache, q_weight, k_weight)
     S = k_cache.shape[1] if k_cache.dim() == 4 else 0
     for c in (k_cache, v_cache):
         if c.shape != (B, S, k.shape[2], D) or c.dtype != k.dtype or c.device != k.device or S == 0:
@@ -369,7 +379,7 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     in bfloat16, whose slots hold the positions 0, 1, ...; token t of sequence b stands at position start[b] + t (its own
     key already in the cache, as qk_norm_rotary_append leaves it) and sees the slots up to there that the window and the
     sinks allow. A token at a negative position (an idle sequence has a start of -T) gets zeros. Slots that no token of
-    the call sees may hold anything. Not differentiable."""
+    the call sees may hold anything. Not differentiable: while gradients are recorded, tensors that require one are refused."""
     fn = 'sink_attention_decode'
     window, sinks = min(int(window), FAR), min(int(sinks), FAR)
     B, T, H, D, S, Hk = _check(fn, q, k_cache, v_cache)
@@ -383,6 +393,7 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     if window < 0 or sinks < 0:
         raise ValueError(f'{fn}: window and sinks must not be negative, got {window} and {sinks}')
     _no_tangents(fn, q, k_cache, v_cache)
+    _no_gradients(fn, q, k_cache, v_cache)
     start, wide = _ints(fn, 'start', start, B, q.device)
     _cache_rows(fn, k_cache)
     _cache_rows(fn, v_cache)

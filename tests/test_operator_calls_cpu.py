@@ -121,3 +121,24 @@ def test_append_raises_the_caches_versions(launches):
     with torch.inference_mode():
         CALLS['qk_norm_rotary_append'][1](operands())
     assert len(launches) == 5
+
+
+@pytest.mark.parametrize('name', ['qk_norm_rotary_append', 'sink_attention_decode'])
+def test_calls_without_a_derivative_refuse_to_drop_one(name, launches):
+    """A tensor that requires a gradient, a leaf or not, is refused while gradients are recorded, nothing launched; under
+    no_grad it is a tensor like others. The operator's backward pass is refused."""
+    tensors, call, operator = CALLS[name]
+    for which in tensors:
+        for of in (lambda x: x, lambda x: x * 1):
+            t = operands()
+            t[which] = of(t[which].requires_grad_())
+            with pytest.raises(ValueError, match='not differentiable'):
+                call(t)
+            assert not launches
+            with torch.no_grad():
+                assert not call(t).requires_grad
+            out = operator(t)
+            with pytest.raises(RuntimeError, match='no autograd formula'):
+                out.float().sum().backward()
+            assert len(launches) == 2
+            launches.clear()
