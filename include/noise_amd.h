@@ -639,6 +639,7 @@ typedef struct {
  * With a cache (capacity > 0), y[1] and v_out are [batch, capacity, heads, D] tensors: the key of position p is written to
  * their token p, and so is the row of v (any values, copied). A token whose position lies outside the tables or the
  * cache then gets zeros in y[0] and is not written. Slots of other positions are left as they are.
+ * The rows of y[1] and v_out share no memory, among themselves, with one another or with the inputs (not checked here).
  * capacity 0: y[1] is [batch, tokens, heads, D], v and v_out are NULL. */
 int noise_qk_norm_rotary(const noise_heads_t x[2], const noise_heads_t y[2], const float *const w[2],
                          const noise_heads_t *v, const noise_heads_t *v_out, const float *rope_cos,

@@ -78,6 +78,37 @@ def _no_gradients(fn, *tensors):
                 raise ValueError(f'{fn}: not differentiable, and a tensor requires a gradient: call it under torch.no_grad()')
 
 
+@functools.lru_cache(maxsize=1024)
+def _span(shape, strides):
+    """(elements from a tensor's first to behind its last, its (stride, size) from the outermost dimension in), or None where it
+    is not made of dimensions inside one another: where a step along one lands on what the shorter steps reach"""
+    end, dims = 1, sorted((s, n) for s, n in zip(strides, shape) if n > 1)
+    for s, n in dims:
+        if s < end:
+            return None
+        end += s * (n - 1)
+    return end, dims[::-1]
+
+
+def _share(a, b):
+    """Whether tensors of one shape and type, each with a _span, have memory in common (or may have, where their ranges meet
+    and their strides differ)"""
+    (end_a, dims), (end_b, others) = _span(a.shape, a.stride()), _span(b.shape, b.stride())
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if off >= end_a or -off >= end_b:
+        return False
+    return dims != others or _reach(off, dims)
+
+
+def _reach(off, dims):
+    """Whether two elements of such a tensor lie `off` apart: a dimension's steps miss `off` by less than one of them, which
+    leaves two numbers of steps, and the rest to the dimensions inside"""
+    if not dims:
+        return off == 0
+    (s, n), *inner = dims
+    return any(abs(d) < n and _reach(off - d * s, inner) for d in (off // s, off // s + 1))
+
+
 _HEADS = 5 * 8   # bytes of a noise_heads_t: five 64-bit numbers
 
 
@@ -249,7 +280,8 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     """q' of qk_norm_rotary for new tokens at positions start[b] + t, with k' and v [B, T, Hk, D] written to those slots of
     k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
     cache or the tables gets zeros in q' and leaves the cache as it is, so an idle sequence has a start of -T; no other
-    slot is touched. q, k and v must not share memory with the caches. Not differentiable (it writes in place): while
+    slot is touched. The caches may be views of one buffer (refused where their slots overlap); q, k and v must not share
+    memory with them. Not differentiable (it writes in place): while
     gradients are recorded, tensors that require one are refused."""
     fn = 'qk_norm_rotary_append'
     cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
@@ -266,10 +298,10 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
             raise ValueError(f'{fn}: caches must be [{B}, capacity, {k.shape[2]}, {D}] {k.dtype} on {k.device}, got '
                              f'{tuple(c.shape)} {c.dtype} on {c.device}')
         _cache_rows(fn, c)
-        if 0 in c.stride() and any(s == 0 and n > 1 for s, n in zip(c.stride(), c.shape)):
-            raise ValueError(f'{fn}: a broadcast cache has no slots of its own to write to')
-    if k_cache.data_ptr() == v_cache.data_ptr():
-        raise ValueError(f'{fn}: k_cache and v_cache are the same memory')
+        if _span(c.shape, c.stride()) is None:
+            raise ValueError(f'{fn}: slots of a cache overlap (a broadcast cache has none of its own to write to)')
+    if B and _share(k_cache, v_cache):
+        raise ValueError(f'{fn}: k_cache and v_cache have slots in the same memory')
     out = _new(q)
     q, k, v = _rows(q), _rows(k), _rows(v)
     table, at = _table(q, k, out, k_cache, v, v_cache, pointers=(qw, kw))

@@ -142,3 +142,74 @@ def test_calls_without_a_derivative_refuse_to_drop_one(name, launches):
                 out.float().sum().backward()
             assert len(launches) == 2
             launches.clear()
+
+
+def append_into(k_cache, v_cache):
+    B, S, Hk, D = k_cache.shape
+    t = operands(B=B, Hk=Hk, H=Hk, D=D)
+    return sinks.qk_norm_rotary_append(t['q'], t['k'], t['v'], t['cos'], t['sin'], k_cache, v_cache, t['start'])
+
+
+def test_caches_that_share_slots_are_refused(launches):
+    """Of one another and of their own sequences, slots and heads."""
+    buf = torch.zeros(2, 12, 2, 64, dtype=BF16)
+    flat = torch.zeros(5000, dtype=BF16)
+    other = torch.zeros_like(buf)
+    for k, v in ((buf[:, :8], buf[:, 1:9]), (buf[:, 4:], buf[:, :8]), (buf[:, :7], buf[:, 5:]),
+                 (buf[:, :, :1], buf[:, :, :1].clone().set_(buf[:, :, :1])),
+                 (buf[:1], buf.as_strided((1, 12, 2, 64), (80, 128, 64, 1), 12 * 128 - 128)),
+                 (flat.as_strided((2, 8, 2, 64), (1024, 128, 64, 1)), flat.as_strided((2, 8, 2, 64), (1024, 64, 512, 1), 1024))):
+        for a, b in ((k, v), (v, k)):
+            with pytest.raises(ValueError, match='same memory'):
+                append_into(a, b)
+    for c in (flat.as_strided((2, 8, 2, 64), (512, 128, 64, 1)), flat.as_strided((2, 8, 2, 64), (1024, 64, 64, 1)),
+              flat.as_strided((2, 8, 2, 64), (2048, 128, 56, 1)), flat.as_strided((1, 8, 2, 64), (0, 128, 120, 1))):
+        for a, b in ((c, other[:c.shape[0], :8]), (other[:c.shape[0], :8], c)):
+            with pytest.raises(ValueError, match='overlap'):
+                append_into(a, b)
+    assert not launches
+
+
+def test_caches_side_by_side_are_taken(launches):
+    """Keys and values next to each other per slot, per head, per sequence and one after the other; sequences of one."""
+    flat = torch.zeros(2 * 9 * 2 * 2 * 64, dtype=BF16)
+    slot, head = flat.view(2, 9, 2, 2, 64), flat.view(2, 9, 2, 128)
+    rows = flat.view(2, 2, 2, 9, 64)
+    pairs = [(slot[:, :, 0], slot[:, :, 1]), (slot[:, :, :, 0], slot[:, :, :, 1]), (head[..., :64], head[..., 64:]),
+             (rows[:, :, 0].transpose(1, 2), rows[:, :, 1].transpose(1, 2)), (rows[:, 0].transpose(1, 2), rows[:, 1].transpose(1, 2)),
+             tuple(flat.view(2, 2, 9, 2, 64)), tuple(flat.view(2, 2, 9, 2, 64).unbind(1)),
+             (flat.view(4, 9, 2, 64)[:1], flat.view(4, 9, 2, 64)[1:2]), (flat.view(4, 9, 128)[:, :, None, :64][:1], slot[1:, :, :1, 0]),
+             (flat.as_strided((1, 9, 1, 64), (8, 64, 24, 1)), flat.as_strided((1, 9, 1, 64), (16, 64, 40, 1), 9 * 64))]
+    for n, (k, v) in enumerate([*pairs, *((v, k) for k, v in pairs)], 1):
+        append_into(k, v)
+        assert len(launches) == n
+    empty = torch.zeros(0, 9, 2, 64, dtype=BF16)
+    append_into(empty, empty.clone())
+
+
+def test_caches_that_share_memory_against_enumeration(launches):
+    """Of random layouts, those in which an element belongs to two slots are refused; others with sequences, slots and heads
+    inside one another, in any order, are taken."""
+    import random
+    rng = random.Random(0)
+    taken = refused = 0
+    for _ in range(600):
+        shape = (rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 2))
+        strides, end = [0, 0, 0], 64
+        for d in rng.sample(range(3), 3):
+            strides[d] = end + 8 * rng.choice([0, 0, 1, 8, 30]) - 8 * rng.choice([0] * 9 + [1])
+            end = strides[d] * (shape[d] - 1) + end
+        flat = torch.zeros(3 * end + 5000, dtype=BF16)
+        at = [8 * rng.randint(0, end // 4) for _ in range(2)]
+        k, v = (flat.as_strided((*shape, 64), (*strides, 1), a) for a in at)
+        own = [{a + sum(i * s for i, s in zip((b, t, h), strides)) + d for b in range(shape[0]) for t in range(shape[1])
+                for h in range(shape[2]) for d in range(64)} for a in at]
+        meets = len(own[0]) < k.numel() or not own[0].isdisjoint(own[1])
+        try:
+            append_into(k, v)
+            assert not meets, (shape, strides, at)
+            taken += 1
+        except ValueError:
+            assert meets, (shape, strides, at)
+            refused += 1
+    assert taken > 50 and refused > 50
