@@ -78,7 +78,6 @@ def _no_gradients(fn, *tensors):
                 raise ValueError(f'{fn}: not differentiable, and a tensor requires a gradient: call it under torch.no_grad()')
 
 
-@functools.lru_cache(maxsize=1024)
 def _span(shape, strides):
     """(elements from a tensor's first to behind its last, its (stride, size) from the outermost dimension in), or None where it
     is not made of dimensions inside one another: where a step along one lands on what the shorter steps reach"""
@@ -90,14 +89,20 @@ def _span(shape, strides):
     return end, dims[::-1]
 
 
-def _share(a, b):
-    """Whether tensors of one shape and type, each with a _span, have memory in common (or may have, where their ranges meet
-    and their strides differ)"""
-    (end_a, dims), (end_b, others) = _span(a.shape, a.stride()), _span(b.shape, b.stride())
-    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
-    if off >= end_a or -off >= end_b:
-        return False
-    return dims != others or _reach(off, dims)
+@functools.lru_cache(maxsize=1024)
+def _spans(shape, strides, others):
+    return _span(shape, strides), _span(shape, others)
+
+
+def _own_memory(fn, k_cache, v_cache):
+    """Refuses caches of one shape and type in which two slots are the same memory (or may be: where the caches' ranges meet and
+    their strides differ)"""
+    k, v = _spans(k_cache.shape, k_cache.stride(), v_cache.stride())
+    if k is None or v is None:
+        raise ValueError(f'{fn}: slots of a cache overlap (a broadcast cache has none of its own to write to)')
+    off = (v_cache.data_ptr() - k_cache.data_ptr()) // k_cache.element_size()
+    if -v[0] < off < k[0] and k_cache.numel() and (k[1] != v[1] or _reach(off, k[1])):
+        raise ValueError(f'{fn}: k_cache and v_cache have slots in the same memory')
 
 
 def _reach(off, dims):
@@ -298,10 +303,7 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
             raise ValueError(f'{fn}: caches must be [{B}, capacity, {k.shape[2]}, {D}] {k.dtype} on {k.device}, got '
                              f'{tuple(c.shape)} {c.dtype} on {c.device}')
         _cache_rows(fn, c)
-        if _span(c.shape, c.stride()) is None:
-            raise ValueError(f'{fn}: slots of a cache overlap (a broadcast cache has none of its own to write to)')
-    if B and _share(k_cache, v_cache):
-        raise ValueError(f'{fn}: k_cache and v_cache have slots in the same memory')
+    _own_memory(fn, k_cache, v_cache)
     out = _new(q)
     q, k, v = _rows(q), _rows(k), _rows(v)
     table, at = _table(q, k, out, k_cache, v, v_cache, pointers=(qw, kw))
