@@ -659,11 +659,11 @@ int noise_qk_norm_rotary_bwd(const noise_heads_t x[2], const noise_heads_t dy[2]
 
 /* Causal attention with a left window and `sinks` first tokens that stay visible: query i sees the keys j <= i with
  * i - j <= window or j < sinks (sinks 0: the mask of utils/model.py:17-21). o = softmax(scale q k^T) v in bf16 with fp32
- * scores and sums. q, o have H heads and k, v Hk, H a multiple of Hk (query head h reads key head h / (H / Hk)); head_dim
- * 64 or 128. lengths (NULL: tokens): [batch] int32, or int64 with lengths_wide; keys from lengths[b] on are seen by no
- * query and queries from there on get zeros (rows there may hold anything). For the backward pass (else NULL, both): lse,
- * fp32 [batch][H][tokens], the log2 of each row's sum of exponentials (not written past the lengths), and o_rest, like o,
- * what o's rounding to bf16 left out. */
+ * scores and sums; scale is positive, 1e-30 .. 1e30, here and in the calls below. q, o have H heads and k, v Hk, H a
+ * multiple of Hk (query head h reads key head h / (H / Hk)); head_dim 64 or 128. lengths (NULL: tokens): [batch] int32, or
+ * int64 with lengths_wide; keys from lengths[b] on are seen by no query and queries from there on get zeros (rows there may
+ * hold anything). For the backward pass (else NULL, both): lse, fp32 [batch][H][tokens], the log2 of each row's sum of
+ * exponentials (not written past the lengths), and o_rest, like o, what o's rounding to bf16 left out. */
 int noise_sink_attention_fwd(const noise_heads_t *q, const noise_heads_t *k, const noise_heads_t *v,
                              const noise_heads_t *o, const noise_heads_t *o_rest, float *lse, const void *lengths,
                              int lengths_wide, int64_t batch, int64_t tokens, int64_t head_dim, int64_t window,

@@ -612,8 +612,7 @@ extern "C" int noise_sink_attention_bwd(const noise_heads_t *q, const noise_head
                         q->heads == dq->heads && k->heads == v->heads && k->heads == dk->heads && k->heads == dv->heads,
                     "%s: tensors missing or of other heads", fn);
     int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
-    if (st) return st;
-    NOISE_CHECK_ARG(scale > 0.f && scale < __builtin_inff(), "%s: scale must be positive", fn);
+    if (st || (st = check_scale(fn, scale))) return st;
     if (batch == 0 || tokens == 0) return NOISE_OK;
     NOISE_CHECK_ARG(lse && aligned(lse, 4), "%s: lse is required", fn);
     NOISE_CHECK_ARG(!lengths || aligned(lengths, lengths_wide ? 8 : 4), "%s: lengths misaligned", fn);

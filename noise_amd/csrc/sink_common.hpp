@@ -62,6 +62,13 @@ int check_heads(const char *fn, const char *name, const noise_heads_t *h, Rows *
     return NOISE_OK;
 }
 
+// Hidden scores are -inf before the scale is applied, and maxima are taken there: it has to be positive. Within these limits its
+// product with log2 e and the backward pass's quotient of a log-sum-exp by it are normal numbers.
+int check_scale(const char *fn, float scale) {
+    NOISE_CHECK_ARG(scale >= 1e-30f && scale <= 1e30f, "%s: scale must be positive, 1e-30 .. 1e30", fn);
+    return NOISE_OK;
+}
+
 int check_sizes(const char *fn, int64_t batch, int64_t tokens, int64_t slots, int64_t heads, int64_t kv_heads,
                 int64_t head_dim, int64_t window, int64_t sinks) {
     NOISE_CHECK_ARG(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128, got %lld", fn, (long long)head_dim);

@@ -297,7 +297,7 @@ extern "C" int noise_sink_decode(const noise_heads_t *q, const noise_heads_t *k,
     const char *fn = "noise_sink_decode";
     NOISE_CHECK_ARG(q && k && v && o && q->heads == o->heads && k->heads == v->heads, "%s: tensors missing or of other heads", fn);
     int st = check_sizes(fn, batch, tokens, capacity, q->heads, k->heads, head_dim, window, sinks);
-    if (st) return st;
+    if (st || (st = check_scale(fn, scale))) return st;
     NOISE_CHECK_ARG(tokens <= 16, "%s: at most 16 new tokens, got %lld", fn, (long long)tokens);
     if (batch == 0 || tokens == 0) return NOISE_OK;
     NOISE_CHECK_ARG(capacity > 0, "%s: the cache has no slots", fn);

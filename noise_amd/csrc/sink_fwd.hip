@@ -375,7 +375,7 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     const char *fn = "noise_sink_attention_fwd";
     NOISE_CHECK_ARG(q && k && v && o && q->heads == o->heads && k->heads == v->heads, "%s: tensors missing or of other heads", fn);
     int st = check_sizes(fn, batch, tokens, tokens, q->heads, k->heads, head_dim, window, sinks);
-    if (st) return st;
+    if (st || (st = check_scale(fn, scale))) return st;
     if (batch == 0 || tokens == 0) return NOISE_OK;
     FwdArgs a;
     if ((st = check_heads(fn, "q", q, &a.q)) || (st = check_heads(fn, "k", k, &a.k)) ||

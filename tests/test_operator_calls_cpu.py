@@ -1,10 +1,13 @@
 """What the calls of noise_amd.sinks and noise_amd.distill do around their kernels, without a GPU: the launches are left out, and
 what would have been launched is kept."""
+import ctypes
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from noise_amd import distill, sinks
+from noise_amd import _lib, distill, sinks
 
 BF16 = torch.bfloat16
 
@@ -213,3 +216,17 @@ def test_caches_that_share_memory_against_enumeration(launches):
             assert meets, (shape, strides, at)
             refused += 1
     assert taken > 50 and refused > 50
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.125, math.nan, math.inf, -math.inf, 1e-40, 1e38])
+def test_entry_points_refuse_a_scale_that_is_not_positive(scale):
+    """Hidden keys are -inf before the scale is applied: 0 would make them NaN and a negative one inf. (No sequences: a scale that
+    is taken launches nothing.)"""
+    lib = _lib.lib()
+    heads = ctypes.byref(_lib.Heads(16, 5 * 128, 128, 64, 2))
+    forward = lambda x: lib.noise_sink_attention_fwd(*[heads] * 4, None, None, None, 0, 0, 5, 64, 3, 0, x, None)
+    decode = lambda x: lib.noise_sink_decode(*[heads] * 4, 16, 0, 0, 1, 9, 64, 3, 0, x, None, 0, None)
+    backward = lambda x: lib.noise_sink_attention_bwd(*[heads] * 6, 16, *[heads] * 3, None, 0, 0, 5, 64, 3, 0, x, None, 0, None)
+    for call in (forward, decode, backward):
+        assert call(scale) == -1 and 'scale' in lib.noise_last_error().decode()
+        assert call(0.125) == 0
