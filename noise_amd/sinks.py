@@ -45,22 +45,30 @@ def _check(fn, q, k, v=None):
     return B, T, H, D, S, Hk
 
 
+def _strides(t):
+    """The strides of t's batch, tokens and heads, 0 where there is one of them (torch keeps any number there)"""
+    (B, T, H, _), (a, b, c, _) = t.shape, t.stride()
+    return a if B > 1 else 0, b if T > 1 else 0, c if H > 1 else 0
+
+
 def _rows(t):
     """t with unit inner stride and rows of whole 16 B at 16 B addresses, less than 2^25 elements from token to token (copied
     if it has not)."""
     if t.is_contiguous() and not t.data_ptr() % 16:
         return t
-    s, unit = t.stride(), 16 // t.element_size()
-    if s[3] != 1 or (s[0] | s[1] | s[2]) % unit or s[1] >= 1 << 25 or t.data_ptr() % 16:
+    (a, b, c), unit = _strides(t), 16 // t.element_size()
+    if t.stride(3) != 1 or (a | b | c) % unit or b >= 1 << 25 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
     return t
 
 
-def _cache_rows(fn, c):
-    a, b, s, unit = c.stride()
-    if unit != 1 or (a | b | s) % (16 // c.element_size()) or c.data_ptr() % 16:
+def _cache_rows(fn, cache):
+    (a, b, c, one), unit = cache.stride(), 16 // cache.element_size()
+    if (a | b | c) % unit:
+        a, b, c = _strides(cache)
+    if one != 1 or (a | b | c) % unit or cache.data_ptr() % 16:
         raise ValueError(f'{fn}: cache rows must be whole 16 B at 16 B addresses with unit inner stride')
 
 
@@ -123,6 +131,8 @@ def _table(*tensors, pointers=()):
     flat = []
     for t in tensors:
         a, b, c, _ = t.stride()
+        if (a | b | c) % 8 or b >= 1 << 25:
+            a, b, c = _strides(t)
         flat += (t.data_ptr(), a, b, c, t.size(2))
     for t in pointers:
         flat.append(0 if t is None else t.data_ptr())

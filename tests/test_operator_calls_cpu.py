@@ -230,3 +230,52 @@ def test_entry_points_refuse_a_scale_that_is_not_positive(scale):
     for call in (forward, decode, backward):
         assert call(scale) == -1 and 'scale' in lib.noise_last_error().decode()
         assert call(0.125) == 0
+
+
+def odd(B, T, H, D=64, dtype=BF16):
+    """A [B, T, H, D] view with a pitch that is no multiple of 16 B in every dimension of one element"""
+    unit = 16 // torch.empty(0, dtype=dtype).element_size()
+    h = D if H > 1 else D + 3
+    t = H * D if T > 1 else H * D + 1 + unit
+    b = T * H * D if B > 1 else T * H * D + 5
+    return torch.randn(2 * B * T * H * D + 64).to(dtype).as_strided((B, T, H, D), (b, t, h, 1))
+
+
+@pytest.mark.parametrize('dtype', [BF16, torch.float32])
+@pytest.mark.parametrize('B,T,H', [(1, 7, 4), (2, 1, 4), (2, 7, 1), (1, 1, 4), (1, 7, 1), (2, 1, 1), (1, 1, 1)])
+def test_strides_of_single_elements_do_not_matter(B, T, H, dtype, monkeypatch):
+    """Views whose only odd strides are those of dimensions with one element are taken as they are (torch calls them contiguous),
+    their outputs and caches too: every stride that reaches an entry point is a multiple of 16 B."""
+    unit = 16 // torch.empty(0, dtype=dtype).element_size()
+    checked = []
+
+    def call(name, device, *args):
+        at = args[0]
+        for n in range({'noise_qk_norm_rotary': 4 if args[3] is None else 6, 'noise_qk_norm_rotary_bwd': 6, 'noise_sink_attention_fwd': 4,
+                        'noise_sink_attention_bwd': 9, 'noise_sink_decode': 4}[name]):
+            t = _lib.Heads.from_address(at + n * sinks._HEADS)
+            assert t.ptr % 16 == 0 and not any(s % unit for s in (t.s_b, t.s_t, t.s_h)), (name, n, t.s_b, t.s_t, t.s_h)
+            checked.append((t.ptr, t.heads))
+
+    monkeypatch.setattr(sinks, '_call', call)
+    x = lambda: odd(B, T, H, dtype=dtype)
+    pointers = lambda: {p for p, _ in checked}
+    cos = sin = torch.rand(9, 32)
+    start = torch.zeros(B, dtype=torch.int32)
+    q, k, v = (x().requires_grad_() for _ in range(3))
+    for n, s in enumerate((B, T, H)):
+        assert s > 1 or q.stride(n) % unit
+    torch.autograd.grad(sinks.qk_norm_rotary(q, k, cos, sin), (q, k), (x(), x()))
+    assert {q.data_ptr(), k.data_ptr()} <= pointers()
+    with torch.no_grad():
+        caches = odd(B, 9, H, dtype=dtype), odd(B, 9, H, dtype=dtype)
+        sinks.qk_norm_rotary_append(q, k, v, cos, sin, *caches, start)
+        assert {c.data_ptr() for c in caches} <= pointers()
+        one = odd(B, 1, H, dtype=dtype)
+        sinks.qk_norm_rotary_append(q[:, :1], k[:, :1], v[:, :1], cos, sin, one, odd(B, 1, H, dtype=dtype), start)
+        assert one.data_ptr() in pointers()
+    if dtype == BF16:
+        torch.autograd.grad(sinks.sink_attention(q, k, v, 3, 1), (q, k, v), x())
+        assert v.data_ptr() in pointers()
+        with torch.no_grad():
+            sinks.sink_attention_decode(q, *caches, start, 3)

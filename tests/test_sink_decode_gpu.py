@@ -216,3 +216,33 @@ def test_a_conversation(D, H, Hk):
     want, weight = oracle.attend(*qk_norm_rotary(q, k, cos, sin), v, window, sinks)
     bound = MORE * U * (weight + want.abs())
     assert ((rows - want).abs() <= bound).all() and ((whole.double() - want).abs() <= bound).all()
+
+
+def test_views_with_odd_strides_of_single_elements():
+    """A batch of one, one token and one head, cut out of buffers whose pitch is no multiple of 16 B: the bits of their copies."""
+    from noise_amd.sinks import qk_norm_rotary, qk_norm_rotary_append, sink_attention, sink_attention_decode
+    g = torch.Generator(DEV).manual_seed(6)
+    cos, sin = tables(70, 64)
+    for B, T, H in ((1, 70, 2), (2, 1, 2), (2, 70, 1), (1, 1, 1)):
+        strides = (T * H * 64 + (5 if B == 1 else 0), H * 64 + (9 if T == 1 else 0), 64 + (3 if H == 1 else 0), 1)
+        if H == 1:
+            strides = (T * 72, 72, 67, 1) if B > 1 else (T * 72 + 5, 72, 67, 1)
+        if T == 1:
+            strides = (strides[0] if B == 1 else 256, 73, strides[2], 1)
+        x = [torch.randn(20000, device=DEV, generator=g).bfloat16().as_strided((B, T, H, 64), strides) for _ in range(4)]
+        caches = [torch.zeros(40000, device=DEV, dtype=torch.bfloat16).as_strided((B, 70, H, 64), (70 * H * 72 + (5 if B == 1 else 0),
+                  H * 72, 67 if H == 1 else 72, 1)) for _ in range(2)]
+        start = torch.zeros(B, device=DEV, dtype=torch.int32)
+
+        def run(q, k, v, dout, kc, vc):
+            q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+            normed = qk_norm_rotary(q, k, cos, sin)
+            out = sink_attention(q, k, v, 20, 2)
+            grads = [*torch.autograd.grad(normed, (q, k), (dout, dout)), *torch.autograd.grad(out, (q, k, v), dout)]
+            with torch.no_grad():
+                new = qk_norm_rotary_append(q, k, v, cos, sin, kc, vc, start)
+                return [*normed, out, *grads, new, kc, vc, sink_attention_decode(q[:, -1:], kc, vc, start + T - 1, 20, 2)]
+
+        for got, want in zip(run(*x, *caches), run(*(t.clone(memory_format=torch.contiguous_format) for t in x),
+                                                   *(torch.zeros(B, 70, H, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2)))):
+            assert torch.equal(got, want)
