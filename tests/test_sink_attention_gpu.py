@@ -185,6 +185,36 @@ def test_enough_rows(B, T, window, padded, D):
             check(grads[i][b:b + 1, :, h:h + 1], wants[i], bounds[i], 'dk, dv')
 
 
+@pytest.mark.parametrize('D', [64, 128])
+def test_a_padded_batch_with_a_long_window(D):
+    """The 256-query workgroups (8 sequences of 8 heads, a window past 2048) over sequences that end in their first tile, at and
+    behind a tile's and a wave's edge, and nowhere; rows past the lengths hold NaN."""
+    from noise_amd.sinks import sink_attention
+    T, window, sinks = 2500, 2100, 70
+    q, k, v, dout = inputs(8, T, 8, 4, D, 22, 4)
+    lengths = torch.tensor([T, 1, 64, 65, 129, 257, 700, 0], device=DEV)
+    for b, n in enumerate(lengths.tolist()):
+        for t in (q, k, v, dout):
+            t[b, n:] = math.nan
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = sink_attention(*leaves, window, sinks, lengths)
+    plain = sink_attention(q, k, v, window, sinks, lengths)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for b in range(8):
+        h = b % 4
+        print(D, b, h, flush=True)
+        heads = [t[b:b + 1, :, 2 * h:2 * h + 2] for t in (q, dout)]
+        kv = [t[b:b + 1, :, h:h + 1] for t in (k, v)]
+        n = lengths[b:b + 1]
+        want, weight = oracle.attend(heads[0], *kv, window, sinks, n)
+        for got in (out.detach(), plain):
+            check(got[b:b + 1, :, 2 * h:2 * h + 2], want, U * (weight + want.abs()), 'out')
+        wants, bounds = oracle.attend_grads(heads[0], *kv, heads[1], window, sinks, n)
+        check(grads[0][b:b + 1, :, 2 * h:2 * h + 2], wants[0], bounds[0], 'dq')
+        for i in (1, 2):
+            check(grads[i][b:b + 1, :, h:h + 1], wants[i], bounds[i], 'dk, dv')
+
+
 def test_growing_scores():
     """Scores far apart, and rows whose largest weight stands in the last tile or the first key."""
     q, k, v, dout = inputs(1, 400, 2, 2, 64, 8, 4)
