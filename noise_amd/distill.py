@@ -87,6 +87,9 @@ def distill_loss(logits, teacher_logits, teacher_index, vocab=None, temperature=
     with p over the entries in use: an index outside 0 .. vocab - 1 or a teacher logit of -inf leaves its entry out, and a
     token without entries has loss and gradient 0; at most 1024 entries. The same index may stand in several entries. Statistics and sums are in
     fp32. Differentiable in the logits (once); the teacher has no gradient."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.distill_loss(logits, teacher_logits, teacher_index,
+                                                logits.shape[-1] if vocab is None else int(vocab), float(temperature), softcap)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Distill.apply(logits, teacher_logits, teacher_index, vocab, float(temperature), softcap)
     return distill('distill_loss', logits, teacher_logits, teacher_index, None, vocab, temperature, softcap, False)[0]
@@ -97,4 +100,8 @@ def distill_loss_grad(logits, teacher_logits, teacher_index, weight=None, vocab=
     the loss: the gradient, of the logits' shape and type, is that of sum(weight * loss), weight [...] (None: ones).
     Columns from `vocab` on get zeros. Both results are plain tensors, for logits that require a gradient too
     (logits.backward(gradient) goes on from there)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.distill_loss_grad(logits, teacher_logits, teacher_index, weight,
+                                                     logits.shape[-1] if vocab is None else int(vocab), float(temperature),
+                                                     softcap)
     return distill('distill_loss_grad', logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap, True)

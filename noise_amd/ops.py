@@ -194,6 +194,18 @@ def _sink_attention_fake(q, k, v, window, sinks, lengths):
     return q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
 
 
+@custom_op('noise_amd::sink_attention_output', mutates_args=())
+def sink_attention_output(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, lengths: Optional[Tensor]) -> Tensor:
+    """sink_attention's output alone, without what its backward pass needs"""
+    _backwards_only('sink_attention_output')
+    return _sinks.attend_forward(q, k, v, window, sinks, lengths, False)[0]
+
+
+@sink_attention_output.register_fake
+def _sink_attention_output_fake(q, k, v, window, sinks, lengths):
+    return q.new_empty(q.shape)
+
+
 @custom_op('noise_amd::sink_attention_backward', mutates_args=())
 def sink_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: Tensor, lse: Tensor,
                             window: int, sinks: int, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:

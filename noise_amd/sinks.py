@@ -8,7 +8,7 @@
 Tensors are [batch, token, head, dim] with dim 64 or 128, as in utils/model.py; the queries' heads are a multiple of the
 keys' (query head h reads key head h // (H // Hk)). The norm and rotation are those of utils/model.py:46-47, 55-58 and
 88-94 (rotated halves; without learned weights the rotation and the norm commute), the mask that of utils/model.py:17-21
-with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators for compiled callers.
+with the first `sinks` tokens beside the window. The same calls are torch.ops.noise_amd operators, which compiled callers trace.
 
 Derivatives are taken backwards and once; tensors with forward-mode tangents (torch.autograd.forward_ad) are refused.
 """
@@ -285,6 +285,8 @@ def qk_norm_rotary(q, k, cos, sin, q_weight=None, k_weight=None, start=None, eps
     sin are tables [positions, D / 2] over absolute positions (used in fp32); a token whose position lies outside them
     gets zeros (and has no gradient). q and k are bfloat16 or float32, and so are q' and k' (contiguous), rounded once.
     Differentiable in q, k and the weights (once); the weights' gradients are summed in fp32 in a fixed order."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.qk_norm_rotary(q, k, cos, sin, q_weight, k_weight, start, float(eps))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         return _Norm.apply(q, k, cos, sin, q_weight, k_weight, start, float(eps))
@@ -298,6 +300,9 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     slot is touched. The caches may be views of one buffer (refused where their slots overlap); q, k and v must not share
     memory with them. Not differentiable (it writes in place): while
     gradients are recorded, tensors that require one are refused."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight, k_weight,
+                                                         float(eps))
     fn = 'qk_norm_rotary_append'
     cos, sin, qw, kw, start, wide = _norm_operands(fn, q, k, cos, sin, q_weight, k_weight, start)
     B, T, H, D = q.shape
@@ -408,7 +413,12 @@ def sink_attention(q, k, v, window, sinks=0, lengths=None):
     are taken to be finite, with scores (q . k / sqrt(D)) below 2^28 in size; gradients take the scores' exponents from fp32
     sums, whose steps are 2^-7 of a weight at scores of 2^15. Differentiable in q, k and v (once), with sums in a fixed order."""
     window, sinks = min(int(window), FAR), min(int(sinks), FAR)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    training = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    if torch.compiler.is_compiling():
+        if training:
+            return torch.ops.noise_amd.sink_attention(q, k, v, window, sinks, lengths)[0]
+        return torch.ops.noise_amd.sink_attention_output(q, k, v, window, sinks, lengths)
+    if training:
         return _Attend.apply(q, k, v, window, sinks, lengths)
     return attend_forward(q, k, v, window, sinks, lengths, False)[0]
 
@@ -424,6 +434,8 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     key already in the cache, as qk_norm_rotary_append leaves it) and sees the slots up to there that the window and the
     sinks allow. A token at a negative position (an idle sequence has a start of -T) gets zeros. Slots that no token of
     the call sees may hold anything. Not differentiable: while gradients are recorded, tensors that require one are refused."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.sink_attention_decode(q, k_cache, v_cache, start, min(int(window), FAR), min(int(sinks), FAR))
     fn = 'sink_attention_decode'
     window, sinks = min(int(window), FAR), min(int(sinks), FAR)
     B, T, H, D, S, Hk = _check(fn, q, k_cache, v_cache)

@@ -279,3 +279,28 @@ def test_strides_of_single_elements_do_not_matter(B, T, H, dtype, monkeypatch):
         assert v.data_ptr() in pointers()
         with torch.no_grad():
             sinks.sink_attention_decode(q, *caches, start, 3)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+@pytest.mark.parametrize('name', CALLS)
+def test_compiled_callers_trace_the_calls(name, grad, launches):
+    """fullgraph, as the framework's other calls: the same launches as the eager call makes, the caches written where it does."""
+    tensors, call, _ = CALLS[name]
+    differentiable = name in ('qk_norm_rotary', 'sink_attention', 'distill_loss')
+    made = []
+    for f in (call, torch.compile(call, backend='aot_eager', fullgraph=True)):
+        torch.manual_seed(0)
+        t = operands()
+        if grad and differentiable:
+            t[tensors[0]].requires_grad_()
+        before = t['k_cache']._version
+        outs = f(t)
+        outs = outs if isinstance(outs, tuple) else (outs,)
+        if grad and differentiable:
+            assert torch.autograd.grad(outs, t[tensors[0]], [torch.ones_like(o) for o in outs])[0].shape == t[tensors[0]].shape
+        assert t['k_cache']._version > before or name != 'qk_norm_rotary_append'
+        # (which pointers are given, and every number)
+        made.append([(o.shape, o.dtype) for o in outs] +
+                    [(n, [a is None if a is None or isinstance(a, int) and a > 2 ** 32 else a for a in args]) for n, args in launches])
+        launches.clear()
+    assert made[0] == made[1] and len(made[0]) > len(outs)

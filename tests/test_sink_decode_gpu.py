@@ -246,3 +246,33 @@ def test_views_with_odd_strides_of_single_elements():
         for got, want in zip(run(*x, *caches), run(*(t.clone(memory_format=torch.contiguous_format) for t in x),
                                                    *(torch.zeros(B, 70, H, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2)))):
             assert torch.equal(got, want)
+
+
+def test_compiled_calls():
+    """The calls themselves in compiled functions without a graph break, a training step, a prompt and a serving step: the eager
+    bits."""
+    from noise_amd.distill import distill_loss, distill_loss_grad
+    from noise_amd.sinks import qk_norm_rotary, qk_norm_rotary_append, sink_attention, sink_attention_decode
+    g = torch.Generator(DEV).manual_seed(7)
+    q, k, v = (torch.randn(2, 64, h, 64, device=DEV, generator=g).bfloat16() for h in (4, 2, 2))
+    cos, sin = tables(100, 64)
+    t, i = torch.randn(2, 64, 4, 3, device=DEV, generator=g), torch.randint(0, 64, (2, 64, 4, 3), device=DEV, generator=g)
+    start = torch.full((2,), 64, device=DEV)
+
+    def train(q, k, v, w):
+        q, k = qk_norm_rotary(q, k, cos, sin, w)
+        return distill_loss(sink_attention(q, k, v, 20, 2), t, i, softcap=15.0)
+
+    def serve(q, k, v, kc, vc):
+        first = qk_norm_rotary_append(q, k, v, cos, sin, kc, vc, start - 64)
+        out = sink_attention(first, kc[:, :64], vc[:, :64], 20, 2)
+        new = qk_norm_rotary_append(q[:, :1], k[:, :1], v[:, :1], cos, sin, kc, vc, start)
+        return out, sink_attention_decode(new, kc, vc, start, 20, 2), *distill_loss_grad(out, t, i, None, 60, 2.0)
+
+    results = []
+    for wrap in (lambda f: f, lambda f: torch.compile(f, backend='aot_eager', fullgraph=True)):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, torch.ones(64, device=DEV))]
+        loss = wrap(train)(*leaves)
+        caches = [torch.zeros(2, 100, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
+        results.append((loss, *torch.autograd.grad(loss.sum(), leaves), *wrap(serve)(q, k, v, *caches), *caches))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
