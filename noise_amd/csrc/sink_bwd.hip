@@ -12,8 +12,9 @@
 // Recomputing the scores in both kernels costs 8 products per pair where 5 would do (dQ's takes two); it keeps dQ's partial
 // sums out of memory and their order fixed. Heads of 128 hold 250 registers, two waves per SIMD. 16384 tokens, 16 heads of 128
 // on 4, window 2048, 4 first tokens: sink_dq_kernel 510 us (1.0 PFLOP/s), sink_dkv_kernel 510 us (1.0 PFLOP/s), matrix
-// cores busy 0.45 to 0.5 of the time and the waves waiting for LDS reads between the products. 8 x 2048 tokens, 8 heads of 64,
-// window 1024: 67 us (770 TFLOP/s) and 62 us (830), with the vector work on the scores beside the products.
+// cores busy 0.52 and 0.49 of the time and the waves waiting for LDS reads between the products. 8 x 2048 tokens, 8 heads of
+// 64, window 1024: 67 us (770 TFLOP/s) and 62 us (830), with the vector work on the scores (0.58 and 0.42 of the cycles) beside
+// the products (0.40 and 0.41).
 #include "sink_common.hpp"
 
 namespace noise {
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256, 2) void sink_dq_kernel(BwdArgs a
                         sc[r] = (unsigned)(16 * (r >> 3) + (r & 7) - ds) >= wd ? sc[r] : -__builtin_inff();
             }
             // the scores' gradients as two bf16 each, of 16 bits together: a row's add up to zero, and with keys that have much in
-            // common the roundings of a single one (2^-9 each) would outweigh the result's own (dq's error against 64 bits, 300
+            // common the roundings of a single one (up to 2^-8 each) would outweigh the result's own (dq's error against 64 bits, 300
             // keys and 70 first tokens: 3.1e-3 with one, 2.2e-3 with two, 1.7e-3 the rounding of the result alone; a third
             // more products, 55 -> 67 us at 8 x 2048 tokens, 8 heads of 64)
             bf16x8 g[2], rest[2];

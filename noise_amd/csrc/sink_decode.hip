@@ -1,6 +1,6 @@
 // A few new tokens against a cache, with a sliding window and first tokens that stay visible.
 //
-// Bound by the reading of the visible keys and values, once per key head. The slots that a sequence's tokens see between them
+// Bound by the reading of the visible keys and values, once for every 32 rows (tokens times query heads) of a key head. The slots that a sequence's tokens see between them
 // are listed without gaps (the first tokens, then the window's), cut into tiles of 32 and dealt out to the waves of the
 // workgroups that share the list. A wave keeps two tiles of its own in LDS, one being copied (whole lines, straight to
 // LDS) while the other is worked on, and needs no barrier before the end: four waves of a CU have 64 KB in flight. The
@@ -8,8 +8,9 @@
 // key head) as the columns. The waves join their sums in LDS; the parts of a list over several workgroups go to the workspace
 // in fp32 and sink_decode_join_kernel adds them up.
 //
-// 64 sequences, 32 heads of 128 on 8, 4100 visible slots each: 184 us, 5.9 TB/s (a large copy runs at 4.9 TB/s here, read and
-// write together). One sequence of 8 heads of 64, 1028 slots: 5.4 us over 72 workgroups and 4.8 us for the join, where the
+// 64 sequences, 32 heads of 128 on 8, 4101 visible slots each: 184 us, 5.9 TB/s (a large copy runs at 4.9 TB/s here, read and
+// write together); with 8 new tokens (32 rows) 190 us, with 9 or 16, which read everything twice, 311 and 315. One sequence of
+// 8 heads of 64, 1029 slots: 5.4 us over 72 workgroups and 4.8 us for the join, where the
 // call's host part takes 12 us.
 #include "sink_common.hpp"
 
@@ -261,8 +262,12 @@ __global__ __launch_bounds__(256) void sink_decode_join_kernel(DecodeArgs a) {
     for (int e = 0; e < D / 64; ++e) out[lane + 64 * e] = (__bf16)(weight != 0.f ? s[e] * inv : 0.f);
 }
 
-// Workgroups that share a list: enough for two on each of the 256 CUs, of four tiles (one per wave) or more. (One workgroup
-// for each list of 1028 slots, 8 in all, took 15 us.)
+// Workgroups that share a list: enough for two on each of the 256 CUs, of four tiles (one per wave) or more. One workgroup for
+// each list of 1029 slots, 8 in all, took 15 us. 32 heads of 128 on 8 (8 lists a sequence, one workgroup on a CU at a time), 4101
+// slots, in us: 32 sequences in two parts (as here) 100, whole 96; 33 sequences 124 and 141; 64 sequences whole (as here) 185,
+// in two 191; 128 sequences 362 and 373. Whole lists a little past a full round of workgroups are the costly case: 65
+// sequences 229 (in three 199), 97 sequences 316 (in three 287). 8 heads of 64 (two workgroups on a CU): 64 sequences 107 whole,
+// 102 in eight; 65 sequences 135 and 103.
 int64_t splits_of(int64_t units, int64_t tokens, int64_t slots, int64_t window, int64_t sinks) {
     int64_t most = window < slots && sinks < slots && window + sinks + tokens < slots ? window + sinks + tokens : slots;
     const int64_t useful = (most + kWaves * kKeys - 1) / (kWaves * kKeys), wanted = (512 + units - 1) / units;

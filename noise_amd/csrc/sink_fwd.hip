@@ -10,9 +10,10 @@
 // does S, softmax and O of tile t, group B softmax and O of tile t - 1, then S of tile t.
 //
 // Heads of 128: bound by the matrix products (16384 tokens, 16 heads on 4, window 2048, 4 first tokens: 290 us, 890 TFLOP/s
-// of the visible pairs, 1 PFLOP/s with the tiles' edges; a large bf16 product runs at 1250 here). Heads of 64: by the
-// vector work on the scores and the products together, 58 and 31 % of the cycles (8 x 2048 tokens, 8 heads, window 1024:
-// 43 us, 600 TFLOP/s; 47 us with what the backward pass needs).
+// of the visible pairs, 1 PFLOP/s with the tiles' edges; a large bf16 product runs at 1250 here; matrix cores busy 0.44 of the
+// time, vector units 0.45). Heads of 64: by the vector work on the scores and the products together, 64 and 34 % of the cycles
+// (8 x 2048 tokens, 8 heads, window 1024, which 128-query workgroups take: 44 us, 590 TFLOP/s; 47 us with what the backward
+// pass needs).
 #include "sink_common.hpp"
 
 namespace noise {
@@ -34,9 +35,9 @@ struct FwdArgs {
 // FORM: kPaired, as above, 256 queries by 8 waves, for long windows; kFour, 128 queries by 4 waves and two stages; for no more
 // workgroups than there are CUs, kSplit, 128 queries by 8 waves, every second tile by either half, which are joined in LDS.
 // TRAIN: with what the backward pass needs beside o, the rows' lse and o's own rounding error. The backward pass forms
-// dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (2^-9 of o) would drown it. With o and its
-// error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is left
-// is 2^-9 of the other weights, in proportion to the difference itself.
+// dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (up to 2^-8 of o) would drown it. With o
+// and its error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is
+// left is up to 2^-8 of the other weights, in proportion to the difference itself.
 template <int D, int FORM, bool TRAIN>
 __global__ __launch_bounds__(FORM == kFour ? 256 : 512) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void sink_fwd_kernel(FwdArgs a) {
@@ -393,11 +394,14 @@ extern "C" int noise_sink_attention_fwd(const noise_heads_t *q, const noise_head
     a.sinks = (int)(sinks < tokens ? sinks : tokens);
     a.rows = (int)(batch * q->heads);
     // 256-query workgroups where they fill the CUs twice and their windows are long, else smaller ones, which have less to do
-    // past the window's edges (us): 16 heads of 128 on 4 x 4096 tokens, window 1024, kPaired 160, kFour 150; 8 heads of 64,
-    // 8 x 2048 tokens, window 1024, 48.4 and 46.4; 16 x 2048 tokens, causal, 99 and 104; 16 heads of 128, 2 x 4096 tokens,
-    // causal, 141 and 153. With fewer: 8 heads of 64, 4 x 2048 tokens, window 1024 (256 of 256), kPaired 32.9, kFour
-    // 28.3; 8 heads of 128, 4096 tokens (256 of 128), kFour 33.0, kSplit 28.3; 4 heads of 64, 4096 tokens, causal (128 of
-    // 128), kPaired 76, kFour 61, kSplit 41
+    // past the window's edges. kPaired and kFour (us, TRAIN), 16 heads of 128 on 4, 4 x 4096 tokens: window 1024 182 and 167,
+    // 1536 216 and 208, 2048 249 and 244, 4096 302 and 303; 16384 tokens: 1024 195 and 184, 2048 319 and 315, 3000 434 and
+    // 419; 8 heads of 64, 8 x 2048 tokens: 1024 49.4 and 46.4, 1536 55.7 and 53.1, causal 57.6 and 55.0; 16 x 2048 tokens:
+    // 1024 84.7 and 85.7, causal 95.3 and 98.8; 16384 tokens: 1024 58.0 and 58.4, 2048 93 and 98, 4000 162 and 170, 8000 288
+    // and 271. So from 1536 on the two lie within 5 % of one another, on either side, and the border is not a sharp one.
+    // With fewer workgroups: 8 heads of 64, 4 x 2048 tokens, window 1024 (256 of 256), kPaired 32.9, kFour 28.3; 8 heads of
+    // 128, 4096 tokens (256 of 128), kFour 33.0, kSplit 28.3; 4 heads of 64, 4096 tokens, causal (128 of 128), kPaired 76,
+    // kFour 61, kSplit 41
     const int64_t paired = (tokens + 255) / 256 * a.rows, fours = (tokens + 127) / 128 * a.rows;
     const int form = paired >= 512 && a.window >= 2048 ? kPaired : fours > 256 ? kFour : kSplit;
     a.qtiles = (int)(form == kPaired ? (tokens + 255) / 256 : (tokens + 127) / 128);

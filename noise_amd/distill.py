@@ -85,8 +85,9 @@ def distill_loss(logits, teacher_logits, teacher_index, vocab=None, temperature=
         loss = temperature^2 * sum_k p_k (log p_k - log softmax(z)[index_k])
 
     with p over the entries in use: an index outside 0 .. vocab - 1 or a teacher logit of -inf leaves its entry out, and a
-    token without entries has loss and gradient 0; at most 1024 entries. The same index may stand in several entries. Statistics and sums are in
-    fp32. Differentiable in the logits (once); the teacher has no gradient."""
+    token without entries has loss and gradient 0; at most 1024 entries (a gradient's work grows with their square: past 256 of
+    them it outweighs a row of 4096). The same index may stand in several entries. Statistics and sums are in fp32.
+    Differentiable in the logits (once); the teacher has no gradient."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.distill_loss(logits, teacher_logits, teacher_index,
                                                 logits.shape[-1] if vocab is None else int(vocab), float(temperature), softcap)

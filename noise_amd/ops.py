@@ -119,7 +119,8 @@ def _coordinate_differences_fake(raw, y, sigma):
 
 
 # --- operators with gradients ---
-# (an absent gradient of an optional tensor leaves the backward operators as an empty tensor)
+# (an absent gradient of an optional tensor leaves the backward operators as an empty tensor; sink_attention always computes what
+# its backward pass needs, sink_attention_output never does)
 
 
 def _backwards_only(name):
