@@ -276,3 +276,41 @@ def test_compiled_calls():
         caches = [torch.zeros(2, 100, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2)]
         results.append((loss, *torch.autograd.grad(loss.sum(), leaves), *wrap(serve)(q, k, v, *caches), *caches))
     assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+@pytest.mark.parametrize('D', [64, 128])
+def test_captured_serving_step(D):
+    """A step as it is served, new tokens into the cache, attention and the positions moved on, captured once and replayed with
+    new tokens, beside eager steps on caches of their own; one sequence is idle, one runs past its cache."""
+    from noise_amd.sinks import qk_norm_rotary_append, sink_attention_decode
+    g = torch.Generator(DEV).manual_seed(8)
+    B, T, H, Hk, S = 4, 2, 8, 2, 1100
+    new = lambda: [torch.randn(B, T, h, D, device=DEV, generator=g).bfloat16() for h in (H, Hk, Hk)]
+    cos, sin = tables(S, D)
+    q, k, v = new()
+    both = torch.randn(2, B, S, 2, Hk, D, device=DEV, generator=g).bfloat16()     # keys and values side by side
+    begin = torch.tensor([0, 1000, -10 ** 6, S - 5], device=DEV)
+    starts = [begin.clone(), begin.clone()]
+
+    def step(n):
+        kc, vc = both[n, :, :, 0], both[n, :, :, 1]
+        out = sink_attention_decode(qk_norm_rotary_append(q, k, v, cos, sin, kc, vc, starts[n]), kc, vc, starts[n], 700, 4)
+        starts[n] += T
+        return out
+
+    both[1] = both[0]
+    step(0)
+    both[0] = both[1]
+    starts[0].copy_(begin)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(0)
+    for _ in range(6):
+        for t, x in zip((q, k, v), new()):
+            t.copy_(x)
+        want = step(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(both[0], both[1]) and torch.equal(*starts)
+        assert (out[2] == 0).all() and bool(torch.isfinite(out).all())
