@@ -37,7 +37,7 @@ struct FwdArgs {
 // TRAIN: with what the backward pass needs beside o, the rows' lse and o's own rounding error. The backward pass forms
 // dP - dO.o, which nearly cancels where one weight is close to 1: there o's rounding (up to 2^-8 of o) would drown it. With o
 // and its error, and with a running maximum that is exact (so that the largest weight is 1 and its rounding nothing), what is
-// left is up to 2^-8 of the other weights, in proportion to the difference itself.
+// left is up to 2^-8 of the other weights' terms of dO.o, which vanish with them.
 template <int D, int FORM, bool TRAIN>
 __global__ __launch_bounds__(FORM == kFour ? 256 : 512) __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 2, D == 64 ? 4 : 2)))
 void sink_fwd_kernel(FwdArgs a) {
