@@ -304,3 +304,16 @@ def test_compiled_callers_trace_the_calls(name, grad, launches):
                     [(n, [a is None if a is None or isinstance(a, int) and a > 2 ** 32 else a for a in args]) for n, args in launches])
         launches.clear()
     assert made[0] == made[1] and len(made[0]) > len(outs)
+
+
+def test_compiled_callers_may_give_whole_numbers(launches):
+    t = operands()
+    torch.compile(lambda t: distill.distill_loss(t['logits'], t['teacher'], t['index'], temperature=2, softcap=15),
+                  backend='aot_eager', fullgraph=True)(t)
+    torch.compile(lambda t: distill.distill_loss_grad(t['logits'], t['teacher'], t['index'], vocab=9, temperature=2, softcap=15),
+                  backend='aot_eager', fullgraph=True)(t)
+    torch.compile(lambda t: sinks.sink_attention(t['q'], t['k'], t['v'], 10 ** 30, 10 ** 30), backend='aot_eager',
+                  fullgraph=True)(t)
+    torch.compile(lambda t: sinks.qk_norm_rotary(t['q'], t['k'], t['cos'], t['sin'], eps=1), backend='aot_eager',
+                  fullgraph=True)(t)
+    assert len(launches) == 4
