@@ -298,8 +298,8 @@ def qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight=N
     k_cache and v_cache [B, capacity, Hk, D] (of k's type) in the same launch. A token whose position lies outside the
     cache or the tables gets zeros in q' and leaves the cache as it is, so an idle sequence has a start of -T; no other
     slot is touched. The caches may be views of one buffer (refused where their slots overlap); q, k and v must not share
-    memory with them. Not differentiable (it writes in place): while
-    gradients are recorded, tensors that require one are refused."""
+    memory with them. Not differentiable (it writes in place): while gradients are recorded, tensors that require one are
+    refused."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.qk_norm_rotary_append(q, k, v, cos, sin, k_cache, v_cache, start, q_weight, k_weight,
                                                          float(eps))
