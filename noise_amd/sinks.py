@@ -432,8 +432,9 @@ def sink_attention_decode(q, k_cache, v_cache, start, window, sinks=0):
     """sink_attention of T new tokens (1 to 16) against a cache: q [B, T, H, D], k_cache and v_cache [B, capacity, Hk, D]
     in bfloat16, whose slots hold the positions 0, 1, ... (every position has its slot: the window saves reading, not room);
     token t of sequence b stands at position start[b] + t (its own key already in the cache, as qk_norm_rotary_append leaves
-    it) and sees the slots up to there that the window and the sinks allow. A token at a negative position (an idle sequence has a start of -T) gets zeros. Slots that no token of
-    the call sees may hold anything. Not differentiable: while gradients are recorded, tensors that require one are refused."""
+    it) and sees the slots up to there that the window and the sinks allow. A token at a negative position (an idle sequence
+    has a start of -T) gets zeros. Slots that no token of the call sees may hold anything. Not differentiable: while gradients
+    are recorded, tensors that require one are refused."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.sink_attention_decode(q, k_cache, v_cache, start, min(int(window), FAR), min(int(sinks), FAR))
     fn = 'sink_attention_decode'
