@@ -707,6 +707,51 @@ int noise_distill(const void *x, int type, int64_t rows, int64_t vocab, int64_t 
                   float temperature, float softcap, float *loss, void *grad, int64_t width, int64_t grad_stride,
                   noise_stream_t stream);
 
+/* Global norm of `count` gradients (fp32 and bf16, any sizes), and the gradients scaled to a bound on it:
+ *   norm = sqrt(sum of all squares) (summed in fp64, stored in fp32),
+ *   factor = min(1, max_norm / (norm + 1e-6)),  g <- factor g in place, rounded once (not written where the factor is 1).
+ * max_norm infinite: the norm alone. A norm that is NaN makes every gradient NaN; an infinite one makes the finite ones 0 and
+ * the infinite ones NaN. The table is read on the host, before the call returns; gradients that share memory are refused.
+ * workspace: noise_clip_workspace_bytes(count) bytes, 8 B aligned. */
+typedef struct {
+    void *ptr;      /* contiguous elements, aligned to their type */
+    int64_t numel;  /* 0: left out */
+    int64_t type;   /* NOISE_BF16 or NOISE_FP32 */
+} noise_gradient_t;
+int64_t noise_clip_workspace_bytes(int64_t count);
+int noise_clip_gradients(const noise_gradient_t *gradients, int64_t count, float max_norm, float *norm, void *workspace,
+                         int64_t workspace_bytes, noise_stream_t stream);
+
+/* The residual stream between two blocks, and what the next one reads, for `rows` rows of `dim` (1 .. 8192) elements:
+ *   b = y, or with norm_y y / sqrt(mean y^2 + eps) y_weight;  out = scale (x + gate b) + x0_scale x0;
+ *   h = out / sqrt(mean out^2 + eps) weight   (from out before it is rounded)
+ * x, x0 and out have x_type, y and h y_type (fp32 and fp32, fp32 and bf16, bf16 and bf16); x, y and x0 have row strides in
+ * elements, out and h are contiguous. y, x0, scale, x0_scale (one fp32 value each), gate, y_weight and weight (fp32 [dim])
+ * may be NULL: left out. gate: [rows / gate_rows][dim], row i uses gate i / gate_rows. */
+typedef struct {
+    const void *x, *y, *x0;
+    int64_t x_stride, y_stride, x0_stride;
+    const float *scale, *x0_scale;
+    const void *gate;
+    const float *y_weight, *weight;
+    int64_t rows, gate_rows, dim, x_type, y_type, gate_type, norm_y;
+} noise_residual_t;
+int noise_residual_norm(const noise_residual_t *r, void *out, void *h, float eps, noise_stream_t stream);
+
+/* Its gradients from dout and dh (contiguous; NULL: zeros), each optional (NULL), contiguous and of its tensor's type: dx, dy,
+ * dx0 as the tensors, dscale, dx0_scale, dy_weight, dweight in fp32 and dgate in gate_type, summed over rows in fp32 (the two
+ * scalars in fp64) in a fixed order. With rows 0 nothing is written. workspace (not needed for dx, dy, dx0 and the gradient of
+ * a gate with gate_rows 1 alone): noise_residual_norm_bwd_workspace_bytes, 16 B aligned; gate_rows: rows without a gate. */
+typedef struct {
+    void *dx, *dy, *dx0;
+    float *dscale, *dx0_scale;
+    void *dgate;
+    float *dy_weight, *dweight;
+} noise_residual_grads_t;
+int64_t noise_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t gate_rows, int64_t dim);
+int noise_residual_norm_bwd(const noise_residual_t *r, const void *dout, const void *dh, const noise_residual_grads_t *grads,
+                            float eps, void *workspace, int64_t workspace_bytes, noise_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -86,12 +86,18 @@ SIGNATURES = {
     'noise_sink_decode_workspace_bytes': [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64],
     'noise_sink_decode': [_p, _p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p, _i64, _p],
     'noise_distill': [_p, _i32, _i64, _i64, _i64, _p, _i32, _p, _i32, _i64, _p, _f32, _f32, _p, _p, _i64, _i64, _p],
+    'noise_residual_norm': [_p, _p, _p, _f32, _p],
+    'noise_residual_norm_bwd_workspace_bytes': [_i64, _i64, _i64],
+    'noise_residual_norm_bwd': [_p, _p, _p, _p, _f32, _p, _i64, _p],
+    'noise_clip_workspace_bytes': [_i64],
+    'noise_clip_gradients': [_p, _i64, _f32, _p, _p, _i64, _p],
 }
 _RESTYPES = {'noise_last_error': ctypes.c_char_p, 'noise_update_workspace_bytes': ctypes.c_int64,
              'noise_head_ce_workspace_bytes': ctypes.c_int64, 'noise_block_split_workspace_bytes': ctypes.c_int64,
              'noise_dust_block_workspace_bytes': ctypes.c_int64, 'noise_dust_block_static_max_bytes': ctypes.c_int64,
              'noise_qk_norm_rotary_bwd_workspace_bytes': ctypes.c_int64,
-             'noise_sink_attention_bwd_workspace_bytes': ctypes.c_int64, 'noise_sink_decode_workspace_bytes': ctypes.c_int64}
+             'noise_sink_attention_bwd_workspace_bytes': ctypes.c_int64, 'noise_sink_decode_workspace_bytes': ctypes.c_int64,
+             'noise_clip_workspace_bytes': ctypes.c_int64, 'noise_residual_norm_bwd_workspace_bytes': ctypes.c_int64}
 
 # y_fp32 of noise_pop_linear / noise_rank1_expand: fp32 output in autocast's form (bf16 product and dot)
 LINEAR_AUTOCAST = 2
@@ -131,6 +137,11 @@ class Heads(ctypes.Structure):
     """noise_heads_t: a [batch, tokens, heads, dim] tensor with unit inner stride."""
     _fields_ = [('ptr', ctypes.c_void_p), ('s_b', ctypes.c_int64), ('s_t', ctypes.c_int64), ('s_h', ctypes.c_int64),
                 ('heads', ctypes.c_int64)]
+
+
+class Gradient(ctypes.Structure):
+    """noise_gradient_t: a contiguous tensor of noise_clip_gradients."""
+    _fields_ = [('ptr', ctypes.c_void_p), ('numel', ctypes.c_int64), ('type', ctypes.c_int64)]
 
 
 SLICE_GROUPS_MAX = 64  # NOISE_SLICE_GROUPS_MAX

@@ -1,0 +1,582 @@
+// The residual stream between two blocks: a block's output, through a norm if asked, times its gate onto the scaled stream, and
+// the norm that the next block reads; and the gradients (utils/model.py:46-47 and the mixing of the forward that
+// train/val/eggroll.py:77-94 repeats, with learned weights, a gate and a norm of the block's output as options). Per row of D:
+//   b = y  or  y ry wy, ry = 1 / sqrt(mean y^2 + eps);  t = x + g b;  x' = s t + s0 x0;  n = x' r;  h = n w
+//   backward, G = dx' + r (u - n mean(u n)), u = dh w:  dx = s G,  dx0 = s0 G,  dg = s G b,  db = s G g,
+//   dy = db  or  ry (e - ny mean(e ny)), e = db wy, ny = y ry;  ds = sum G t, ds0 = sum G x0, dw = sum dh n, dwy = sum db ny
+// The backward pass forms x' again from x, y and x0 in fp32, so that n carries none of x's rounding to its stored type (and
+// reads what ds, ds0 and dg need anyway).
+//
+// Memory bound. TEAM lanes hold a row, 8 consecutive elements of each of C chunks per lane; sums over a row are wave shuffles for
+// teams of up to a wave, and one exchange through LDS per sum for larger ones. Workgroups of the backward pass take a run of
+// rows of one gate each, keep the sums over rows in registers and leave one row of partial sums; a second kernel adds those up
+// in a fixed order.
+#include "common.hpp"
+#include "mfma.hpp"
+
+namespace noise {
+namespace {
+
+constexpr int64_t kLaunchGroups = 1 << 20;   // a launch has fewer than 2^32 threads
+constexpr int kMaxDim = 8192;
+
+struct ResArgs {
+    const void *x, *y, *x0, *gate, *dout, *dh;
+    const float *scale, *x0_scale, *wy, *w;
+    void *out, *h;                   // backward: dx, dy
+    void *dx0, *dgate;               // dgate: of a gate per row only
+    float *part_w, *part_wy, *part_g;   // [parts][D] partial sums
+    double *part_s;                  // [parts][2]
+    int64_t rows, gate_rows, s_x, s_y, s_x0, first;
+    int64_t gates, gates_per_part, parts_per_gate, part_rows;  // backward: how the rows are cut (Cut)
+    int D, gate_bf16;
+    float eps;
+};
+
+// 8 elements at any address of their type, in fp32; n: how many of them exist (zeros for the others)
+template <class E>
+__device__ __forceinline__ void get8(const E *p, int n, float (&o)[8]) {
+    E v[8];
+    if (n >= 8) {
+        __builtin_memcpy(v, p, 8 * sizeof(E));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (float)v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = e < n ? (float)p[e] : 0.f;
+    }
+}
+template <class E>
+__device__ __forceinline__ void put8(E *p, int n, const float (&o)[8]) {
+    if (n >= 8) {
+        E v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (E)o[e];
+        __builtin_memcpy(p, v, 8 * sizeof(E));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = (E)o[e];
+    }
+}
+
+// N sums over a team of TEAM lanes. Teams larger than a wave are the workgroup: the sums go through LDS, in two alternating sets of
+// slots, so that one barrier per call is enough.
+template <int TEAM, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float *slots, int &turn) {
+#pragma unroll
+    for (int o = 1; o < (TEAM < 64 ? TEAM : 64); o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+    if constexpr (TEAM > 64) {
+        constexpr int NW = TEAM / 64;
+        float *s = slots + 2 * NW * turn;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i * NW + (threadIdx.x >> 6)] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = s[i * NW];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) v[i] += s[i * NW + w];
+        }
+    }
+}
+
+template <int TEAM>
+constexpr int group_threads() { return TEAM > 256 ? TEAM : 256; }
+
+__device__ __forceinline__ void get_gate(const ResArgs &a, int64_t at, int n, float (&o)[8]) {
+    if (a.gate_bf16) get8(static_cast<const __bf16 *>(a.gate) + at, n, o);
+    else get8(static_cast<const float *>(a.gate) + at, n, o);
+}
+
+template <class EX, class EY, int TEAM, int C, bool POST>
+__global__ __launch_bounds__(group_threads<TEAM>()) void residual_kernel(ResArgs a) {
+    constexpr int NT = group_threads<TEAM>(), TEAMS = NT / TEAM;
+    __shared__ float slots[4 * (TEAM > 64 ? TEAM / 64 : 1)];
+    int turn = 0;
+    const int64_t row = (a.first + blockIdx.x) * TEAMS + threadIdx.x / TEAM;
+    if (row >= a.rows) return;   // (whole teams: a team larger than a wave is the workgroup)
+    const int lane = threadIdx.x % TEAM, D = a.D;
+    const EX *x = static_cast<const EX *>(a.x) + row * a.s_x, *x0 = static_cast<const EX *>(a.x0) + row * a.s_x0;
+    const EY *y = static_cast<const EY *>(a.y) + row * a.s_y;
+    const int64_t gate = a.gate ? row / a.gate_rows * D : 0;
+    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = a.x0_scale ? *a.x0_scale : 1.f;
+    float b[C][8], t[C][8], v0[C][8];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int c = 8 * (i * TEAM + lane), n = D - c;
+        get8(x + c, n, t[i]);
+        if (a.y) get8(y + c, n, b[i]);
+        if (a.x0) get8(x0 + c, n, v0[i]);
+    }
+    float ry = 1.f;
+    if constexpr (POST) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[0] += b[i][e] * b[i][e];
+        team_sum<TEAM>(s, slots, turn);
+        ry = rsqrtf(s[0] * inv + a.eps);
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int c = 8 * (i * TEAM + lane), n = D - c;
+        float f[8];
+        if constexpr (POST) {
+            if (a.wy) get8(a.wy + c, n, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[i][e] = b[i][e] * ry * (a.wy ? f[e] : 1.f);
+        }
+        if (a.y) {
+            if (a.gate) get_gate(a, gate + c, n, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[i][e] += a.gate ? f[e] * b[i][e] : b[i][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            t[i][e] *= scale;
+            if (a.x0) t[i][e] += x0_scale * v0[i][e];
+            s[0] += t[i][e] * t[i][e];
+        }
+    }
+    team_sum<TEAM>(s, slots, turn);
+    const float r = rsqrtf(s[0] * inv + a.eps);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int c = 8 * (i * TEAM + lane), n = D - c;
+        put8(static_cast<EX *>(a.out) + row * D + c, n, t[i]);
+        float f[8];
+        if (a.w) get8(a.w + c, n, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[i][e] = t[i][e] * r * (a.w ? f[e] : 1.f);
+        put8(static_cast<EY *>(a.h) + row * D + c, n, t[i]);
+    }
+}
+
+// SUMS: with weights or a gate whose gradients are sums over rows
+template <class EX, class EY, int TEAM, int C, bool POST, bool SUMS>
+__global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(ResArgs a) {
+    constexpr int NT = group_threads<TEAM>(), TEAMS = NT / TEAM;
+    __shared__ float slots[4 * (TEAM > 64 ? TEAM / 64 : 1)];
+    __shared__ double scalars[2][NT / 64];
+    __shared__ float fold[SUMS && TEAMS > 1 ? TEAMS * TEAM * 8 : 1];
+    int turn = 0;
+    const int64_t part = a.first + blockIdx.x;
+    const bool row_gate = a.gate_rows == 1;   // (a gate per row is not summed: all rows are one unit)
+    const int64_t unit_rows = row_gate ? a.rows : a.gate_rows, at = part % a.parts_per_gate;
+    const int64_t first_unit = part / a.parts_per_gate * a.gates_per_part;
+    const int64_t last_unit = first_unit + a.gates_per_part < a.gates ? first_unit + a.gates_per_part : a.gates;
+    const int lane = threadIdx.x % TEAM, D = a.D;
+    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = a.x0_scale ? *a.x0_scale : 1.f;
+    float sw[SUMS ? C : 1][8] = {}, swy[SUMS ? C : 1][8] = {}, sg[SUMS ? C : 1][8] = {};
+    double ds = 0., ds0 = 0.;
+    // the teams' sums, added in LDS, one array and chunk at a time
+    auto leave = [&](float *to, float (&v)[SUMS ? C : 1][8]) {
+#pragma unroll
+        for (int i = 0; i < (SUMS ? C : 1); ++i) {
+            const int c = 8 * (i * TEAM + lane), n = D - c;
+            if constexpr (TEAMS > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) fold[(threadIdx.x / TEAM * 8 + e) * TEAM + lane] = v[i][e];
+                __syncthreads();
+                if (threadIdx.x < TEAM) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        for (int k = 1; k < TEAMS; ++k) v[i][e] += fold[(k * 8 + e) * TEAM + lane];
+                }
+            }
+            if (threadIdx.x < TEAM) put8(to + c, n, v[i]);
+        }
+    };
+    for (int64_t unit = first_unit; unit < last_unit; ++unit) {
+    const int64_t begin = unit * unit_rows + at * a.part_rows;
+    const int64_t end = (unit + 1) * unit_rows, stop = begin + a.part_rows < end ? begin + a.part_rows : end;
+    for (int64_t row = begin + threadIdx.x / TEAM; row < stop; row += TEAMS) {
+        const EX *x = static_cast<const EX *>(a.x) + row * a.s_x, *x0 = static_cast<const EX *>(a.x0) + row * a.s_x0;
+        const EY *y = static_cast<const EY *>(a.y) + row * a.s_y;
+        const EX *dout = static_cast<const EX *>(a.dout) + row * D;
+        const EY *dh = static_cast<const EY *>(a.dh) + row * D;
+        float vy[C][8], t[C][8], v0[C][8], G[C][8], H[C][8], g[C][8];
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 8 * (i * TEAM + lane), n = D - c;
+            get8(x + c, n, t[i]);
+            if (a.y) get8(y + c, n, vy[i]);
+            if (a.x0) get8(x0 + c, n, v0[i]);
+            if (a.dout) get8(dout + c, n, G[i]);
+            if (a.dh) get8(dh + c, n, H[i]);
+            if (a.gate) get_gate(a, (row_gate ? row : unit) * D + c, n, g[i]);
+        }
+        float ry = 1.f;
+        if constexpr (POST) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[0] += vy[i][e] * vy[i][e];
+            team_sum<TEAM>(s, slots, turn);
+            ry = rsqrtf(s[0] * inv + a.eps);
+        }
+        // t and x' (out); the sums of x'^2 and u x'
+        float out[C][8], s2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 8 * (i * TEAM + lane), n = D - c;
+            float f[8];
+            if (a.y) {
+                if (POST && a.wy) get8(a.wy + c, n, f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float b = POST ? vy[i][e] * ry * (a.wy ? f[e] : 1.f) : vy[i][e];
+                    t[i][e] += a.gate ? g[i][e] * b : b;
+                }
+            }
+            if (a.w) get8(a.w + c, n, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                out[i][e] = t[i][e] * scale;
+                if (a.x0) out[i][e] += x0_scale * v0[i][e];
+                s2[0] += out[i][e] * out[i][e];
+                if (a.dh) s2[1] += H[i][e] * (a.w ? f[e] : 1.f) * out[i][e];
+            }
+        }
+        team_sum<TEAM>(s2, slots, turn);
+        const float r = rsqrtf(s2[0] * inv + a.eps), m = s2[1] * r * inv * r;   // (r mean(u n): n = x' r)
+        float ls = 0.f, ls0 = 0.f, s3[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 8 * (i * TEAM + lane), n = D - c;
+            float f[8];
+            if (a.w) get8(a.w + c, n, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float grad = a.dout ? G[i][e] : 0.f;
+                if (a.dh) {
+                    grad += r * (H[i][e] * (a.w ? f[e] : 1.f) - out[i][e] * m);
+                    if constexpr (SUMS) sw[i][e] += H[i][e] * (out[i][e] * r);
+                }
+                ls += grad * t[i][e];
+                if (a.x0) ls0 += grad * v0[i][e];
+                G[i][e] = grad;
+            }
+            if (a.dx0) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = x0_scale * G[i][e];
+                put8(static_cast<EX *>(a.dx0) + row * D + c, n, o);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) G[i][e] *= scale;
+            if (a.out) put8(static_cast<EX *>(a.out) + row * D + c, n, G[i]);
+            if (!a.y) continue;
+            // of y: G becomes db, H e
+            if (POST && a.wy) get8(a.wy + c, n, f);
+            float dg[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float ny = vy[i][e] * ry, wy = POST && a.wy ? f[e] : 1.f;
+                dg[e] = G[i][e] * (POST ? ny * wy : vy[i][e]);
+                if constexpr (SUMS) sg[i][e] += dg[e];
+                if (a.gate) G[i][e] *= g[i][e];
+                if constexpr (POST) {
+                    if constexpr (SUMS) swy[i][e] += G[i][e] * ny;
+                    G[i][e] *= wy;
+                    s3[0] += G[i][e] * ny;
+                }
+            }
+            if (a.dgate) {
+                if (a.gate_bf16) put8(static_cast<__bf16 *>(a.dgate) + row * D + c, n, dg);
+                else put8(static_cast<float *>(a.dgate) + row * D + c, n, dg);
+            }
+        }
+        ds += (double)ls, ds0 += (double)ls0;
+        if (!a.y || !a.h) continue;
+        float m3 = 0.f;
+        if constexpr (POST) {
+            team_sum<TEAM>(s3, slots, turn);
+            m3 = s3[0] * inv;
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = 8 * (i * TEAM + lane), n = D - c;
+            if constexpr (POST) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) G[i][e] = ry * (G[i][e] - vy[i][e] * ry * m3);
+            }
+            put8(static_cast<EY *>(a.h) + row * D + c, n, G[i]);
+        }
+    }
+    if constexpr (SUMS) {
+        if (a.part_g) {
+            leave(a.part_g + (unit * a.parts_per_gate + at) * D, sg);
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sg[i][e] = 0.f;
+        }
+    }
+    }
+    if (a.part_s) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            ds += __shfl_xor(ds, o, 64);
+            ds0 += __shfl_xor(ds0, o, 64);
+        }
+        if ((threadIdx.x & 63) == 0) scalars[0][threadIdx.x >> 6] = ds, scalars[1][threadIdx.x >> 6] = ds0;
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            double s = 0.;
+            for (int w = 0; w < NT / 64; ++w) s += scalars[threadIdx.x][w];
+            a.part_s[2 * part + threadIdx.x] = s;
+        }
+    }
+    if constexpr (SUMS) {
+        if (a.part_w) leave(a.part_w + part * D, sw);
+        if constexpr (POST) {
+            if (a.part_wy) leave(a.part_wy + part * D, swy);
+        }
+    }
+}
+
+struct JoinArgs {
+    const float *part[3];            // of w, wy (all parts together) and the gate (each gate's parts)
+    float *to[2];
+    void *dgate;
+    const double *part_s;
+    float *ds, *ds0;
+    int64_t parts, parts_per_gate, gates;
+    int D, gate_bf16;
+};
+
+// 32 columns of one sum, 32 runs of parts after one another
+__global__ __launch_bounds__(1024) void residual_join_kernel(JoinArgs a) {
+    __shared__ float s[32][33];
+    const int which = blockIdx.z, col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    if (which < 3) {
+        if (!a.part[which]) return;
+        const int64_t n = which < 2 ? a.parts : a.parts_per_gate, sums = which < 2 ? 1 : a.gates;
+        for (int64_t g = blockIdx.y; g < sums; g += gridDim.y) {
+            float v = 0.f;
+            if (col < a.D) {
+#pragma unroll 8
+                for (int64_t p = slice; p < n; p += 32) v += a.part[which][(g * n + p) * a.D + col];
+            }
+            s[slice][threadIdx.x & 31] = v;
+            __syncthreads();
+            if (slice == 0 && col < a.D) {
+                for (int k = 1; k < 32; ++k) v += s[k][threadIdx.x & 31];
+                if (which < 2) a.to[which][col] = v;
+                else if (a.gate_bf16) static_cast<__bf16 *>(a.dgate)[g * a.D + col] = (__bf16)v;
+                else static_cast<float *>(a.dgate)[g * a.D + col] = v;
+            }
+            __syncthreads();
+        }
+        return;
+    }
+    if (!a.part_s || blockIdx.x > 0 || blockIdx.y > 0) return;
+    __shared__ double d[2][16];
+    double v[2] = {0., 0.};
+    for (int64_t p = threadIdx.x; p < a.parts; p += 1024) v[0] += a.part_s[2 * p], v[1] += a.part_s[2 * p + 1];
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+        if ((threadIdx.x & 63) == 0) d[k][threadIdx.x >> 6] = v[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        double t = 0.;
+        for (int w = 0; w < 16; ++w) t += d[threadIdx.x][w];
+        float *to = threadIdx.x == 0 ? a.ds : a.ds0;
+        if (to) *to = (float)t;
+    }
+}
+
+// lanes of a row and chunks per lane
+struct Shape {
+    int team, chunks;
+};
+Shape shape_of(int64_t D) {
+    return D <= 128    ? Shape{16, 1}
+           : D <= 512  ? Shape{64, 1}
+           : D <= 1024 ? Shape{64, 2}
+           : D <= 2048 ? Shape{256, 1}
+           : D <= 4096 ? Shape{256, 2}
+                       : Shape{512, 2};
+}
+int threads_of(int team) { return team > 256 ? team : 256; }
+
+template <class EX, class EY, bool POST>
+void (*forward_of(Shape s))(ResArgs) {
+    return s.team == 16    ? residual_kernel<EX, EY, 16, 1, POST>
+           : s.team == 64  ? (s.chunks == 1 ? residual_kernel<EX, EY, 64, 1, POST> : residual_kernel<EX, EY, 64, 2, POST>)
+           : s.team == 256 ? (s.chunks == 1 ? residual_kernel<EX, EY, 256, 1, POST> : residual_kernel<EX, EY, 256, 2, POST>)
+                           : residual_kernel<EX, EY, 512, 2, POST>;
+}
+template <class EX, class EY, bool POST, bool SUMS>
+void (*backward_of(Shape s))(ResArgs) {
+    return s.team == 16    ? residual_bwd_kernel<EX, EY, 16, 1, POST, SUMS>
+           : s.team == 64  ? (s.chunks == 1 ? residual_bwd_kernel<EX, EY, 64, 1, POST, SUMS> : residual_bwd_kernel<EX, EY, 64, 2, POST, SUMS>)
+           : s.team == 256 ? (s.chunks == 1 ? residual_bwd_kernel<EX, EY, 256, 1, POST, SUMS> : residual_bwd_kernel<EX, EY, 256, 2, POST, SUMS>)
+                           : residual_bwd_kernel<EX, EY, 512, 2, POST, SUMS>;
+}
+// f.operator()<EX, EY> for a pair of types
+template <class F>
+auto of_types(int64_t x, int64_t y, F f) {
+    return x == NOISE_FP32 ? (y == NOISE_FP32 ? f(0.f, 0.f) : f(0.f, (__bf16)0.f)) : f((__bf16)0.f, (__bf16)0.f);
+}
+
+// How the backward pass cuts the rows into the parts of its workgroups: several gates' rows each, or a gate's rows (all rows where
+// no gate is summed) in several parts. About four workgroups of 256 threads per CU, or their threads in larger ones.
+struct Cut {
+    int64_t gates, gates_per_part, parts_per_gate, rows, parts;
+};
+Cut cut_of(int64_t rows, int64_t gate_rows, int64_t D) {
+    const Shape s = shape_of(D);
+    const int64_t teams = threads_of(s.team) / s.team, want = 1024 * 256 / threads_of(s.team);
+    const int64_t unit = gate_rows > 1 ? gate_rows : rows;
+    Cut c;
+    c.gates = rows / unit;
+    const int64_t most = (unit + teams - 1) / teams;
+    int64_t per = (want + c.gates - 1) / c.gates;
+    if (per > most) per = most;
+    c.rows = ((unit + per - 1) / per + teams - 1) / teams * teams;
+    c.parts_per_gate = (unit + c.rows - 1) / c.rows;
+    c.gates_per_part = c.parts_per_gate > 1 ? 1 : (c.gates + want - 1) / want;
+    c.parts = (c.gates + c.gates_per_part - 1) / c.gates_per_part * c.parts_per_gate;
+    return c;
+}
+
+int check(const char *fn, const noise_residual_t *a, float eps) {
+    NOISE_CHECK_ARG(a && a->rows >= 0 && a->dim > 0 && a->dim <= kMaxDim, "%s: rows >= 0 and dim 1 .. %d required", fn, kMaxDim);
+    const bool types = (a->x_type == NOISE_FP32 && (a->y_type == NOISE_FP32 || a->y_type == NOISE_BF16)) ||
+                       (a->x_type == NOISE_BF16 && a->y_type == NOISE_BF16);
+    NOISE_CHECK_ARG(types, "%s: types %lld and %lld", fn, (long long)a->x_type, (long long)a->y_type);
+    NOISE_CHECK_ARG(eps >= 0.f && eps < 3e38f, "%s: eps must be 0 or more", fn);
+    if (a->rows == 0) return NOISE_OK;
+    const size_t sx = a->x_type == NOISE_BF16 ? 2 : 4, sy = a->y_type == NOISE_BF16 ? 2 : 4;
+    NOISE_CHECK_ARG(a->x && aligned(a->x, sx) && aligned(a->y, sy) && aligned(a->x0, sx), "%s: x NULL or a pointer not aligned", fn);
+    NOISE_CHECK_ARG(a->rows <= INT64_MAX / 8 / kMaxDim, "%s: too many rows", fn);
+    NOISE_CHECK_ARG(a->y || (!a->gate && !a->norm_y), "%s: a gate or norm of y without y", fn);
+    NOISE_CHECK_ARG(a->norm_y || !a->y_weight, "%s: a weight of y's norm without the norm", fn);
+    NOISE_CHECK_ARG(a->x0 || !a->x0_scale, "%s: x0_scale without x0", fn);
+    NOISE_CHECK_ARG(aligned(a->scale, 4) && aligned(a->x0_scale, 4) && aligned(a->y_weight, 4) && aligned(a->weight, 4),
+                    "%s: a pointer is not aligned to its type", fn);
+    if (a->gate) {
+        NOISE_CHECK_ARG(a->gate_type == NOISE_BF16 || a->gate_type == NOISE_FP32, "%s: unknown gate type", fn);
+        NOISE_CHECK_ARG(a->gate_rows > 0 && a->rows % a->gate_rows == 0 && aligned(a->gate, a->gate_type == NOISE_BF16 ? 2 : 4),
+                        "%s: rows must be a multiple of gate_rows", fn);
+    }
+    return NOISE_OK;
+}
+
+ResArgs args_of(const noise_residual_t *r, float eps) {
+    ResArgs a = {};
+    a.x = r->x, a.y = r->y, a.x0 = r->x0, a.gate = r->gate;
+    a.scale = r->scale, a.x0_scale = r->x0_scale, a.wy = r->y_weight, a.w = r->weight;
+    a.rows = r->rows, a.gate_rows = r->gate ? r->gate_rows : r->rows;
+    a.s_x = r->x_stride, a.s_y = r->y_stride, a.s_x0 = r->x0_stride;
+    a.D = (int)r->dim, a.gate_bf16 = r->gate_type == NOISE_BF16, a.eps = eps;
+    return a;
+}
+
+}  // namespace
+}  // namespace noise
+
+using namespace noise;
+
+extern "C" int noise_residual_norm(const noise_residual_t *r, void *out, void *h, float eps, noise_stream_t stream) {
+    clear_error();
+    const char *fn = "noise_residual_norm";
+    if (int e = check(fn, r, eps)) return e;
+    if (r->rows == 0) return NOISE_OK;
+    NOISE_CHECK_ARG(out && h && aligned(out, r->x_type == NOISE_BF16 ? 2 : 4) && aligned(h, r->y_type == NOISE_BF16 ? 2 : 4),
+                    "%s: an output is NULL or not aligned to its type", fn);
+    ResArgs a = args_of(r, eps);
+    a.out = out, a.h = h;
+    const Shape s = shape_of(r->dim);
+    auto kernel = of_types(r->x_type, r->y_type, [&](auto x, auto y) {
+        return r->norm_y ? forward_of<decltype(x), decltype(y), true>(s) : forward_of<decltype(x), decltype(y), false>(s);
+    });
+    const int threads = threads_of(s.team);
+    const int64_t teams = threads / s.team, groups = (r->rows + teams - 1) / teams;
+    for (a.first = 0; a.first < groups; a.first += kLaunchGroups) {
+        const int64_t n = groups - a.first < kLaunchGroups ? groups - a.first : kLaunchGroups;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 0, (hipStream_t)stream, a);
+    }
+    return launch_status(fn);
+}
+
+extern "C" int64_t noise_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t gate_rows, int64_t dim) {
+    if (rows <= 0 || gate_rows <= 0 || dim <= 0 || dim > kMaxDim) return 0;
+    const Cut c = cut_of(rows, gate_rows, dim);
+    return c.parts * (2 * 4 * dim + 16) + c.gates * c.parts_per_gate * 4 * dim;
+}
+
+extern "C" int noise_residual_norm_bwd(const noise_residual_t *r, const void *dout, const void *dh,
+                                       const noise_residual_grads_t *d, float eps, void *workspace, int64_t workspace_bytes,
+                                       noise_stream_t stream) {
+    clear_error();
+    const char *fn = "noise_residual_norm_bwd";
+    if (int e = check(fn, r, eps)) return e;
+    NOISE_CHECK_ARG(d, "%s: NULL pointer", fn);
+    const size_t sx = r->x_type == NOISE_BF16 ? 2 : 4, sy = r->y_type == NOISE_BF16 ? 2 : 4;
+    NOISE_CHECK_ARG(aligned(dout, sx) && aligned(dh, sy) && aligned(d->dx, sx) && aligned(d->dy, sy) && aligned(d->dx0, sx) &&
+                        aligned(d->dgate, r->gate_type == NOISE_BF16 ? 2 : 4) && aligned(d->dscale, 4) &&
+                        aligned(d->dx0_scale, 4) && aligned(d->dy_weight, 4) && aligned(d->dweight, 4),
+                    "%s: a pointer is not aligned to its type", fn);
+    NOISE_CHECK_ARG((r->y || !d->dy) && (r->x0 || (!d->dx0 && !d->dx0_scale)) && (r->gate || !d->dgate) &&
+                        (r->norm_y || !d->dy_weight),
+                    "%s: a gradient of an absent tensor", fn);
+    ResArgs a = args_of(r, eps);
+    const bool row_gate = r->gate && r->gate_rows == 1 && r->rows > 1;
+    const bool sums = d->dweight || d->dy_weight || (d->dgate && !row_gate);
+    const bool scalars = d->dscale || d->dx0_scale;
+    a.dout = dout, a.dh = dh, a.out = d->dx, a.h = d->dy, a.dx0 = d->dx0;
+    a.dgate = row_gate ? d->dgate : nullptr;
+    if (r->rows == 0) return NOISE_OK;
+    const Cut c = cut_of(r->rows, a.gate_rows, r->dim);
+    const int64_t parts = c.parts;
+    if (sums || scalars) {
+        const int64_t need = noise_residual_norm_bwd_workspace_bytes(r->rows, a.gate_rows, r->dim);
+        NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= need,
+                        "%s: workspace of %lld bytes (16 B aligned) required", fn, (long long)need);
+        char *w = static_cast<char *>(workspace);
+        if (scalars) a.part_s = reinterpret_cast<double *>(w);
+        w += 16 * parts;
+        if (d->dweight) a.part_w = reinterpret_cast<float *>(w);
+        w += 4 * parts * r->dim;
+        if (d->dy_weight) a.part_wy = reinterpret_cast<float *>(w);
+        w += 4 * parts * r->dim;
+        if (d->dgate && !row_gate) a.part_g = reinterpret_cast<float *>(w);
+    }
+    const Shape s = shape_of(r->dim);
+    auto kernel = of_types(r->x_type, r->y_type, [&](auto x, auto y) {
+        using X = decltype(x);
+        using Y = decltype(y);
+        return r->norm_y ? (sums ? backward_of<X, Y, true, true>(s) : backward_of<X, Y, true, false>(s))
+                         : (sums ? backward_of<X, Y, false, true>(s) : backward_of<X, Y, false, false>(s));
+    });
+    a.gates = c.gates, a.gates_per_part = c.gates_per_part, a.parts_per_gate = c.parts_per_gate, a.part_rows = c.rows;
+    for (a.first = 0; a.first < parts; a.first += kLaunchGroups) {
+        const int64_t n = parts - a.first < kLaunchGroups ? parts - a.first : kLaunchGroups;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads_of(s.team)), 0, (hipStream_t)stream, a);
+    }
+    if (sums || scalars) {
+        JoinArgs j;
+        j.part[0] = a.part_w, j.part[1] = a.part_wy, j.part[2] = a.part_g, j.part_s = a.part_s;
+        j.to[0] = d->dweight, j.to[1] = d->dy_weight, j.dgate = d->dgate, j.ds = d->dscale, j.ds0 = d->dx0_scale;
+        j.parts = parts, j.parts_per_gate = c.parts_per_gate, j.gates = c.gates, j.D = (int)r->dim, j.gate_bf16 = a.gate_bf16;
+        const unsigned gates = !a.part_g ? 1 : c.gates < 4096 ? (unsigned)c.gates : 4096;
+        hipLaunchKernelGGL(residual_join_kernel, dim3((unsigned)(r->dim + 31) / 32, gates, 4), dim3(1024), 0,
+                           (hipStream_t)stream, j);
+    }
+    return launch_status(fn);
+}

@@ -19,6 +19,7 @@ import torch
 
 from . import _lib
 from ._lib import ATTN_QK_NORMED, ATTN_V_TRANSPOSED
+from .clip import clip_gradients
 from .model import rotary_tables, window_sizes, has_ve, N_EMBD, N_HEAD, HEAD_DIM, VOCAB
 from .noise import GATHER_ROWS, DeviceGenerator, OrthogonalDraws
 
@@ -856,9 +857,10 @@ class Eggroll:
                       need, stream)
         return grads
 
-    def step(self, x, y, optimizer, step, chunk=512, update_chunk=4096):
+    def step(self, x, y, optimizer, step, chunk=512, update_chunk=4096, max_norm=None):
         """eggroll.py:131-168 on one GPU: evaluate the population, rebuild the update, step the optimizer;
-        returns the mean loss."""
+        returns the mean loss. max_norm (None, as there: no bound) clips the update's global norm first
+        (noise_amd.clip.clip_gradients)."""
         if self.world != 1:
             raise NotImplementedError('Eggroll.step gathers losses across ranks in the reference; this library '
                                       'runs one GPU (call population() per rank and gather the losses first)')
@@ -867,6 +869,8 @@ class Eggroll:
         optimizer.zero_grad(set_to_none=True)
         for name, p in self.params.items():
             p.grad = grads[name]
+        if max_norm is not None:
+            clip_gradients(grads.values(), max_norm)
         optimizer.step()
         return losses.mean().item()
 

@@ -25,8 +25,10 @@ from torch import Tensor
 from torch.autograd import forward_ad
 from torch.library import custom_op
 
+from . import clip as _clip
 from . import distill as _distill
 from . import dust, eggroll, model
+from . import residual as _residual
 from . import sinks as _sinks
 
 BLOCK_WEIGHTS = ('q', 'k', 'v', 'gate', 'proj', 'fc', 'out')
@@ -282,3 +284,60 @@ def _distill_loss_backward(ctx, weight):
 
 
 distill_loss.register_autograd(_distill_loss_backward, setup_context=_distill_loss_setup)
+
+
+@custom_op('noise_amd::clip_gradients', mutates_args=('gradients',))
+def clip_gradients(gradients: List[Tensor], max_norm: float) -> Tensor:
+    _backwards_only('clip_gradients')
+    with torch.no_grad():
+        return _clip.clip('clip_gradients', gradients, max_norm)
+
+
+@clip_gradients.register_fake
+def _clip_gradients_fake(gradients, max_norm):
+    return gradients[0].new_empty((), dtype=torch.float32)
+
+
+@custom_op('noise_amd::residual_norm', mutates_args=())
+def residual_norm(x: Tensor, y: Optional[Tensor], x0: Optional[Tensor], scale: Optional[Tensor], x0_scale: Optional[Tensor],
+                  gate: Optional[Tensor], y_weight: Optional[Tensor], weight: Optional[Tensor], norm_y: bool,
+                  dtype: Optional[torch.dtype], eps: float) -> Tuple[Tensor, Tensor]:
+    _backwards_only('residual_norm')
+    return _residual.forward(x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps)
+
+
+@residual_norm.register_fake
+def _residual_norm_fake(x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps):
+    return x.new_empty(x.shape), x.new_empty(x.shape, dtype=dtype or (x if y is None else y).dtype)
+
+
+@custom_op('noise_amd::residual_norm_backward', mutates_args=())
+def residual_norm_backward(dout: Optional[Tensor], dh: Optional[Tensor], x: Tensor, y: Optional[Tensor], x0: Optional[Tensor],
+                           scale: Optional[Tensor], x0_scale: Optional[Tensor], gate: Optional[Tensor],
+                           y_weight: Optional[Tensor], weight: Optional[Tensor], norm_y: bool, dtype: Optional[torch.dtype],
+                           eps: float, needs: List[bool]) -> List[Tensor]:
+    """The gradients that `needs` asks for, in its order (empty tensors in the others' places)"""
+    _backwards_only('residual_norm_backward')
+    grads = _residual.backward(dout, dh, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps, needs)
+    return [x.new_empty(0) if g is None else g for g in grads]
+
+
+@residual_norm_backward.register_fake
+def _residual_norm_backward_fake(dout, dh, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps, needs):
+    given = (x, y, x0, scale, x0_scale, gate, y_weight, weight)
+    return [t.new_empty(t.shape) if n and t is not None else x.new_empty(0) for t, n in zip(given, needs)]
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    *tensors, ctx.norm_y, ctx.dtype, ctx.eps = inputs
+    ctx.save_for_backward(*tensors)
+    ctx.set_materialize_grads(False)
+
+
+def _residual_norm_backward(ctx, dout, dh):
+    tensors, needs = ctx.saved_tensors, [bool(n) for n in ctx.needs_input_grad[:8]]
+    grads = torch.ops.noise_amd.residual_norm_backward(dout, dh, *tensors, ctx.norm_y, ctx.dtype, ctx.eps, needs)
+    return (*(g if n and t is not None else None for g, n, t in zip(grads, needs, tensors)), None, None, None)
+
+
+residual_norm.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
