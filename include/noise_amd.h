@@ -752,6 +752,31 @@ int64_t noise_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t gate_rows,
 int noise_residual_norm_bwd(const noise_residual_t *r, const void *dout, const void *dh, const noise_residual_grads_t *grads,
                             float eps, void *workspace, int64_t workspace_bytes, noise_stream_t stream);
 
+/* Cross entropy of a linear head, without its logits in memory: for each of `rows` rows x_r [dim] with a target t_r in 0 ..
+ * vocab - 1,
+ *   z = cap(x weight^T),  cap(z) = softcap tanh(z / softcap) (softcap 0: z; else 1e-6 .. 1e6),
+ *   loss_r = lse_r - z[t_r],  lse_r = log sum_{v < vocab} exp z[v].
+ * A row with any other target has loss 0 and no gradient, and may hold anything. x and weight are of `type` (bf16, or fp32, whose
+ * products keep 21 bits of each operand), with row strides in elements; rows 0 .. 2^30, dim 1 .. 65536, vocab 1 .. 2^22. targets: int32,
+ * or int64 with targets_wide. workspace: noise_vocab_workspace_bytes (16 B aligned; -1 for arguments that would be refused). */
+typedef struct {
+    const void *x;
+    int64_t x_stride;
+    const void *weight;
+    int64_t weight_stride;
+    const void *targets;
+    int64_t targets_wide, rows, dim, vocab, type;
+} noise_vocab_t;
+int64_t noise_vocab_workspace_bytes(const noise_vocab_t *v, int with_grad);
+/* loss: fp32 [rows]; lse (NULL: not asked for): fp32 [rows], what the gradients need (0 without a target) */
+int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace, int64_t workspace_bytes,
+                     noise_stream_t stream);
+/* The gradients of sum_r weight[r] loss[r] (weight fp32 [rows], NULL: ones), each optional (NULL): dx [rows][dim] and dweight
+ * [width][dim], contiguous, of `type`; rows of dweight from vocab on are zeros. Either lse of the loss call comes in, or the
+ * losses come out in the same call. With rows 0 nothing is written. */
+int noise_vocab_grad(const noise_vocab_t *v, float softcap, const float *weight, const float *lse, float *loss, void *dx,
+                     void *dweight, int64_t width, void *workspace, int64_t workspace_bytes, noise_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -89,6 +89,9 @@ SIGNATURES = {
     'noise_residual_norm': [_p, _p, _p, _f32, _p],
     'noise_residual_norm_bwd_workspace_bytes': [_i64, _i64, _i64],
     'noise_residual_norm_bwd': [_p, _p, _p, _p, _f32, _p, _i64, _p],
+    'noise_vocab_workspace_bytes': [_p, _i32],
+    'noise_vocab_loss': [_p, _f32, _p, _p, _p, _i64, _p],
+    'noise_vocab_grad': [_p, _f32, _p, _p, _p, _p, _p, _i64, _p, _i64, _p],
     'noise_clip_workspace_bytes': [_i64],
     'noise_clip_gradients': [_p, _i64, _f32, _p, _p, _i64, _p],
 }
@@ -97,7 +100,8 @@ _RESTYPES = {'noise_last_error': ctypes.c_char_p, 'noise_update_workspace_bytes'
              'noise_dust_block_workspace_bytes': ctypes.c_int64, 'noise_dust_block_static_max_bytes': ctypes.c_int64,
              'noise_qk_norm_rotary_bwd_workspace_bytes': ctypes.c_int64,
              'noise_sink_attention_bwd_workspace_bytes': ctypes.c_int64, 'noise_sink_decode_workspace_bytes': ctypes.c_int64,
-             'noise_clip_workspace_bytes': ctypes.c_int64, 'noise_residual_norm_bwd_workspace_bytes': ctypes.c_int64}
+             'noise_clip_workspace_bytes': ctypes.c_int64, 'noise_residual_norm_bwd_workspace_bytes': ctypes.c_int64,
+             'noise_vocab_workspace_bytes': ctypes.c_int64}
 
 # y_fp32 of noise_pop_linear / noise_rank1_expand: fp32 output in autocast's form (bf16 product and dot)
 LINEAR_AUTOCAST = 2

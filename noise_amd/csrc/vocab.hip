@@ -1,0 +1,666 @@
+// Cross entropy of a linear head over a vocabulary, with its gradients, without the logits in memory: for each row x_r with a target
+// t_r in 0 .. V - 1, z = cap(x W^T),
+//   loss_r = lse_r - z_{r,t_r},  dZ_rv = w_r (exp(z_rv - lse_r) - [v = t_r]) cap'(z_rv),  dx = dZ W,  dW = dZ^T x,
+// cap(z) = softcap tanh(z / softcap), cap' = 1 - (cap / softcap)^2. (The head is utils/model.py:204-206 and train/val/run.py:89-94.)
+//
+// Rows without a target take no part: the others are packed one after the other (which also zeroes what stands between them and
+// the end of a tile), and all counts of rows are read on the device. Rows are worked on in pieces, so that dZ never takes more
+// than kPieceBytes. Per piece, four products of R V D multiply-adds (two for the loss alone):
+//   loss_kernel     a tile of logits in registers, its rows' maxima and sums of exponentials left per 128 vocabulary entries;
+//                   lse_join_kernel adds those up
+//   dz_kernel       the logits once more, and dZ from them in 16 bits
+//   dx_kernel, dw_kernel  the gradients; k is split over workgroups where there are few tiles, with fp32 sums joined in order
+// fp32 operands are held as sums of two fp16 values, scaled by a power of two per tensor (hi carries 11 bits of a value, lo the next
+// 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term.
+#include "vocab_gemm.hpp"
+
+namespace noise {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.4028234663852886e38f;
+constexpr int64_t kPieceBytes = 1ll << 31;   // of dZ
+constexpr int kSegment = 128;                // vocabulary entries per partial maximum and sum
+constexpr int kPad = 256;                    // rows of the packed matrices and of dZ come in these
+
+using Tile = Tiling<256, 256, 2, 4, 64, 2>;
+
+// What the kernels share. Row indices are those of the packed rows.
+struct HeadArgs {
+    Operand x, w, dz;
+    const int *count;            // packed rows
+    const int *live;             // packed row -> row
+    const int *target;           // of a packed row
+    const float *scales;         // 2^ex, 2^ew, 2^ed of fp32 operands (x, w, dZ), else 1
+    const float *weight;         // of a packed row's loss
+    float *lse, *zt;             // of a packed row
+    float2 *partial;             // [segments][rows]
+    int64_t row0;                // the piece's first packed row
+    int64_t rows;                // packed rows, at most (the partials' stride)
+    int64_t piece;               // rows of the piece, at most
+    int vocab, dim, nk;          // nk: stages of k over dim
+    int tiles_m, tiles_n, splits;
+    float softcap;
+    void *out;                   // dx or dW
+    int64_t out_ld;
+    float *slabs;                // [splits][n][m] where k is split
+    float *sum;                  // dW over several pieces: fp32 [vocab][dim]
+    int add, fp32;               // add: to sum's values; fp32: out's type
+};
+
+__device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
+    const int64_t n = *a.count - a.row0;
+    return n < 0 ? 0 : n < a.piece ? n : a.piece;
+}
+
+// softcap tanh(z / softcap) with an error of 2^-22 softcap: what enters exp(z) is absolute
+__device__ __forceinline__ float cap_of(float z, float cap, float k) {
+    return cap - 2.f * cap * __builtin_amdgcn_rcpf(exp2_fast(z * k) + 1.f);
+}
+
+// --- rows with a target, packed ---
+
+__global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, int wide, int64_t rows, int64_t vocab,
+                                                          const float *weight, int *count, int *live, int *place, int *target,
+                                                          float *live_weight, float *weight_max) {
+    __shared__ int sums[16];
+    __shared__ float tops[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int base = 0;
+    float top = 0.f;
+    for (int64_t r0 = 0; r0 < rows; r0 += 1024) {
+        const int64_t r = r0 + threadIdx.x;
+        int64_t t = -1;
+        if (r < rows) t = wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
+        const bool in = t >= 0 && t < vocab;
+        const uint64_t mask = __ballot(in);
+        if (lane == 0) sums[wave] = __popcll(mask);
+        __syncthreads();
+        int before = base, all = 0;
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) before += sums[w];
+            all += sums[w];
+        }
+        before += __popcll(mask & ((1ull << lane) - 1));
+        if (r < rows) place[r] = in ? before : -1;
+        if (in) {
+            live[before] = (int)r;
+            target[before] = (int)t;
+            const float w = weight ? weight[r] : 1.f;
+            if (live_weight) live_weight[before] = w;
+            if (fabsf(w) < __builtin_inff()) top = fmaxf(top, fabsf(w));
+        }
+        base += all;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) top = fmaxf(top, tops[w]);
+        *weight_max = top;
+        *count = base;
+    }
+}
+
+// --- operands ---
+
+// Largest finite |v| of the matrix's rows (x: of those with a target), one value per workgroup
+__global__ __launch_bounds__(256) void vocab_max_kernel(const float *src, int64_t ld, int64_t rows, int64_t dim, const int *place,
+                                                        float *to) {
+    __shared__ float tops[4];
+    float top = 0.f;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        if (place && place[r] < 0) continue;
+        for (int64_t c = threadIdx.x; c < dim; c += 256) {
+            const float v = fabsf(src[r * ld + c]);
+            if (v < __builtin_inff()) top = fmaxf(top, v);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) to[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+
+constexpr int kMaxParts = 512;
+
+// The power of two that takes `top` to 2^14 .. 2^15 (within 2^-100 .. 2^100)
+__device__ __forceinline__ float scale_of(float top) {
+    if (!(top > 0.f)) return 1.f;
+    int e = 14 - ilogbf(top);
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    return ldexpf(1.f, e);
+}
+
+__global__ __launch_bounds__(64) void vocab_scale_kernel(const float *x_max, const float *w_max, int n, const float *d_max, float *scales) {
+    float x = 0.f, w = 0.f;
+    for (int i = threadIdx.x; i < n; i += 64) x = fmaxf(x, x_max[i]), w = fmaxf(w, w_max[i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64)), w = fmaxf(w, __shfl_xor(w, o, 64));
+    if (threadIdx.x == 0) scales[0] = scale_of(x), scales[1] = scale_of(w), scales[2] = scale_of(*d_max);
+}
+
+// v s as a sum of two fp16 values, as bits
+__device__ __forceinline__ void halves(float v, float s, uint16_t &hi, uint16_t &lo) {
+    const float f = v * s;
+    const _Float16 h = (_Float16)f;
+    const float rest = fabsf(f) < __builtin_inff() ? f - (float)h : 0.f;
+    const _Float16 l = (_Float16)rest;
+    __builtin_memcpy(&hi, &h, 2);
+    __builtin_memcpy(&lo, &l, 2);
+}
+
+// One workgroup per source row: the row to its place (none: left out), zeros from dim to ld; and zeros in the rows behind the last,
+// `padded` in all. dx: gradient rows to zero where a row has no place.
+template <class E, bool SPLIT>
+__global__ __launch_bounds__(256) void vocab_pack_kernel(const E *src, int64_t src_ld, int64_t rows, int64_t first, int64_t dim,
+                                                         const int *place, const int *count, int64_t padded, const float *scale,
+                                                         Operand to, E *dx) {
+    const int64_t r = first + blockIdx.x;
+    uint16_t *dst = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(to.ptr));
+    auto zero = [&](int64_t at) {
+        for (int64_t c = threadIdx.x; c < to.ld; c += 256) {
+            dst[at * to.ld + c] = 0;
+            if (SPLIT) dst[to.lo + at * to.ld + c] = 0;
+        }
+    };
+    const int64_t behind = place ? *count : rows;
+    if (r >= behind && r < padded) zero(r);
+    if (r >= rows) return;
+    const int64_t at = place ? place[r] : r;
+    if (at < 0) {
+        if (dx)
+            for (int64_t c = threadIdx.x; c < dim; c += 256) dx[r * dim + c] = (E)0.f;
+        return;
+    }
+    const float s = SPLIT ? *scale : 1.f;
+    for (int64_t c = threadIdx.x; c < to.ld; c += 256) {
+        if constexpr (SPLIT) {
+            uint16_t hi = 0, lo = 0;
+            if (c < dim) halves((float)src[r * src_ld + c], s, hi, lo);
+            dst[at * to.ld + c] = hi, dst[to.lo + at * to.ld + c] = lo;
+        } else {
+            uint16_t bits = 0;
+            if (c < dim) __builtin_memcpy(&bits, src + r * src_ld + c, 2);
+            dst[at * to.ld + c] = bits;
+        }
+    }
+}
+
+// --- logits ---
+
+// The tile's logits, capped and unscaled; -inf past the vocabulary
+template <class T, bool CAP>
+__device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, float unit, f32x16 (&acc)[T::FB][T::NB]) {
+    const float k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
+    const bool edge = m0 + T::FB * 32 > a.vocab;
+#pragma unroll
+    for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+        for (int j = 0; j < T::NB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float z = acc[i][j][r] * unit;
+                if (CAP) z = cap_of(z, a.softcap, k);
+                if (edge && m0 + 32 * i + 16 * (r / 8) + 8 * (lane >> 5) + r % 8 >= a.vocab) z = -__builtin_inff();
+                acc[i][j][r] = z;
+            }
+}
+
+template <class T, bool SPLIT, bool CAP>
+__global__ __launch_bounds__(64 * T::NW) void vocab_loss_kernel(HeadArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    if ((int64_t)tn * T::NT >= piece_rows(a)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f32x16 acc[T::FB][T::NB];
+    product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
+                                           T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
+    const int m0 = tm * T::MT + T::wm(wave);
+    if (m0 >= a.vocab) return;
+    const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f;
+    to_logits<T, CAP>(a, m0, lane, unit, acc);
+    static_assert(T::FB * 32 == kSegment, "a wave's entries are a segment");
+#pragma unroll
+    for (int j = 0; j < T::NB; ++j) {
+        const int64_t row = a.row0 + (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
+        float top = kLowest;
+#pragma unroll
+        for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+        top = fmaxf(top, swap_halves(top));
+        const float shift = top * kLog2e;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -shift));
+        s += swap_halves(s);
+        if (lane < 32) a.partial[(int64_t)(m0 / kSegment) * a.rows + row] = float2{top, s};
+        const int t = row < *a.count ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
+        if (t >= 0 && t < kSegment && !(t & 8)) {
+#pragma unroll
+            for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t == 32 * i + 16 * (r / 8) + r % 8) a.zt[row] = acc[i][j][r];
+        }
+    }
+}
+
+// lse of 32 rows, 8 runs of segments each; the losses
+__global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segments, float *loss, float *lse) {
+    __shared__ float tops[8][33], sums[8][33];
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int slice = threadIdx.x >> 5;
+    const int64_t end = a.row0 + piece_rows(a);
+    float top = kLowest, s = 0.f;
+    if (row < end)
+#pragma unroll 4
+        for (int g = slice; g < segments; g += 8) {
+            const float2 p = a.partial[(int64_t)g * a.rows + row];
+            const float m = fmaxf(top, p.x);
+            s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
+            top = m;
+        }
+    tops[slice][threadIdx.x & 31] = top;
+    sums[slice][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (slice || row >= end) return;
+    for (int k = 1; k < 8; ++k) {
+        const float x = tops[k][threadIdx.x & 31], m = fmaxf(top, x);
+        s = s * exp2_fast((top - m) * kLog2e) + sums[k][threadIdx.x & 31] * exp2_fast((x - m) * kLog2e);
+        top = m;
+    }
+    const float l = top + logf(s);
+    const int to = a.live[row];
+    a.lse[row] = l;
+    if (loss) loss[to] = l - a.zt[row];
+    if (lse) lse[to] = l;
+}
+
+// lse of the packed rows from the forward pass's
+__global__ __launch_bounds__(256) void vocab_lse_gather_kernel(const int *count, const int *live, const float *lse, float *to) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r < *count) to[r] = lse[live[r]];
+}
+
+// zeros: losses (and lse) of rows without a target; rows of dW past the vocabulary
+__global__ __launch_bounds__(256) void vocab_zero_kernel(float *loss, float *lse, const int *place, int64_t rows) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= rows || place[r] >= 0) return;
+    if (loss) loss[r] = 0.f;
+    if (lse) lse[r] = 0.f;
+}
+__global__ __launch_bounds__(256) void vocab_fill_kernel(uint16_t *p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+template <class T, bool SPLIT, bool CAP>
+__global__ __launch_bounds__(64 * T::NW) void vocab_dz_kernel(HeadArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t rows = piece_rows(a);
+    if ((int64_t)tn * T::NT >= rows) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f32x16 acc[T::FB][T::NB];
+    product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
+                                           T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
+    const int m0 = tm * T::MT + T::wm(wave);
+    const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f;
+    to_logits<T, CAP>(a, m0, lane, unit, acc);
+    uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr));
+#pragma unroll
+    for (int j = 0; j < T::NB; ++j) {
+        const int64_t at = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31), row = a.row0 + at;
+        const bool there = at < rows;
+        const float w = there ? (a.weight ? a.weight[row] : 1.f) * (SPLIT ? a.scales[2] : 1.f) : 0.f;
+        const float shift = there ? a.lse[row] * kLog2e : 0.f;
+        const int t = there ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
+#pragma unroll
+        for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint16_t hi[8], lo[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = acc[i][j][8 * h + e];
+                    float d = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
+                    if (t == 32 * i + 16 * h + e) d -= 1.f;
+                    if (CAP) {
+                        const float u = z / a.softcap;
+                        d *= z == -__builtin_inff() ? 0.f : 1.f - u * u;
+                    }
+                    d = there ? d * w : 0.f;
+                    if constexpr (SPLIT) halves(d, 1.f, hi[e], lo[e]);
+                    else {
+                        const __bf16 b = (__bf16)d;
+                        __builtin_memcpy(&hi[e], &b, 2);
+                    }
+                }
+                uint16_t *to = dz + at * a.dz.ld + m0 + 32 * i + 16 * h + 8 * (lane >> 5);
+                __builtin_memcpy(__builtin_assume_aligned(to, 16), hi, 16);
+                if constexpr (SPLIT) __builtin_memcpy(__builtin_assume_aligned(to + a.dz.lo, 16), lo, 16);
+            }
+    }
+}
+
+// --- gradients ---
+
+// 8 consecutive results, of which n exist, in the output's type at any address of that type
+__device__ __forceinline__ void put_out(const HeadArgs &a, int64_t at, int n, const float (&v)[8]) {
+    if (a.fp32) {
+        float *p = static_cast<float *>(a.out) + at;
+        if (n >= 8) __builtin_memcpy(p, v, 32);
+        else
+            for (int e = 0; e < 8; ++e)
+                if (e < n) p[e] = v[e];
+    } else {
+        __bf16 o[8], *p = static_cast<__bf16 *>(a.out) + at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (__bf16)v[e];
+        if (n >= 8) __builtin_memcpy(p, o, 16);
+        else
+            for (int e = 0; e < 8; ++e)
+                if (e < n) p[e] = o[e];
+    }
+}
+
+// DX: out row = row of x, n = packed row; otherwise (dW) n = vocabulary entry. m: columns of dim.
+template <class T, bool DX, bool SPLIT>
+__global__ __launch_bounds__(64 * T::NW) void vocab_grad_kernel(HeadArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+    const int tiles = a.tiles_m * a.tiles_n, split = blockIdx.x / tiles;
+    int tm, tn;
+    tile_of(blockIdx.x - split * tiles, a.tiles_m, a.tiles_n, tm, tn);
+    const int64_t rows = piece_rows(a);
+    const int64_t n_end = DX ? rows : a.vocab;
+    if ((int64_t)tn * T::NT >= n_end) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nk = (int)(((DX ? a.vocab : rows) + T::BK - 1) / T::BK), all = SPLIT ? 3 * nk : nk;
+    const int first = (int)((int64_t)all * split / a.splits), last = (int)((int64_t)all * (split + 1) / a.splits);
+    const int dim8 = (int)a.x.ld / 8;   // chunks of a packed row
+    f32x16 acc[T::FB][T::NB];
+    if (DX)
+        product<T, true, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
+                                              T::NT - 1, nk, first, last, a.vocab, lds, acc);
+    else {
+        Operand x = a.x;
+        x.ptr += a.row0 * x.ld;
+        product<T, true, true, SPLIT, SPLIT>(x, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
+                                             (int)(a.dz.ld - (int64_t)tn * T::NT) / 8 - 1, nk, first, last, 1ll << 40, lds, acc);
+    }
+    const float unit = SPLIT ? 1.f / a.scales[2] / a.scales[DX ? 1 : 0] : 1.f;
+#pragma unroll
+    for (int j = 0; j < T::NB; ++j) {
+        const int64_t n = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
+        if (n >= n_end) continue;
+        const int64_t to = DX ? a.live[a.row0 + n] : n;
+#pragma unroll
+        for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int m = tm * T::MT + T::wm(wave) + 32 * i + 16 * h + 8 * (lane >> 5);
+                if (m >= a.dim) continue;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * h + e] * unit;
+                const int left = a.dim - m;
+                if (a.splits > 1) {
+                    float *p = a.slabs + ((int64_t)split * (DX ? a.piece : a.vocab) + n) * a.x.ld + m;
+                    __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
+                    continue;
+                }
+                if (a.sum) {
+                    float *p = a.sum + n * a.x.ld + m;
+                    if (a.add)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += p[e];
+                    if (!a.out) __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
+                }
+                if (a.out) put_out(a, to * a.out_ld + m, left, v);
+            }
+    }
+}
+
+// The splits' sums, in order
+template <bool DX>
+__global__ __launch_bounds__(256) void vocab_sum_kernel(HeadArgs a) {
+    const int64_t rows = piece_rows(a), n_end = DX ? rows : a.vocab, per = a.x.ld / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / per;
+    const int m = (int)(i - n * per) * 8;
+    if (n >= n_end || m >= a.dim) return;
+    float v[8] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float *p = a.slabs + ((int64_t)s * (DX ? a.piece : a.vocab) + n) * a.x.ld + m;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += p[e];
+    }
+    if (a.sum) {
+        float *p = a.sum + n * a.x.ld + m;
+        if (a.add)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += p[e];
+        if (!a.out) __builtin_memcpy(p, v, 32);
+    }
+    if (a.out) put_out(a, (DX ? a.live[a.row0 + n] : n) * a.out_ld + m, a.dim - m, v);
+}
+
+// --- host ---
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// The workspace's parts, and how the work is cut
+struct Plan {
+    int64_t ld, rows, piece, pieces, vocab_ld, segments;
+    int nk;
+    bool split, pack_w;
+    int dx_splits, dw_splits;
+    int64_t at_int, at_float, at_partial, at_x, at_w, at_dz, at_slabs, at_sum, bytes;
+};
+
+int splits_of(int64_t tiles, int64_t stages) {
+    // a tile per CU, but no fewer than 8 stages of k per workgroup
+    int64_t s = 256 / (tiles > 256 ? 256 : tiles);
+    if (s > stages / 8) s = stages / 8;
+    return s < 1 ? 1 : (int)s;
+}
+
+Plan plan_of(const noise_vocab_t *v, bool grad) {
+    Plan p = {};
+    p.split = v->type == NOISE_FP32;
+    p.ld = up(v->dim, Tile::BK);
+    p.nk = (int)(p.ld / Tile::BK);
+    p.rows = up(v->rows, kPad);
+    p.vocab_ld = up(v->vocab, Tile::MT);
+    p.segments = (v->vocab + kSegment - 1) / kSegment;
+    const int64_t parts = p.split ? 2 : 1;
+    int64_t most = kPieceBytes / (2 * parts * p.vocab_ld) / kPad * kPad;
+    if (most < kPad) most = kPad;
+    p.piece = p.rows < most ? p.rows : most;
+    // pieces of one size
+    p.pieces = (p.rows + p.piece - 1) / p.piece;
+    p.piece = up((p.rows + p.pieces - 1) / p.pieces, kPad);
+    p.pieces = (p.rows + p.piece - 1) / p.piece;
+    // the weight is read where it is if its rows are whole stages of k at 16 B addresses
+    p.pack_w = p.split || v->dim % Tile::BK || v->weight_stride % 8 || !aligned(v->weight, 16) || v->weight_stride >= (1 << 23);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += up(bytes, 1024);
+        return here;
+    };
+    p.at_int = take(4 * (3 * p.rows + 1));
+    p.at_float = take(4 * (3 * p.rows + 4 + 2 * kMaxParts));
+    p.at_partial = take(8 * p.segments * p.rows);
+    p.at_x = take(2 * parts * p.rows * p.ld);
+    if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
+    if (grad) {
+        p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
+        const int64_t tm = (p.ld + Tile::MT - 1) / Tile::MT;
+        p.dx_splits = splits_of(tm * (p.piece / Tile::NT), (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK);
+        p.dw_splits = splits_of(tm * ((v->vocab + Tile::NT - 1) / Tile::NT), (p.split ? 3 : 1) * p.piece / Tile::BK);
+        int64_t slabs = p.dx_splits > 1 ? 4 * p.dx_splits * p.piece * p.ld : 0;
+        const int64_t dw = p.dw_splits > 1 ? 4 * p.dw_splits * v->vocab * p.ld : 0;
+        if (dw > slabs) slabs = dw;
+        p.at_slabs = take(slabs);
+        if (p.pieces > 1) p.at_sum = take(4 * v->vocab * p.ld);
+    }
+    p.bytes = at;
+    return p;
+}
+
+int check(const char *fn, const noise_vocab_t *v, float softcap) {
+    NOISE_CHECK_ARG(v, "%s: NULL pointer", fn);
+    NOISE_CHECK_ARG(v->type == NOISE_BF16 || v->type == NOISE_FP32, "%s: unknown type %lld", fn, (long long)v->type);
+    NOISE_CHECK_ARG(v->rows >= 0 && v->rows <= (1 << 30) && v->dim > 0 && v->dim <= (1 << 16) && v->vocab > 0 && v->vocab <= (1 << 22),
+                    "%s: rows 0 .. 2^30, dim 1 .. 65536 and vocab 1 .. 2^22 required", fn);
+    NOISE_CHECK_ARG(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e6f), "%s: softcap must be 1e-6 .. 1e6, or 0 for none", fn);
+    if (v->rows == 0) return NOISE_OK;
+    const size_t size = v->type == NOISE_BF16 ? 2 : 4;
+    NOISE_CHECK_ARG(v->x && v->weight && v->targets && aligned(v->x, size) && aligned(v->weight, size) &&
+                        aligned(v->targets, v->targets_wide ? 8 : 4),
+                    "%s: a pointer is NULL or not aligned to its type", fn);
+    return NOISE_OK;
+}
+
+// loss and lse (out, or with `given` lse in); dx and dw where grad
+int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weight, float *loss, float *lse, const float *given,
+        void *dx, void *dw, int64_t width, bool grad, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const Plan p = plan_of(v, grad);
+    NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes,
+                    "%s: workspace of %lld bytes (16 B aligned) required", fn, (long long)p.bytes);
+    char *ws = static_cast<char *>(workspace);
+    int *place = reinterpret_cast<int *>(ws + p.at_int), *live = place + p.rows, *target = live + p.rows, *count = target + p.rows;
+    float *f = reinterpret_cast<float *>(ws + p.at_float);
+    float *packed_weight = f, *packed_lse = f + p.rows, *zt = f + 2 * p.rows, *scales = f + 3 * p.rows, *x_max = scales + 4,
+          *w_max = x_max + kMaxParts;
+    const int64_t rows = v->rows;
+    const unsigned row_groups = (unsigned)((rows + 255) / 256);
+    hipLaunchKernelGGL(vocab_live_kernel, dim3(1), dim3(1024), 0, stream, v->targets, (int)v->targets_wide, rows, v->vocab, weight,
+                       count, live, place, target, packed_weight, scales + 3);
+    if (loss || lse) hipLaunchKernelGGL(vocab_zero_kernel, dim3(row_groups), dim3(256), 0, stream, loss, lse, place, rows);
+    if (p.split) {
+        hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts), dim3(256), 0, stream, static_cast<const float *>(v->x), v->x_stride,
+                           rows, v->dim, place, x_max);
+        hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts), dim3(256), 0, stream, static_cast<const float *>(v->weight),
+                           v->weight_stride, v->vocab, v->dim, (const int *)nullptr, w_max);
+        hipLaunchKernelGGL(vocab_scale_kernel, dim3(1), dim3(64), 0, stream, x_max, w_max, kMaxParts, scales + 3, scales);
+    }
+    HeadArgs a = {};
+    a.x = Operand{reinterpret_cast<__bf16 *>(ws + p.at_x), p.ld, p.rows * p.ld};
+    a.w = p.pack_w ? Operand{reinterpret_cast<__bf16 *>(ws + p.at_w), p.ld, v->vocab * p.ld}
+                   : Operand{static_cast<const __bf16 *>(v->weight), v->weight_stride, 0};
+    constexpr int64_t kRows = 1 << 22;   // a launch has fewer than 2^32 threads
+    for (int64_t r = 0; r < p.rows; r += kRows) {
+        const unsigned n = (unsigned)(p.rows - r < kRows ? p.rows - r : kRows);
+        if (p.split)
+            hipLaunchKernelGGL((vocab_pack_kernel<float, true>), dim3(n), dim3(256), 0, stream, static_cast<const float *>(v->x),
+                               v->x_stride, rows, r, v->dim, place, count, p.rows, scales, a.x, static_cast<float *>(dx));
+        else
+            hipLaunchKernelGGL((vocab_pack_kernel<__bf16, false>), dim3(n), dim3(256), 0, stream, static_cast<const __bf16 *>(v->x),
+                               v->x_stride, rows, r, v->dim, place, count, p.rows, scales, a.x, static_cast<__bf16 *>(dx));
+    }
+    if (p.pack_w) {
+        if (p.split)
+            hipLaunchKernelGGL((vocab_pack_kernel<float, true>), dim3((unsigned)v->vocab), dim3(256), 0, stream,
+                               static_cast<const float *>(v->weight), v->weight_stride, v->vocab, (int64_t)0, v->dim,
+                               (const int *)nullptr, (const int *)nullptr, v->vocab, scales + 1, a.w, (float *)nullptr);
+        else
+            hipLaunchKernelGGL((vocab_pack_kernel<__bf16, false>), dim3((unsigned)v->vocab), dim3(256), 0, stream,
+                               static_cast<const __bf16 *>(v->weight), v->weight_stride, v->vocab, (int64_t)0, v->dim,
+                               (const int *)nullptr, (const int *)nullptr, v->vocab, scales, a.w, (__bf16 *)nullptr);
+    }
+    a.count = count, a.live = live, a.target = target, a.scales = scales;
+    a.weight = weight ? packed_weight : nullptr;
+    a.lse = packed_lse, a.zt = zt, a.partial = reinterpret_cast<float2 *>(ws + p.at_partial);
+    a.rows = p.rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
+    a.fp32 = p.split;
+    if (given) hipLaunchKernelGGL(vocab_lse_gather_kernel, dim3(row_groups), dim3(256), 0, stream, count, live, given, packed_lse);
+    if (dw && width > v->vocab) {
+        const int64_t n = (width - v->vocab) * v->dim * (p.split ? 2 : 1);
+        hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,
+                           static_cast<uint16_t *>(dw) + v->vocab * v->dim * (p.split ? 2 : 1), n);
+    }
+    const int threads = 64 * Tile::NW;
+    const bool cap = softcap > 0.f;
+    for (int64_t i = 0; i < p.pieces; ++i) {
+        a.row0 = i * p.piece, a.piece = p.rows - a.row0 < p.piece ? p.rows - a.row0 : p.piece;
+        a.tiles_m = (int)((v->vocab + Tile::MT - 1) / Tile::MT), a.tiles_n = (int)(a.piece / Tile::NT), a.splits = 1;
+        const dim3 tiles((unsigned)(a.tiles_m * a.tiles_n));
+        if (!given) {
+            auto kernel = p.split ? (cap ? vocab_loss_kernel<Tile, true, true> : vocab_loss_kernel<Tile, true, false>)
+                                  : (cap ? vocab_loss_kernel<Tile, false, true> : vocab_loss_kernel<Tile, false, false>);
+            hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
+            hipLaunchKernelGGL(vocab_lse_kernel, dim3((unsigned)((a.piece + 31) / 32)), dim3(256), 0, stream, a, (int)p.segments, loss, lse);
+        }
+        if (!grad) continue;
+        a.dz = Operand{reinterpret_cast<__bf16 *>(ws + p.at_dz), p.vocab_ld, p.piece * p.vocab_ld};
+        auto kernel = p.split ? (cap ? vocab_dz_kernel<Tile, true, true> : vocab_dz_kernel<Tile, true, false>)
+                              : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
+        hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
+        a.slabs = reinterpret_cast<float *>(ws + p.at_slabs);
+        a.out_ld = v->dim;
+        const int64_t per = p.ld / 8;
+        a.tiles_m = (int)((p.ld + Tile::MT - 1) / Tile::MT);
+        if (dx) {
+            a.out = dx, a.splits = p.dx_splits, a.sum = nullptr;
+            hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, true, true> : vocab_grad_kernel<Tile, true, false>),
+                               dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(threads), 0, stream, a);
+            if (a.splits > 1)
+                hipLaunchKernelGGL(vocab_sum_kernel<true>, dim3((unsigned)((a.piece * per + 255) / 256)), dim3(256), 0, stream, a);
+        }
+        if (dw) {
+            a.tiles_n = (int)((v->vocab + Tile::NT - 1) / Tile::NT);
+            a.splits = p.dw_splits;
+            a.sum = p.pieces > 1 ? reinterpret_cast<float *>(ws + p.at_sum) : nullptr;
+            a.add = i > 0, a.out = i + 1 == p.pieces ? dw : nullptr;
+            hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, false, true> : vocab_grad_kernel<Tile, false, false>),
+                               dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(threads), 0, stream, a);
+            if (a.splits > 1)
+                hipLaunchKernelGGL(vocab_sum_kernel<false>, dim3((unsigned)((v->vocab * per + 255) / 256)), dim3(256), 0, stream, a);
+        }
+    }
+    return launch_status(fn);
+}
+
+}  // namespace
+}  // namespace noise
+
+using namespace noise;
+
+extern "C" int64_t noise_vocab_workspace_bytes(const noise_vocab_t *v, int with_grad) {
+    clear_error();
+    if (check("noise_vocab_workspace_bytes", v, 0.f)) return -1;
+    return v->rows ? plan_of(v, with_grad != 0).bytes : 0;
+}
+
+extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace,
+                                int64_t workspace_bytes, noise_stream_t stream) {
+    clear_error();
+    const char *fn = "noise_vocab_loss";
+    if (int e = check(fn, v, softcap)) return e;
+    if (v->rows == 0) return NOISE_OK;
+    NOISE_CHECK_ARG(loss && aligned(loss, 4) && aligned(lse, 4), "%s: loss NULL or not 4 B aligned", fn);
+    return run(fn, v, softcap, nullptr, loss, lse, nullptr, nullptr, nullptr, 0, false, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int noise_vocab_grad(const noise_vocab_t *v, float softcap, const float *weight, const float *lse, float *loss, void *dx,
+                                void *dweight, int64_t width, void *workspace, int64_t workspace_bytes, noise_stream_t stream) {
+    clear_error();
+    const char *fn = "noise_vocab_grad";
+    if (int e = check(fn, v, softcap)) return e;
+    const size_t size = v->type == NOISE_BF16 ? 2 : 4;
+    NOISE_CHECK_ARG((lse != nullptr) != (loss != nullptr) || v->rows == 0, "%s: either lse in or loss out", fn);
+    NOISE_CHECK_ARG(aligned(weight, 4) && aligned(lse, 4) && aligned(loss, 4) && aligned(dx, size) && aligned(dweight, size),
+                    "%s: a pointer is not aligned to its type", fn);
+    NOISE_CHECK_ARG(!dweight || (width >= v->vocab && width <= (1 << 30)), "%s: dweight needs vocab <= width", fn);
+    if (v->rows == 0) return NOISE_OK;
+    return run(fn, v, softcap, weight, loss, nullptr, lse, dx, dweight, width, true, workspace, workspace_bytes, (hipStream_t)stream);
+}

@@ -30,6 +30,7 @@ from . import distill as _distill
 from . import dust, eggroll, model
 from . import residual as _residual
 from . import sinks as _sinks
+from . import vocab as _vocab
 
 BLOCK_WEIGHTS = ('q', 'k', 'v', 'gate', 'proj', 'fc', 'out')
 
@@ -341,3 +342,57 @@ def _residual_norm_backward(ctx, dout, dh):
 
 
 residual_norm.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
+
+
+@custom_op('noise_amd::linear_cross_entropy', mutates_args=())
+def linear_cross_entropy(x: Tensor, weight: Tensor, targets: Tensor, vocab: int, softcap: Optional[float]) -> Tuple[Tensor, Tensor]:
+    """The losses, and what their backward pass needs"""
+    _backwards_only('linear_cross_entropy')
+    return _vocab.forward(x, weight, targets, vocab, softcap, True)
+
+
+@linear_cross_entropy.register_fake
+def _linear_cross_entropy_fake(x, weight, targets, vocab, softcap):
+    return x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@custom_op('noise_amd::linear_cross_entropy_backward', mutates_args=())
+def linear_cross_entropy_backward(dloss: Tensor, x: Tensor, weight: Tensor, targets: Tensor, lse: Tensor, vocab: int,
+                                  softcap: Optional[float], need_x: bool, need_weight: bool) -> Tuple[Tensor, Tensor]:
+    """dx and dweight (empty where not needed)"""
+    _backwards_only('linear_cross_entropy_backward')
+    grads = _vocab.gradients('linear_cross_entropy', x, weight, targets, dloss, lse, vocab, softcap, need_x, need_weight)[1:]
+    return tuple(x.new_empty(0) if g is None else g for g in grads)
+
+
+@linear_cross_entropy_backward.register_fake
+def _linear_cross_entropy_backward_fake(dloss, x, weight, targets, lse, vocab, softcap, need_x, need_weight):
+    return x.new_empty(x.shape if need_x else 0), weight.new_empty(weight.shape if need_weight else 0)
+
+
+@custom_op('noise_amd::linear_cross_entropy_grad', mutates_args=())
+def linear_cross_entropy_grad(x: Tensor, weight: Tensor, targets: Tensor, token_weight: Optional[Tensor], vocab: int,
+                              softcap: Optional[float]) -> Tuple[Tensor, Tensor, Tensor]:
+    _backwards_only('linear_cross_entropy_grad')
+    return _vocab.gradients('linear_cross_entropy_grad', x, weight, targets, token_weight, None, vocab, softcap)
+
+
+@linear_cross_entropy_grad.register_fake
+def _linear_cross_entropy_grad_fake(x, weight, targets, token_weight, vocab, softcap):
+    return x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape), weight.new_empty(weight.shape)
+
+
+def _linear_cross_entropy_setup(ctx, inputs, output):
+    x, weight, targets, *ctx.more = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, weight, targets, output[1])
+
+
+def _linear_cross_entropy_backward(ctx, dloss, _):
+    x, weight, targets, lse = ctx.saved_tensors
+    needs = [bool(n) for n in ctx.needs_input_grad[:2]]
+    grads = torch.ops.noise_amd.linear_cross_entropy_backward(dloss, x, weight, targets, lse, *ctx.more, *needs)
+    return (*(g if n else None for g, n in zip(grads, needs)), None, None, None)
+
+
+linear_cross_entropy.register_autograd(_linear_cross_entropy_backward, setup_context=_linear_cross_entropy_setup)

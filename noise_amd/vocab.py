@@ -1,0 +1,135 @@
+"""The cross entropy of a linear head over a vocabulary of any size, without its logits in memory, beside noise_amd.dust's forward-only
+head_loss of the fixed model.
+
+  linear_cross_entropy(x, weight, targets, vocab, softcap)                      per-token losses; differentiable in x and weight
+  linear_cross_entropy_grad(x, weight, targets, token_weight, vocab, softcap)   losses and the weighted sum's gradients in one call
+
+The head is utils/model.py:204-206's with its soft cap as an option, the loss that of train/val/run.py:89-94. The calls are
+torch.ops.noise_amd operators too. Derivatives are taken backwards and once, as in noise_amd.sinks.
+"""
+from array import array
+
+import torch
+
+from . import _lib
+from .sinks import F32, TYPES, _call, _no_tangents
+
+
+def _rows(t):
+    """t [rows, dim], or a copy of it, with unit inner stride and rows after one another"""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1) else t.contiguous()
+
+
+class _Operands:
+    """The checked operands as noise_vocab_t takes them; the copies among them live as long as this does"""
+
+    def __init__(self, fn, x, weight, targets, vocab, softcap):
+        if x.dtype not in TYPES or x.dim() < 1 or weight.dtype != x.dtype or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+            raise ValueError(f'{fn}: bfloat16 or float32 x [..., dim] and weight [width, dim] of its type, got {x.dtype} '
+                             f'{tuple(x.shape)} and {weight.dtype} {tuple(weight.shape)}')
+        width, dim = weight.shape
+        self.vocab = width if vocab is None else int(vocab)
+        if not 0 < self.vocab <= width or self.vocab > 1 << 22:
+            raise ValueError(f'{fn}: vocab must be 1 .. {min(width, 1 << 22)}, got {self.vocab}')
+        if not 0 < dim <= 1 << 16:
+            raise ValueError(f'{fn}: dim must be 1 .. {1 << 16}, got {dim}')
+        if softcap is not None and not 1e-6 <= softcap <= 1e6:
+            raise ValueError(f'{fn}: softcap must be 1e-6 .. 1e6 (None: no cap), got {softcap}')
+        if targets.shape != x.shape[:-1] or targets.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f'{fn}: targets must be int32 or int64 of shape {tuple(x.shape[:-1])}, got {targets.dtype} '
+                             f'{tuple(targets.shape)}')
+        if weight.device != x.device or targets.device != x.device:
+            raise ValueError(f'{fn}: tensors on {x.device}, {weight.device} and {targets.device}')
+        _no_tangents(fn, x, weight)
+        self.shape, self.device = x.shape[:-1], x.device
+        self.x, self.weight = _rows(x if x.dim() == 2 else x.reshape(-1, dim)), _rows(weight)
+        self.targets = targets if targets.is_contiguous() else targets.contiguous()
+        self.rows, self.softcap = self.x.shape[0], float(softcap or 0.0)
+        if self.rows > 1 << 30:
+            raise ValueError(f'{fn}: at most 2^30 tokens, got {self.rows}')
+        self.table = array('q', (self.x.data_ptr(), self.x.stride(0) if self.rows > 1 else dim, self.weight.data_ptr(),
+                                 self.weight.stride(0) if width > 1 else dim, self.targets.data_ptr(),
+                                 int(targets.dtype == torch.int64), self.rows, dim, self.vocab, TYPES[x.dtype]))
+        self.at = self.table.buffer_info()[0]
+
+    def workspace(self, grad):
+        need = _lib.lib().noise_vocab_workspace_bytes(self.at, grad)
+        return torch.empty(need, dtype=torch.uint8, device=self.device), need
+
+
+def forward(x, weight, targets, vocab, softcap, with_lse):
+    """(losses, lse or None)"""
+    a = _Operands('linear_cross_entropy', x, weight, targets, vocab, softcap)
+    loss = x.new_empty(a.shape, dtype=F32)
+    lse = x.new_empty(a.shape, dtype=F32) if with_lse else None
+    if a.rows:
+        work, need = a.workspace(0)
+        _call('noise_vocab_loss', a.device, a.at, a.softcap, loss.data_ptr(), _lib.ptr(lse), work.data_ptr(), need)
+    return loss, lse
+
+
+def gradients(fn, x, weight, targets, token_weight, lse, vocab, softcap, need_x=True, need_weight=True):
+    """(losses or, where lse is given, None; dx; dweight)"""
+    a = _Operands(fn, x, weight, targets, vocab, softcap)
+    _no_tangents(fn, token_weight)
+    if token_weight is not None:
+        if token_weight.shape != a.shape or token_weight.device != a.device:
+            raise ValueError(f'{fn}: token weights must be {tuple(a.shape)} on {a.device}, got {tuple(token_weight.shape)} on '
+                             f'{token_weight.device}')
+        if token_weight.dtype != F32 or not token_weight.is_contiguous():
+            token_weight = token_weight.to(F32).contiguous()
+    loss = x.new_empty(a.shape, dtype=F32) if lse is None else None
+    dx = x.new_empty(x.shape) if need_x else None
+    dw = weight.new_empty(weight.shape) if need_weight else None
+    if a.rows:
+        work, need = a.workspace(1)
+        _call('noise_vocab_grad', a.device, a.at, a.softcap, _lib.ptr(token_weight), _lib.ptr(lse), _lib.ptr(loss), _lib.ptr(dx),
+              _lib.ptr(dw), weight.shape[0], work.data_ptr(), need)
+    elif dw is not None:
+        dw.zero_()
+    return loss, dx, dw
+
+
+class _Head(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, vocab, softcap):
+        loss, lse = forward(x, weight, targets, vocab, softcap, True)
+        ctx.save_for_backward(x, weight, targets, lse)
+        ctx.more = (vocab, softcap)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, weight, targets, lse = ctx.saved_tensors
+        return (*gradients('linear_cross_entropy', x, weight, targets, dloss, lse, *ctx.more, *ctx.needs_input_grad[:2])[1:],
+                None, None, None)
+
+
+def linear_cross_entropy(x, weight, targets, vocab=None, softcap=None):
+    """Per-token cross entropies, fp32 [...], of hidden states x [..., dim] under the head weight [width, dim] (both bfloat16 or
+    both float32, the weight's first `vocab` rows in use) against targets [...] (int32 or int64):
+
+        z = cap(x weight^T),  cap(z) = softcap * tanh(z / softcap),  loss = log sum exp z - z[target]
+
+    A token whose target lies outside 0 .. vocab - 1 has loss 0 and no gradient, whatever its x holds. The logits are formed a
+    tile at a time and never stored; their products, sums and softmax are in fp32, float32 operands with 21 bits in the products.
+    Differentiable in x and weight (once): the backward pass forms the logits again, and holds their gradients in 16 bits (two
+    times 16 for float32) for at most 2 GiB of tokens and vocabulary at a time. Rows may lie at any distance from each other."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.linear_cross_entropy(x, weight, targets, weight.shape[0] if vocab is None else int(vocab),
+                                                        softcap)[0]
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _Head.apply(x, weight, targets, vocab, softcap)
+    return forward(x, weight, targets, vocab, softcap, False)[0]
+
+
+def linear_cross_entropy_grad(x, weight, targets, token_weight=None, vocab=None, softcap=None):
+    """(losses, dx, dweight) of linear_cross_entropy in one call, for a training step that knows its tokens' weights before the
+    losses: the gradients, of x's and weight's shapes and type, are those of sum(token_weight * loss), token_weight [...] (None:
+    ones). Rows of dweight from `vocab` on are zeros. The results are plain tensors, for operands that require a gradient too
+    (x.backward(dx) goes on from there)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.noise_amd.linear_cross_entropy_grad(x, weight, targets, token_weight,
+                                                             weight.shape[0] if vocab is None else int(vocab), softcap)
+    return gradients('linear_cross_entropy_grad', x, weight, targets, token_weight, None, vocab, softcap)
