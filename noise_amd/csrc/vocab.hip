@@ -34,11 +34,10 @@ struct HeadArgs {
     const float *scales;         // 2^ex, 2^ew, 2^ed of fp32 operands (x, w, dZ), else 1
     const float *weight;         // of a packed row's loss
     float *lse, *zt;             // of a packed row
-    float2 *partial;             // [segments][rows]
+    float2 *partial;             // [rows][segments]: a segment's largest logit, and the sum of exponentials from there
     int64_t row0;                // the piece's first packed row
-    int64_t rows;                // packed rows, at most (the partials' stride)
     int64_t piece;               // rows of the piece, at most
-    int vocab, dim, nk;          // nk: stages of k over dim
+    int vocab, dim, nk, segments;  // nk: stages of k over dim
     int tiles_m, tiles_n, splits;
     float softcap;
     void *out;                   // dx or dW
@@ -60,37 +59,57 @@ __device__ __forceinline__ float cap_of(float z, float cap, float k) {
 
 // --- rows with a target, packed ---
 
+// One workgroup: N rows per thread at a time (4 for few rows, which then take all its waves)
+template <int N>
 __global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, int wide, int64_t rows, int64_t vocab,
-                                                          const float *weight, int *count, int *live, int *place, int *target,
-                                                          float *live_weight, float *weight_max) {
+                                                          const float *weight, const float *lse, int *count, int *live, int *place,
+                                                          int *target, float *live_weight, float *live_lse, float *weight_max) {
     __shared__ int sums[16];
     __shared__ float tops[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int base = 0;
     float top = 0.f;
-    for (int64_t r0 = 0; r0 < rows; r0 += 1024) {
-        const int64_t r = r0 + threadIdx.x;
-        int64_t t = -1;
-        if (r < rows) t = wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
-        const bool in = t >= 0 && t < vocab;
-        const uint64_t mask = __ballot(in);
-        if (lane == 0) sums[wave] = __popcll(mask);
+    for (int64_t r0 = 0; r0 < rows; r0 += 1024 * N) {
+        // thread t of a wave takes rows r0 + 64 N wave + 64 i + t: consecutive lanes read consecutive targets
+        const int64_t first = r0 + 64 * N * wave + lane;
+        int64_t t[N];
+        float w[N], l[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t r = first + 64 * i;
+            t[i] = r >= rows ? -1 : wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
+            w[i] = weight && r < rows ? weight[r] : 1.f;
+            l[i] = lse && r < rows ? lse[r] : 0.f;
+        }
+        uint64_t mask[N];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            mask[i] = __ballot(t[i] >= 0 && t[i] < vocab);
+            n += __popcll(mask[i]);
+        }
+        if (lane == 0) sums[wave] = n;
         __syncthreads();
-        int before = base, all = 0;
+        int before = base;
         for (int w = 0; w < 16; ++w) {
             if (w < wave) before += sums[w];
-            all += sums[w];
+            base += sums[w];
         }
-        before += __popcll(mask & ((1ull << lane) - 1));
-        if (r < rows) place[r] = in ? before : -1;
-        if (in) {
-            live[before] = (int)r;
-            target[before] = (int)t;
-            const float w = weight ? weight[r] : 1.f;
-            if (live_weight) live_weight[before] = w;
-            if (fabsf(w) < __builtin_inff()) top = fmaxf(top, fabsf(w));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t r = first + 64 * i;
+            const int at = before + __popcll(mask[i] & ((1ull << lane) - 1));
+            before += __popcll(mask[i]);
+            if (r >= rows) continue;
+            const bool in = t[i] >= 0 && t[i] < vocab;
+            place[r] = in ? at : -1;
+            if (!in) continue;
+            live[at] = (int)r;
+            target[at] = (int)t[i];
+            if (lse) live_lse[at] = l[i];
+            if (weight) live_weight[at] = w[i];
+            if (fabsf(w[i]) < __builtin_inff()) top = fmaxf(top, fabsf(w[i]));
         }
-        base += all;
         __syncthreads();
     }
 #pragma unroll
@@ -106,26 +125,54 @@ __global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, i
 
 // --- operands ---
 
-// Largest finite |v| of the matrix's rows (x: of those with a target), one value per workgroup
-__global__ __launch_bounds__(256) void vocab_max_kernel(const float *src, int64_t ld, int64_t rows, int64_t dim, const int *place,
-                                                        float *to) {
+// x and the weight as they come, and where they go
+struct PackArgs {
+    const void *src[2];
+    int64_t src_ld[2], rows[2], padded[2];   // padded: rows of the packed matrix (0: not packed)
+    Operand to[2];
+    int64_t dim;
+    const int *place, *count;
+    const float *max, *weight_max;           // fp32: kMaxParts values of x's and of the weight's largest
+    float *scales;
+    void *dx;
+    float *loss, *lse;
+};
+
+constexpr int kMaxParts = 512;
+
+// 8 values of 4 or 2 B at any address of their type; n of them exist
+template <class E>
+__device__ __forceinline__ void load8(const E *p, int64_t n, E (&v)[8]) {
+    if (n >= 8) __builtin_memcpy(v, p, sizeof v);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (E)0.f;
+}
+
+// Largest finite |v| of a matrix's rows (x: of those with a target), one value per workgroup; a wave takes a row
+__global__ __launch_bounds__(256) void vocab_max_kernel(PackArgs a, float *to) {
     __shared__ float tops[4];
+    const int which = blockIdx.y, lane = threadIdx.x & 63;
+    const float *src = static_cast<const float *>(a.src[which]);
     float top = 0.f;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        if (place && place[r] < 0) continue;
-        for (int64_t c = threadIdx.x; c < dim; c += 256) {
-            const float v = fabsf(src[r * ld + c]);
-            if (v < __builtin_inff()) top = fmaxf(top, v);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows[which]; r += 4 * kMaxParts) {
+        if (which == 0 && a.place[r] < 0) continue;
+        for (int64_t c = 8 * lane; c < a.dim; c += 512) {
+            float v[8];
+            load8(src + r * a.src_ld[which] + c, a.dim - c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = fabsf(v[e]);
+                if (f < __builtin_inff()) top = fmaxf(top, f);
+            }
         }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    if (lane == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) to[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (threadIdx.x == 0) to[which * kMaxParts + blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
-
-constexpr int kMaxParts = 512;
 
 // The power of two that takes `top` to 2^14 .. 2^15 (within 2^-100 .. 2^100)
 __device__ __forceinline__ float scale_of(float top) {
@@ -135,17 +182,8 @@ __device__ __forceinline__ float scale_of(float top) {
     return ldexpf(1.f, e);
 }
 
-__global__ __launch_bounds__(64) void vocab_scale_kernel(const float *x_max, const float *w_max, int n, const float *d_max, float *scales) {
-    float x = 0.f, w = 0.f;
-    for (int i = threadIdx.x; i < n; i += 64) x = fmaxf(x, x_max[i]), w = fmaxf(w, w_max[i]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64)), w = fmaxf(w, __shfl_xor(w, o, 64));
-    if (threadIdx.x == 0) scales[0] = scale_of(x), scales[1] = scale_of(w), scales[2] = scale_of(*d_max);
-}
-
-// v s as a sum of two fp16 values, as bits
-__device__ __forceinline__ void halves(float v, float s, uint16_t &hi, uint16_t &lo) {
-    const float f = v * s;
+// f as a sum of two fp16 values, as bits
+__device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
     const _Float16 h = (_Float16)f;
     const float rest = fabsf(f) < __builtin_inff() ? f - (float)h : 0.f;
     const _Float16 l = (_Float16)rest;
@@ -153,39 +191,60 @@ __device__ __forceinline__ void halves(float v, float s, uint16_t &hi, uint16_t 
     __builtin_memcpy(&lo, &l, 2);
 }
 
-// One workgroup per source row: the row to its place (none: left out), zeros from dim to ld; and zeros in the rows behind the last,
-// `padded` in all. dx: gradient rows to zero where a row has no place.
+// The packed matrices: x's rows at their places (zeros behind the last) and the weight's where it is packed, with zeros from dim to
+// the packed row's end. Rows of x without a place: their losses, lse and rows of dx to zero. A wave takes a row; blockIdx.y: x or
+// the weight.
 template <class E, bool SPLIT>
-__global__ __launch_bounds__(256) void vocab_pack_kernel(const E *src, int64_t src_ld, int64_t rows, int64_t first, int64_t dim,
-                                                         const int *place, const int *count, int64_t padded, const float *scale,
-                                                         Operand to, E *dx) {
-    const int64_t r = first + blockIdx.x;
-    uint16_t *dst = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(to.ptr));
-    auto zero = [&](int64_t at) {
-        for (int64_t c = threadIdx.x; c < to.ld; c += 256) {
-            dst[at * to.ld + c] = 0;
-            if (SPLIT) dst[to.lo + at * to.ld + c] = 0;
+__global__ __launch_bounds__(256) void vocab_pack_kernel(PackArgs a) {
+    const int which = blockIdx.y, lane = threadIdx.x & 63;
+    const int64_t rows = a.rows[which], padded = a.padded[which], ld = a.to[which].ld, waves = (int64_t)gridDim.x * 4;
+    float scale = 1.f;
+    if constexpr (SPLIT) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMaxParts / 64; ++i) top = fmaxf(top, a.max[which * kMaxParts + lane + 64 * i]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        scale = scale_of(top);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.scales[which] = scale;
+            if (which == 0) a.scales[2] = scale_of(*a.weight_max);
         }
-    };
-    const int64_t behind = place ? *count : rows;
-    if (r >= behind && r < padded) zero(r);
-    if (r >= rows) return;
-    const int64_t at = place ? place[r] : r;
-    if (at < 0) {
-        if (dx)
-            for (int64_t c = threadIdx.x; c < dim; c += 256) dx[r * dim + c] = (E)0.f;
-        return;
     }
-    const float s = SPLIT ? *scale : 1.f;
-    for (int64_t c = threadIdx.x; c < to.ld; c += 256) {
-        if constexpr (SPLIT) {
-            uint16_t hi = 0, lo = 0;
-            if (c < dim) halves((float)src[r * src_ld + c], s, hi, lo);
-            dst[at * to.ld + c] = hi, dst[to.lo + at * to.ld + c] = lo;
-        } else {
-            uint16_t bits = 0;
-            if (c < dim) __builtin_memcpy(&bits, src + r * src_ld + c, 2);
-            dst[at * to.ld + c] = bits;
+    if (!padded) return;
+    const E *src = static_cast<const E *>(a.src[which]);
+    uint16_t *dst = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.to[which].ptr));
+    const int64_t behind = which == 0 ? *a.count : rows;
+    uint16_t none[8] = {};
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < (rows > padded ? rows : padded); r += waves) {
+        if (r >= behind && r < padded)
+            for (int64_t c = 8 * lane; c < ld; c += 512) {
+                __builtin_memcpy(__builtin_assume_aligned(dst + r * ld + c, 16), none, 16);
+                if (SPLIT) __builtin_memcpy(__builtin_assume_aligned(dst + a.to[which].lo + r * ld + c, 16), none, 16);
+            }
+        if (r >= rows) continue;
+        const int64_t at = which == 0 ? a.place[r] : r;
+        if (at < 0) {
+            if (a.dx)
+                for (int64_t c = lane; c < a.dim; c += 64) static_cast<E *>(a.dx)[r * a.dim + c] = (E)0.f;
+            if (lane == 0) {
+                if (a.loss) a.loss[r] = 0.f;
+                if (a.lse) a.lse[r] = 0.f;
+            }
+            continue;
+        }
+        for (int64_t c = 8 * lane; c < ld; c += 512) {
+            E v[8];
+            load8(src + r * a.src_ld[which] + c, a.dim - c, v);
+            uint16_t hi[8], lo[8];
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) halves(v[e] * scale, hi[e], lo[e]);
+                __builtin_memcpy(__builtin_assume_aligned(dst + a.to[which].lo + at * ld + c, 16), lo, 16);
+            } else {
+                __builtin_memcpy(hi, v, 16);
+            }
+            __builtin_memcpy(__builtin_assume_aligned(dst + at * ld + c, 16), hi, 16);
         }
     }
 }
@@ -210,12 +269,15 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
             }
 }
 
-template <class T, bool SPLIT, bool CAP>
+// STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_kernel turns into dZ. (Its rounding, 2^-11,
+// comes before dZ's own, 2^-8; below 2^-29 of the segment's largest it has fewer bits, below 2^-39 none.)
+template <class T, bool SPLIT, bool CAP, bool STORE>
 __global__ __launch_bounds__(64 * T::NW) void vocab_loss_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
     int tm, tn;
     tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
-    if ((int64_t)tn * T::NT >= piece_rows(a)) return;
+    const int64_t rows = piece_rows(a);
+    if ((int64_t)tn * T::NT >= rows) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
@@ -224,79 +286,128 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_loss_kernel(HeadArgs a) {
     if (m0 >= a.vocab) return;
     const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f;
     to_logits<T, CAP>(a, m0, lane, unit, acc);
+    const float inv_cap = CAP ? 1.f / a.softcap : 0.f;
     static_assert(T::FB * 32 == kSegment, "a wave's entries are a segment");
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
-        const int64_t row = a.row0 + (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
+        const int64_t at = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31), row = a.row0 + at;
+        const bool there = at < rows;
         float top = kLowest;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
         top = fmaxf(top, swap_halves(top));
+        const int t = there ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
+        const bool mine = t >= 0 && t < kSegment && !(t & 8);
+        if (__any(mine)) {
+            float z = 0.f;
+#pragma unroll
+            for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z = t == 32 * i + 16 * (r / 8) + r % 8 ? acc[i][j][r] : z;
+            if (mine) a.zt[row] = z;
+        }
         const float shift = top * kLog2e;
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -shift));
+            for (int h = 0; h < 2; ++h) {
+                _Float16 v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float z = acc[i][j][8 * h + e];
+                    float p = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
+                    s += p;
+                    if constexpr (STORE) {
+                        if (CAP) {
+                            const float u = z * inv_cap;
+                            p *= z == -__builtin_inff() ? 0.f : 1.f - u * u;
+                        }
+                        v[e] = (_Float16)(there ? p * 32768.f : 0.f);   // (rows behind the last one are multiplied by zeros)
+                    }
+                }
+                if constexpr (STORE) {
+                    uint16_t *to = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld + m0 + 32 * i +
+                                   16 * h + 8 * (lane >> 5);
+                    __builtin_memcpy(__builtin_assume_aligned(to, 16), v, 16);
+                }
+            }
         s += swap_halves(s);
-        if (lane < 32) a.partial[(int64_t)(m0 / kSegment) * a.rows + row] = float2{top, s};
-        const int t = row < *a.count ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
-        if (t >= 0 && t < kSegment && !(t & 8)) {
-#pragma unroll
-            for (int i = 0; i < T::FB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t == 32 * i + 16 * (r / 8) + r % 8) a.zt[row] = acc[i][j][r];
-        }
+        if (lane < 32 && there) a.partial[row * a.segments + m0 / kSegment] = float2{top, s};
     }
 }
 
-// lse of 32 rows, 8 runs of segments each; the losses
-__global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segments, float *loss, float *lse) {
-    __shared__ float tops[8][33], sums[8][33];
-    const int64_t row = a.row0 + (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int slice = threadIdx.x >> 5;
-    const int64_t end = a.row0 + piece_rows(a);
-    float top = kLowest, s = 0.f;
-    if (row < end)
-#pragma unroll 4
-        for (int g = slice; g < segments; g += 8) {
-            const float2 p = a.partial[(int64_t)g * a.rows + row];
-            const float m = fmaxf(top, p.x);
-            s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
-            top = m;
-        }
-    tops[slice][threadIdx.x & 31] = top;
-    sums[slice][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (slice || row >= end) return;
-    for (int k = 1; k < 8; ++k) {
-        const float x = tops[k][threadIdx.x & 31], m = fmaxf(top, x);
-        s = s * exp2_fast((top - m) * kLog2e) + sums[k][threadIdx.x & 31] * exp2_fast((x - m) * kLog2e);
+// Sum over the workgroup of sums s with maxima top: every thread gets both
+__device__ __forceinline__ void join_sums(float &top, float &s, float2 (&slots)[4]) {
+    auto join = [&](float m2, float s2) {
+        const float m = fmaxf(top, m2);
+        s = s * exp2_fast((top - m) * kLog2e) + s2 * exp2_fast((m2 - m) * kLog2e);
+        top = m;
+    };
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(s, o, 64);
+        // (the lower lane's pair first, so that both lanes get the same bits)
+        const bool low = !(threadIdx.x & o);
+        const float m = fmaxf(top, m2), a = s * exp2_fast((top - m) * kLog2e), b = s2 * exp2_fast((m2 - m) * kLog2e);
+        s = low ? a + b : b + a;
         top = m;
     }
-    const float l = top + logf(s);
-    const int to = a.live[row];
-    a.lse[row] = l;
-    if (loss) loss[to] = l - a.zt[row];
-    if (lse) lse[to] = l;
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = float2{top, s};
+    __syncthreads();
+    top = slots[0].x, s = slots[0].y;
+    for (int w = 1; w < 4; ++w) join(slots[w].x, slots[w].y);
 }
 
-// lse of the packed rows from the forward pass's
-__global__ __launch_bounds__(256) void vocab_lse_gather_kernel(const int *count, const int *live, const float *lse, float *to) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r < *count) to[r] = lse[live[r]];
+// A row's lse and loss from its segments; with STORE also dZ from what vocab_loss_kernel left:
+// dZ_v = weight exp(top - lse) 2^-15 stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
+template <bool STORE>
+__global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segment, float *loss, float *lse) {
+    __shared__ float2 slots[4];
+    const int64_t at = blockIdx.x, row = a.row0 + at;
+    if (at >= piece_rows(a)) return;
+    const float2 *part = a.partial + row * a.segments;
+    float top = kLowest, s = 0.f;
+    for (int g = threadIdx.x; g < a.segments; g += 256) {
+        const float2 p = part[g];
+        const float m = fmaxf(top, p.x);
+        s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
+        top = m;
+    }
+    join_sums(top, s, slots);
+    const float l = top + logf(s), z = a.zt[row];
+    if (threadIdx.x == 0) {
+        const int to = a.live ? a.live[row] : (int)row;
+        if (a.lse) a.lse[row] = l;
+        if (loss) loss[to] = l - z;
+        if (lse) lse[to] = l;
+    }
+    if constexpr (STORE) {
+        const float w = a.weight ? a.weight[row] : 1.f, u = a.softcap > 0.f ? z / a.softcap : 0.f;
+        const float own = w * (exp2_fast((z - l) * kLog2e) - 1.f) * (1.f - u * u);
+        const int t = a.target[row], end = a.segments * segment;
+        uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld;
+#pragma unroll 4
+        for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
+            __bf16 o[8];
+            if (c < end) {
+                _Float16 v[8];
+                __builtin_memcpy(v, __builtin_assume_aligned(dz + c, 16), 16);
+                const float f = w * exp2_fast(__builtin_fmaf(part[c / segment].x - l, kLog2e, -15.f));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = (__bf16)(c + e == t ? own : (float)v[e] * f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = (__bf16)0.f;
+            }
+            __builtin_memcpy(__builtin_assume_aligned(dz + c, 16), o, 16);
+        }
+    }
 }
 
-// zeros: losses (and lse) of rows without a target; rows of dW past the vocabulary
-__global__ __launch_bounds__(256) void vocab_zero_kernel(float *loss, float *lse, const int *place, int64_t rows) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= rows || place[r] >= 0) return;
-    if (loss) loss[r] = 0.f;
-    if (lse) lse[r] = 0.f;
-}
+// zeros: rows of dW past the vocabulary
 __global__ __launch_bounds__(256) void vocab_fill_kernel(uint16_t *p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
@@ -320,6 +431,7 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_dz_kernel(HeadArgs a) {
     for (int j = 0; j < T::NB; ++j) {
         const int64_t at = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31), row = a.row0 + at;
         const bool there = at < rows;
+        const float inv_cap = CAP ? 1.f / a.softcap : 0.f;
         const float w = there ? (a.weight ? a.weight[row] : 1.f) * (SPLIT ? a.scales[2] : 1.f) : 0.f;
         const float shift = there ? a.lse[row] * kLog2e : 0.f;
         const int t = there ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
@@ -334,11 +446,11 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_dz_kernel(HeadArgs a) {
                     float d = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
                     if (t == 32 * i + 16 * h + e) d -= 1.f;
                     if (CAP) {
-                        const float u = z / a.softcap;
+                        const float u = z * inv_cap;
                         d *= z == -__builtin_inff() ? 0.f : 1.f - u * u;
                     }
                     d = there ? d * w : 0.f;
-                    if constexpr (SPLIT) halves(d, 1.f, hi[e], lo[e]);
+                    if constexpr (SPLIT) halves(d, hi[e], lo[e]);
                     else {
                         const __bf16 b = (__bf16)d;
                         __builtin_memcpy(&hi[e], &b, 2);
@@ -539,50 +651,29 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     char *ws = static_cast<char *>(workspace);
     int *place = reinterpret_cast<int *>(ws + p.at_int), *live = place + p.rows, *target = live + p.rows, *count = target + p.rows;
     float *f = reinterpret_cast<float *>(ws + p.at_float);
-    float *packed_weight = f, *packed_lse = f + p.rows, *zt = f + 2 * p.rows, *scales = f + 3 * p.rows, *x_max = scales + 4,
-          *w_max = x_max + kMaxParts;
+    float *packed_weight = f, *packed_lse = f + p.rows, *zt = f + 2 * p.rows, *scales = f + 3 * p.rows,
+          *maxima = scales + 4;
     const int64_t rows = v->rows;
-    const unsigned row_groups = (unsigned)((rows + 255) / 256);
-    hipLaunchKernelGGL(vocab_live_kernel, dim3(1), dim3(1024), 0, stream, v->targets, (int)v->targets_wide, rows, v->vocab, weight,
-                       count, live, place, target, packed_weight, scales + 3);
-    if (loss || lse) hipLaunchKernelGGL(vocab_zero_kernel, dim3(row_groups), dim3(256), 0, stream, loss, lse, place, rows);
-    if (p.split) {
-        hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts), dim3(256), 0, stream, static_cast<const float *>(v->x), v->x_stride,
-                           rows, v->dim, place, x_max);
-        hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts), dim3(256), 0, stream, static_cast<const float *>(v->weight),
-                           v->weight_stride, v->vocab, v->dim, (const int *)nullptr, w_max);
-        hipLaunchKernelGGL(vocab_scale_kernel, dim3(1), dim3(64), 0, stream, x_max, w_max, kMaxParts, scales + 3, scales);
-    }
+    hipLaunchKernelGGL((rows <= 4096 ? vocab_live_kernel<4> : vocab_live_kernel<16>), dim3(1), dim3(1024), 0, stream, v->targets, (int)v->targets_wide, rows, v->vocab, weight,
+                       given, count, live, place, target, packed_weight, packed_lse, scales + 3);
     HeadArgs a = {};
     a.x = Operand{reinterpret_cast<__bf16 *>(ws + p.at_x), p.ld, p.rows * p.ld};
     a.w = p.pack_w ? Operand{reinterpret_cast<__bf16 *>(ws + p.at_w), p.ld, v->vocab * p.ld}
                    : Operand{static_cast<const __bf16 *>(v->weight), v->weight_stride, 0};
-    constexpr int64_t kRows = 1 << 22;   // a launch has fewer than 2^32 threads
-    for (int64_t r = 0; r < p.rows; r += kRows) {
-        const unsigned n = (unsigned)(p.rows - r < kRows ? p.rows - r : kRows);
-        if (p.split)
-            hipLaunchKernelGGL((vocab_pack_kernel<float, true>), dim3(n), dim3(256), 0, stream, static_cast<const float *>(v->x),
-                               v->x_stride, rows, r, v->dim, place, count, p.rows, scales, a.x, static_cast<float *>(dx));
-        else
-            hipLaunchKernelGGL((vocab_pack_kernel<__bf16, false>), dim3(n), dim3(256), 0, stream, static_cast<const __bf16 *>(v->x),
-                               v->x_stride, rows, r, v->dim, place, count, p.rows, scales, a.x, static_cast<__bf16 *>(dx));
-    }
-    if (p.pack_w) {
-        if (p.split)
-            hipLaunchKernelGGL((vocab_pack_kernel<float, true>), dim3((unsigned)v->vocab), dim3(256), 0, stream,
-                               static_cast<const float *>(v->weight), v->weight_stride, v->vocab, (int64_t)0, v->dim,
-                               (const int *)nullptr, (const int *)nullptr, v->vocab, scales + 1, a.w, (float *)nullptr);
-        else
-            hipLaunchKernelGGL((vocab_pack_kernel<__bf16, false>), dim3((unsigned)v->vocab), dim3(256), 0, stream,
-                               static_cast<const __bf16 *>(v->weight), v->weight_stride, v->vocab, (int64_t)0, v->dim,
-                               (const int *)nullptr, (const int *)nullptr, v->vocab, scales, a.w, (__bf16 *)nullptr);
-    }
+    PackArgs k = {};
+    k.src[0] = v->x, k.src[1] = v->weight, k.src_ld[0] = v->x_stride, k.src_ld[1] = v->weight_stride;
+    k.rows[0] = rows, k.rows[1] = v->vocab, k.padded[0] = p.rows, k.padded[1] = p.pack_w ? v->vocab : 0;
+    k.to[0] = a.x, k.to[1] = a.w, k.dim = v->dim, k.place = place, k.count = count;
+    k.max = maxima, k.weight_max = scales + 3, k.scales = scales, k.dx = dx, k.loss = loss, k.lse = lse;
+    if (p.split) hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts, 2), dim3(256), 0, stream, k, maxima);
+    const int64_t most = p.rows > k.padded[1] ? p.rows : k.padded[1], packs = (most + 3) / 4;
+    hipLaunchKernelGGL((p.split ? vocab_pack_kernel<float, true> : vocab_pack_kernel<__bf16, false>),
+                       dim3((unsigned)(packs < 4096 ? packs : 4096), p.pack_w ? 2 : 1), dim3(256), 0, stream, k);
     a.count = count, a.live = live, a.target = target, a.scales = scales;
     a.weight = weight ? packed_weight : nullptr;
     a.lse = packed_lse, a.zt = zt, a.partial = reinterpret_cast<float2 *>(ws + p.at_partial);
-    a.rows = p.rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
+    a.segments = (int)p.segments, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
     a.fp32 = p.split;
-    if (given) hipLaunchKernelGGL(vocab_lse_gather_kernel, dim3(row_groups), dim3(256), 0, stream, count, live, given, packed_lse);
     if (dw && width > v->vocab) {
         const int64_t n = (width - v->vocab) * v->dim * (p.split ? 2 : 1);
         hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,
@@ -594,17 +685,22 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
         a.row0 = i * p.piece, a.piece = p.rows - a.row0 < p.piece ? p.rows - a.row0 : p.piece;
         a.tiles_m = (int)((v->vocab + Tile::MT - 1) / Tile::MT), a.tiles_n = (int)(a.piece / Tile::NT), a.splits = 1;
         const dim3 tiles((unsigned)(a.tiles_m * a.tiles_n));
+        a.dz = Operand{reinterpret_cast<__bf16 *>(ws + p.at_dz), p.vocab_ld, p.piece * p.vocab_ld};
+        const bool store = grad && !p.split;
         if (!given) {
-            auto kernel = p.split ? (cap ? vocab_loss_kernel<Tile, true, true> : vocab_loss_kernel<Tile, true, false>)
-                                  : (cap ? vocab_loss_kernel<Tile, false, true> : vocab_loss_kernel<Tile, false, false>);
+            auto kernel = p.split ? (cap ? vocab_loss_kernel<Tile, true, true, false> : vocab_loss_kernel<Tile, true, false, false>)
+                          : store ? (cap ? vocab_loss_kernel<Tile, false, true, true> : vocab_loss_kernel<Tile, false, false, true>)
+                                  : (cap ? vocab_loss_kernel<Tile, false, true, false> : vocab_loss_kernel<Tile, false, false, false>);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
-            hipLaunchKernelGGL(vocab_lse_kernel, dim3((unsigned)((a.piece + 31) / 32)), dim3(256), 0, stream, a, (int)p.segments, loss, lse);
+            hipLaunchKernelGGL((store ? vocab_lse_kernel<true> : vocab_lse_kernel<false>), dim3((unsigned)a.piece), dim3(256), 0,
+                               stream, a, kSegment, loss, lse);
         }
         if (!grad) continue;
-        a.dz = Operand{reinterpret_cast<__bf16 *>(ws + p.at_dz), p.vocab_ld, p.piece * p.vocab_ld};
-        auto kernel = p.split ? (cap ? vocab_dz_kernel<Tile, true, true> : vocab_dz_kernel<Tile, true, false>)
-                              : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
-        hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
+        if (given || !store) {
+            auto kernel = p.split ? (cap ? vocab_dz_kernel<Tile, true, true> : vocab_dz_kernel<Tile, true, false>)
+                                  : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
+            hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
+        }
         a.slabs = reinterpret_cast<float *>(ws + p.at_slabs);
         a.out_ld = v->dim;
         const int64_t per = p.ld / 8;
