@@ -38,7 +38,7 @@ struct HeadArgs {
     int64_t row0;                // the piece's first packed row
     int64_t piece;               // rows of the piece, at most
     int vocab, dim, nk, segments;  // nk: stages of k over dim
-    int tiles_m, tiles_n, splits;
+    int tiles_m;
     float softcap;
     void *out;                   // dx or dW
     int64_t out_ld;
@@ -50,6 +50,20 @@ struct HeadArgs {
 __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
     const int64_t n = *a.count - a.row0;
     return n < 0 ? 0 : n < a.piece ? n : a.piece;
+}
+
+// In how many parts workgroups share the stages of k of a product with this many tiles, by what was measured: a tile takes 1.8 us per
+// stage and 3 us more, 256 of them run at a time, and a part's tile of fp32 sums costs 0.12 us of the whole chip's time. At most
+// kSplitTiles parts of tiles in all, at least 4 stages each.
+constexpr uint32_t kSplitTiles = 512;
+__device__ inline int splits_of(uint32_t tiles, uint32_t stages) {
+    if (tiles == 0 || 2 * tiles > kSplitTiles) return 1;
+    uint32_t best = stages * 18 + 30, splits = 1;   // in 100 ns (stages of 2^22 entries or a piece's rows: far from 32 bits)
+    for (uint32_t s = 2; s * tiles <= kSplitTiles && 4 * s <= stages; ++s) {
+        const uint32_t ns = (tiles * s + 255) / 256 * ((stages + s - 1) / s * 18 + 30) + tiles * s * 6 / 5;
+        if (ns < best) best = ns, splits = s;
+    }
+    return (int)splits;
 }
 
 // softcap tanh(z / softcap) with an error of 2^-22 softcap: what enters exp(z) is absolute
@@ -251,42 +265,51 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(PackArgs a) {
 
 // --- logits ---
 
-// The tile's logits, capped and unscaled; -inf past the vocabulary
-template <class T, bool CAP>
-__device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, float unit, f32x16 (&acc)[T::FB][T::NB]) {
-    const float k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
-    const bool edge = m0 + T::FB * 32 > a.vocab;
+// The tile's logits, unscaled and capped. Past the vocabulary: -inf, or under the cap (where they are multiplied by cap') a value whose
+// exponential vanishes beside any other's.
+template <class T, bool SPLIT, bool CAP>
+__device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f32x16 (&acc)[T::FB][T::NB]) {
+    const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f, k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
 #pragma unroll
     for (int i = 0; i < T::FB; ++i)
 #pragma unroll
         for (int j = 0; j < T::NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float z = acc[i][j][r] * unit;
+                float z = SPLIT ? acc[i][j][r] * unit : acc[i][j][r];
                 if (CAP) z = cap_of(z, a.softcap, k);
-                if (edge && m0 + 32 * i + 16 * (r / 8) + 8 * (lane >> 5) + r % 8 >= a.vocab) z = -__builtin_inff();
                 acc[i][j][r] = z;
             }
+    if (m0 + T::FB * 32 > a.vocab) {
+        const float none = CAP ? -8.f * a.softcap - 200.f : -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (m0 + 32 * i + 16 * (r / 8) + 8 * (lane >> 5) + r % 8 >= a.vocab)
+#pragma unroll
+                    for (int j = 0; j < T::NB; ++j) acc[i][j][r] = none;
+    }
 }
 
 // STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_kernel turns into dZ. (Its rounding, 2^-11,
 // comes before dZ's own, 2^-8; below 2^-29 of the segment's largest it has fewer bits, below 2^-39 none.)
 template <class T, bool SPLIT, bool CAP, bool STORE>
-__global__ __launch_bounds__(64 * T::NW) void vocab_loss_kernel(HeadArgs a) {
+__global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
-    int tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
     const int64_t rows = piece_rows(a);
-    if ((int64_t)tn * T::NT >= rows) return;
+    const int tiles_n = (int)((rows + T::NT - 1) / T::NT);   // (of the rows that there are: XCDs share those evenly)
+    if ((int)blockIdx.x >= a.tiles_m * tiles_n) return;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
                                            T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
     if (m0 >= a.vocab) return;
-    const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f;
-    to_logits<T, CAP>(a, m0, lane, unit, acc);
-    const float inv_cap = CAP ? 1.f / a.softcap : 0.f;
+    to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
+    const float bend = CAP ? -32768.f / a.softcap / a.softcap : 0.f;   // of cap' 2^15
     static_assert(T::FB * 32 == kSegment, "a wave's entries are a segment");
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
@@ -321,16 +344,17 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_loss_kernel(HeadArgs a) {
                     float p = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
                     s += p;
                     if constexpr (STORE) {
-                        if (CAP) {
-                            const float u = z * inv_cap;
-                            p *= z == -__builtin_inff() ? 0.f : 1.f - u * u;
-                        }
-                        v[e] = (_Float16)(there ? p * 32768.f : 0.f);   // (rows behind the last one are multiplied by zeros)
+                        p *= CAP ? __builtin_fmaf(z * bend, z, 32768.f) : 32768.f;
+                        v[e] = (_Float16)p;
                     }
                 }
                 if constexpr (STORE) {
                     uint16_t *to = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld + m0 + 32 * i +
                                    16 * h + 8 * (lane >> 5);
+                    // (rows behind the last one are multiplied by zeros)
+                    if (!there)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = (_Float16)0.f;
                     __builtin_memcpy(__builtin_assume_aligned(to, 16), v, 16);
                 }
             }
@@ -361,6 +385,16 @@ __device__ __forceinline__ void join_sums(float &top, float &s, float2 (&slots)[
     for (int w = 1; w < 4; ++w) join(slots[w].x, slots[w].y);
 }
 
+// This thread's share of a row's segments
+__device__ __forceinline__ void row_sums(const float2 *part, int segments, float &top, float &s) {
+    for (int g = threadIdx.x; g < segments; g += 256) {
+        const float2 p = part[g];
+        const float m = fmaxf(top, p.x);
+        s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
+        top = m;
+    }
+}
+
 // A row's lse and loss from its segments; with STORE also dZ from what vocab_loss_kernel left:
 // dZ_v = weight exp(top - lse) 2^-15 stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
 template <bool STORE>
@@ -370,12 +404,7 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segment,
     if (at >= piece_rows(a)) return;
     const float2 *part = a.partial + row * a.segments;
     float top = kLowest, s = 0.f;
-    for (int g = threadIdx.x; g < a.segments; g += 256) {
-        const float2 p = part[g];
-        const float m = fmaxf(top, p.x);
-        s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
-        top = m;
-    }
+    row_sums(part, a.segments, top, s);
     join_sums(top, s, slots);
     const float l = top + logf(s), z = a.zt[row];
     if (threadIdx.x == 0) {
@@ -407,32 +436,185 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segment,
     }
 }
 
+// --- the losses of a few rows ---
+
+// What is read is the weight, once: a workgroup takes 16 VB vocabulary entries for up to 16 RB rows, its four waves a quarter of dim
+// each, straight from memory into v_mfma_f32_16x16x32_bf16's (fp32: v_mfma_f32_16x16x4_f32's, exact products) operands: 16 lanes on
+// 16 rows of the weight, and the rows of x from the caches. The waves' sums meet in LDS; wave v takes entries 16 v on from there.
+struct FewArgs {
+    const void *x, *w, *targets;
+    int64_t x_ld, w_ld;
+    float2 *partial;
+    float *zt;
+    int rows, vocab, dim, segments, wide;
+    float softcap;
+};
+
+template <class E, int VB, int RB, bool CAP>
+__global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
+    constexpr int N = sizeof(E) == 2 ? 8 : 4, U = 4;   // elements per load, loads in flight per block
+    __shared__ float sums[4][VB][RB][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int v0 = blockIdx.x * 16 * VB;
+    const E *w[VB], *x[RB];
+#pragma unroll
+    for (int b = 0; b < VB; ++b) {
+        const int v = v0 + 16 * b + i;
+        w[b] = static_cast<const E *>(a.w) + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.w_ld;
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int r = 16 * b + i;
+        x[b] = static_cast<const E *>(a.x) + (int64_t)(r < a.rows ? r : a.rows - 1) * a.x_ld;
+    }
+    f32x4 acc[VB][RB] = {};
+    auto multiply = [&](const E (&vw)[N], const E (&vx)[N], f32x4 &c) {
+        if constexpr (sizeof(E) == 2) {
+            bf16x8 p, q;
+            __builtin_memcpy(&p, vw, 16);
+            __builtin_memcpy(&q, vx, 16);
+            c = mfma16x16x32(p, q, c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(vw[e], vx[e], c, 0, 0, 0);
+        }
+    };
+    // steps of 4 N consecutive elements of dim, wave after wave; the last one may be cut
+    const int steps = (a.dim + 4 * N - 1) / (4 * N), whole = a.dim / (4 * N);
+    const int first = steps * wave / 4, last = steps * (wave + 1) / 4;
+    int s = first;
+    for (; s + U <= (last < whole ? last : whole); s += U) {
+        E vw[VB][U][N];
+#pragma unroll
+        for (int b = 0; b < VB; ++b)
+#pragma unroll
+            for (int u = 0; u < U; ++u) __builtin_memcpy(vw[b][u], w[b] + (s + u) * 4 * N + g * N, 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+                E vx[N];
+                __builtin_memcpy(vx, x[r] + (s + u) * 4 * N + g * N, 16);
+#pragma unroll
+                for (int b = 0; b < VB; ++b) multiply(vw[b][u], vx, acc[b][r]);
+            }
+        }
+    }
+    for (; s < last; ++s) {
+        const int at = s * 4 * N + g * N, n = a.dim - at;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            E vx[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) vx[e] = e < n ? x[r][at + e] : (E)0.f;
+#pragma unroll
+            for (int b = 0; b < VB; ++b) {
+                E vw[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) vw[e] = e < n ? w[b][at + e] : (E)0.f;
+                multiply(vw, vx, acc[b][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) __builtin_memcpy(sums[wave][b][r][lane], &acc[b][r], 16);
+    __syncthreads();
+    // entries v0 + 16 wave + 4 g + e of row 16 r + i
+    __shared__ float2 tops[4][RB][16];
+    if (wave < VB) {
+        const float k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+            const int row = 16 * r + i, v = v0 + 16 * wave + 4 * g;
+            float z[4], top = kLowest, t = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                z[e] = sums[0][wave][r][lane][e] + sums[1][wave][r][lane][e] + sums[2][wave][r][lane][e] + sums[3][wave][r][lane][e];
+                if (CAP) z[e] = cap_of(z[e], a.softcap, k);
+                if (v + e >= a.vocab) z[e] = -__builtin_inff();
+                top = fmaxf(top, z[e]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t += exp2_fast((z[e] - top) * kLog2e);
+            t += __shfl_xor(t, 16, 64);
+            t += __shfl_xor(t, 32, 64);
+            if (g == 0) tops[wave][r][i] = float2{top, t};
+            if (row < a.rows) {
+                const int64_t target = a.wide ? static_cast<const int64_t *>(a.targets)[row]
+                                              : (int64_t)static_cast<const int32_t *>(a.targets)[row];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (target == v + e && v + e < a.vocab) a.zt[row] = z[e];
+            }
+        }
+    }
+    __syncthreads();
+    for (int row = threadIdx.x; row < 16 * RB; row += 256) {
+        if (row >= a.rows) continue;
+        float2 p = tops[0][row / 16][row % 16];
+#pragma unroll
+        for (int b = 1; b < VB; ++b) {
+            const float2 q = tops[b][row / 16][row % 16];
+            const float m = fmaxf(p.x, q.x);
+            p = float2{m, p.y * exp2_fast((p.x - m) * kLog2e) + q.y * exp2_fast((q.x - m) * kLog2e)};
+        }
+        a.partial[(int64_t)row * a.segments + blockIdx.x] = p;
+    }
+}
+
+__global__ __launch_bounds__(256) void vocab_few_join_kernel(FewArgs a, float *loss, float *lse) {
+    __shared__ float2 slots[4];
+    const int row = blockIdx.x;
+    const int64_t t = a.wide ? static_cast<const int64_t *>(a.targets)[row] : (int64_t)static_cast<const int32_t *>(a.targets)[row];
+    const bool in = t >= 0 && t < a.vocab;
+    float top = kLowest, s = 0.f;
+    if (in) row_sums(a.partial + (int64_t)row * a.segments, a.segments, top, s);
+    join_sums(top, s, slots);
+    if (threadIdx.x) return;
+    const float l = top + logf(s);
+    loss[row] = in ? l - a.zt[row] : 0.f;
+    if (lse) lse[row] = in ? l : 0.f;
+}
+
+constexpr int kFewRows = 64;
+
+template <class E, int VB>
+void (*few_of(int64_t rows, bool cap))(FewArgs) {
+    return rows <= 16   ? (cap ? vocab_few_kernel<E, VB, 1, true> : vocab_few_kernel<E, VB, 1, false>)
+           : rows <= 32 ? (cap ? vocab_few_kernel<E, VB, 2, true> : vocab_few_kernel<E, VB, 2, false>)
+                        : (cap ? vocab_few_kernel<E, VB, 4, true> : vocab_few_kernel<E, VB, 4, false>);
+}
+
 // zeros: rows of dW past the vocabulary
 __global__ __launch_bounds__(256) void vocab_fill_kernel(uint16_t *p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
 template <class T, bool SPLIT, bool CAP>
-__global__ __launch_bounds__(64 * T::NW) void vocab_dz_kernel(HeadArgs a) {
+__global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
-    int tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
     const int64_t rows = piece_rows(a);
-    if ((int64_t)tn * T::NT >= rows) return;
+    const int tiles_n = (int)((rows + T::NT - 1) / T::NT);   // (of the rows that there are: XCDs share those evenly)
+    if ((int)blockIdx.x >= a.tiles_m * tiles_n) return;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
                                            T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
-    const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f;
-    to_logits<T, CAP>(a, m0, lane, unit, acc);
+    to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
     uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr));
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int64_t at = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31), row = a.row0 + at;
         const bool there = at < rows;
-        const float inv_cap = CAP ? 1.f / a.softcap : 0.f;
         const float w = there ? (a.weight ? a.weight[row] : 1.f) * (SPLIT ? a.scales[2] : 1.f) : 0.f;
+        const float bend = CAP ? -w / a.softcap / a.softcap : 0.f;   // of w cap'
         const float shift = there ? a.lse[row] * kLog2e : 0.f;
         const int t = there ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
 #pragma unroll
@@ -445,11 +627,8 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_dz_kernel(HeadArgs a) {
                     const float z = acc[i][j][8 * h + e];
                     float d = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
                     if (t == 32 * i + 16 * h + e) d -= 1.f;
-                    if (CAP) {
-                        const float u = z * inv_cap;
-                        d *= z == -__builtin_inff() ? 0.f : 1.f - u * u;
-                    }
-                    d = there ? d * w : 0.f;
+                    d *= CAP ? __builtin_fmaf(z * bend, z, w) : w;
+                    if (!there) d = 0.f;
                     if constexpr (SPLIT) halves(d, hi[e], lo[e]);
                     else {
                         const __bf16 b = (__bf16)d;
@@ -484,19 +663,35 @@ __device__ __forceinline__ void put_out(const HeadArgs &a, int64_t at, int n, co
     }
 }
 
+// How a gradient's product is cut, from the rows that there are
+struct Cut {
+    int64_t n_end;             // results along n: packed rows (dx) or vocabulary entries (dW)
+    int tiles_n, tiles, stages, splits;
+    template <class T, bool DX, bool SPLIT>
+    __device__ static Cut of(int64_t rows, int vocab, int tiles_m) {
+        Cut c;
+        c.n_end = DX ? rows : vocab;
+        c.tiles_n = (int)((c.n_end + T::NT - 1) / T::NT);
+        c.tiles = tiles_m * c.tiles_n;
+        c.stages = (SPLIT ? 3 : 1) * (int)(((DX ? vocab : rows) + T::BK - 1) / T::BK);
+        c.splits = splits_of(c.tiles, c.stages);
+        return c;
+    }
+};
+
 // DX: out row = row of x, n = packed row; otherwise (dW) n = vocabulary entry. m: columns of dim.
 template <class T, bool DX, bool SPLIT>
-__global__ __launch_bounds__(64 * T::NW) void vocab_grad_kernel(HeadArgs a) {
+__global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
-    const int tiles = a.tiles_m * a.tiles_n, split = blockIdx.x / tiles;
-    int tm, tn;
-    tile_of(blockIdx.x - split * tiles, a.tiles_m, a.tiles_n, tm, tn);
     const int64_t rows = piece_rows(a);
-    const int64_t n_end = DX ? rows : a.vocab;
-    if ((int64_t)tn * T::NT >= n_end) return;
+    const Cut c = Cut::of<T, DX, SPLIT>(rows, a.vocab, a.tiles_m);
+    if ((int)blockIdx.x >= c.tiles * c.splits) return;
+    const int split = blockIdx.x / c.tiles;
+    int tm, tn;
+    tile_of(blockIdx.x - split * c.tiles, a.tiles_m, c.tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nk = (int)(((DX ? a.vocab : rows) + T::BK - 1) / T::BK), all = SPLIT ? 3 * nk : nk;
-    const int first = (int)((int64_t)all * split / a.splits), last = (int)((int64_t)all * (split + 1) / a.splits);
+    const int nk = SPLIT ? c.stages / 3 : c.stages;
+    const int first = (int)((int64_t)c.stages * split / c.splits), last = (int)((int64_t)c.stages * (split + 1) / c.splits);
     const int dim8 = (int)a.x.ld / 8;   // chunks of a packed row
     f32x16 acc[T::FB][T::NB];
     if (DX)
@@ -512,7 +707,7 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_grad_kernel(HeadArgs a) {
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
         const int64_t n = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
-        if (n >= n_end) continue;
+        if (n >= c.n_end) continue;
         const int64_t to = DX ? a.live[a.row0 + n] : n;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
@@ -524,8 +719,8 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_grad_kernel(HeadArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * h + e] * unit;
                 const int left = a.dim - m;
-                if (a.splits > 1) {
-                    float *p = a.slabs + ((int64_t)split * (DX ? a.piece : a.vocab) + n) * a.x.ld + m;
+                if (c.splits > 1) {
+                    float *p = a.slabs + ((int64_t)split * c.n_end + n) * a.x.ld + m;
                     __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
                     continue;
                 }
@@ -542,15 +737,16 @@ __global__ __launch_bounds__(64 * T::NW) void vocab_grad_kernel(HeadArgs a) {
 }
 
 // The splits' sums, in order
-template <bool DX>
+template <class T, bool DX, bool SPLIT>
 __global__ __launch_bounds__(256) void vocab_sum_kernel(HeadArgs a) {
-    const int64_t rows = piece_rows(a), n_end = DX ? rows : a.vocab, per = a.x.ld / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / per;
+    const Cut k = Cut::of<T, DX, SPLIT>(piece_rows(a), a.vocab, a.tiles_m);
+    if (k.splits == 1) return;   // (the product has written its results)
+    const int64_t per = a.x.ld / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / per;
     const int m = (int)(i - n * per) * 8;
-    if (n >= n_end || m >= a.dim) return;
+    if (n >= k.n_end || m >= a.dim) return;
     float v[8] = {};
-    for (int s = 0; s < a.splits; ++s) {
-        const float *p = a.slabs + ((int64_t)s * (DX ? a.piece : a.vocab) + n) * a.x.ld + m;
+    for (int s = 0; s < k.splits; ++s) {
+        const float *p = a.slabs + ((int64_t)s * k.n_end + n) * a.x.ld + m;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += p[e];
     }
@@ -572,16 +768,21 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Plan {
     int64_t ld, rows, piece, pieces, vocab_ld, segments;
     int nk;
-    bool split, pack_w;
-    int dx_splits, dw_splits;
+    bool split, pack_w, split_dx, split_dw;   // split_dx, split_dw: the product's k may be split
+    int64_t dx_groups, dw_groups;
     int64_t at_int, at_float, at_partial, at_x, at_w, at_dz, at_slabs, at_sum, bytes;
 };
 
-int splits_of(int64_t tiles, int64_t stages) {
-    // a tile per CU, but no fewer than 8 stages of k per workgroup
-    int64_t s = 256 / (tiles > 256 ? 256 : tiles);
-    if (s > stages / 8) s = stages / 8;
-    return s < 1 ? 1 : (int)s;
+// For any number of rows up to the piece's: the most workgroups of a gradient's product, and the fp32 values of its splits' sums.
+// rows: whether the results are rows (dx), of which there may be fewer than n_end
+void most_of(bool rows, int64_t n_end, int64_t stages, int64_t ld, int64_t *groups, int64_t *slabs) {
+    const int64_t tiles_m = (ld + Tile::MT - 1) / Tile::MT, tiles = tiles_m * ((n_end + Tile::NT - 1) / Tile::NT);
+    *groups = tiles > kSplitTiles ? tiles : kSplitTiles;
+    // s parts where s tiles <= kSplitTiles and 4 s <= stages
+    const int64_t least = rows ? tiles_m : tiles, s = stages / 4 < kSplitTiles / least ? stages / 4 : kSplitTiles / least;
+    int64_t n = s * n_end;
+    if (rows && kSplitTiles / tiles_m * Tile::NT < n) n = kSplitTiles / tiles_m * Tile::NT;
+    *slabs = s < 2 ? 0 : n * ld;
 }
 
 Plan plan_of(const noise_vocab_t *v, bool grad) {
@@ -615,13 +816,11 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
-        const int64_t tm = (p.ld + Tile::MT - 1) / Tile::MT;
-        p.dx_splits = splits_of(tm * (p.piece / Tile::NT), (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK);
-        p.dw_splits = splits_of(tm * ((v->vocab + Tile::NT - 1) / Tile::NT), (p.split ? 3 : 1) * p.piece / Tile::BK);
-        int64_t slabs = p.dx_splits > 1 ? 4 * p.dx_splits * p.piece * p.ld : 0;
-        const int64_t dw = p.dw_splits > 1 ? 4 * p.dw_splits * v->vocab * p.ld : 0;
-        if (dw > slabs) slabs = dw;
-        p.at_slabs = take(slabs);
+        int64_t dx, dw;
+        most_of(true, p.piece, (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK, p.ld, &p.dx_groups, &dx);
+        most_of(false, v->vocab, (p.split ? 3 : 1) * p.piece / Tile::BK, p.ld, &p.dw_groups, &dw);
+        p.split_dx = dx > 0, p.split_dw = dw > 0;
+        p.at_slabs = take(4 * (dx > dw ? dx : dw));
         if (p.pieces > 1) p.at_sum = take(4 * v->vocab * p.ld);
     }
     p.bytes = at;
@@ -640,6 +839,38 @@ int check(const char *fn, const noise_vocab_t *v, float softcap) {
                         aligned(v->targets, v->targets_wide ? 8 : 4),
                     "%s: a pointer is NULL or not aligned to its type", fn);
     return NOISE_OK;
+}
+
+struct FewPlan {
+    int blocks;   // of 16 entries per workgroup
+    int64_t segments, bytes;
+};
+FewPlan few_plan(const noise_vocab_t *v) {
+    FewPlan p;
+    // four workgroups per CU with 64 entries each, or 16 each
+    p.blocks = v->vocab >= 64 * 512 ? 4 : 1;
+    p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
+    p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
+    return p;
+}
+
+int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace, int64_t workspace_bytes,
+            hipStream_t stream) {
+    const FewPlan p = few_plan(v);
+    NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes,
+                    "%s: workspace of %lld bytes (16 B aligned) required", fn, (long long)p.bytes);
+    FewArgs a;
+    a.x = v->x, a.w = v->weight, a.targets = v->targets, a.x_ld = v->x_stride, a.w_ld = v->weight_stride;
+    a.zt = static_cast<float *>(workspace);
+    a.partial = reinterpret_cast<float2 *>(a.zt + kFewRows);
+    a.rows = (int)v->rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.segments = (int)p.segments, a.wide = (int)v->targets_wide;
+    a.softcap = softcap;
+    const bool cap = softcap > 0.f;
+    auto kernel = v->type == NOISE_FP32 ? (p.blocks == 4 ? few_of<float, 4>(v->rows, cap) : few_of<float, 1>(v->rows, cap))
+                                        : (p.blocks == 4 ? few_of<__bf16, 4>(v->rows, cap) : few_of<__bf16, 1>(v->rows, cap));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)p.segments), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(vocab_few_join_kernel, dim3((unsigned)v->rows), dim3(256), 0, stream, a, loss, lse);
+    return launch_status(fn);
 }
 
 // loss and lse (out, or with `given` lse in); dx and dw where grad
@@ -683,8 +914,8 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     const bool cap = softcap > 0.f;
     for (int64_t i = 0; i < p.pieces; ++i) {
         a.row0 = i * p.piece, a.piece = p.rows - a.row0 < p.piece ? p.rows - a.row0 : p.piece;
-        a.tiles_m = (int)((v->vocab + Tile::MT - 1) / Tile::MT), a.tiles_n = (int)(a.piece / Tile::NT), a.splits = 1;
-        const dim3 tiles((unsigned)(a.tiles_m * a.tiles_n));
+        a.tiles_m = (int)((v->vocab + Tile::MT - 1) / Tile::MT);
+        const dim3 tiles((unsigned)(a.tiles_m * (a.piece / Tile::NT)));
         a.dz = Operand{reinterpret_cast<__bf16 *>(ws + p.at_dz), p.vocab_ld, p.piece * p.vocab_ld};
         const bool store = grad && !p.split;
         if (!given) {
@@ -706,21 +937,21 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
         const int64_t per = p.ld / 8;
         a.tiles_m = (int)((p.ld + Tile::MT - 1) / Tile::MT);
         if (dx) {
-            a.out = dx, a.splits = p.dx_splits, a.sum = nullptr;
+            a.out = dx, a.sum = nullptr;
             hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, true, true> : vocab_grad_kernel<Tile, true, false>),
-                               dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(threads), 0, stream, a);
-            if (a.splits > 1)
-                hipLaunchKernelGGL(vocab_sum_kernel<true>, dim3((unsigned)((a.piece * per + 255) / 256)), dim3(256), 0, stream, a);
+                               dim3((unsigned)p.dx_groups), dim3(threads), 0, stream, a);
+            if (p.split_dx)
+                hipLaunchKernelGGL((p.split ? vocab_sum_kernel<Tile, true, true> : vocab_sum_kernel<Tile, true, false>),
+                                   dim3((unsigned)((a.piece * per + 255) / 256)), dim3(256), 0, stream, a);
         }
         if (dw) {
-            a.tiles_n = (int)((v->vocab + Tile::NT - 1) / Tile::NT);
-            a.splits = p.dw_splits;
             a.sum = p.pieces > 1 ? reinterpret_cast<float *>(ws + p.at_sum) : nullptr;
             a.add = i > 0, a.out = i + 1 == p.pieces ? dw : nullptr;
             hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, false, true> : vocab_grad_kernel<Tile, false, false>),
-                               dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)), dim3(threads), 0, stream, a);
-            if (a.splits > 1)
-                hipLaunchKernelGGL(vocab_sum_kernel<false>, dim3((unsigned)((v->vocab * per + 255) / 256)), dim3(256), 0, stream, a);
+                               dim3((unsigned)p.dw_groups), dim3(threads), 0, stream, a);
+            if (p.split_dw)
+                hipLaunchKernelGGL((p.split ? vocab_sum_kernel<Tile, false, true> : vocab_sum_kernel<Tile, false, false>),
+                                   dim3((unsigned)((v->vocab * per + 255) / 256)), dim3(256), 0, stream, a);
         }
     }
     return launch_status(fn);
@@ -734,7 +965,8 @@ using namespace noise;
 extern "C" int64_t noise_vocab_workspace_bytes(const noise_vocab_t *v, int with_grad) {
     clear_error();
     if (check("noise_vocab_workspace_bytes", v, 0.f)) return -1;
-    return v->rows ? plan_of(v, with_grad != 0).bytes : 0;
+    if (v->rows == 0) return 0;
+    return !with_grad && v->rows <= kFewRows ? few_plan(v).bytes : plan_of(v, with_grad != 0).bytes;
 }
 
 extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace,
@@ -744,6 +976,7 @@ extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *lo
     if (int e = check(fn, v, softcap)) return e;
     if (v->rows == 0) return NOISE_OK;
     NOISE_CHECK_ARG(loss && aligned(loss, 4) && aligned(lse, 4), "%s: loss NULL or not 4 B aligned", fn);
+    if (v->rows <= kFewRows) return run_few(fn, v, softcap, loss, lse, workspace, workspace_bytes, (hipStream_t)stream);
     return run(fn, v, softcap, nullptr, loss, lse, nullptr, nullptr, nullptr, 0, false, workspace, workspace_bytes, (hipStream_t)stream);
 }
 

@@ -123,6 +123,14 @@ def test_rows(R, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('V', [17, 32767, 32768, 40001])
+def test_few_rows(V, dtype):
+    """The losses of up to 64 tokens, which have a kernel of their own, next to those of more."""
+    for R, D in ((1, 1), (4, 130), (16, 128), (17, 7), (31, 257), (33, 96), (64, 1000), (65, 64)):
+        check(*make(R, V, D, dtype, R, V + R % 3, masked=R % 2 == 1), V, 15.0 if R % 4 == 0 else None)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
 def test_masks(dtype):
     """Rows without a target hold NaN and infinities; all of them, all but one; weights with NaN there; int32 targets."""
     x, weight, targets, w = make(300, 500, 96, dtype, 3, 520, masked=True)
@@ -206,7 +214,7 @@ def test_values():
         loss = linear_cross_entropy(bad, weight, targets)
         dx = linear_cross_entropy_grad(bad, weight, targets, w)[1]
         rest = [r for r in range(50) if r not in (10, 20)]
-        assert not torch.isfinite(loss[[10, 20]]).any() and torch.equal(loss[rest], clean[0][rest])
+        assert not torch.isfinite(loss[[10, 20]]).any() and torch.equal(loss[rest], linear_cross_entropy(x, weight, targets)[rest])
         assert torch.isnan(dx[10]).all() and torch.equal(dx[rest], clean[1][rest])
     # tensors of very different sizes in fp32
     x, weight, targets, w = make(50, 400, 64, F32, 8)
