@@ -40,11 +40,19 @@ struct HeadArgs {
     int vocab, dim, nk, segments;  // nk: stages of k over dim
     int tiles_m;
     float softcap;
-    void *out;                   // dx or dW
-    int64_t out_ld;
+};
+
+// A gradient: dx (of rows) or dW (of vocabulary entries)
+struct Result {
+    void *out;                   // NULL: not asked for, or (with sum) not yet
     float *slabs;                // [splits][n][m] where k is split
     float *sum;                  // dW over several pieces: fp32 [vocab][dim]
-    int add, fp32;               // add: to sum's values; fp32: out's type
+    uint32_t groups;             // workgroups of its product, at most
+    uint32_t sums;               // workgroups that join its splits (0: it has none)
+};
+struct GradArgs {
+    Result dx, dw;
+    int add, fp32, tiles_m;      // add: to dw.sum's values; fp32: the results' type
 };
 
 __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
@@ -644,16 +652,16 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
 
 // --- gradients ---
 
-// 8 consecutive results, of which n exist, in the output's type at any address of that type
-__device__ __forceinline__ void put_out(const HeadArgs &a, int64_t at, int n, const float (&v)[8]) {
-    if (a.fp32) {
-        float *p = static_cast<float *>(a.out) + at;
+// 8 consecutive results, of which n exist, in their type at any address of it
+__device__ __forceinline__ void put_out(void *out, int fp32, int64_t at, int n, const float (&v)[8]) {
+    if (fp32) {
+        float *p = static_cast<float *>(out) + at;
         if (n >= 8) __builtin_memcpy(p, v, 32);
         else
             for (int e = 0; e < 8; ++e)
                 if (e < n) p[e] = v[e];
     } else {
-        __bf16 o[8], *p = static_cast<__bf16 *>(a.out) + at;
+        __bf16 o[8], *p = static_cast<__bf16 *>(out) + at;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = (__bf16)v[e];
         if (n >= 8) __builtin_memcpy(p, o, 16);
@@ -661,6 +669,20 @@ __device__ __forceinline__ void put_out(const HeadArgs &a, int64_t at, int n, co
             for (int e = 0; e < 8; ++e)
                 if (e < n) p[e] = o[e];
     }
+}
+
+// Columns m .. m + 7 of result n: added to the pieces before, and stored as its row
+template <bool DX>
+__device__ __forceinline__ void finish(const HeadArgs &a, const GradArgs &g, int64_t n, int m, float (&v)[8]) {
+    const Result &r = DX ? g.dx : g.dw;
+    if (!DX && r.sum) {
+        float *p = r.sum + n * a.x.ld + m;
+        if (g.add)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += p[e];
+        if (!r.out) __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
+    }
+    if (r.out) put_out(r.out, g.fp32, (DX ? (int64_t)a.live[a.row0 + n] : n) * a.dim + m, a.dim - m, v);
 }
 
 // How a gradient's product is cut, from the rows that there are
@@ -679,16 +701,16 @@ struct Cut {
     }
 };
 
-// DX: out row = row of x, n = packed row; otherwise (dW) n = vocabulary entry. m: columns of dim.
+// n: packed rows (DX) or vocabulary entries; m: columns of dim
 template <class T, bool DX, bool SPLIT>
-__global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+__device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, uint32_t group, char *lds) {
+    const Result &res = DX ? g.dx : g.dw;
     const int64_t rows = piece_rows(a);
-    const Cut c = Cut::of<T, DX, SPLIT>(rows, a.vocab, a.tiles_m);
-    if ((int)blockIdx.x >= c.tiles * c.splits) return;
-    const int split = blockIdx.x / c.tiles;
+    const Cut c = Cut::of<T, DX, SPLIT>(rows, a.vocab, g.tiles_m);
+    if (group >= (uint32_t)c.tiles * c.splits) return;
+    const int split = group / c.tiles;
     int tm, tn;
-    tile_of(blockIdx.x - split * c.tiles, a.tiles_m, c.tiles_n, tm, tn);
+    tile_of(group - split * c.tiles, g.tiles_m, c.tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nk = SPLIT ? c.stages / 3 : c.stages;
     const int first = (int)((int64_t)c.stages * split / c.splits), last = (int)((int64_t)c.stages * (split + 1) / c.splits);
@@ -708,7 +730,6 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a) {
     for (int j = 0; j < T::NB; ++j) {
         const int64_t n = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
         if (n >= c.n_end) continue;
-        const int64_t to = DX ? a.live[a.row0 + n] : n;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
 #pragma unroll
@@ -717,47 +738,45 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a) {
                 if (m >= a.dim) continue;
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = acc[i][j][8 * h + e] * unit;
-                const int left = a.dim - m;
-                if (c.splits > 1) {
-                    float *p = a.slabs + ((int64_t)split * c.n_end + n) * a.x.ld + m;
-                    __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
-                    continue;
-                }
-                if (a.sum) {
-                    float *p = a.sum + n * a.x.ld + m;
-                    if (a.add)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += p[e];
-                    if (!a.out) __builtin_memcpy(__builtin_assume_aligned(p, 16), v, 32);
-                }
-                if (a.out) put_out(a, to * a.out_ld + m, left, v);
+                for (int e = 0; e < 8; ++e) v[e] = SPLIT ? acc[i][j][8 * h + e] * unit : acc[i][j][8 * h + e];
+                if (c.splits > 1)
+                    __builtin_memcpy(__builtin_assume_aligned(res.slabs + ((int64_t)split * c.n_end + n) * a.x.ld + m, 16), v, 32);
+                else
+                    finish<DX>(a, g, n, m, v);
             }
     }
 }
 
+// Both gradients in one launch: neither waits for the other's last workgroups
+template <class T, bool SPLIT>
+__global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a, GradArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
+    if (blockIdx.x < g.dx.groups) gradient<T, true, SPLIT>(a, g, blockIdx.x, lds);
+    else gradient<T, false, SPLIT>(a, g, blockIdx.x - g.dx.groups, lds);
+}
+
 // The splits' sums, in order
 template <class T, bool DX, bool SPLIT>
-__global__ __launch_bounds__(256) void vocab_sum_kernel(HeadArgs a) {
-    const Cut k = Cut::of<T, DX, SPLIT>(piece_rows(a), a.vocab, a.tiles_m);
+__device__ __forceinline__ void join_splits(const HeadArgs &a, const GradArgs &g, uint32_t group) {
+    const Cut k = Cut::of<T, DX, SPLIT>(piece_rows(a), a.vocab, g.tiles_m);
     if (k.splits == 1) return;   // (the product has written its results)
-    const int64_t per = a.x.ld / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = i / per;
+    const int64_t i = (int64_t)group * 256 + threadIdx.x;
+    const uint32_t per = (uint32_t)(a.x.ld / 8);
+    const int64_t n = i / per;
     const int m = (int)(i - n * per) * 8;
     if (n >= k.n_end || m >= a.dim) return;
     float v[8] = {};
     for (int s = 0; s < k.splits; ++s) {
-        const float *p = a.slabs + ((int64_t)s * k.n_end + n) * a.x.ld + m;
+        const float *p = (DX ? g.dx : g.dw).slabs + ((int64_t)s * k.n_end + n) * a.x.ld + m;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += p[e];
     }
-    if (a.sum) {
-        float *p = a.sum + n * a.x.ld + m;
-        if (a.add)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += p[e];
-        if (!a.out) __builtin_memcpy(p, v, 32);
-    }
-    if (a.out) put_out(a, (DX ? a.live[a.row0 + n] : n) * a.out_ld + m, a.dim - m, v);
+    finish<DX>(a, g, n, m, v);
+}
+template <class T, bool SPLIT>
+__global__ __launch_bounds__(256) void vocab_sum_kernel(HeadArgs a, GradArgs g) {
+    if (blockIdx.x < g.dx.sums) join_splits<T, true, SPLIT>(a, g, blockIdx.x);
+    else join_splits<T, false, SPLIT>(a, g, blockIdx.x - g.dx.sums);
 }
 
 // --- host ---
@@ -768,9 +787,9 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Plan {
     int64_t ld, rows, piece, pieces, vocab_ld, segments;
     int nk;
-    bool split, pack_w, split_dx, split_dw;   // split_dx, split_dw: the product's k may be split
-    int64_t dx_groups, dw_groups;
-    int64_t at_int, at_float, at_partial, at_x, at_w, at_dz, at_slabs, at_sum, bytes;
+    bool split, pack_w;
+    int64_t dx_groups, dw_groups, dx_slabs, dw_slabs;
+    int64_t at_int, at_float, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
 };
 
 // For any number of rows up to the piece's: the most workgroups of a gradient's product, and the fp32 values of its splits' sums.
@@ -816,11 +835,10 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
-        int64_t dx, dw;
-        most_of(true, p.piece, (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK, p.ld, &p.dx_groups, &dx);
-        most_of(false, v->vocab, (p.split ? 3 : 1) * p.piece / Tile::BK, p.ld, &p.dw_groups, &dw);
-        p.split_dx = dx > 0, p.split_dw = dw > 0;
-        p.at_slabs = take(4 * (dx > dw ? dx : dw));
+        most_of(true, p.piece, (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK, p.ld, &p.dx_groups, &p.dx_slabs);
+        most_of(false, v->vocab, (p.split ? 3 : 1) * p.piece / Tile::BK, p.ld, &p.dw_groups, &p.dw_slabs);
+        p.at_dx = take(4 * p.dx_slabs);
+        p.at_dw = take(4 * p.dw_slabs);
         if (p.pieces > 1) p.at_sum = take(4 * v->vocab * p.ld);
     }
     p.bytes = at;
@@ -904,7 +922,6 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     a.weight = weight ? packed_weight : nullptr;
     a.lse = packed_lse, a.zt = zt, a.partial = reinterpret_cast<float2 *>(ws + p.at_partial);
     a.segments = (int)p.segments, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
-    a.fp32 = p.split;
     if (dw && width > v->vocab) {
         const int64_t n = (width - v->vocab) * v->dim * (p.split ? 2 : 1);
         hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,
@@ -932,27 +949,28 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
                                   : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
         }
-        a.slabs = reinterpret_cast<float *>(ws + p.at_slabs);
-        a.out_ld = v->dim;
+        GradArgs g = {};
         const int64_t per = p.ld / 8;
-        a.tiles_m = (int)((p.ld + Tile::MT - 1) / Tile::MT);
+        g.tiles_m = (int)((p.ld + Tile::MT - 1) / Tile::MT);
+        g.add = i > 0, g.fp32 = p.split;
         if (dx) {
-            a.out = dx, a.sum = nullptr;
-            hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, true, true> : vocab_grad_kernel<Tile, true, false>),
-                               dim3((unsigned)p.dx_groups), dim3(threads), 0, stream, a);
-            if (p.split_dx)
-                hipLaunchKernelGGL((p.split ? vocab_sum_kernel<Tile, true, true> : vocab_sum_kernel<Tile, true, false>),
-                                   dim3((unsigned)((a.piece * per + 255) / 256)), dim3(256), 0, stream, a);
+            g.dx.out = dx, g.dx.slabs = reinterpret_cast<float *>(ws + p.at_dx), g.dx.groups = (uint32_t)p.dx_groups;
+            // (past kSplitTiles / 2 tiles nothing is split)
+            const int64_t most = kSplitTiles / 2 / g.tiles_m * Tile::NT;
+            if (p.dx_slabs) g.dx.sums = (uint32_t)(((a.piece < most ? a.piece : most) * per + 255) / 256);
         }
         if (dw) {
-            a.sum = p.pieces > 1 ? reinterpret_cast<float *>(ws + p.at_sum) : nullptr;
-            a.add = i > 0, a.out = i + 1 == p.pieces ? dw : nullptr;
-            hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, false, true> : vocab_grad_kernel<Tile, false, false>),
-                               dim3((unsigned)p.dw_groups), dim3(threads), 0, stream, a);
-            if (p.split_dw)
-                hipLaunchKernelGGL((p.split ? vocab_sum_kernel<Tile, false, true> : vocab_sum_kernel<Tile, false, false>),
-                                   dim3((unsigned)((v->vocab * per + 255) / 256)), dim3(256), 0, stream, a);
+            g.dw.out = i + 1 == p.pieces ? dw : nullptr, g.dw.slabs = reinterpret_cast<float *>(ws + p.at_dw);
+            g.dw.sum = p.pieces > 1 ? reinterpret_cast<float *>(ws + p.at_sum) : nullptr;
+            g.dw.groups = (uint32_t)p.dw_groups;
+            if (p.dw_slabs) g.dw.sums = (uint32_t)((v->vocab * per + 255) / 256);
         }
+        if (g.dx.groups + g.dw.groups)
+            hipLaunchKernelGGL((p.split ? vocab_grad_kernel<Tile, true> : vocab_grad_kernel<Tile, false>),
+                               dim3(g.dx.groups + g.dw.groups), dim3(threads), 0, stream, a, g);
+        if (g.dx.sums + g.dw.sums)
+            hipLaunchKernelGGL((p.split ? vocab_sum_kernel<Tile, true> : vocab_sum_kernel<Tile, false>),
+                               dim3(g.dx.sums + g.dw.sums), dim3(256), 0, stream, a, g);
     }
     return launch_status(fn);
 }

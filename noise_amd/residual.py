@@ -14,7 +14,7 @@ from array import array
 import torch
 
 from . import _lib
-from .sinks import BF16, EPS, F32, TYPES, _call, _no_tangents
+from .sinks import BF16, EPS, F32, TYPES, _call, _new, _no_tangents
 
 MAX_DIM = 8192
 
@@ -49,69 +49,76 @@ def _rows(t, D):
 
 def _gate(fn, gate, x):
     """(gate as contiguous rows of D, rows of x that share one)"""
-    if gate is None:
-        return None, 0
-    shape, D, n = gate.shape, x.shape[-1], x.dim()
-    full = (1,) * (n - len(shape)) + tuple(shape)
-    # as x up to some dimension, ones from there on
-    same = 0
-    while same < n - 1 and full[:same + 1] == x.shape[:same + 1]:
-        same += 1
-    if len(shape) > n or len(shape) < 1 or shape[-1] != D or any(s != 1 for s in full[same:n - 1]):
-        raise ValueError(f'{fn}: gate must be [{D}], or as x with ones from some dimension on, got {tuple(shape)} for '
-                         f'{tuple(x.shape)}')
+    shape, full = gate.shape, x.shape
     if gate.device != x.device or gate.dtype not in TYPES:
         raise ValueError(f'{fn}: gate must be bfloat16 or float32 on {x.device}, got {gate.dtype} on {gate.device}')
-    return gate if gate.is_contiguous() else gate.contiguous(), math.prod(x.shape[same:n - 1])
+    n, same = len(full), 0
+    over = (1,) * (n - len(shape)) + tuple(shape)
+    # as x up to some dimension, ones from there on
+    while same < n - 1 and over[same] == full[same]:
+        same += 1
+    if not 1 <= len(shape) <= n or shape[-1] != full[-1] or any(s != 1 for s in over[same:n - 1]):
+        raise ValueError(f'{fn}: gate must be [{full[-1]}], or as x with ones from some dimension on, got {tuple(shape)} for '
+                         f'{tuple(full)}')
+    return gate if gate.is_contiguous() else gate.contiguous(), math.prod(full[same:n - 1])
 
 
-class _Operands:
-    """The checked operands as noise_residual_t takes them; the copies among them live as long as this does"""
+def _operands(fn, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype):
+    """The operands as the kernels take them, copies among them, and what else goes into a noise_residual_t"""
+    shape, device, xt = x.shape, x.device, x.dtype
+    if xt not in TYPES or not shape:
+        raise ValueError(f'{fn}: bfloat16 or float32 x [..., dim], got {xt} {tuple(shape)}')
+    D = shape[-1]
+    if not 0 < D <= MAX_DIM:
+        raise ValueError(f'{fn}: dim must be 1 .. {MAX_DIM}, got {D}')
+    for name, t in (('y', y), ('x0', x0)):
+        if t is not None and (t.shape != shape or t.device != device):
+            raise ValueError(f'{fn}: {name} must be {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}')
+    if x0 is not None and x0.dtype != xt:
+        raise ValueError(f'{fn}: x and x0 must have one type, got {xt} and {x0.dtype}')
+    if y is None and (gate is not None or norm_y):
+        raise ValueError(f'{fn}: a gate or norm of y without y')
+    if y_weight is not None and not norm_y:
+        raise ValueError(f"{fn}: y_weight is the weight of y's norm, which norm_y=True asks for")
+    if x0 is None and x0_scale is not None:
+        raise ValueError(f'{fn}: x0_scale without x0')
+    if dtype is None:
+        dtype = xt if y is None else y.dtype
+    if dtype not in TYPES or (y is not None and y.dtype != dtype) or (xt == BF16 and dtype == F32):
+        raise ValueError(f'{fn}: h has the type of y, bfloat16, or float32 where x is float32; got x {xt}, '
+                         f'y {None if y is None else y.dtype} and {dtype}')
+    _no_tangents(fn, x, y, x0, scale, x0_scale, gate, y_weight, weight)
+    rows = x.numel() // D
+    x, sx = _rows(x, D)
+    sy = s0 = 0
+    if y is not None:
+        y, sy = _rows(y, D)
+    if x0 is not None:
+        x0, s0 = _rows(x0, D)
+    gate_rows, gate_type = rows, BF16
+    if gate is not None:
+        gate, gate_rows = _gate(fn, gate, x)
+        gate_type = gate.dtype
+    tensors = (x, y, x0, _scalar(fn, 'scale', scale, device), _scalar(fn, 'x0_scale', x0_scale, device), gate,
+               _vector(fn, 'y_weight', y_weight, D, device), _vector(fn, 'weight', weight, D, device))
+    return tensors, (sx, sy, s0), (rows, gate_rows, D, TYPES[xt], TYPES[dtype], TYPES[gate_type], int(norm_y)), dtype
 
-    def __init__(self, fn, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype):
-        if x.dtype not in TYPES or x.dim() < 1:
-            raise ValueError(f'{fn}: bfloat16 or float32 x [..., dim], got {x.dtype} {tuple(x.shape)}')
-        shape, device, D = x.shape, x.device, x.shape[-1]
-        if not 0 < D <= MAX_DIM:
-            raise ValueError(f'{fn}: dim must be 1 .. {MAX_DIM}, got {D}')
-        for name, t in (('y', y), ('x0', x0)):
-            if t is not None and (t.shape != shape or t.device != device):
-                raise ValueError(f'{fn}: {name} must be {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}')
-        if x0 is not None and x0.dtype != x.dtype:
-            raise ValueError(f'{fn}: x and x0 must have one type, got {x.dtype} and {x0.dtype}')
-        if y is None and (gate is not None or norm_y):
-            raise ValueError(f'{fn}: a gate or norm of y without y')
-        if y_weight is not None and not norm_y:
-            raise ValueError(f'{fn}: y_weight is the weight of y\'s norm, which norm_y=True asks for')
-        if x0 is None and x0_scale is not None:
-            raise ValueError(f'{fn}: x0_scale without x0')
-        if dtype is None:
-            dtype = x.dtype if y is None else y.dtype
-        if dtype not in TYPES or (y is not None and y.dtype != dtype) or (x.dtype == BF16 and dtype == F32):
-            raise ValueError(f'{fn}: h has the type of y, bfloat16, or float32 where x is float32; got x {x.dtype}, '
-                             f'y {None if y is None else y.dtype} and {dtype}')
-        _no_tangents(fn, x, y, x0, scale, x0_scale, gate, y_weight, weight)
-        self.shape, self.dtype, self.device, self.D = shape, dtype, device, D
-        self.rows = x.numel() // D
-        self.scale, self.x0_scale = _scalar(fn, 'scale', scale, device), _scalar(fn, 'x0_scale', x0_scale, device)
-        self.gate, self.gate_rows = _gate(fn, gate, x)
-        self.y_weight, self.weight = _vector(fn, 'y_weight', y_weight, D, device), _vector(fn, 'weight', weight, D, device)
-        self.x, sx = _rows(x, D)
-        self.y, sy = (None, 0) if y is None else _rows(y, D)
-        self.x0, s0 = (None, 0) if x0 is None else _rows(x0, D)
-        p = lambda t: 0 if t is None else t.data_ptr()
-        self.table = array('q', (self.x.data_ptr(), p(self.y), p(self.x0), sx, sy, s0, p(self.scale), p(self.x0_scale),
-                                 p(self.gate), p(self.y_weight), p(self.weight), self.rows,
-                                 self.gate_rows if gate is not None else self.rows, D, TYPES[x.dtype], TYPES[dtype],
-                                 TYPES[BF16] if gate is None else TYPES[gate.dtype], int(norm_y)))
-        self.at = self.table.buffer_info()[0]
+
+def _table(tensors, strides, numbers):
+    """A noise_residual_t, and its address (the array holds it for as long as it lives)"""
+    p = [0 if t is None else t.data_ptr() for t in tensors]
+    table = array('q', (*p[:3], *strides, *p[3:], *numbers))
+    return table, table.buffer_info()[0]
 
 
-def forward(x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps):
-    a = _Operands('residual_norm', x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype)
-    out, h = x.new_empty(a.shape), x.new_empty(a.shape, dtype=a.dtype)
-    if a.rows:
-        _call('noise_residual_norm', a.device, a.at, out.data_ptr(), h.data_ptr(), eps)
+def _forward(tensors, strides, numbers, dtype, eps):
+    """residual_norm of checked operands"""
+    x = tensors[0]
+    out = _new(x)
+    h = torch.empty_like(out, dtype=dtype)
+    if numbers[0]:
+        table, at = _table(tensors, strides, numbers)
+        _call('noise_residual_norm', x.device, at, out.data_ptr(), h.data_ptr(), eps)
     return out, h
 
 
@@ -127,38 +134,54 @@ def _upstream(grad, dtype):
     return grad if grad.is_contiguous() else grad.contiguous()
 
 
-def backward(dout, dh, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps, needs):
-    """The gradients of x, y, x0, scale, x0_scale, gate, y_weight and weight, None where `needs` says False"""
+def _backward(dout, dh, tensors, strides, numbers, dtype, eps, needs):
+    """The gradients of checked operands, None where `needs` says False; the scalars' and weights' in fp32"""
     _no_tangents('residual_norm', dout, dh)
-    a = _Operands('residual_norm', x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype)
-    given = (x, y, x0, scale, x0_scale, gate, y_weight, weight)
-    if not a.rows or (dout is None and dh is None):
-        return [torch.zeros_like(t) if n and t is not None else None for t, n in zip(given, needs)]
-    dout, dh = _upstream(dout, x.dtype), _upstream(dh, a.dtype)
-    # (those that are sums over rows, but for the gate's, come in fp32)
-    grads = [t.new_empty(t.shape, dtype=F32 if i in (3, 4, 6, 7) else t.dtype) if n and t is not None else None
-             for i, (t, n) in enumerate(zip(given, needs))]
+    x = tensors[0]
+    if not numbers[0] or (dout is None and dh is None):
+        return [torch.zeros_like(t) if n and t is not None else None for t, n in zip(tensors, needs)]
+    dout, dh = _upstream(dout, x.dtype), _upstream(dh, dtype)
+    grads = [_new(t) if n and t is not None else None for t, n in zip(tensors, needs)]
     need, work = 0, None
-    if any(grads[i] is not None for i in (3, 4, 5, 6, 7)):
-        need = _workspace(a.rows, a.gate_rows or a.rows, a.D)
+    if any([g is not None for g in grads[3:]]):
+        need = _workspace(*numbers[:3])
         work = x.new_empty(need, dtype=torch.uint8)
-    table = array('q', [0 if g is None else g.data_ptr() for g in grads])
-    _call('noise_residual_norm_bwd', a.device, a.at, _lib.ptr(dout), _lib.ptr(dh), table.buffer_info()[0], eps, _lib.ptr(work), need)
+    table, at = _table(tensors, strides, numbers)
+    to = array('q', [0 if g is None else g.data_ptr() for g in grads])
+    _call('noise_residual_norm_bwd', x.device, at, _lib.ptr(dout), _lib.ptr(dh), to.buffer_info()[0], eps, _lib.ptr(work), need)
+    return grads
+
+
+def forward(x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps):
+    return _forward(*_operands('residual_norm', x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype), eps)
+
+
+def backward(dout, dh, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps, needs):
+    """The gradients of x, y, x0, scale, x0_scale, gate, y_weight and weight in their types, None where `needs` says False"""
+    given = x, y, x0, scale, x0_scale, gate, y_weight, weight
+    grads = _backward(dout, dh, *_operands('residual_norm', *given, norm_y, dtype), eps, needs)
     return [g if g is None or g.dtype == t.dtype else g.to(t.dtype) for g, t in zip(grads, given)]
 
 
 class _Residual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps):
-        ctx.save_for_backward(x, y, x0, scale, x0_scale, gate, y_weight, weight)
-        ctx.more = norm_y, dtype, eps
+        tensors, *more = _operands('residual_norm', x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype)
+        # (what the kernels take is saved: the tensors themselves, or the copies made of them)
+        ctx.save_for_backward(*tensors)
+        ctx.more = *more, eps
+        ctx.types = [None if t is None or t.dtype == F32 else t.dtype for t in (scale, x0_scale, y_weight, weight)]
         ctx.set_materialize_grads(False)
-        return forward(x, y, x0, scale, x0_scale, gate, y_weight, weight, norm_y, dtype, eps)
+        return _forward(tensors, *more, eps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dh):
-        return (*backward(dout, dh, *ctx.saved_tensors, *ctx.more, ctx.needs_input_grad), None, None, None)
+        grads = _backward(dout, dh, ctx.saved_tensors, *ctx.more, ctx.needs_input_grad)
+        for i, t in zip((3, 4, 6, 7), ctx.types):
+            if t is not None and grads[i] is not None:
+                grads[i] = grads[i].to(t)
+        return (*grads, None, None, None)
 
 
 def residual_norm(x, y=None, x0=None, scale=None, x0_scale=None, gate=None, y_weight=None, weight=None, norm_y=False, dtype=None,

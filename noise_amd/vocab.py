@@ -7,12 +7,15 @@ head_loss of the fixed model.
 The head is utils/model.py:204-206's with its soft cap as an option, the loss that of train/val/run.py:89-94. The calls are
 torch.ops.noise_amd operators too. Derivatives are taken backwards and once, as in noise_amd.sinks.
 """
+import functools
 from array import array
 
 import torch
 
 from . import _lib
-from .sinks import F32, TYPES, _call, _no_tangents
+from .sinks import F32, TYPES, _call, _new, _no_tangents
+
+MAX_VOCAB, MAX_DIM, MAX_ROWS = 1 << 22, 1 << 16, 1 << 30
 
 
 def _rows(t):
@@ -20,90 +23,107 @@ def _rows(t):
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1) else t.contiguous()
 
 
-class _Operands:
-    """The checked operands as noise_vocab_t takes them; the copies among them live as long as this does"""
-
-    def __init__(self, fn, x, weight, targets, vocab, softcap):
-        if x.dtype not in TYPES or x.dim() < 1 or weight.dtype != x.dtype or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
-            raise ValueError(f'{fn}: bfloat16 or float32 x [..., dim] and weight [width, dim] of its type, got {x.dtype} '
-                             f'{tuple(x.shape)} and {weight.dtype} {tuple(weight.shape)}')
-        width, dim = weight.shape
-        self.vocab = width if vocab is None else int(vocab)
-        if not 0 < self.vocab <= width or self.vocab > 1 << 22:
-            raise ValueError(f'{fn}: vocab must be 1 .. {min(width, 1 << 22)}, got {self.vocab}')
-        if not 0 < dim <= 1 << 16:
-            raise ValueError(f'{fn}: dim must be 1 .. {1 << 16}, got {dim}')
-        if softcap is not None and not 1e-6 <= softcap <= 1e6:
-            raise ValueError(f'{fn}: softcap must be 1e-6 .. 1e6 (None: no cap), got {softcap}')
-        if targets.shape != x.shape[:-1] or targets.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f'{fn}: targets must be int32 or int64 of shape {tuple(x.shape[:-1])}, got {targets.dtype} '
-                             f'{tuple(targets.shape)}')
-        if weight.device != x.device or targets.device != x.device:
-            raise ValueError(f'{fn}: tensors on {x.device}, {weight.device} and {targets.device}')
-        _no_tangents(fn, x, weight)
-        self.shape, self.device = x.shape[:-1], x.device
-        self.x, self.weight = _rows(x if x.dim() == 2 else x.reshape(-1, dim)), _rows(weight)
-        self.targets = targets if targets.is_contiguous() else targets.contiguous()
-        self.rows, self.softcap = self.x.shape[0], float(softcap or 0.0)
-        if self.rows > 1 << 30:
-            raise ValueError(f'{fn}: at most 2^30 tokens, got {self.rows}')
-        self.table = array('q', (self.x.data_ptr(), self.x.stride(0) if self.rows > 1 else dim, self.weight.data_ptr(),
-                                 self.weight.stride(0) if width > 1 else dim, self.targets.data_ptr(),
-                                 int(targets.dtype == torch.int64), self.rows, dim, self.vocab, TYPES[x.dtype]))
-        self.at = self.table.buffer_info()[0]
-
-    def workspace(self, grad):
-        need = _lib.lib().noise_vocab_workspace_bytes(self.at, grad)
-        return torch.empty(need, dtype=torch.uint8, device=self.device), need
+def _operands(fn, x, weight, targets, vocab, softcap):
+    """x [rows, dim], the weight and targets as the kernels take them, copies among them; then vocab and softcap"""
+    if x.dtype not in TYPES or x.dim() < 1 or weight.dtype != x.dtype or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f'{fn}: bfloat16 or float32 x [..., dim] and weight [width, dim] of its type, got {x.dtype} '
+                         f'{tuple(x.shape)} and {weight.dtype} {tuple(weight.shape)}')
+    width, dim = weight.shape
+    vocab = width if vocab is None else int(vocab)
+    if not 0 < vocab <= min(width, MAX_VOCAB):
+        raise ValueError(f'{fn}: vocab must be 1 .. {min(width, MAX_VOCAB)}, got {vocab}')
+    if not 0 < dim <= MAX_DIM:
+        raise ValueError(f'{fn}: dim must be 1 .. {MAX_DIM}, got {dim}')
+    if softcap is not None and not 1e-6 <= softcap <= 1e6:
+        raise ValueError(f'{fn}: softcap must be 1e-6 .. 1e6 (None: no cap), got {softcap}')
+    if targets.shape != x.shape[:-1] or targets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f'{fn}: targets must be int32 or int64 of shape {tuple(x.shape[:-1])}, got {targets.dtype} '
+                         f'{tuple(targets.shape)}')
+    if weight.device != x.device or targets.device != x.device:
+        raise ValueError(f'{fn}: tensors on {x.device}, {weight.device} and {targets.device}')
+    _no_tangents(fn, x, weight)
+    x = _rows(x if x.dim() == 2 else x.reshape(-1, dim))
+    if x.shape[0] > MAX_ROWS:
+        raise ValueError(f'{fn}: at most {MAX_ROWS} tokens, got {x.shape[0]}')
+    return x, _rows(weight), targets if targets.is_contiguous() else targets.contiguous(), vocab, float(softcap or 0.0)
 
 
-def forward(x, weight, targets, vocab, softcap, with_lse):
-    """(losses, lse or None)"""
-    a = _Operands('linear_cross_entropy', x, weight, targets, vocab, softcap)
-    loss = x.new_empty(a.shape, dtype=F32)
-    lse = x.new_empty(a.shape, dtype=F32) if with_lse else None
-    if a.rows:
-        work, need = a.workspace(0)
-        _call('noise_vocab_loss', a.device, a.at, a.softcap, loss.data_ptr(), _lib.ptr(lse), work.data_ptr(), need)
+def _table(x, weight, targets, vocab, with_grad):
+    """A noise_vocab_t, its address (the array holds it for as long as it lives), a workspace and its bytes"""
+    (rows, dim), width, kind, at = x.shape, weight.shape[0], TYPES[x.dtype], weight.data_ptr()
+    pitch = weight.stride(0) if width > 1 else dim
+    table = array('q', (x.data_ptr(), x.stride(0) if rows > 1 else dim, at, pitch, targets.data_ptr(),
+                        int(targets.dtype == torch.int64), rows, dim, vocab, kind))
+    need = _workspace(at % 16, pitch, rows, dim, vocab, kind, with_grad)
+    return table, table.buffer_info()[0], x.new_empty(need, dtype=torch.uint8), need
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(offset, pitch, rows, dim, vocab, kind, with_grad):
+    # (of addresses like these, of which none is read)
+    table = array('q', (4096, dim, 4096 + offset, pitch, 4096, 0, rows, dim, vocab, kind))
+    return _lib.lib().noise_vocab_workspace_bytes(table.buffer_info()[0], with_grad)
+
+
+def _forward(shape, x, weight, targets, vocab, softcap, with_lse):
+    """(losses, lse or None) of checked operands"""
+    loss = x.new_empty(shape, dtype=F32)
+    lse = torch.empty_like(loss) if with_lse else None
+    if x.shape[0]:
+        table, at, work, need = _table(x, weight, targets, vocab, 0)
+        _call('noise_vocab_loss', x.device, at, softcap, loss.data_ptr(), _lib.ptr(lse), work.data_ptr(), need)
     return loss, lse
 
 
-def gradients(fn, x, weight, targets, token_weight, lse, vocab, softcap, need_x=True, need_weight=True):
-    """(losses or, where lse is given, None; dx; dweight)"""
-    a = _Operands(fn, x, weight, targets, vocab, softcap)
+def _gradients(fn, shape, token_weight, lse, x, weight, targets, vocab, softcap, need_x, need_weight):
+    """(losses or, where lse is given, None; dx [rows, dim]; dweight) of checked operands"""
     _no_tangents(fn, token_weight)
     if token_weight is not None:
-        if token_weight.shape != a.shape or token_weight.device != a.device:
-            raise ValueError(f'{fn}: token weights must be {tuple(a.shape)} on {a.device}, got {tuple(token_weight.shape)} on '
+        if token_weight.shape != shape or token_weight.device != x.device:
+            raise ValueError(f'{fn}: token weights must be {tuple(shape)} on {x.device}, got {tuple(token_weight.shape)} on '
                              f'{token_weight.device}')
         if token_weight.dtype != F32 or not token_weight.is_contiguous():
             token_weight = token_weight.to(F32).contiguous()
-    loss = x.new_empty(a.shape, dtype=F32) if lse is None else None
-    dx = x.new_empty(x.shape) if need_x else None
-    dw = weight.new_empty(weight.shape) if need_weight else None
-    if a.rows:
-        work, need = a.workspace(1)
-        _call('noise_vocab_grad', a.device, a.at, a.softcap, _lib.ptr(token_weight), _lib.ptr(lse), _lib.ptr(loss), _lib.ptr(dx),
+    loss = x.new_empty(shape, dtype=F32) if lse is None else None
+    dx = _new(x) if need_x else None
+    dw = _new(weight) if need_weight else None
+    if x.shape[0]:
+        table, at, work, need = _table(x, weight, targets, vocab, 1)
+        _call('noise_vocab_grad', x.device, at, softcap, _lib.ptr(token_weight), _lib.ptr(lse), _lib.ptr(loss), _lib.ptr(dx),
               _lib.ptr(dw), weight.shape[0], work.data_ptr(), need)
     elif dw is not None:
         dw.zero_()
     return loss, dx, dw
 
 
+def forward(x, weight, targets, vocab, softcap, with_lse):
+    """(losses, lse or None)"""
+    return _forward(targets.shape, *_operands('linear_cross_entropy', x, weight, targets, vocab, softcap), with_lse)
+
+
+def gradients(fn, x, weight, targets, token_weight, lse, vocab, softcap, need_x=True, need_weight=True):
+    """(losses or, where lse is given, None; dx; dweight)"""
+    operands = _operands(fn, x, weight, targets, vocab, softcap)
+    loss, dx, dw = _gradients(fn, targets.shape, token_weight, lse, *operands, need_x, need_weight)
+    return loss, None if dx is None else dx.view(x.shape), dw
+
+
 class _Head(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, vocab, softcap):
-        loss, lse = forward(x, weight, targets, vocab, softcap, True)
-        ctx.save_for_backward(x, weight, targets, lse)
-        ctx.more = (vocab, softcap)
+        ctx.shapes = x.shape, targets.shape
+        x, weight, targets, *ctx.more = _operands('linear_cross_entropy', x, weight, targets, vocab, softcap)
+        loss, lse = _forward(ctx.shapes[1], x, weight, targets, *ctx.more, True)
+        # (what the kernels take is saved: the tensors themselves, or the copies made of them)
+        ctx.save_for_backward(lse, x, weight, targets)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, weight, targets, lse = ctx.saved_tensors
-        return (*gradients('linear_cross_entropy', x, weight, targets, dloss, lse, *ctx.more, *ctx.needs_input_grad[:2])[1:],
-                None, None, None)
+        _, dx, dw = _gradients('linear_cross_entropy', ctx.shapes[1], dloss, *ctx.saved_tensors, *ctx.more,
+                               *ctx.needs_input_grad[:2])
+        return None if dx is None else dx.view(ctx.shapes[0]), dw, None, None, None
 
 
 def linear_cross_entropy(x, weight, targets, vocab=None, softcap=None):
