@@ -7,15 +7,19 @@
 // The backward pass forms x' again from x, y and x0 in fp32, so that n carries none of x's rounding to its stored type (and
 // reads what ds, ds0 and dg need anyway).
 //
-// Memory bound. TEAM lanes hold a row, 8 consecutive elements of each of C chunks per lane; sums over a row are wave shuffles for
-// teams of up to a wave, and one exchange through LDS per sum for larger ones. Workgroups of the backward pass take a run of
-// rows of one gate each, keep the sums over rows in registers and leave one row of partial sums; a second kernel adds those up
-// in a fixed order.
+// Memory bound. TEAM lanes hold a row, 8 consecutive elements each; sums over a row are wave shuffles for teams of up to a wave, and
+// one exchange through LDS per sum for larger ones, which are a workgroup. Workgroups of the backward pass take a run of rows of one
+// gate each, hold the weights and the sums over rows in registers, and leave one row of partial sums; a second kernel adds those up in a fixed
+// order.
 #include "common.hpp"
 #include "mfma.hpp"
 
+#include <type_traits>
+
 namespace noise {
 namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int64_t kLaunchGroups = 1 << 20;   // a launch has fewer than 2^32 threads
 constexpr int kMaxDim = 8192;
@@ -33,41 +37,63 @@ struct ResArgs {
     float eps;
 };
 
-// 8 elements at any address of their type, in fp32; n: how many of them exist (zeros for the others)
-template <class E>
-__device__ __forceinline__ void get8(const E *p, int n, float (&o)[8]) {
-    E v[8];
-    if (n >= 8) {
-        __builtin_memcpy(v, p, 8 * sizeof(E));
+// 8 elements at any address of their type; n: how many of them exist (zeros for the others). FULL: 8 or none do
+template <class E, bool FULL>
+struct Eight {
+    static constexpr int W = sizeof(E) / 2;   // 16 B words
+    u32x4 v[W];
+    __device__ __forceinline__ void load(const E *p, int n) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (float)v[e];
-    } else {
+        for (int i = 0; i < W; ++i) v[i] = u32x4{0, 0, 0, 0};
+        if (n >= 8) {
+            __builtin_memcpy(v, p, sizeof v);
+        } else if (!FULL && n > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = e < n ? (float)p[e] : 0.f;
+            for (int e = 0; e < 7; ++e)
+                if (e < n) {
+                    if constexpr (W == 2) v[e / 4][e % 4] = __float_as_uint(p[e]);
+                    else v[0][e / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[e] << (16 * (e % 2));
+                }
+        }
     }
-}
-template <class E>
+    __device__ __forceinline__ float operator[](int e) const {
+        if constexpr (W == 2) return __uint_as_float(v[e / 4][e % 4]);
+        return __uint_as_float(e % 2 ? v[0][e / 2] & 0xffff0000u : v[0][e / 2] << 16);
+    }
+};
+template <bool FULL, class E>
 __device__ __forceinline__ void put8(E *p, int n, const float (&o)[8]) {
     if (n >= 8) {
         E v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (E)o[e];
         __builtin_memcpy(p, v, 8 * sizeof(E));
-    } else {
+    } else if constexpr (!FULL) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (e < n) p[e] = (E)o[e];
     }
 }
 
-// N sums over a team of TEAM lanes. Teams larger than a wave are the workgroup: the sums go through LDS, in two alternating sets of
-// slots, so that one barrier per call is enough.
+// v + the value of the lane that `control` (a DPP one) pairs this lane with
+template <int CONTROL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true));
+}
+
+// N sums over a team of TEAM lanes. Within a wave by DPP (lanes 1, 2, 4 and 8 apart: pairs and halves of four swapped, halves of 8 and
+// 16 lanes mirrored) and lane swaps: a sixth of the time of shuffles, which go through LDS. Teams larger than a wave are the
+// workgroup: their waves' sums go through LDS, in two alternating sets of slots, so that one barrier per call is enough.
 template <int TEAM, int N>
 __device__ __forceinline__ void team_sum(float (&v)[N], float *slots, int &turn) {
 #pragma unroll
-    for (int o = 1; o < (TEAM < 64 ? TEAM : 64); o <<= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+    for (int i = 0; i < N; ++i) {
+        v[i] = add_dpp<0xb1>(v[i]);    // quad_perm 1 0 3 2
+        v[i] = add_dpp<0x4e>(v[i]);    // quad_perm 2 3 0 1
+        v[i] = add_dpp<0x141>(v[i]);   // row_half_mirror
+        v[i] = add_dpp<0x140>(v[i]);   // row_mirror
+        if constexpr (TEAM >= 64) v[i] = sum_lanes_16_32(v[i]);
+    }
     if constexpr (TEAM > 64) {
         constexpr int NW = TEAM / 64;
         float *s = slots + 2 * NW * turn;
@@ -87,242 +113,216 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float *slots, int &turn)
 }
 
 template <int TEAM>
-constexpr int group_threads() { return TEAM > 256 ? TEAM : 256; }
+constexpr int group_threads() { return TEAM > 64 ? TEAM : 256; }
 
+// 8 values of a gate's row at `at`, of a weight from c on: ones where there is none
+template <bool FULL>
 __device__ __forceinline__ void get_gate(const ResArgs &a, int64_t at, int n, float (&o)[8]) {
-    if (a.gate_bf16) get8(static_cast<const __bf16 *>(a.gate) + at, n, o);
-    else get8(static_cast<const float *>(a.gate) + at, n, o);
+    if (a.gate_bf16) {
+        Eight<__bf16, FULL> v;
+        v.load(static_cast<const __bf16 *>(a.gate) + at, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[e];
+    } else {
+        Eight<float, FULL> v;
+        v.load(static_cast<const float *>(a.gate) + at, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[e];
+    }
+}
+template <bool FULL>
+__device__ __forceinline__ void get_weight(const float *w, int c, int n, float (&o)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 1.f;
+    if (!w) return;
+    Eight<float, FULL> v;
+    v.load(w + c, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = v[e];
 }
 
-template <class EX, class EY, int TEAM, int C, bool POST>
+template <class EX, class EY, int TEAM, bool POST, bool FULL>
 __global__ __launch_bounds__(group_threads<TEAM>()) void residual_kernel(ResArgs a) {
     constexpr int NT = group_threads<TEAM>(), TEAMS = NT / TEAM;
     __shared__ float slots[4 * (TEAM > 64 ? TEAM / 64 : 1)];
     int turn = 0;
     const int64_t row = (a.first + blockIdx.x) * TEAMS + threadIdx.x / TEAM;
     if (row >= a.rows) return;   // (whole teams: a team larger than a wave is the workgroup)
-    const int lane = threadIdx.x % TEAM, D = a.D;
-    const EX *x = static_cast<const EX *>(a.x) + row * a.s_x, *x0 = static_cast<const EX *>(a.x0) + row * a.s_x0;
-    const EY *y = static_cast<const EY *>(a.y) + row * a.s_y;
-    const int64_t gate = a.gate ? row / a.gate_rows * D : 0;
-    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = a.x0_scale ? *a.x0_scale : 1.f;
-    float b[C][8], t[C][8], v0[C][8];
+    const int c = 8 * (threadIdx.x % TEAM), D = a.D, n = D - c;
+    Eight<EX, FULL> x, x0;
+    Eight<EY, FULL> y;
+    x.load(static_cast<const EX *>(a.x) + row * a.s_x + c, n);
+    if (a.y) y.load(static_cast<const EY *>(a.y) + row * a.s_y + c, n);
+    if (a.x0) x0.load(static_cast<const EX *>(a.x0) + row * a.s_x0 + c, n);
+    float g[8], w[8], wy[8];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int c = 8 * (i * TEAM + lane), n = D - c;
-        get8(x + c, n, t[i]);
-        if (a.y) get8(y + c, n, b[i]);
-        if (a.x0) get8(x0 + c, n, v0[i]);
-    }
+    for (int e = 0; e < 8; ++e) g[e] = 1.f;
+    if (a.gate) get_gate<FULL>(a, row / a.gate_rows * D + c, n, g);
+    get_weight<FULL>(a.w, c, n, w);
+    if (POST) get_weight<FULL>(a.wy, c, n, wy);
+    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = a.x0_scale ? *a.x0_scale : 1.f;
     float ry = 1.f;
     if constexpr (POST) {
         float s[1] = {0.f};
 #pragma unroll
-        for (int i = 0; i < C; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[0] += b[i][e] * b[i][e];
+        for (int e = 0; e < 8; ++e) s[0] += y[e] * y[e];
         team_sum<TEAM>(s, slots, turn);
         ry = rsqrtf(s[0] * inv + a.eps);
     }
-    float s[1] = {0.f};
+    float t[8], s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int c = 8 * (i * TEAM + lane), n = D - c;
-        float f[8];
-        if constexpr (POST) {
-            if (a.wy) get8(a.wy + c, n, f);
+    for (int e = 0; e < 8; ++e) t[e] = x[e];
+    if (a.y) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b[i][e] = b[i][e] * ry * (a.wy ? f[e] : 1.f);
-        }
-        if (a.y) {
-            if (a.gate) get_gate(a, gate + c, n, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[i][e] += a.gate ? f[e] * b[i][e] : b[i][e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            t[i][e] *= scale;
-            if (a.x0) t[i][e] += x0_scale * v0[i][e];
-            s[0] += t[i][e] * t[i][e];
-        }
+        for (int e = 0; e < 8; ++e) t[e] += g[e] * (POST ? y[e] * ry * wy[e] : y[e]);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] *= scale;
+    if (a.x0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] += x0_scale * x0[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[0] += t[e] * t[e];
     team_sum<TEAM>(s, slots, turn);
     const float r = rsqrtf(s[0] * inv + a.eps);
+    put8<FULL>(static_cast<EX *>(a.out) + row * D + c, n, t);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        const int c = 8 * (i * TEAM + lane), n = D - c;
-        put8(static_cast<EX *>(a.out) + row * D + c, n, t[i]);
-        float f[8];
-        if (a.w) get8(a.w + c, n, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[i][e] = t[i][e] * r * (a.w ? f[e] : 1.f);
-        put8(static_cast<EY *>(a.h) + row * D + c, n, t[i]);
-    }
+    for (int e = 0; e < 8; ++e) t[e] = t[e] * r * w[e];
+    put8<FULL>(static_cast<EY *>(a.h) + row * D + c, n, t);
 }
 
-// SUMS: with weights or a gate whose gradients are sums over rows
-template <class EX, class EY, int TEAM, int C, bool POST, bool SUMS>
+// MIX: with x0. (Loading the next row before working on the present one was slower, by 5 to 10 %: it takes registers from other rows.)
+template <class EX, class EY, int TEAM, bool POST, bool MIX, bool FULL>
 __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(ResArgs a) {
     constexpr int NT = group_threads<TEAM>(), TEAMS = NT / TEAM;
     __shared__ float slots[4 * (TEAM > 64 ? TEAM / 64 : 1)];
     __shared__ double scalars[2][NT / 64];
-    __shared__ float fold[SUMS && TEAMS > 1 ? TEAMS * TEAM * 8 : 1];
+    __shared__ float fold[TEAMS > 1 ? TEAMS * TEAM * 8 : 1];
     int turn = 0;
     const int64_t part = a.first + blockIdx.x;
     const bool row_gate = a.gate_rows == 1;   // (a gate per row is not summed: all rows are one unit)
     const int64_t unit_rows = row_gate ? a.rows : a.gate_rows, at = part % a.parts_per_gate;
     const int64_t first_unit = part / a.parts_per_gate * a.gates_per_part;
     const int64_t last_unit = first_unit + a.gates_per_part < a.gates ? first_unit + a.gates_per_part : a.gates;
-    const int lane = threadIdx.x % TEAM, D = a.D;
-    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = a.x0_scale ? *a.x0_scale : 1.f;
-    float sw[SUMS ? C : 1][8] = {}, swy[SUMS ? C : 1][8] = {}, sg[SUMS ? C : 1][8] = {};
+    const int lane = threadIdx.x % TEAM, D = a.D, c = 8 * lane, n = D - c;
+    const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = MIX && a.x0_scale ? *a.x0_scale : 1.f;
+    float w[8], wy[8], g[8], sw[8] = {}, swy[8] = {}, sg[8] = {};
+    get_weight<FULL>(a.w, c, n, w);
+    if (POST) get_weight<FULL>(a.wy, c, n, wy);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = 1.f;
     double ds = 0., ds0 = 0.;
-    // the teams' sums, added in LDS, one array and chunk at a time
-    auto leave = [&](float *to, float (&v)[SUMS ? C : 1][8]) {
+    // the teams' sums, added in LDS
+    auto leave = [&](float *to, float (&v)[8]) {
+        if constexpr (TEAMS > 1) {
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < (SUMS ? C : 1); ++i) {
-            const int c = 8 * (i * TEAM + lane), n = D - c;
-            if constexpr (TEAMS > 1) {
-                __syncthreads();
+            for (int e = 0; e < 8; ++e) fold[(threadIdx.x / TEAM * 8 + e) * TEAM + lane] = v[e];
+            __syncthreads();
+            if (threadIdx.x < TEAM) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) fold[(threadIdx.x / TEAM * 8 + e) * TEAM + lane] = v[i][e];
-                __syncthreads();
-                if (threadIdx.x < TEAM) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        for (int k = 1; k < TEAMS; ++k) v[i][e] += fold[(k * 8 + e) * TEAM + lane];
-                }
+                for (int e = 0; e < 8; ++e)
+                    for (int k = 1; k < TEAMS; ++k) v[e] += fold[(k * 8 + e) * TEAM + lane];
             }
-            if (threadIdx.x < TEAM) put8(to + c, n, v[i]);
         }
+        if (threadIdx.x < TEAM) put8<FULL>(to + c, n, v);
     };
     for (int64_t unit = first_unit; unit < last_unit; ++unit) {
-    const int64_t begin = unit * unit_rows + at * a.part_rows;
-    const int64_t end = (unit + 1) * unit_rows, stop = begin + a.part_rows < end ? begin + a.part_rows : end;
-    for (int64_t row = begin + threadIdx.x / TEAM; row < stop; row += TEAMS) {
-        const EX *x = static_cast<const EX *>(a.x) + row * a.s_x, *x0 = static_cast<const EX *>(a.x0) + row * a.s_x0;
-        const EY *y = static_cast<const EY *>(a.y) + row * a.s_y;
-        const EX *dout = static_cast<const EX *>(a.dout) + row * D;
-        const EY *dh = static_cast<const EY *>(a.dh) + row * D;
-        float vy[C][8], t[C][8], v0[C][8], G[C][8], H[C][8], g[C][8];
+        const int64_t begin = unit * unit_rows + at * a.part_rows, end = (unit + 1) * unit_rows;
+        const int64_t stop = begin + a.part_rows < end ? begin + a.part_rows : end, from = begin + threadIdx.x / TEAM;
+        if (a.gate && !row_gate) get_gate<FULL>(a, unit * D + c, n, g);
+        // this lane's elements of the row, of the contiguous tensors and of the others
+        int64_t o = from * D + c;
+        const EX *x = static_cast<const EX *>(a.x) + from * a.s_x + c, *x0 = static_cast<const EX *>(a.x0) + from * a.s_x0 + c;
+        const EY *y = static_cast<const EY *>(a.y) + from * a.s_y + c;
+        for (int64_t row = from; row < stop; row += TEAMS, o += TEAMS * D, x += TEAMS * a.s_x, y += TEAMS * a.s_y, x0 += TEAMS * a.s_x0) {
+            Eight<EX, FULL> vx, vx0, vdo;
+            Eight<EY, FULL> vy, vdh;
+            vx.load(x, n);
+            if (a.y) vy.load(y, n);
+            if (MIX) vx0.load(x0, n);
+            vdo.load(static_cast<const EX *>(a.dout) + o, a.dout ? n : 0);
+            if (a.dh) vdh.load(static_cast<const EY *>(a.dh) + o, n);
+            if (a.gate && row_gate) get_gate<FULL>(a, o, n, g);
+            float ry = 1.f;
+            if constexpr (POST) {
+                float s[1] = {0.f};
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 8 * (i * TEAM + lane), n = D - c;
-            get8(x + c, n, t[i]);
-            if (a.y) get8(y + c, n, vy[i]);
-            if (a.x0) get8(x0 + c, n, v0[i]);
-            if (a.dout) get8(dout + c, n, G[i]);
-            if (a.dh) get8(dh + c, n, H[i]);
-            if (a.gate) get_gate(a, (row_gate ? row : unit) * D + c, n, g[i]);
-        }
-        float ry = 1.f;
-        if constexpr (POST) {
-            float s[1] = {0.f};
+                for (int e = 0; e < 8; ++e) s[0] += vy[e] * vy[e];
+                team_sum<TEAM>(s, slots, turn);
+                ry = rsqrtf(s[0] * inv + a.eps);
+            }
+            // t and x' (out), G
+            float t[8], out[8], G[8], ls = 0.f, ls0 = 0.f;
 #pragma unroll
-            for (int i = 0; i < C; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[0] += vy[i][e] * vy[i][e];
-            team_sum<TEAM>(s, slots, turn);
-            ry = rsqrtf(s[0] * inv + a.eps);
-        }
-        // t and x' (out); the sums of x'^2 and u x'
-        float out[C][8], s2[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 8 * (i * TEAM + lane), n = D - c;
-            float f[8];
+            for (int e = 0; e < 8; ++e) t[e] = vx[e], G[e] = vdo[e];
             if (a.y) {
-                if (POST && a.wy) get8(a.wy + c, n, f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] += g[e] * (POST ? vy[e] * ry * wy[e] : vy[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = MIX ? t[e] * scale + x0_scale * vx0[e] : t[e] * scale;
+            if (a.dh) {
+                float s[2] = {0.f, 0.f};   // of x'^2 and u x'
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[0] += out[e] * out[e], s[1] += vdh[e] * w[e] * out[e];
+                team_sum<TEAM>(s, slots, turn);
+                const float r = rsqrtf(s[0] * inv + a.eps), m = s[1] * r * inv * r;   // (r mean(u n): n = x' r)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float b = POST ? vy[i][e] * ry * (a.wy ? f[e] : 1.f) : vy[i][e];
-                    t[i][e] += a.gate ? g[i][e] * b : b;
+                    G[e] += r * (vdh[e] * w[e] - out[e] * m);
+                    sw[e] += vdh[e] * (out[e] * r);
                 }
             }
-            if (a.w) get8(a.w + c, n, f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                out[i][e] = t[i][e] * scale;
-                if (a.x0) out[i][e] += x0_scale * v0[i][e];
-                s2[0] += out[i][e] * out[i][e];
-                if (a.dh) s2[1] += H[i][e] * (a.w ? f[e] : 1.f) * out[i][e];
+                ls += G[e] * t[e];
+                if (MIX) ls0 += G[e] * vx0[e];
             }
-        }
-        team_sum<TEAM>(s2, slots, turn);
-        const float r = rsqrtf(s2[0] * inv + a.eps), m = s2[1] * r * inv * r;   // (r mean(u n): n = x' r)
-        float ls = 0.f, ls0 = 0.f, s3[1] = {0.f};
+            ds += (double)ls, ds0 += (double)ls0;
+            if (MIX && a.dx0) {
+                float v[8];
 #pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 8 * (i * TEAM + lane), n = D - c;
-            float f[8];
-            if (a.w) get8(a.w + c, n, f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float grad = a.dout ? G[i][e] : 0.f;
-                if (a.dh) {
-                    grad += r * (H[i][e] * (a.w ? f[e] : 1.f) - out[i][e] * m);
-                    if constexpr (SUMS) sw[i][e] += H[i][e] * (out[i][e] * r);
-                }
-                ls += grad * t[i][e];
-                if (a.x0) ls0 += grad * v0[i][e];
-                G[i][e] = grad;
-            }
-            if (a.dx0) {
-                float o[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = x0_scale * G[i][e];
-                put8(static_cast<EX *>(a.dx0) + row * D + c, n, o);
+                for (int e = 0; e < 8; ++e) v[e] = x0_scale * G[e];
+                put8<FULL>(static_cast<EX *>(a.dx0) + o, n, v);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) G[i][e] *= scale;
-            if (a.out) put8(static_cast<EX *>(a.out) + row * D + c, n, G[i]);
+            for (int e = 0; e < 8; ++e) G[e] *= scale;
+            if (a.out) put8<FULL>(static_cast<EX *>(a.out) + o, n, G);
             if (!a.y) continue;
-            // of y: G becomes db, H e
-            if (POST && a.wy) get8(a.wy + c, n, f);
-            float dg[8];
+            // of y: G becomes db, then e
+            float dg[8], s3[1] = {0.f};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float ny = vy[i][e] * ry, wy = POST && a.wy ? f[e] : 1.f;
-                dg[e] = G[i][e] * (POST ? ny * wy : vy[i][e]);
-                if constexpr (SUMS) sg[i][e] += dg[e];
-                if (a.gate) G[i][e] *= g[i][e];
+                const float ny = vy[e] * ry;
+                dg[e] = G[e] * (POST ? ny * wy[e] : vy[e]);
+                sg[e] += dg[e];
+                G[e] *= g[e];
                 if constexpr (POST) {
-                    if constexpr (SUMS) swy[i][e] += G[i][e] * ny;
-                    G[i][e] *= wy;
-                    s3[0] += G[i][e] * ny;
+                    swy[e] += G[e] * ny;
+                    G[e] *= wy[e];
+                    s3[0] += G[e] * ny;
                 }
             }
             if (a.dgate) {
-                if (a.gate_bf16) put8(static_cast<__bf16 *>(a.dgate) + row * D + c, n, dg);
-                else put8(static_cast<float *>(a.dgate) + row * D + c, n, dg);
+                if (a.gate_bf16) put8<FULL>(static_cast<__bf16 *>(a.dgate) + o, n, dg);
+                else put8<FULL>(static_cast<float *>(a.dgate) + o, n, dg);
             }
-        }
-        ds += (double)ls, ds0 += (double)ls0;
-        if (!a.y || !a.h) continue;
-        float m3 = 0.f;
-        if constexpr (POST) {
-            team_sum<TEAM>(s3, slots, turn);
-            m3 = s3[0] * inv;
-        }
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int c = 8 * (i * TEAM + lane), n = D - c;
+            if (!a.h) continue;
             if constexpr (POST) {
+                team_sum<TEAM>(s3, slots, turn);
+                const float m3 = s3[0] * inv * ry;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) G[i][e] = ry * (G[i][e] - vy[i][e] * ry * m3);
+                for (int e = 0; e < 8; ++e) G[e] = ry * (G[e] - vy[e] * m3);
             }
-            put8(static_cast<EY *>(a.h) + row * D + c, n, G[i]);
+            put8<FULL>(static_cast<EY *>(a.h) + o, n, G);
         }
-    }
-    if constexpr (SUMS) {
         if (a.part_g) {
             leave(a.part_g + (unit * a.parts_per_gate + at) * D, sg);
 #pragma unroll
-            for (int i = 0; i < C; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sg[i][e] = 0.f;
+            for (int e = 0; e < 8; ++e) sg[e] = 0.f;
         }
-    }
     }
     if (a.part_s) {
 #pragma unroll
@@ -334,15 +334,13 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
         __syncthreads();
         if (threadIdx.x < 2) {
             double s = 0.;
-            for (int w = 0; w < NT / 64; ++w) s += scalars[threadIdx.x][w];
+            for (int k = 0; k < NT / 64; ++k) s += scalars[threadIdx.x][k];
             a.part_s[2 * part + threadIdx.x] = s;
         }
     }
-    if constexpr (SUMS) {
-        if (a.part_w) leave(a.part_w + part * D, sw);
-        if constexpr (POST) {
-            if (a.part_wy) leave(a.part_wy + part * D, swy);
-        }
+    if (a.part_w) leave(a.part_w + part * D, sw);
+    if constexpr (POST) {
+        if (a.part_wy) leave(a.part_wy + part * D, swy);
     }
 }
 
@@ -399,33 +397,28 @@ __global__ __launch_bounds__(1024) void residual_join_kernel(JoinArgs a) {
     }
 }
 
-// lanes of a row and chunks per lane
-struct Shape {
-    int team, chunks;
-};
-Shape shape_of(int64_t D) {
-    return D <= 128    ? Shape{16, 1}
-           : D <= 512  ? Shape{64, 1}
-           : D <= 1024 ? Shape{64, 2}
-           : D <= 2048 ? Shape{256, 1}
-           : D <= 4096 ? Shape{256, 2}
-                       : Shape{512, 2};
-}
-int threads_of(int team) { return team > 256 ? team : 256; }
+// lanes of a row, and threads of a workgroup
+int team_of(int64_t D) { return D <= 128 ? 16 : D <= 512 ? 64 : D <= 1024 ? 128 : D <= 2048 ? 256 : D <= 4096 ? 512 : 1024; }
+int threads_of(int team) { return team > 64 ? team : 256; }
 
-template <class EX, class EY, bool POST>
-void (*forward_of(Shape s))(ResArgs) {
-    return s.team == 16    ? residual_kernel<EX, EY, 16, 1, POST>
-           : s.team == 64  ? (s.chunks == 1 ? residual_kernel<EX, EY, 64, 1, POST> : residual_kernel<EX, EY, 64, 2, POST>)
-           : s.team == 256 ? (s.chunks == 1 ? residual_kernel<EX, EY, 256, 1, POST> : residual_kernel<EX, EY, 256, 2, POST>)
-                           : residual_kernel<EX, EY, 512, 2, POST>;
+// FULL: rows of whole 8 elements
+template <class EX, class EY, bool POST, bool FULL>
+void (*forward_of(int team))(ResArgs) {
+    return team == 16    ? residual_kernel<EX, EY, 16, POST, FULL>
+           : team == 64  ? residual_kernel<EX, EY, 64, POST, FULL>
+           : team == 128 ? residual_kernel<EX, EY, 128, POST, FULL>
+           : team == 256 ? residual_kernel<EX, EY, 256, POST, FULL>
+           : team == 512 ? residual_kernel<EX, EY, 512, POST, FULL>
+                         : residual_kernel<EX, EY, 1024, POST, FULL>;
 }
-template <class EX, class EY, bool POST, bool SUMS>
-void (*backward_of(Shape s))(ResArgs) {
-    return s.team == 16    ? residual_bwd_kernel<EX, EY, 16, 1, POST, SUMS>
-           : s.team == 64  ? (s.chunks == 1 ? residual_bwd_kernel<EX, EY, 64, 1, POST, SUMS> : residual_bwd_kernel<EX, EY, 64, 2, POST, SUMS>)
-           : s.team == 256 ? (s.chunks == 1 ? residual_bwd_kernel<EX, EY, 256, 1, POST, SUMS> : residual_bwd_kernel<EX, EY, 256, 2, POST, SUMS>)
-                           : residual_bwd_kernel<EX, EY, 512, 2, POST, SUMS>;
+template <class EX, class EY, bool POST, bool MIX, bool FULL>
+void (*backward_of(int team))(ResArgs) {
+    return team == 16    ? residual_bwd_kernel<EX, EY, 16, POST, MIX, FULL>
+           : team == 64  ? residual_bwd_kernel<EX, EY, 64, POST, MIX, FULL>
+           : team == 128 ? residual_bwd_kernel<EX, EY, 128, POST, MIX, FULL>
+           : team == 256 ? residual_bwd_kernel<EX, EY, 256, POST, MIX, FULL>
+           : team == 512 ? residual_bwd_kernel<EX, EY, 512, POST, MIX, FULL>
+                         : residual_bwd_kernel<EX, EY, 1024, POST, MIX, FULL>;
 }
 // f.operator()<EX, EY> for a pair of types
 template <class F>
@@ -434,13 +427,14 @@ auto of_types(int64_t x, int64_t y, F f) {
 }
 
 // How the backward pass cuts the rows into the parts of its workgroups: several gates' rows each, or a gate's rows (all rows where
-// no gate is summed) in several parts. About four workgroups of 256 threads per CU, or their threads in larger ones.
+// no gate is summed) in several parts. Eight waves per CU, which is
+// what the registers leave room for (twice as many parts cost norm-wide's join 6 us more).
 struct Cut {
     int64_t gates, gates_per_part, parts_per_gate, rows, parts;
 };
 Cut cut_of(int64_t rows, int64_t gate_rows, int64_t D) {
-    const Shape s = shape_of(D);
-    const int64_t teams = threads_of(s.team) / s.team, want = 1024 * 256 / threads_of(s.team);
+    const int team = team_of(D);
+    const int64_t teams = threads_of(team) / team, want = threads_of(team) > 512 ? 256 : 131072 / threads_of(team);
     const int64_t unit = gate_rows > 1 ? gate_rows : rows;
     Cut c;
     c.gates = rows / unit;
@@ -501,12 +495,15 @@ extern "C" int noise_residual_norm(const noise_residual_t *r, void *out, void *h
                     "%s: an output is NULL or not aligned to its type", fn);
     ResArgs a = args_of(r, eps);
     a.out = out, a.h = h;
-    const Shape s = shape_of(r->dim);
+    const int team = team_of(r->dim), threads = threads_of(team);
     auto kernel = of_types(r->x_type, r->y_type, [&](auto x, auto y) {
-        return r->norm_y ? forward_of<decltype(x), decltype(y), true>(s) : forward_of<decltype(x), decltype(y), false>(s);
+        using X = decltype(x);
+        using Y = decltype(y);
+        const bool full = r->dim % 8 == 0;
+        return r->norm_y ? (full ? forward_of<X, Y, true, true>(team) : forward_of<X, Y, true, false>(team))
+                         : (full ? forward_of<X, Y, false, true>(team) : forward_of<X, Y, false, false>(team));
     });
-    const int threads = threads_of(s.team);
-    const int64_t teams = threads / s.team, groups = (r->rows + teams - 1) / teams;
+    const int64_t teams = threads / team, groups = (r->rows + teams - 1) / teams;
     for (a.first = 0; a.first < groups; a.first += kLaunchGroups) {
         const int64_t n = groups - a.first < kLaunchGroups ? groups - a.first : kLaunchGroups;
         hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 0, (hipStream_t)stream, a);
@@ -557,17 +554,21 @@ extern "C" int noise_residual_norm_bwd(const noise_residual_t *r, const void *do
         w += 4 * parts * r->dim;
         if (d->dgate && !row_gate) a.part_g = reinterpret_cast<float *>(w);
     }
-    const Shape s = shape_of(r->dim);
+    const int team = team_of(r->dim);
     auto kernel = of_types(r->x_type, r->y_type, [&](auto x, auto y) {
         using X = decltype(x);
         using Y = decltype(y);
-        return r->norm_y ? (sums ? backward_of<X, Y, true, true>(s) : backward_of<X, Y, true, false>(s))
-                         : (sums ? backward_of<X, Y, false, true>(s) : backward_of<X, Y, false, false>(s));
+        auto of = [&](auto full) {
+            constexpr bool F = decltype(full)::value;
+            return r->norm_y ? (r->x0 ? backward_of<X, Y, true, true, F>(team) : backward_of<X, Y, true, false, F>(team))
+                             : (r->x0 ? backward_of<X, Y, false, true, F>(team) : backward_of<X, Y, false, false, F>(team));
+        };
+        return r->dim % 8 ? of(std::false_type{}) : of(std::true_type{});
     });
     a.gates = c.gates, a.gates_per_part = c.gates_per_part, a.parts_per_gate = c.parts_per_gate, a.part_rows = c.rows;
     for (a.first = 0; a.first < parts; a.first += kLaunchGroups) {
         const int64_t n = parts - a.first < kLaunchGroups ? parts - a.first : kLaunchGroups;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads_of(s.team)), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads_of(team)), 0, (hipStream_t)stream, a);
     }
     if (sums || scalars) {
         JoinArgs j;
