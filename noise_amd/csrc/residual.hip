@@ -207,11 +207,33 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
     const int64_t last_unit = first_unit + a.gates_per_part < a.gates ? first_unit + a.gates_per_part : a.gates;
     const int lane = threadIdx.x % TEAM, D = a.D, c = 8 * lane, n = D - c;
     const float inv = 1.f / (float)D, scale = a.scale ? *a.scale : 1.f, x0_scale = MIX && a.x0_scale ? *a.x0_scale : 1.f;
-    float w[8], wy[8], g[8], sw[8] = {}, swy[8] = {}, sg[8] = {};
-    get_weight<FULL>(a.w, c, n, w);
-    if (POST) get_weight<FULL>(a.wy, c, n, wy);
+    float sw[8] = {}, swy[8] = {}, sg[8] = {};
+    // the weights and the gate: in registers, or in LDS where 16 waves leave 128 registers to each
+    constexpr bool SHARED = TEAM == 1024;
+    constexpr int W = 0, WY = 1, GATE = 2;
+    __shared__ __attribute__((aligned(16))) float shared[SHARED ? 3 : 1][SHARED ? 8 * TEAM : 1];
+    float own[SHARED ? 1 : 3][8];
+    auto hold = [&](int which, const float (&v)[8]) {
+        if constexpr (SHARED) __builtin_memcpy(&shared[which][c], v, 32);
+        else
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = 1.f;
+            for (int e = 0; e < 8; ++e) own[which][e] = v[e];
+    };
+    auto take = [&](int which, float (&v)[8]) {
+        if constexpr (SHARED) __builtin_memcpy(v, &shared[which][c], 32);   // (each lane its own: no barrier)
+        else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = own[which][e];
+    };
+    {
+        float v[8];
+        get_weight<FULL>(a.w, c, n, v);
+        hold(W, v);
+        if (POST) get_weight<FULL>(a.wy, c, n, v), hold(WY, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 1.f;
+        hold(GATE, v);
+    }
     double ds = 0., ds0 = 0.;
     // the teams' sums, added in LDS
     auto leave = [&](float *to, float (&v)[8]) {
@@ -231,7 +253,8 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
     for (int64_t unit = first_unit; unit < last_unit; ++unit) {
         const int64_t begin = unit * unit_rows + at * a.part_rows, end = (unit + 1) * unit_rows;
         const int64_t stop = begin + a.part_rows < end ? begin + a.part_rows : end, from = begin + threadIdx.x / TEAM;
-        if (a.gate && !row_gate) get_gate<FULL>(a, unit * D + c, n, g);
+        float w[8], wy[8], g[8];
+        if (a.gate && !row_gate) get_gate<FULL>(a, unit * D + c, n, g), hold(GATE, g);
         // this lane's elements of the row, of the contiguous tensors and of the others
         int64_t o = from * D + c;
         const EX *x = static_cast<const EX *>(a.x) + from * a.s_x + c, *x0 = static_cast<const EX *>(a.x0) + from * a.s_x0 + c;
@@ -244,7 +267,7 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
             if (MIX) vx0.load(x0, n);
             vdo.load(static_cast<const EX *>(a.dout) + o, a.dout ? n : 0);
             if (a.dh) vdh.load(static_cast<const EY *>(a.dh) + o, n);
-            if (a.gate && row_gate) get_gate<FULL>(a, o, n, g);
+            if (a.gate && row_gate) get_gate<FULL>(a, o, n, g), hold(GATE, g);
             float ry = 1.f;
             if constexpr (POST) {
                 float s[1] = {0.f};
@@ -258,6 +281,8 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = vx[e], G[e] = vdo[e];
             if (a.y) {
+                take(GATE, g);
+                if (POST) take(WY, wy);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) t[e] += g[e] * (POST ? vy[e] * ry * wy[e] : vy[e]);
             }
@@ -265,10 +290,12 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
             for (int e = 0; e < 8; ++e) out[e] = MIX ? t[e] * scale + x0_scale * vx0[e] : t[e] * scale;
             if (a.dh) {
                 float s[2] = {0.f, 0.f};   // of x'^2 and u x'
+                take(W, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[0] += out[e] * out[e], s[1] += vdh[e] * w[e] * out[e];
                 team_sum<TEAM>(s, slots, turn);
                 const float r = rsqrtf(s[0] * inv + a.eps), m = s[1] * r * inv * r;   // (r mean(u n): n = x' r)
+                take(W, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     G[e] += r * (vdh[e] * w[e] - out[e] * m);
@@ -293,6 +320,8 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(Res
             if (!a.y) continue;
             // of y: G becomes db, then e
             float dg[8], s3[1] = {0.f};
+            take(GATE, g);
+            if (POST) take(WY, wy);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float ny = vy[e] * ry;
