@@ -61,14 +61,14 @@ __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
 }
 
 // In how many parts workgroups share the stages of k of a product with this many tiles, by what was measured: a tile takes 1.8 us per
-// stage and 3 us more, 256 of them run at a time, and a part's tile of fp32 sums costs 0.12 us of the whole chip's time. At most
+// stage (2.7 where operands are sums of two) and 3 us more, 256 of them run at a time, and a part's tile of fp32 sums costs 0.12 us of the whole chip's time. At most
 // kSplitTiles parts of tiles in all, at least 4 stages each.
 constexpr uint32_t kSplitTiles = 512;
-__device__ inline int splits_of(uint32_t tiles, uint32_t stages) {
+__device__ inline int splits_of(uint32_t tiles, uint32_t stages, uint32_t stage) {
     if (tiles == 0 || 2 * tiles > kSplitTiles) return 1;
-    uint32_t best = stages * 18 + 30, splits = 1;   // in 100 ns (stages of 2^22 entries or a piece's rows: far from 32 bits)
+    uint32_t best = stages * stage + 30, splits = 1;   // in 100 ns (stages of 2^22 entries or a piece's rows: far from 32 bits)
     for (uint32_t s = 2; s * tiles <= kSplitTiles && 4 * s <= stages; ++s) {
-        const uint32_t ns = (tiles * s + 255) / 256 * ((stages + s - 1) / s * 18 + 30) + tiles * s * 6 / 5;
+        const uint32_t ns = (tiles * s + 255) / 256 * ((stages + s - 1) / s * stage + 30) + tiles * s * 6 / 5;
         if (ns < best) best = ns, splits = s;
     }
     return (int)splits;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
-                                           T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
+                                           T::NT - 1, 0, a.nk, 1ll << 40, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
     if (m0 >= a.vocab) return;
     to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
@@ -460,7 +460,7 @@ struct FewArgs {
 
 template <class E, int VB, int RB, bool CAP>
 __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
-    constexpr int N = sizeof(E) == 2 ? 8 : 4, U = 4;   // elements per load, loads in flight per block
+    constexpr int N = sizeof(E) == 2 ? 8 : 4, U = 8;   // elements per load, loads in flight per block
     __shared__ float sums[4][VB][RB][64][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const int v0 = blockIdx.x * 16 * VB;
@@ -613,7 +613,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
-                                           T::NT - 1, a.nk, 0, SPLIT ? 3 * a.nk : a.nk, 1ll << 40, lds, acc);
+                                           T::NT - 1, 0, a.nk, 1ll << 40, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
     to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
     uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr));
@@ -695,8 +695,8 @@ struct Cut {
         c.n_end = DX ? rows : vocab;
         c.tiles_n = (int)((c.n_end + T::NT - 1) / T::NT);
         c.tiles = tiles_m * c.tiles_n;
-        c.stages = (SPLIT ? 3 : 1) * (int)(((DX ? vocab : rows) + T::BK - 1) / T::BK);
-        c.splits = splits_of(c.tiles, c.stages);
+        c.stages = (int)(((DX ? vocab : rows) + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>);
+        c.splits = splits_of(c.tiles, c.stages, SPLIT ? 27 : 18);
         return c;
     }
 };
@@ -712,18 +712,17 @@ __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, u
     int tm, tn;
     tile_of(group - split * c.tiles, g.tiles_m, c.tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nk = SPLIT ? c.stages / 3 : c.stages;
     const int first = (int)((int64_t)c.stages * split / c.splits), last = (int)((int64_t)c.stages * (split + 1) / c.splits);
     const int dim8 = (int)a.x.ld / 8;   // chunks of a packed row
     f32x16 acc[T::FB][T::NB];
     if (DX)
         product<T, true, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
-                                              T::NT - 1, nk, first, last, a.vocab, lds, acc);
+                                              T::NT - 1, first, last, a.vocab, lds, acc);
     else {
         Operand x = a.x;
         x.ptr += a.row0 * x.ld;
         product<T, true, true, SPLIT, SPLIT>(x, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
-                                             (int)(a.dz.ld - (int64_t)tn * T::NT) / 8 - 1, nk, first, last, 1ll << 40, lds, acc);
+                                             (int)(a.dz.ld - (int64_t)tn * T::NT) / 8 - 1, first, last, 1ll << 40, lds, acc);
     }
     const float unit = SPLIT ? 1.f / a.scales[2] / a.scales[DX ? 1 : 0] : 1.f;
 #pragma unroll
@@ -808,7 +807,8 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     Plan p = {};
     p.split = v->type == NOISE_FP32;
     p.ld = up(v->dim, Tile::BK);
-    p.nk = (int)(p.ld / Tile::BK);
+    const int64_t step = p.split ? kStep<Tile, true> : kStep<Tile, false>;
+    p.nk = (int)(p.ld / step);
     p.rows = up(v->rows, kPad);
     p.vocab_ld = up(v->vocab, Tile::MT);
     p.segments = (v->vocab + kSegment - 1) / kSegment;
@@ -835,8 +835,8 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
-        most_of(true, p.piece, (p.split ? 3 : 1) * (v->vocab + Tile::BK - 1) / Tile::BK, p.ld, &p.dx_groups, &p.dx_slabs);
-        most_of(false, v->vocab, (p.split ? 3 : 1) * p.piece / Tile::BK, p.ld, &p.dw_groups, &p.dw_slabs);
+        most_of(true, p.piece, (v->vocab + step - 1) / step, p.ld, &p.dx_groups, &p.dx_slabs);
+        most_of(false, v->vocab, p.piece / step, p.ld, &p.dw_groups, &p.dw_slabs);
         p.at_dx = take(4 * p.dx_slabs);
         p.at_dw = take(4 * p.dw_slabs);
         if (p.pieces > 1) p.at_sum = take(4 * v->vocab * p.ld);
@@ -865,8 +865,8 @@ struct FewPlan {
 };
 FewPlan few_plan(const noise_vocab_t *v) {
     FewPlan p;
-    // four workgroups per CU with 64 entries each, or 16 each
-    p.blocks = v->vocab >= 64 * 512 ? 4 : 1;
+    // 32 entries per workgroup, or 16 where that leaves fewer than two workgroups per CU
+    p.blocks = v->vocab >= 32 * 512 ? 2 : 1;
     p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
     p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
     return p;
@@ -884,8 +884,8 @@ int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, 
     a.rows = (int)v->rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.segments = (int)p.segments, a.wide = (int)v->targets_wide;
     a.softcap = softcap;
     const bool cap = softcap > 0.f;
-    auto kernel = v->type == NOISE_FP32 ? (p.blocks == 4 ? few_of<float, 4>(v->rows, cap) : few_of<float, 1>(v->rows, cap))
-                                        : (p.blocks == 4 ? few_of<__bf16, 4>(v->rows, cap) : few_of<__bf16, 1>(v->rows, cap));
+    auto kernel = v->type == NOISE_FP32 ? (p.blocks == 2 ? few_of<float, 2>(v->rows, cap) : few_of<float, 1>(v->rows, cap))
+                                        : (p.blocks == 2 ? few_of<__bf16, 2>(v->rows, cap) : few_of<__bf16, 1>(v->rows, cap));
     hipLaunchKernelGGL(kernel, dim3((unsigned)p.segments), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(vocab_few_join_kernel, dim3((unsigned)v->rows), dim3(256), 0, stream, a, loss, lse);
     return launch_status(fn);

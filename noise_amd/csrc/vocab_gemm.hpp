@@ -119,16 +119,21 @@ struct Tiling {
     __device__ static int wn(int wave) { return wave / WM * (NT / WN); }
 };
 
-// acc += the product over the stages first .. last - 1 of k (BK each). With SPLIT, operands are sums of two: the stages run three
-// times over the nk stages of k, for hi hi, hi lo and lo hi. k_rows: how many k a crossed A has rows for. Ends with a barrier.
+// k per stage. Operands that are sums of two values have both in a stage, for half the k.
+template <class T, bool SPLIT>
+constexpr int kStep = SPLIT ? T::BK / 2 : T::BK;
+
+// acc = the product over the stages first .. last - 1 of k. With SPLIT, operands are sums of two, multiplied hi hi + hi lo + lo hi
+// from one reading of each. k_rows: how many k a crossed A has rows for. Ends with a barrier.
 template <class T, bool CA, bool CB, bool F16, bool SPLIT>
-__device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last, const Operand &b, int64_t b0, int b_last, int nk,
-                                        int first, int last, int64_t k_rows, char *lds, f32x16 (&acc)[T::FB][T::NB]) {
-    constexpr int BK = T::BK, NS = T::NS, SPK = BK / 16;
+__device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last, const Operand &b, int64_t b0, int b_last, int first,
+                                        int last, int64_t k_rows, char *lds, f32x16 (&acc)[T::FB][T::NB]) {
+    constexpr int BK = kStep<T, SPLIT>, NS = T::NS, SPK = BK / 16, P = SPLIT ? 2 : 1;
     using SA = Side<T::MT, BK, T::NW, CA>;
     using SB = Side<T::NT, BK, T::NW, CB>;
-    constexpr int G = SA::N + SB::N;
+    constexpr int G = P * (SA::N + SB::N);
     static_assert(NS >= 2 && NS <= 4 && G * (NS - 1) < 64 && SPK % 2 == 0, "pipeline depth");
+    static_assert(P * (SA::kBytes + SB::kBytes) == T::kStage, "a stage");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned lbase = lds_addr(lds);
     SA sa;
@@ -146,22 +151,22 @@ __device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last
     const int n = last - first;
     auto issue = [&](int p) {
         const unsigned st = lbase + (p % NS) * T::kStage;
-        int64_t la = 0, lb = 0;
-        int s = first + p;
-        if (SPLIT) {
-            if (s >= 2 * nk) s -= 2 * nk, la = a.lo;
-            else if (s >= nk) s -= nk, lb = b.lo;
+        const int64_t k = (int64_t)(first + p) * BK;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            sa.copy(k, q ? a.lo : 0, k_rows - k < BK ? (int)(k_rows - k) : BK, st + q * SA::kBytes, wave);
+            sb.copy(k, q ? b.lo : 0, BK, st + P * SA::kBytes + q * SB::kBytes, wave);
         }
-        const int64_t k = (int64_t)s * BK;
-        sa.copy(k, la, k_rows - k < BK ? (int)(k_rows - k) : BK, st, wave);
-        sb.copy(k, lb, BK, st + SA::kBytes, wave);
     };
-    bf16x8 va[2][T::FB], vb[2][T::NB];
+    bf16x8 va[2][P][T::FB], vb[2][P][T::NB];
     auto fetch = [&](int buf, const char *st, int s) {
 #pragma unroll
-        for (int i = 0; i < T::FB; ++i) va[buf][i] = fa.get(st, s, i);
+        for (int q = 0; q < P; ++q) {
 #pragma unroll
-        for (int j = 0; j < T::NB; ++j) vb[buf][j] = fb.get(st + SA::kBytes, s, j);
+            for (int i = 0; i < T::FB; ++i) va[buf][q][i] = fa.get(st + q * SA::kBytes, s, i);
+#pragma unroll
+            for (int j = 0; j < T::NB; ++j) vb[buf][q][j] = fb.get(st + P * SA::kBytes + q * SB::kBytes, s, j);
+        }
     };
 #pragma unroll
     for (int p = 0; p < NS; ++p)
@@ -186,9 +191,12 @@ __device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last
                 fetch(cur ^ 1, lds + ((p + 1) % NS) * T::kStage, 0);
             }
 #pragma unroll
-            for (int i = 0; i < T::FB; ++i)
+            for (int q = 0; q < 2 * P - 1; ++q)
 #pragma unroll
-                for (int j = 0; j < T::NB; ++j) acc[i][j] = mfma16bit<F16>(va[cur][i], vb[cur][j], acc[i][j]);
+                for (int i = 0; i < T::FB; ++i)
+#pragma unroll
+                    for (int j = 0; j < T::NB; ++j)
+                        acc[i][j] = mfma16bit<F16>(va[cur][q == 2][i], vb[cur][q == 1][j], acc[i][j]);
         }
     }
     __syncthreads();
