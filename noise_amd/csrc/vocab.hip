@@ -52,26 +52,13 @@ struct Result {
 };
 struct GradArgs {
     Result dx, dw;
+    const uint2 *cut;            // the piece's (shares_of)
     int add, fp32, tiles_m;      // add: to dw.sum's values; fp32: the results' type
 };
 
 __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
     const int64_t n = *a.count - a.row0;
     return n < 0 ? 0 : n < a.piece ? n : a.piece;
-}
-
-// In how many parts workgroups share the stages of k of a product with this many tiles, by what was measured: a tile takes 1.8 us per
-// stage (2.7 where operands are sums of two) and 3 us more, 256 of them run at a time, and a part's tile of fp32 sums costs 0.12 us of the whole chip's time. At most
-// kSplitTiles parts of tiles in all, at least 4 stages each.
-constexpr uint32_t kSplitTiles = 512;
-__device__ inline int splits_of(uint32_t tiles, uint32_t stages, uint32_t stage) {
-    if (tiles == 0 || 2 * tiles > kSplitTiles) return 1;
-    uint32_t best = stages * stage + 30, splits = 1;   // in 100 ns (stages of 2^22 entries or a piece's rows: far from 32 bits)
-    for (uint32_t s = 2; s * tiles <= kSplitTiles && 4 * s <= stages; ++s) {
-        const uint32_t ns = (tiles * s + 255) / 256 * ((stages + s - 1) / s * stage + 30) + tiles * s * 6 / 5;
-        if (ns < best) best = ns, splits = s;
-    }
-    return (int)splits;
 }
 
 // softcap tanh(z / softcap) with an error of 2^-22 softcap: what enters exp(z) is absolute
@@ -81,58 +68,52 @@ __device__ __forceinline__ float cap_of(float z, float cap, float k) {
 
 // --- rows with a target, packed ---
 
-// One workgroup: N rows per thread at a time (4 for few rows, which then take all its waves)
-template <int N>
-__global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, int wide, int64_t rows, int64_t vocab,
+// Up to kLiveParts workgroups with `chunk` rows each: how many rows before them have a target they count themselves
+constexpr int kLiveParts = 64;
+__global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, int wide, int64_t rows, int64_t chunk, int64_t vocab,
                                                           const float *weight, const float *lse, int *count, int *live, int *place,
                                                           int *target, float *live_weight, float *live_lse, float *weight_max) {
-    __shared__ int sums[16];
+    __shared__ int sums[2][16];
     __shared__ float tops[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    auto at = [&](int64_t r) {
+        return wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
+    };
+    const int64_t begin = blockIdx.x * chunk, end = begin + chunk < rows ? begin + chunk : rows;
+    int n = 0;
+#pragma unroll 8
+    for (int64_t r = threadIdx.x; r < begin; r += 1024) {
+        const int64_t t = at(r);
+        n += t >= 0 && t < vocab;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if (lane == 0) sums[1][wave] = n;
+    __syncthreads();
     int base = 0;
+    for (int w = 0; w < 16; ++w) base += sums[1][w];
     float top = 0.f;
-    for (int64_t r0 = 0; r0 < rows; r0 += 1024 * N) {
-        // thread t of a wave takes rows r0 + 64 N wave + 64 i + t: consecutive lanes read consecutive targets
-        const int64_t first = r0 + 64 * N * wave + lane;
-        int64_t t[N];
-        float w[N], l[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t r = first + 64 * i;
-            t[i] = r >= rows ? -1 : wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
-            w[i] = weight && r < rows ? weight[r] : 1.f;
-            l[i] = lse && r < rows ? lse[r] : 0.f;
-        }
-        uint64_t mask[N];
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            mask[i] = __ballot(t[i] >= 0 && t[i] < vocab);
-            n += __popcll(mask[i]);
-        }
-        if (lane == 0) sums[wave] = n;
+    for (int64_t r0 = begin; r0 < end; r0 += 1024) {
+        const int64_t r = r0 + threadIdx.x;
+        const int64_t t = r < end ? at(r) : -1;
+        const float w = weight && r < end ? weight[r] : 1.f, l = lse && r < end ? lse[r] : 0.f;
+        const bool in = t >= 0 && t < vocab;
+        const uint64_t mask = __ballot(in);
+        if (lane == 0) sums[0][wave] = __popcll(mask);
         __syncthreads();
-        int before = base;
-        for (int w = 0; w < 16; ++w) {
-            if (w < wave) before += sums[w];
-            base += sums[w];
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t r = first + 64 * i;
-            const int at = before + __popcll(mask[i] & ((1ull << lane) - 1));
-            before += __popcll(mask[i]);
-            if (r >= rows) continue;
-            const bool in = t[i] >= 0 && t[i] < vocab;
-            place[r] = in ? at : -1;
-            if (!in) continue;
-            live[at] = (int)r;
-            target[at] = (int)t[i];
-            if (lse) live_lse[at] = l[i];
-            if (weight) live_weight[at] = w[i];
-            if (fabsf(w[i]) < __builtin_inff()) top = fmaxf(top, fabsf(w[i]));
+        int to = base + __popcll(mask & ((1ull << lane) - 1));
+        for (int k = 0; k < 16; ++k) {
+            if (k < wave) to += sums[0][k];
+            base += sums[0][k];
         }
         __syncthreads();
+        if (r < end) place[r] = in ? to : -1;
+        if (!in) continue;
+        live[to] = (int)r;
+        target[to] = (int)t;
+        if (lse) live_lse[to] = l;
+        if (weight) live_weight[to] = w;
+        if (fabsf(w) < __builtin_inff()) top = fmaxf(top, fabsf(w));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -140,8 +121,8 @@ __global__ __launch_bounds__(1024) void vocab_live_kernel(const void *targets, i
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) top = fmaxf(top, tops[w]);
-        *weight_max = top;
-        *count = base;
+        weight_max[blockIdx.x] = top;
+        if (blockIdx.x + 1 == gridDim.x) *count = base;
     }
 }
 
@@ -154,10 +135,15 @@ struct PackArgs {
     Operand to[2];
     int64_t dim;
     const int *place, *count;
-    const float *max, *weight_max;           // fp32: kMaxParts values of x's and of the weight's largest
+    const float *max, *weight_max;           // fp32: kMaxParts values of x's and of the weight's largest, and of the tokens' weights'
+    int live_parts;
     float *scales;
     void *dx;
     float *loss, *lse;
+    uint2 *cuts;                             // of each piece's gradients (NULL: none are asked for)
+    int64_t piece, pieces;
+    uint32_t tiles_m;
+    bool need_dx, need_dw;
 };
 
 constexpr int kMaxParts = 512;
@@ -213,6 +199,45 @@ __device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
     __builtin_memcpy(&lo, &l, 2);
 }
 
+// In how many shares workgroups take the stages of k of a tile of dx (x) and of dW (y), whose fp32 sums are then joined. Both products
+// run in one launch. Of no shares, and shares of one, a half and a third of what all stages take on 256 CUs, those that come out best
+// by what was measured: a workgroup takes 2.2 us per stage (3.3 where operands are sums of two) and 3 us more, 256 run at a time, and
+// joining costs 5 us and 0.09 us of the whole chip's time per tile's share. At most kSplitTiles shares of tiles, at least 4 stages each. (At
+// 16384 x 4096 x 512 dx then has 1 share and dW 4, and both take 154 us with the join; in two launches, with 2 and 8, it was 195.)
+constexpr uint32_t kSplitTiles = 512;
+template <class T, bool SPLIT>
+__device__ uint2 shares_of(int64_t rows, int64_t vocab, uint32_t tiles_m, bool dx, bool dw) {
+    constexpr uint32_t kStage = SPLIT ? 33 : 22;   // in 100 ns
+    uint32_t tiles[2] = {dx ? tiles_m * (uint32_t)((rows + T::NT - 1) / T::NT) : 0, dw ? tiles_m * (uint32_t)((vocab + T::NT - 1) / T::NT) : 0};
+    uint32_t stages[2] = {(uint32_t)((vocab + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>), (uint32_t)((rows + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>)};
+    const uint64_t work = (uint64_t)tiles[0] * stages[0] + (uint64_t)tiles[1] * stages[1];
+    uint2 take = {1, 1};
+    if (tiles[0] + tiles[1] >= 2048 || work == 0) return take;
+    uint64_t best = 0;
+    for (uint32_t k = 0; k < 4; ++k) {
+        const uint32_t each = k ? (uint32_t)((work + 256 * k - 1) / (256 * k)) : 0;
+        uint32_t s[2], groups = 0, longest = 0, sums = 0;
+        uint64_t all = 0;
+        for (int w = 0; w < 2; ++w) {
+            s[w] = each ? (stages[w] + each - 1) / each : 1;
+            if (s[w] > stages[w] / 4) s[w] = stages[w] / 4;
+            if (tiles[w] && s[w] > kSplitTiles / tiles[w]) s[w] = kSplitTiles / tiles[w];
+            if (s[w] < 1) s[w] = 1;
+            const uint32_t n = (stages[w] + s[w] - 1) / s[w];
+            groups += tiles[w] * s[w];
+            all += (uint64_t)tiles[w] * s[w] * n;
+            if (tiles[w] && n > longest) longest = n;
+            if (s[w] > 1) sums += tiles[w] * s[w];
+        }
+        const uint32_t rounds = (groups + 255) / 256;
+        uint64_t time = all * rounds / groups;
+        if (time < longest) time = longest;
+        time = time * kStage + rounds * 30 + (sums ? 50 + sums * 9 / 10 : 0);
+        if (k == 0 || time < best) best = time, take = uint2{s[0], s[1]};
+    }
+    return take;
+}
+
 // The packed matrices: x's rows at their places (zeros behind the last) and the weight's where it is packed, with zeros from dim to
 // the packed row's end. Rows of x without a place: their losses, lse and rows of dx to zero. A wave takes a row; blockIdx.y: x or
 // the weight.
@@ -230,9 +255,18 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(PackArgs a) {
         scale = scale_of(top);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             a.scales[which] = scale;
-            if (which == 0) a.scales[2] = scale_of(*a.weight_max);
+            if (which == 0) {
+                float most = 0.f;
+                for (int i = 0; i < a.live_parts; ++i) most = fmaxf(most, a.weight_max[i]);
+                a.scales[2] = scale_of(most);
+            }
         }
     }
+    if (a.cuts && blockIdx.x == 0 && which == 0)
+        for (int64_t i = threadIdx.x; i < a.pieces; i += 256) {
+            const int64_t left = *a.count - i * a.piece, there = left < 0 ? 0 : left < a.piece ? left : a.piece;
+            a.cuts[i] = shares_of<Tile, SPLIT>(there, a.rows[1], a.tiles_m, a.need_dx, a.need_dw);
+        }
     if (!padded) return;
     const E *src = static_cast<const E *>(a.src[which]);
     uint16_t *dst = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.to[which].ptr));
@@ -300,7 +334,7 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
     }
 }
 
-// STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_kernel turns into dZ. (Its rounding, 2^-11,
+// STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_dz_kernel turns into dZ. (Its rounding, 2^-11,
 // comes before dZ's own, 2^-8; below 2^-29 of the segment's largest it has fewer bits, below 2^-39 none.)
 template <class T, bool SPLIT, bool CAP, bool STORE>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
@@ -371,26 +405,27 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     }
 }
 
-// Sum over the workgroup of sums s with maxima top: every thread gets both
-__device__ __forceinline__ void join_sums(float &top, float &s, float2 (&slots)[4]) {
-    auto join = [&](float m2, float s2) {
-        const float m = fmaxf(top, m2);
-        s = s * exp2_fast((top - m) * kLog2e) + s2 * exp2_fast((m2 - m) * kLog2e);
-        top = m;
-    };
+// Sum over the wave of sums s with maxima top, which every lane gets: the same bits (the lower lane's first in each pair)
+__device__ __forceinline__ void wave_sums(float &top, float &s) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const float m2 = __shfl_xor(top, o, 64), s2 = __shfl_xor(s, o, 64);
-        // (the lower lane's pair first, so that both lanes get the same bits)
-        const bool low = !(threadIdx.x & o);
         const float m = fmaxf(top, m2), a = s * exp2_fast((top - m) * kLog2e), b = s2 * exp2_fast((m2 - m) * kLog2e);
-        s = low ? a + b : b + a;
+        s = threadIdx.x & o ? b + a : a + b;
         top = m;
     }
+}
+// The same over the workgroup
+__device__ __forceinline__ void join_sums(float &top, float &s, float2 (&slots)[4]) {
+    wave_sums(top, s);
     if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = float2{top, s};
     __syncthreads();
     top = slots[0].x, s = slots[0].y;
-    for (int w = 1; w < 4; ++w) join(slots[w].x, slots[w].y);
+    for (int w = 1; w < 4; ++w) {
+        const float m = fmaxf(top, slots[w].x);
+        s = s * exp2_fast((top - m) * kLog2e) + slots[w].y * exp2_fast((slots[w].x - m) * kLog2e);
+        top = m;
+    }
 }
 
 // This thread's share of a row's segments
@@ -403,10 +438,31 @@ __device__ __forceinline__ void row_sums(const float2 *part, int segments, float
     }
 }
 
-// A row's lse and loss from its segments; with STORE also dZ from what vocab_loss_kernel left:
+// Rows' lse and losses from their segments, a wave per row
+__global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, float *loss, float *lse) {
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = a.row0 + at;
+    if (at >= piece_rows(a)) return;
+    const int lane = threadIdx.x & 63;
+    const float2 *part = a.partial + row * a.segments;
+    float top = kLowest, s = 0.f;
+    for (int g = lane; g < a.segments; g += 64) {
+        const float2 p = part[g];
+        const float m = fmaxf(top, p.x);
+        s = s * exp2_fast((top - m) * kLog2e) + p.y * exp2_fast((p.x - m) * kLog2e);
+        top = m;
+    }
+    wave_sums(top, s);
+    if (lane) return;
+    const float l = top + logf(s);
+    const int to = a.live[row];
+    a.lse[row] = l;
+    loss[to] = l - a.zt[row];
+    if (lse) lse[to] = l;
+}
+
+// A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left:
 // dZ_v = weight exp(top - lse) 2^-15 stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
-template <bool STORE>
-__global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segment, float *loss, float *lse) {
+__global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *loss) {
     __shared__ float2 slots[4];
     const int64_t at = blockIdx.x, row = a.row0 + at;
     if (at >= piece_rows(a)) return;
@@ -415,32 +471,25 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, int segment,
     row_sums(part, a.segments, top, s);
     join_sums(top, s, slots);
     const float l = top + logf(s), z = a.zt[row];
-    if (threadIdx.x == 0) {
-        const int to = a.live ? a.live[row] : (int)row;
-        if (a.lse) a.lse[row] = l;
-        if (loss) loss[to] = l - z;
-        if (lse) lse[to] = l;
-    }
-    if constexpr (STORE) {
-        const float w = a.weight ? a.weight[row] : 1.f, u = a.softcap > 0.f ? z / a.softcap : 0.f;
-        const float own = w * (exp2_fast((z - l) * kLog2e) - 1.f) * (1.f - u * u);
-        const int t = a.target[row], end = a.segments * segment;
-        uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld;
+    if (threadIdx.x == 0) loss[a.live[row]] = l - z;
+    const float w = a.weight ? a.weight[row] : 1.f, u = a.softcap > 0.f ? z / a.softcap : 0.f;
+    const float own = w * (exp2_fast((z - l) * kLog2e) - 1.f) * (1.f - u * u);
+    const int t = a.target[row], end = a.segments * kSegment;
+    uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld;
 #pragma unroll 4
-        for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
-            __bf16 o[8];
-            if (c < end) {
-                _Float16 v[8];
-                __builtin_memcpy(v, __builtin_assume_aligned(dz + c, 16), 16);
-                const float f = w * exp2_fast(__builtin_fmaf(part[c / segment].x - l, kLog2e, -15.f));
+    for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
+        __bf16 o[8];
+        if (c < end) {
+            _Float16 v[8];
+            __builtin_memcpy(v, __builtin_assume_aligned(dz + c, 16), 16);
+            const float f = w * exp2_fast(__builtin_fmaf(part[c / kSegment].x - l, kLog2e, -15.f));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = (__bf16)(c + e == t ? own : (float)v[e] * f);
-            } else {
+            for (int e = 0; e < 8; ++e) o[e] = (__bf16)(c + e == t ? own : (float)v[e] * f);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = (__bf16)0.f;
-            }
-            __builtin_memcpy(__builtin_assume_aligned(dz + c, 16), o, 16);
+            for (int e = 0; e < 8; ++e) o[e] = (__bf16)0.f;
         }
+        __builtin_memcpy(__builtin_assume_aligned(dz + c, 16), o, 16);
     }
 }
 
@@ -688,27 +737,27 @@ __device__ __forceinline__ void finish(const HeadArgs &a, const GradArgs &g, int
 // How a gradient's product is cut, from the rows that there are
 struct Cut {
     int64_t n_end;             // results along n: packed rows (dx) or vocabulary entries (dW)
-    int tiles_n, tiles, stages, splits;
-    template <class T, bool DX, bool SPLIT>
-    __device__ static Cut of(int64_t rows, int vocab, int tiles_m) {
-        Cut c;
-        c.n_end = DX ? rows : vocab;
-        c.tiles_n = (int)((c.n_end + T::NT - 1) / T::NT);
-        c.tiles = tiles_m * c.tiles_n;
-        c.stages = (int)(((DX ? vocab : rows) + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>);
-        c.splits = splits_of(c.tiles, c.stages, SPLIT ? 27 : 18);
-        return c;
-    }
+    uint32_t tiles_n, tiles, stages, splits;
 };
+template <class T, bool DX, bool SPLIT>
+__device__ __forceinline__ Cut cut_of(const HeadArgs &a, const GradArgs &g, int64_t rows) {
+    Cut c;
+    c.n_end = DX ? rows : a.vocab;
+    c.tiles_n = (uint32_t)((c.n_end + T::NT - 1) / T::NT);
+    c.tiles = g.tiles_m * c.tiles_n;
+    c.stages = (uint32_t)(((DX ? a.vocab : rows) + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>);
+    c.splits = DX ? g.cut->x : g.cut->y;
+    return c;
+}
 
 // n: packed rows (DX) or vocabulary entries; m: columns of dim
 template <class T, bool DX, bool SPLIT>
 __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, uint32_t group, char *lds) {
     const Result &res = DX ? g.dx : g.dw;
     const int64_t rows = piece_rows(a);
-    const Cut c = Cut::of<T, DX, SPLIT>(rows, a.vocab, g.tiles_m);
-    if (group >= (uint32_t)c.tiles * c.splits) return;
-    const int split = group / c.tiles;
+    const Cut c = cut_of<T, DX, SPLIT>(a, g, rows);
+    if (group >= c.tiles * c.splits) return;
+    const uint32_t split = group / c.tiles;
     int tm, tn;
     tile_of(group - split * c.tiles, g.tiles_m, c.tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -757,7 +806,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a, G
 // The splits' sums, in order
 template <class T, bool DX, bool SPLIT>
 __device__ __forceinline__ void join_splits(const HeadArgs &a, const GradArgs &g, uint32_t group) {
-    const Cut k = Cut::of<T, DX, SPLIT>(piece_rows(a), a.vocab, g.tiles_m);
+    const Cut k = cut_of<T, DX, SPLIT>(a, g, piece_rows(a));
     if (k.splits == 1) return;   // (the product has written its results)
     const int64_t i = (int64_t)group * 256 + threadIdx.x;
     const uint32_t per = (uint32_t)(a.x.ld / 8);
@@ -765,7 +814,7 @@ __device__ __forceinline__ void join_splits(const HeadArgs &a, const GradArgs &g
     const int m = (int)(i - n * per) * 8;
     if (n >= k.n_end || m >= a.dim) return;
     float v[8] = {};
-    for (int s = 0; s < k.splits; ++s) {
+    for (uint32_t s = 0; s < k.splits; ++s) {
         const float *p = (DX ? g.dx : g.dw).slabs + ((int64_t)s * k.n_end + n) * a.x.ld + m;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += p[e];
@@ -788,7 +837,7 @@ struct Plan {
     int nk;
     bool split, pack_w;
     int64_t dx_groups, dw_groups, dx_slabs, dw_slabs;
-    int64_t at_int, at_float, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
+    int64_t at_int, at_float, at_cuts, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
 };
 
 // For any number of rows up to the piece's: the most workgroups of a gradient's product, and the fp32 values of its splits' sums.
@@ -829,11 +878,12 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
         return here;
     };
     p.at_int = take(4 * (3 * p.rows + 1));
-    p.at_float = take(4 * (3 * p.rows + 4 + 2 * kMaxParts));
+    p.at_float = take(4 * (3 * p.rows + 4 + kLiveParts + 2 * kMaxParts));
     p.at_partial = take(8 * p.segments * p.rows);
     p.at_x = take(2 * parts * p.rows * p.ld);
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
+        p.at_cuts = take(8 * p.pieces);
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
         most_of(true, p.piece, (v->vocab + step - 1) / step, p.ld, &p.dx_groups, &p.dx_slabs);
         most_of(false, v->vocab, p.piece / step, p.ld, &p.dw_groups, &p.dw_slabs);
@@ -901,10 +951,12 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     int *place = reinterpret_cast<int *>(ws + p.at_int), *live = place + p.rows, *target = live + p.rows, *count = target + p.rows;
     float *f = reinterpret_cast<float *>(ws + p.at_float);
     float *packed_weight = f, *packed_lse = f + p.rows, *zt = f + 2 * p.rows, *scales = f + 3 * p.rows,
-          *maxima = scales + 4;
+          *weight_max = scales + 4, *maxima = weight_max + kLiveParts;
     const int64_t rows = v->rows;
-    hipLaunchKernelGGL((rows <= 4096 ? vocab_live_kernel<4> : vocab_live_kernel<16>), dim3(1), dim3(1024), 0, stream, v->targets, (int)v->targets_wide, rows, v->vocab, weight,
-                       given, count, live, place, target, packed_weight, packed_lse, scales + 3);
+    const int64_t parts = (rows + 1023) / 1024 < kLiveParts ? (rows + 1023) / 1024 : kLiveParts, chunk = up((rows + parts - 1) / parts, 1024);
+    const int live_parts = (int)((rows + chunk - 1) / chunk);
+    hipLaunchKernelGGL(vocab_live_kernel, dim3(live_parts), dim3(1024), 0, stream, v->targets, (int)v->targets_wide, rows, chunk,
+                       v->vocab, weight, given, count, live, place, target, packed_weight, packed_lse, weight_max);
     HeadArgs a = {};
     a.x = Operand{reinterpret_cast<__bf16 *>(ws + p.at_x), p.ld, p.rows * p.ld};
     a.w = p.pack_w ? Operand{reinterpret_cast<__bf16 *>(ws + p.at_w), p.ld, v->vocab * p.ld}
@@ -913,7 +965,9 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     k.src[0] = v->x, k.src[1] = v->weight, k.src_ld[0] = v->x_stride, k.src_ld[1] = v->weight_stride;
     k.rows[0] = rows, k.rows[1] = v->vocab, k.padded[0] = p.rows, k.padded[1] = p.pack_w ? v->vocab : 0;
     k.to[0] = a.x, k.to[1] = a.w, k.dim = v->dim, k.place = place, k.count = count;
-    k.max = maxima, k.weight_max = scales + 3, k.scales = scales, k.dx = dx, k.loss = loss, k.lse = lse;
+    k.max = maxima, k.weight_max = weight_max, k.live_parts = live_parts, k.scales = scales, k.dx = dx, k.loss = loss, k.lse = lse;
+    k.piece = p.piece, k.pieces = p.pieces, k.tiles_m = (uint32_t)((p.ld + Tile::MT - 1) / Tile::MT);
+    k.cuts = grad ? reinterpret_cast<uint2 *>(ws + p.at_cuts) : nullptr, k.need_dx = dx != nullptr, k.need_dw = dw != nullptr;
     if (p.split) hipLaunchKernelGGL(vocab_max_kernel, dim3(kMaxParts, 2), dim3(256), 0, stream, k, maxima);
     const int64_t most = p.rows > k.padded[1] ? p.rows : k.padded[1], packs = (most + 3) / 4;
     hipLaunchKernelGGL((p.split ? vocab_pack_kernel<float, true> : vocab_pack_kernel<__bf16, false>),
@@ -940,8 +994,8 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
                           : store ? (cap ? vocab_loss_kernel<Tile, false, true, true> : vocab_loss_kernel<Tile, false, false, true>)
                                   : (cap ? vocab_loss_kernel<Tile, false, true, false> : vocab_loss_kernel<Tile, false, false, false>);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
-            hipLaunchKernelGGL((store ? vocab_lse_kernel<true> : vocab_lse_kernel<false>), dim3((unsigned)a.piece), dim3(256), 0,
-                               stream, a, kSegment, loss, lse);
+            if (store) hipLaunchKernelGGL(vocab_lse_dz_kernel, dim3((unsigned)a.piece), dim3(256), 0, stream, a, loss);
+            else hipLaunchKernelGGL(vocab_lse_kernel, dim3((unsigned)(a.piece / 4)), dim3(256), 0, stream, a, loss, lse);
         }
         if (!grad) continue;
         if (given || !store) {
@@ -951,7 +1005,7 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
         }
         GradArgs g = {};
         const int64_t per = p.ld / 8;
-        g.tiles_m = (int)((p.ld + Tile::MT - 1) / Tile::MT);
+        g.tiles_m = (int)k.tiles_m, g.cut = k.cuts + i;
         g.add = i > 0, g.fp32 = p.split;
         if (dx) {
             g.dx.out = dx, g.dx.slabs = reinterpret_cast<float *>(ws + p.at_dx), g.dx.groups = (uint32_t)p.dx_groups;
