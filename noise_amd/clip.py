@@ -13,7 +13,7 @@ from .sinks import F32, TYPES, _call, _no_gradients, _no_tangents
 
 
 def clip(fn, gradients, max_norm):
-    gradients = list(gradients)
+    gradients = [g for g in gradients if g is not None]
     if not gradients:
         raise ValueError(f'{fn}: no gradients')
     if not max_norm >= 0:
@@ -26,7 +26,7 @@ def clip(fn, gradients, max_norm):
             raise ValueError(f'{fn}: gradients on {device} and {g.device}')
         # (elements in any order: a transposed gradient is as good as another)
         if not g.is_contiguous() and not torch.ops.aten.is_non_overlapping_and_dense(g):
-            raise ValueError(f'{fn}: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps')
+            raise ValueError(f'{fn}: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps itself')
         flat += (g.data_ptr(), g.numel(), TYPES[g.dtype])
     _no_tangents(fn, *gradients)
     _no_gradients(fn, *gradients)
@@ -47,10 +47,10 @@ def clip_gradients(gradients, max_norm):
 
         norm = sqrt(sum of all squares),  g <- g min(1, max_norm / (norm + 1e-6))
 
-    `gradients` are bfloat16 and float32 tensors of any sizes on one device, their elements in any order but without gaps, no two
-    of them in the same memory. Squares are summed in 64 bits, in a fixed order; results are rounded once. An infinite `max_norm`
+    `gradients` are bfloat16 and float32 tensors of any sizes on one device (None is left out), their elements in any order but
+    without gaps, no two of them in the same memory. Squares are summed in 64 bits, in a fixed order; results are rounded once. An infinite `max_norm`
     leaves the gradients as they are; a norm that is NaN makes them all NaN, an infinite one makes the finite ones 0 and the
     infinite ones NaN. Nothing waits for the device: the norm stays on it."""
     if torch.compiler.is_compiling():
-        return torch.ops.noise_amd.clip_gradients(list(gradients), float(max_norm))
+        return torch.ops.noise_amd.clip_gradients([g for g in gradients if g is not None], float(max_norm))
     return clip('clip_gradients', gradients, max_norm)

@@ -34,7 +34,7 @@ struct HeadArgs {
     const float *scales;         // 2^ex, 2^ew, 2^ed of fp32 operands (x, w, dZ), else 1
     const float *weight;         // of a packed row's loss
     float *lse, *zt;             // of a packed row
-    float2 *partial;             // [rows][segments]: a segment's largest logit, and the sum of exponentials from there
+    float2 *partial;             // [rows of the piece][segments]: a segment's largest logit, and the sum of exponentials from there
     int64_t row0;                // the piece's first packed row
     int64_t piece;               // rows of the piece, at most
     int vocab, dim, nk, segments;  // nk: stages of k over dim
@@ -182,11 +182,11 @@ __global__ __launch_bounds__(256) void vocab_max_kernel(PackArgs a, float *to) {
     if (threadIdx.x == 0) to[which * kMaxParts + blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
-// The power of two that takes `top` to 2^14 .. 2^15 (within 2^-100 .. 2^100)
+// The power of two that takes `top` to 2^14 .. 2^15 (within the normal ones)
 __device__ __forceinline__ float scale_of(float top) {
     if (!(top > 0.f)) return 1.f;
     int e = 14 - ilogbf(top);
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    e = e < -126 ? -126 : e > 126 ? 126 : e;
     return ldexpf(1.f, e);
 }
 
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
                 }
             }
         s += swap_halves(s);
-        if (lane < 32 && there) a.partial[row * a.segments + m0 / kSegment] = float2{top, s};
+        if (lane < 32 && there) a.partial[at * a.segments + m0 / kSegment] = float2{top, s};
     }
 }
 
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, float *loss,
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = a.row0 + at;
     if (at >= piece_rows(a)) return;
     const int lane = threadIdx.x & 63;
-    const float2 *part = a.partial + row * a.segments;
+    const float2 *part = a.partial + at * a.segments;
     float top = kLowest, s = 0.f;
     for (int g = lane; g < a.segments; g += 64) {
         const float2 p = part[g];
@@ -466,7 +466,7 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
     __shared__ float2 slots[4];
     const int64_t at = blockIdx.x, row = a.row0 + at;
     if (at >= piece_rows(a)) return;
-    const float2 *part = a.partial + row * a.segments;
+    const float2 *part = a.partial + at * a.segments;
     float top = kLowest, s = 0.f;
     row_sums(part, a.segments, top, s);
     join_sums(top, s, slots);
@@ -879,7 +879,7 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     };
     p.at_int = take(4 * (3 * p.rows + 1));
     p.at_float = take(4 * (3 * p.rows + 4 + kLiveParts + 2 * kMaxParts));
-    p.at_partial = take(8 * p.segments * p.rows);
+    p.at_partial = take(8 * p.segments * p.piece);
     p.at_x = take(2 * parts * p.rows * p.ld);
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {

@@ -32,6 +32,8 @@ def _scalar(fn, name, s, device):
     """The scalar in fp32"""
     if s is None:
         return None
+    if not isinstance(s, torch.Tensor):
+        raise ValueError(f'{fn}: {name} must be a tensor of one value on {device}, got {s!r}')
     if s.numel() != 1 or s.device != device or not s.is_floating_point():
         raise ValueError(f'{fn}: {name} must be one value on {device}, got {s.dtype} {tuple(s.shape)} on {s.device}')
     return s if s.dtype == F32 else s.to(F32)
@@ -203,6 +205,6 @@ def residual_norm(x, y=None, x0=None, scale=None, x0_scale=None, gate=None, y_we
                                                  float(eps))
     if torch.is_grad_enabled():
         for t in (x, y, x0, scale, x0_scale, gate, y_weight, weight):
-            if t is not None and t.requires_grad:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
                 return _Residual.apply(x, y, x0, scale, x0_scale, gate, y_weight, weight, bool(norm_y), dtype, float(eps))
     return forward(x, y, x0, scale, x0_scale, gate, y_weight, weight, bool(norm_y), dtype, float(eps))
