@@ -14,6 +14,8 @@
 // 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term.
 #include "vocab_gemm.hpp"
 
+#include <type_traits>
+
 namespace noise {
 namespace {
 
@@ -212,7 +214,7 @@ __device__ uint2 shares_of(int64_t rows, int64_t vocab, uint32_t tiles_m, bool d
     uint32_t stages[2] = {(uint32_t)((vocab + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>), (uint32_t)((rows + kStep<T, SPLIT> - 1) / kStep<T, SPLIT>)};
     const uint64_t work = (uint64_t)tiles[0] * stages[0] + (uint64_t)tiles[1] * stages[1];
     uint2 take = {1, 1};
-    if (tiles[0] + tiles[1] >= 2048 || work == 0) return take;
+    if (work == 0) return take;
     uint64_t best = 0;
     for (uint32_t k = 0; k < 4; ++k) {
         const uint32_t each = k ? (uint32_t)((work + 256 * k - 1) / (256 * k)) : 0;
@@ -495,24 +497,27 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
 
 // --- the losses of a few rows ---
 
-// What is read is the weight, once: a workgroup takes 16 VB vocabulary entries for up to 16 RB rows, its four waves a quarter of dim
+// What is read is the weight: a workgroup takes 16 VB vocabulary entries for 16 RB rows (blockIdx.y counts those), its four waves a quarter of dim
 // each, straight from memory into v_mfma_f32_16x16x32_bf16's (fp32: v_mfma_f32_16x16x4_f32's, exact products) operands: 16 lanes on
 // 16 rows of the weight, and the rows of x from the caches. The waves' sums meet in LDS; wave v takes entries 16 v on from there.
+//
+// With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel.
 struct FewArgs {
     const void *x, *w, *targets;
     int64_t x_ld, w_ld;
     float2 *partial;
-    float *zt;
+    float *zt, *z;
+    int64_t z_ld;
     int rows, vocab, dim, segments, wide;
     float softcap;
 };
 
-template <class E, int VB, int RB, bool CAP>
+template <class E, int VB, int RB, bool CAP, bool WRITE>
 __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
-    constexpr int N = sizeof(E) == 2 ? 8 : 4, U = 8;   // elements per load, loads in flight per block
+    constexpr int N = sizeof(E) == 2 ? 8 : 4;   // elements per load
     __shared__ float sums[4][VB][RB][64][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int v0 = blockIdx.x * 16 * VB;
+    const int v0 = blockIdx.x * 16 * VB, r0 = blockIdx.y * 16 * RB;
     const E *w[VB], *x[RB];
 #pragma unroll
     for (int b = 0; b < VB; ++b) {
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
     }
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-        const int r = 16 * b + i;
+        const int r = r0 + 16 * b + i;
         x[b] = static_cast<const E *>(a.x) + (int64_t)(r < a.rows ? r : a.rows - 1) * a.x_ld;
     }
     f32x4 acc[VB][RB] = {};
@@ -540,23 +545,29 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
     const int steps = (a.dim + 4 * N - 1) / (4 * N), whole = a.dim / (4 * N);
     const int first = steps * wave / 4, last = steps * (wave + 1) / 4;
     int s = first;
-    for (; s + U <= (last < whole ? last : whole); s += U) {
-        E vw[VB][U][N];
+    auto run = [&](auto count) {
+        constexpr int U = decltype(count)::value;
+        for (; s + U <= (last < whole ? last : whole); s += U) {
+            E vw[VB][U][N];
 #pragma unroll
-        for (int b = 0; b < VB; ++b)
+            for (int b = 0; b < VB; ++b)
 #pragma unroll
-            for (int u = 0; u < U; ++u) __builtin_memcpy(vw[b][u], w[b] + (s + u) * 4 * N + g * N, 16);
+                for (int u = 0; u < U; ++u) __builtin_memcpy(vw[b][u], w[b] + (s + u) * 4 * N + g * N, 16);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int r = 0; r < RB; ++r) {
-                E vx[N];
-                __builtin_memcpy(vx, x[r] + (s + u) * 4 * N + g * N, 16);
+                for (int r = 0; r < RB; ++r) {
+                    E vx[N];
+                    __builtin_memcpy(vx, x[r] + (s + u) * 4 * N + g * N, 16);
 #pragma unroll
-                for (int b = 0; b < VB; ++b) multiply(vw[b][u], vx, acc[b][r]);
+                    for (int b = 0; b < VB; ++b) multiply(vw[b][u], vx, acc[b][r]);
+                }
             }
         }
-    }
+    };
+    run(std::integral_constant<int, 8>{});
+    run(std::integral_constant<int, 2>{});
+    run(std::integral_constant<int, 1>{});
     for (; s < last; ++s) {
         const int at = s * 4 * N + g * N, n = a.dim - at;
 #pragma unroll
@@ -578,13 +589,13 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
 #pragma unroll
         for (int r = 0; r < RB; ++r) __builtin_memcpy(sums[wave][b][r][lane], &acc[b][r], 16);
     __syncthreads();
-    // entries v0 + 16 wave + 4 g + e of row 16 r + i
+    // entries v0 + 16 wave + 4 g + e of row r0 + 16 r + i
     __shared__ float2 tops[4][RB][16];
     if (wave < VB) {
         const float k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-            const int row = 16 * r + i, v = v0 + 16 * wave + 4 * g;
+            const int row = r0 + 16 * r + i, v = v0 + 16 * wave + 4 * g;
             float z[4], top = kLowest, t = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -592,6 +603,11 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
                 if (CAP) z[e] = cap_of(z[e], a.softcap, k);
                 if (v + e >= a.vocab) z[e] = -__builtin_inff();
                 top = fmaxf(top, z[e]);
+            }
+            if constexpr (WRITE) {
+                // (rows of the logits are whole 16 entries)
+                if (row < a.rows) __builtin_memcpy(__builtin_assume_aligned(a.z + row * a.z_ld + v, 16), z, 16);
+                continue;
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -609,9 +625,10 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
             }
         }
     }
+    if constexpr (WRITE) return;
     __syncthreads();
     for (int row = threadIdx.x; row < 16 * RB; row += 256) {
-        if (row >= a.rows) continue;
+        if (r0 + row >= a.rows) continue;
         float2 p = tops[0][row / 16][row % 16];
 #pragma unroll
         for (int b = 1; b < VB; ++b) {
@@ -619,7 +636,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
             const float m = fmaxf(p.x, q.x);
             p = float2{m, p.y * exp2_fast((p.x - m) * kLog2e) + q.y * exp2_fast((q.x - m) * kLog2e)};
         }
-        a.partial[(int64_t)row * a.segments + blockIdx.x] = p;
+        a.partial[(int64_t)(r0 + row) * a.segments + blockIdx.x] = p;
     }
 }
 
@@ -637,13 +654,68 @@ __global__ __launch_bounds__(256) void vocab_few_join_kernel(FewArgs a, float *l
     if (lse) lse[row] = in ? l : 0.f;
 }
 
-constexpr int kFewRows = 64;
+// lse and loss of a packed row from its logits, and dZ; zeros in the rows behind the last
+template <bool SPLIT>
+__global__ __launch_bounds__(256) void vocab_z_dz_kernel(HeadArgs a, const float *logits, int64_t z_ld, float *loss) {
+    __shared__ float2 slots[4];
+    const int64_t at = blockIdx.x;
+    const bool there = at < *a.count;
+    const int row = there ? a.live[at] : 0, t = there ? a.target[at] : 0;
+    const float *z = logits + row * z_ld;
+    float top = kLowest, s = 0.f;
+    if (there)
+        for (int c = 4 * threadIdx.x; c < a.vocab; c += 1024) {   // (-inf past the vocabulary)
+            float v[4];
+            __builtin_memcpy(v, __builtin_assume_aligned(z + c, 16), 16);
+            const float m = fmaxf(top, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+            s *= exp2_fast((top - m) * kLog2e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += exp2_fast((v[e] - m) * kLog2e);
+            top = m;
+        }
+    join_sums(top, s, slots);
+    const float l = top + logf(s), zt = z[t];
+    if (there && loss && threadIdx.x == 0) loss[row] = l - zt;
+    const float w = (a.weight ? a.weight[at] : 1.f) * (SPLIT ? a.scales[2] : 1.f);
+    const bool cap = a.softcap > 0.f;
+    const float bend = cap ? -w / a.softcap / a.softcap : 0.f;   // of w cap'
+    uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld;
+    for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
+        uint16_t hi[8] = {}, lo[8] = {};
+        if (there && c < a.vocab) {
+            float v[8];
+            __builtin_memcpy(v, __builtin_assume_aligned(z + c, 16), 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float d = exp2_fast((v[e] - l) * kLog2e);
+                if (c + e == t) d -= 1.f;
+                d *= cap ? __builtin_fmaf(v[e] * bend, v[e], w) : w;
+                if (c + e >= a.vocab) d = 0.f;
+                if constexpr (SPLIT) halves(d, hi[e], lo[e]);
+                else {
+                    const __bf16 b = (__bf16)d;
+                    __builtin_memcpy(&hi[e], &b, 2);
+                }
+            }
+        }
+        __builtin_memcpy(__builtin_assume_aligned(dz + c, 16), hi, 16);
+        if constexpr (SPLIT) __builtin_memcpy(__builtin_assume_aligned(dz + a.dz.lo + c, 16), lo, 16);
+    }
+}
 
-template <class E, int VB>
+constexpr int kFewRows = 256;
+
+template <class E, int VB, bool WRITE>
 void (*few_of(int64_t rows, bool cap))(FewArgs) {
-    return rows <= 16   ? (cap ? vocab_few_kernel<E, VB, 1, true> : vocab_few_kernel<E, VB, 1, false>)
-           : rows <= 32 ? (cap ? vocab_few_kernel<E, VB, 2, true> : vocab_few_kernel<E, VB, 2, false>)
-                        : (cap ? vocab_few_kernel<E, VB, 4, true> : vocab_few_kernel<E, VB, 4, false>);
+    return rows <= 16   ? (cap ? vocab_few_kernel<E, VB, 1, true, WRITE> : vocab_few_kernel<E, VB, 1, false, WRITE>)
+           : rows <= 32 ? (cap ? vocab_few_kernel<E, VB, 2, true, WRITE> : vocab_few_kernel<E, VB, 2, false, WRITE>)
+                        : (cap ? vocab_few_kernel<E, VB, 4, true, WRITE> : vocab_few_kernel<E, VB, 4, false, WRITE>);
+}
+unsigned few_blocks(int64_t rows) { return (unsigned)((rows + 63) / 64); }
+template <bool WRITE>
+void (*few_of(int type, int blocks, int64_t rows, bool cap))(FewArgs) {
+    return type == NOISE_FP32 ? (blocks == 2 ? few_of<float, 2, WRITE>(rows, cap) : few_of<float, 1, WRITE>(rows, cap))
+                              : (blocks == 2 ? few_of<__bf16, 2, WRITE>(rows, cap) : few_of<__bf16, 1, WRITE>(rows, cap));
 }
 
 // zeros: rows of dW past the vocabulary
@@ -835,9 +907,9 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Plan {
     int64_t ld, rows, piece, pieces, vocab_ld, segments;
     int nk;
-    bool split, pack_w;
+    bool split, pack_w, few;   // few: the logits of all rows are kept (at most 1 GiB)
     int64_t dx_groups, dw_groups, dx_slabs, dw_slabs;
-    int64_t at_int, at_float, at_cuts, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
+    int64_t at_int, at_float, at_cuts, at_z, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
 };
 
 // For any number of rows up to the piece's: the most workgroups of a gradient's product, and the fp32 values of its splits' sums.
@@ -850,6 +922,35 @@ void most_of(bool rows, int64_t n_end, int64_t stages, int64_t ld, int64_t *grou
     int64_t n = s * n_end;
     if (rows && kSplitTiles / tiles_m * Tile::NT < n) n = kSplitTiles / tiles_m * Tile::NT;
     *slabs = s < 2 ? 0 : n * ld;
+}
+
+// Whether the logits come from vocab_few_kernel, whose every workgroup forms its own, or from the tiles of vocab_loss_kernel and
+// vocab_dz_kernel, which share operands but are few and long where there are few entries. By what was measured, in ns: the former read
+// 5 TB/s of weight for each 64 rows and then multiply at 268 TFLOP/s (fp32: 119); a tile takes 1.5 us per stage of 64 of dim when it
+// is one of the only 256 and 2.3 otherwise (twice that in fp32, whose gradients have two such passes in one call and whose losses alone need the
+// weight packed, 12 B read and written per value), and 15 us in all. 131072 x 2048 bf16, losses of 16, 32 and 64 rows: 132, 157 and
+// 233 us against 165; 4096 x 512: 6, 7 and 9 against 27; 131072 x 2048 fp32: 257, 322 and 478 against 970.
+bool few_rows(const noise_vocab_t *v, bool grad) {
+    if (v->rows > kFewRows || (grad && v->rows * v->vocab > 1 << 28)) return false;
+    const double R = (double)v->rows, VD = (double)v->vocab * (double)v->dim, size = v->type == NOISE_FP32 ? 4 : 2;
+    const double few = VD * size * (double)((v->rows + 63) / 64) / 5e3 + 2 * R * VD / (size == 4 ? 119e3 : 268e3);
+    const double rounds = (double)((v->vocab + 65535) / 65536), stages = (double)((v->dim + 63) / 64);
+    double tiles = 15e3 + rounds * stages * (rounds > 1 ? 2300 : 1500) * (size == 4 ? (grad ? 4 : 2) : 1);
+    if (size == 4 && !grad) tiles += VD * 12 / 5e3;
+    return few < tiles;
+}
+
+struct FewPlan {
+    int blocks;   // of 16 entries per workgroup
+    int64_t segments, bytes;
+};
+FewPlan few_plan(const noise_vocab_t *v) {
+    FewPlan p;
+    // 32 entries per workgroup, or 16 where that leaves fewer than two workgroups per CU
+    p.blocks = v->vocab >= 32 * 512 ? 2 : 1;
+    p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
+    p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
+    return p;
 }
 
 Plan plan_of(const noise_vocab_t *v, bool grad) {
@@ -883,6 +984,8 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     p.at_x = take(2 * parts * p.rows * p.ld);
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
+        p.few = few_rows(v, true);
+        if (p.few) p.at_z = take(4 * v->rows * up(v->vocab, 32));
         p.at_cuts = take(8 * p.pieces);
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
         most_of(true, p.piece, (v->vocab + step - 1) / step, p.ld, &p.dx_groups, &p.dx_slabs);
@@ -909,19 +1012,6 @@ int check(const char *fn, const noise_vocab_t *v, float softcap) {
     return NOISE_OK;
 }
 
-struct FewPlan {
-    int blocks;   // of 16 entries per workgroup
-    int64_t segments, bytes;
-};
-FewPlan few_plan(const noise_vocab_t *v) {
-    FewPlan p;
-    // 32 entries per workgroup, or 16 where that leaves fewer than two workgroups per CU
-    p.blocks = v->vocab >= 32 * 512 ? 2 : 1;
-    p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
-    p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
-    return p;
-}
-
 int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace, int64_t workspace_bytes,
             hipStream_t stream) {
     const FewPlan p = few_plan(v);
@@ -932,11 +1022,9 @@ int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, 
     a.zt = static_cast<float *>(workspace);
     a.partial = reinterpret_cast<float2 *>(a.zt + kFewRows);
     a.rows = (int)v->rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.segments = (int)p.segments, a.wide = (int)v->targets_wide;
-    a.softcap = softcap;
-    const bool cap = softcap > 0.f;
-    auto kernel = v->type == NOISE_FP32 ? (p.blocks == 2 ? few_of<float, 2>(v->rows, cap) : few_of<float, 1>(v->rows, cap))
-                                        : (p.blocks == 2 ? few_of<__bf16, 2>(v->rows, cap) : few_of<__bf16, 1>(v->rows, cap));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)p.segments), dim3(256), 0, stream, a);
+    a.softcap = softcap, a.z = nullptr, a.z_ld = 0;
+    auto kernel = few_of<false>(v->type, p.blocks, v->rows, softcap > 0.f);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)p.segments, few_blocks(v->rows)), dim3(256), 0, stream, a);
     hipLaunchKernelGGL(vocab_few_join_kernel, dim3((unsigned)v->rows), dim3(256), 0, stream, a, loss, lse);
     return launch_status(fn);
 }
@@ -988,8 +1076,19 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
         a.tiles_m = (int)((v->vocab + Tile::MT - 1) / Tile::MT);
         const dim3 tiles((unsigned)(a.tiles_m * (a.piece / Tile::NT)));
         a.dz = Operand{reinterpret_cast<__bf16 *>(ws + p.at_dz), p.vocab_ld, p.piece * p.vocab_ld};
-        const bool store = grad && !p.split;
-        if (!given) {
+        const bool store = grad && !p.split, few = p.few;
+        if (few) {
+            const FewPlan q = few_plan(v);
+            FewArgs f = {};
+            f.x = v->x, f.w = v->weight, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
+            f.z = reinterpret_cast<float *>(ws + p.at_z), f.z_ld = up(v->vocab, 32);
+            f.rows = (int)rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.softcap = softcap;
+            auto kernel = few_of<true>(v->type, q.blocks, rows, cap);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)q.segments, few_blocks(rows)), dim3(256), 0, stream, f);
+            // (dW's product reads whole stages of rows)
+            hipLaunchKernelGGL((p.split ? vocab_z_dz_kernel<true> : vocab_z_dz_kernel<false>), dim3((unsigned)up(rows, Tile::BK)), dim3(256),
+                               0, stream, a, f.z, f.z_ld, loss);
+        } else if (!given) {
             auto kernel = p.split ? (cap ? vocab_loss_kernel<Tile, true, true, false> : vocab_loss_kernel<Tile, true, false, false>)
                           : store ? (cap ? vocab_loss_kernel<Tile, false, true, true> : vocab_loss_kernel<Tile, false, false, true>)
                                   : (cap ? vocab_loss_kernel<Tile, false, true, false> : vocab_loss_kernel<Tile, false, false, false>);
@@ -998,7 +1097,7 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
             else hipLaunchKernelGGL(vocab_lse_kernel, dim3((unsigned)(a.piece / 4)), dim3(256), 0, stream, a, loss, lse);
         }
         if (!grad) continue;
-        if (given || !store) {
+        if (!few && (given || !store)) {
             auto kernel = p.split ? (cap ? vocab_dz_kernel<Tile, true, true> : vocab_dz_kernel<Tile, true, false>)
                                   : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
@@ -1038,7 +1137,7 @@ extern "C" int64_t noise_vocab_workspace_bytes(const noise_vocab_t *v, int with_
     clear_error();
     if (check("noise_vocab_workspace_bytes", v, 0.f)) return -1;
     if (v->rows == 0) return 0;
-    return !with_grad && v->rows <= kFewRows ? few_plan(v).bytes : plan_of(v, with_grad != 0).bytes;
+    return !with_grad && few_rows(v, false) ? few_plan(v).bytes : plan_of(v, with_grad != 0).bytes;
 }
 
 extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace,
@@ -1048,7 +1147,7 @@ extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *lo
     if (int e = check(fn, v, softcap)) return e;
     if (v->rows == 0) return NOISE_OK;
     NOISE_CHECK_ARG(loss && aligned(loss, 4) && aligned(lse, 4), "%s: loss NULL or not 4 B aligned", fn);
-    if (v->rows <= kFewRows) return run_few(fn, v, softcap, loss, lse, workspace, workspace_bytes, (hipStream_t)stream);
+    if (few_rows(v, false)) return run_few(fn, v, softcap, loss, lse, workspace, workspace_bytes, (hipStream_t)stream);
     return run(fn, v, softcap, nullptr, loss, lse, nullptr, nullptr, nullptr, 0, false, workspace, workspace_bytes, (hipStream_t)stream);
 }
 

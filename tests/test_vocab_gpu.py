@@ -125,8 +125,8 @@ def test_rows(R, dtype):
 @pytest.mark.parametrize('dtype', [BF16, F32])
 @pytest.mark.parametrize('V', [17, 32767, 32768, 40001])
 def test_few_rows(V, dtype):
-    """The losses of up to 64 tokens, which have a kernel of their own, next to those of more."""
-    for R, D in ((1, 1), (4, 130), (16, 128), (17, 7), (31, 257), (33, 96), (64, 1000), (65, 64)):
+    """Up to 256 tokens may have kernels of their own, by the sizes: next to those of more."""
+    for R, D in ((1, 1), (4, 130), (16, 128), (17, 7), (31, 257), (33, 96), (64, 1000), (65, 64), (129, 2000), (200, 776), (256, 64), (257, 72)):
         check(*make(R, V, D, dtype, R, V + R % 3, masked=R % 2 == 1), V, 15.0 if R % 4 == 0 else None)
 
 
@@ -140,10 +140,8 @@ def test_masks(dtype):
     b = check(x, weight, targets.clamp(-2 ** 31, 2 ** 31 - 1).int(), w, 500, 15.0)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     assert not a[0][~used].any() and not a[1][~used].any()
-    # the rows in use alone give the same (dweight up to the order of its sum over tokens, which goes by how many there are)
-    c = check(x[used], weight, targets[used], w[used], 500, 15.0)
-    assert torch.equal(c[0], a[0][used])
-    assert torch.equal(c[1], a[1][used])
+    # (how sums are cut, and which kernels form the logits, goes by the number of rows: the rows in use alone need not give the same bits)
+    check(x[used], weight, targets[used], w[used], 500, 15.0)
     for keep in (0, 1):
         t = torch.full_like(targets, -100)
         t[200:200 + keep] = 7
