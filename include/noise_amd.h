@@ -757,8 +757,9 @@ int noise_residual_norm_bwd(const noise_residual_t *r, const void *dout, const v
  *   z = cap(x weight^T),  cap(z) = softcap tanh(z / softcap) (softcap 0: z; else 1e-6 .. 1e6),
  *   loss_r = lse_r - z[t_r],  lse_r = log sum_{v < vocab} exp z[v].
  * A row with any other target has loss 0 and no gradient, and may hold anything. x and weight are of `type` (bf16, or fp32, whose
- * products keep 21 bits of each operand), with row strides in elements; rows 0 .. 2^30, dim 1 .. 65536, vocab 1 .. 2^22. targets: int32,
- * or int64 with targets_wide. workspace: noise_vocab_workspace_bytes (16 B aligned; -1 for arguments that would be refused). */
+ * products keep 21 bits of each operand, and of each tensor 2^-38 of its largest value), with row strides in elements (0 or more);
+ * rows 0 .. 2^30, dim 1 .. 65536, vocab 1 .. 2^22. targets: int32, or int64 with targets_wide. workspace:
+ * noise_vocab_workspace_bytes (16 B aligned; -1 for arguments that would be refused). */
 typedef struct {
     const void *x;
     int64_t x_stride;

@@ -63,9 +63,20 @@ __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
     return n < 0 ? 0 : n < a.piece ? n : a.piece;
 }
 
-// softcap tanh(z / softcap) with an error of 2^-22 softcap: what enters exp(z) is absolute
+// softcap tanh(z / softcap), k = 2 log2(e) / softcap, with an error of 2^-22 softcap: what enters exp(z) is absolute. Past kWideCap, where
+// that would be more than 2^-17, WIDE: below 0.35 of the cap tanh's odd series up to the 11th power (the next term is 1.2e-8 of the value
+// there), which leaves an error relative to the logit.
+constexpr float kWideCap = 32.f;
+template <bool WIDE>
 __device__ __forceinline__ float cap_of(float z, float cap, float k) {
-    return cap - 2.f * cap * __builtin_amdgcn_rcpf(exp2_fast(z * k) + 1.f);
+    const float far = cap - 2.f * cap * __builtin_amdgcn_rcpf(exp2_fast(z * k) + 1.f);
+    if constexpr (!WIDE) return far;
+    const float u = z * (k * 0.34657359f), u2 = u * u;   // (z / cap: log(2) / 2)
+    float s = __builtin_fmaf(u2, -1382.f / 155925.f, 62.f / 2835.f);
+    s = __builtin_fmaf(u2, s, -17.f / 315.f);
+    s = __builtin_fmaf(u2, s, 2.f / 15.f);
+    s = __builtin_fmaf(u2, s, -1.f / 3.f);
+    return u2 < 0.1225f ? __builtin_fmaf(z * u2, s, z) : far;
 }
 
 // --- rows with a target, packed ---
@@ -310,8 +321,8 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(PackArgs a) {
 // --- logits ---
 
 // The tile's logits, unscaled and capped. Past the vocabulary: -inf, or under the cap (where they are multiplied by cap') a value whose
-// exponential vanishes beside any other's.
-template <class T, bool SPLIT, bool CAP>
+// exponential vanishes beside any other's. CAP: 0 none, 2 past kWideCap.
+template <class T, bool SPLIT, int CAP>
 __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f32x16 (&acc)[T::FB][T::NB]) {
     const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f, k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
 #pragma unroll
@@ -321,7 +332,7 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float z = SPLIT ? acc[i][j][r] * unit : acc[i][j][r];
-                if (CAP) z = cap_of(z, a.softcap, k);
+                if (CAP) z = cap_of<CAP == 2>(z, a.softcap, k);
                 acc[i][j][r] = z;
             }
     if (m0 + T::FB * 32 > a.vocab) {
@@ -338,7 +349,7 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
 
 // STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_dz_kernel turns into dZ. (Its rounding, 2^-11,
 // comes before dZ's own, 2^-8; below 2^-29 of the segment's largest it has fewer bits, below 2^-39 none.)
-template <class T, bool SPLIT, bool CAP, bool STORE>
+template <class T, bool SPLIT, int CAP, bool STORE>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
     const int64_t rows = piece_rows(a);
@@ -600,7 +611,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 z[e] = sums[0][wave][r][lane][e] + sums[1][wave][r][lane][e] + sums[2][wave][r][lane][e] + sums[3][wave][r][lane][e];
-                if (CAP) z[e] = cap_of(z[e], a.softcap, k);
+                if (CAP) z[e] = cap_of<true>(z[e], a.softcap, k);
                 if (v + e >= a.vocab) z[e] = -__builtin_inff();
                 top = fmaxf(top, z[e]);
             }
@@ -723,7 +734,7 @@ __global__ __launch_bounds__(256) void vocab_fill_kernel(uint16_t *p, int64_t n)
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
-template <class T, bool SPLIT, bool CAP>
+template <class T, bool SPLIT, int CAP>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
     const int64_t rows = piece_rows(a);
@@ -940,6 +951,19 @@ bool few_rows(const noise_vocab_t *v, bool grad) {
     return few < tiles;
 }
 
+template <bool SPLIT, bool STORE>
+void (*loss_of(float softcap))(HeadArgs) {
+    return softcap > kWideCap ? vocab_loss_kernel<Tile, SPLIT, 2, STORE>
+           : softcap > 0.f    ? vocab_loss_kernel<Tile, SPLIT, 1, STORE>
+                              : vocab_loss_kernel<Tile, SPLIT, 0, STORE>;
+}
+template <bool SPLIT>
+void (*dz_of(float softcap))(HeadArgs) {
+    return softcap > kWideCap ? vocab_dz_kernel<Tile, SPLIT, 2>
+           : softcap > 0.f    ? vocab_dz_kernel<Tile, SPLIT, 1>
+                              : vocab_dz_kernel<Tile, SPLIT, 0>;
+}
+
 struct FewPlan {
     int blocks;   // of 16 entries per workgroup
     int64_t segments, bytes;
@@ -1005,6 +1029,7 @@ int check(const char *fn, const noise_vocab_t *v, float softcap) {
                     "%s: rows 0 .. 2^30, dim 1 .. 65536 and vocab 1 .. 2^22 required", fn);
     NOISE_CHECK_ARG(softcap == 0.f || (softcap >= 1e-6f && softcap <= 1e6f), "%s: softcap must be 1e-6 .. 1e6, or 0 for none", fn);
     if (v->rows == 0) return NOISE_OK;
+    NOISE_CHECK_ARG(v->x_stride >= 0 && v->weight_stride >= 0, "%s: strides must be 0 or more", fn);
     const size_t size = v->type == NOISE_BF16 ? 2 : 4;
     NOISE_CHECK_ARG(v->x && v->weight && v->targets && aligned(v->x, size) && aligned(v->weight, size) &&
                         aligned(v->targets, v->targets_wide ? 8 : 4),
@@ -1089,17 +1114,14 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
             hipLaunchKernelGGL((p.split ? vocab_z_dz_kernel<true> : vocab_z_dz_kernel<false>), dim3((unsigned)up(rows, Tile::BK)), dim3(256),
                                0, stream, a, f.z, f.z_ld, loss);
         } else if (!given) {
-            auto kernel = p.split ? (cap ? vocab_loss_kernel<Tile, true, true, false> : vocab_loss_kernel<Tile, true, false, false>)
-                          : store ? (cap ? vocab_loss_kernel<Tile, false, true, true> : vocab_loss_kernel<Tile, false, false, true>)
-                                  : (cap ? vocab_loss_kernel<Tile, false, true, false> : vocab_loss_kernel<Tile, false, false, false>);
+            auto kernel = p.split ? loss_of<true, false>(softcap) : store ? loss_of<false, true>(softcap) : loss_of<false, false>(softcap);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
             if (store) hipLaunchKernelGGL(vocab_lse_dz_kernel, dim3((unsigned)a.piece), dim3(256), 0, stream, a, loss);
             else hipLaunchKernelGGL(vocab_lse_kernel, dim3((unsigned)(a.piece / 4)), dim3(256), 0, stream, a, loss, lse);
         }
         if (!grad) continue;
         if (!few && (given || !store)) {
-            auto kernel = p.split ? (cap ? vocab_dz_kernel<Tile, true, true> : vocab_dz_kernel<Tile, true, false>)
-                                  : (cap ? vocab_dz_kernel<Tile, false, true> : vocab_dz_kernel<Tile, false, false>);
+            auto kernel = p.split ? dz_of<true>(softcap) : dz_of<false>(softcap);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
         }
         GradArgs g = {};

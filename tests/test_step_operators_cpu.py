@@ -280,6 +280,17 @@ def test_vocab_entry_points_refuse():
         assert 0 < need <= operands + 2 ** 31 + 2 ** 29 + 4 * V * (dim + 64) + 8 * 2 ** 31 // 256 + 2 ** 22
 
 
+def test_vocab_entry_points_refuse_negative_strides():
+    lib = _lib.lib()
+    for change in (dict(xs=-24), dict(ws=-24)):
+        table = array('q', {**dict(x=4096, xs=24, w=4096, ws=24, t=4096, wide=1, rows=4, dim=24, vocab=30, type=1), **change}.values())
+        at = table.buffer_info()[0]
+        assert lib.noise_vocab_loss(at, 0.0, 16, None, 16, 1 << 40, None) == -1
+        assert 'stride' in lib.noise_last_error().decode()
+        assert lib.noise_vocab_grad(at, 0.0, None, None, 16, 16, 16, 30, 16, 1 << 40, None) == -1
+        assert lib.noise_vocab_workspace_bytes(at, 1) == -1
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     """The tables of 64-bit words that the Python layer packs have the C structs' sizes and orders."""
     fields = {'noise_gradient_t': 'ptr numel type', 'noise_residual_grads_t': 'dx dy dx0 dscale dx0_scale dgate dy_weight dweight',

@@ -3,7 +3,7 @@
 Bounds, with F = 2^-24, N = |x| |W|^T (the sizes of a logit's terms) and A the largest |z| of a row plus log V:
   a logit: products are exact in fp32 for bf16 operands and are added in at most dim / 16 + 24 steps; fp32 operands, held as two fp16
     values, miss 2^-21 of a term and 2^-38 of the tensors' largest values, and take three times the steps; the soft cap adds 2^-21 of
-    itself: ez
+    itself, or past 32 of thrice the logit where that is less: ez
   a loss: two logits, and the maximum, the sum's (V / 128 + 40 steps) and the logarithm's roundings: 2 max ez + F (80 + V / 128 + 8 A)
   dZ = weight (p - 1[t]) cap': p is off by its exponent's error, ez + the loss's, cap' by 4 cap's; then dZ is rounded to bf16 (2^-8) or to
     two fp16 values (2^-21, and 2^-38 of the largest weight): ed
@@ -57,7 +57,7 @@ def bounds(x, weight, targets, w, V, cap, loss, dx, dw):
     if cap:
         z = cap * torch.tanh(raw / cap)
         slope = 1 - (z / cap) ** 2
-        ez = ez * slope + 2.0 ** -21 * cap + ez ** 2 / cap
+        ez = ez * slope + 2.0 ** -21 * (torch.clamp(3 * z.abs(), max=cap) if cap > 32 else cap) + ez ** 2 / cap
         eslope = 4 * ez / cap
     A = z.abs().amax(-1) + math.log(V) + 1
     eloss = 2 * ez.amax(-1) + F * (80 + V / 128 + 8 * A)
@@ -128,6 +128,14 @@ def test_few_rows(V, dtype):
     """Up to 256 tokens may have kernels of their own, by the sizes: next to those of more."""
     for R, D in ((1, 1), (4, 130), (16, 128), (17, 7), (31, 257), (33, 96), (64, 1000), (65, 64), (129, 2000), (200, 776), (256, 64), (257, 72)):
         check(*make(R, V, D, dtype, R, V + R % 3, masked=R % 2 == 1), V, 15.0 if R % 4 == 0 else None)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('cap', [1e-6, 0.01, 1.0, 32.0, 33.0, 100.0, 1e3, 1e6])
+def test_caps(cap, dtype):
+    """Of the whole range, for few rows and for many: far above the logits they leave these as they are."""
+    for R in (9, 300):
+        check(*make(R, 700, 128, dtype, R, masked=R == 300), 700, cap)
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
