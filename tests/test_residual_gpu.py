@@ -224,6 +224,32 @@ def test_no_rows():
         assert d.shape == v.shape and not d.any()
 
 
+def test_past_32_bits():
+    """More than 2^31 elements: a row's results are those of a call of its own; the weight's gradient is off by its sums, of at most
+    rows / 2048 rows in a lane (512 workgroups of 4 teams) and 64 more steps, and its terms' own 256 F (1 + K)."""
+    from noise_amd.residual import residual_norm
+    R, D = 2 ** 22 + 1001, 512
+    t, up = make((R, D), BF16, BF16, 3, ('x', 'y', 'scale', 'weight'))
+    leaves = {n: v.requires_grad_() for n, v in t.items()}
+    outs = residual_norm(**leaves, norm_y=True)
+    grads = torch.autograd.grad(outs, list(leaves.values()), up)
+    sums, sizes = torch.zeros(D, device=DEV, dtype=torch.float64), torch.zeros(D, device=DEV, dtype=torch.float64)
+    for rows in torch.arange(R, device=DEV).tensor_split(16):
+        a, b = int(rows[0]), int(rows[-1]) + 1
+        own = {n: (v.detach()[a:b] if v.dim() == 2 else v.detach()).requires_grad_() for n, v in leaves.items()}
+        part = residual_norm(**own, norm_y=True)
+        assert torch.equal(outs[0][a:b], part[0]) and torch.equal(outs[1][a:b], part[1])
+        dx, dy = torch.autograd.grad(part, (own['x'], own['y']), (up[0][a:b], up[1][a:b]))
+        assert torch.equal(grads[0][a:b], dx) and torch.equal(grads[1][a:b], dy)
+        exact, _ = oracle.residual(own['x'].double(), own['y'].double(), scale=own['scale'].double(), norm_y=True, eps=EPS)
+        terms = oracle.rms_norm(exact, eps=EPS) * up[1][a:b].double()
+        sums += terms.sum(0).detach()
+        sizes += terms.abs().sum(0).detach()
+        del part, own, exact, terms
+    # K: the parts of x' do not cancel to less than a tenth of their sizes
+    assert ((grads[3] - sums).abs() <= F * (R / 2048 + 64 + 256 * 11) * sizes).all()
+
+
 def test_other_types_of_weights_and_dtype():
     """Weights and scalars in bf16 are taken at their value, their gradients come in their type; h in bf16 without y."""
     from noise_amd.residual import residual_norm

@@ -206,6 +206,57 @@ def test_pieces(dtype):
     assert norm <= (2 * HALF[BF16] if dtype == BF16 else 2.0 ** -18), norm
 
 
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_weight_past_32_bits(dtype):
+    """A weight of more than 2^31 elements, zero but for some rows at its ends and in its middle. z: F (steps as above) and 2^-21 of
+    |x| |W|^T, from which p and so a gradient's terms are off by that of themselves."""
+    from noise_amd.vocab import linear_cross_entropy_grad
+    V, D = 33000, 65536
+    at = torch.cat([torch.tensor([0, 1, 16384, 32768]), torch.arange(V - 60, V)]).to(DEV)
+    g = torch.Generator(DEV).manual_seed(11)
+    some = (torch.randn(len(at), D, device=DEV, generator=g) / 256).to(dtype)
+    weight = torch.zeros(V, D, device=DEV, dtype=dtype)
+    weight[at] = some
+    some = some.double()
+    for R in (20, 300):
+        x = torch.randn(R, D, device=DEV, generator=g).to(dtype)
+        which, w = torch.randint(len(at), (R,), device=DEV, generator=g), torch.rand(R, device=DEV, generator=g)
+        loss, dx, dw = linear_cross_entropy_grad(x, weight, at[which], w)
+        z = x.double() @ some.t()
+        lse = torch.log(z.exp().sum(-1) + V - len(at))
+        ez = (F * ((3 if dtype == F32 else 1) * D / 16 + 24) + 2.0 ** -21) * (x.double().abs() @ some.abs().t()).max()
+        want = lse - z.gather(1, which[:, None])[:, 0]
+        assert ((loss - want).abs() <= 2 * ez + F * (80 + V / 128 + 200)).all()
+        p = (z - lse[:, None]).exp()
+        p[torch.arange(R, device=DEV), which] -= 1
+        p *= w.double()[:, None]
+        tol = 2 * ez + 2 * (HALF[BF16] if dtype == BF16 else 2.0 ** -18)
+        for name, a, b in (('dx', dx, p @ some), ('dweight', dw[at], p.t() @ x.double()),
+                           ('elsewhere', dw[[2, 20000, 32769, V - 61]], ((w * (-lse).exp())[None] @ x.double()).expand(4, D))):
+            assert (a - b).norm() <= tol * b.norm(), (name, (a - b).norm() / b.norm(), tol)
+        del loss, dx, dw
+
+
+def test_rows_past_32_bits():
+    """More than 2^31 elements of x: the last tokens' results are those of a call of their own, dW the calls' sum."""
+    from noise_amd.vocab import linear_cross_entropy_grad
+    R, V, D, N = 2 ** 20 + 4321, 200, 2048, 8
+    g = torch.Generator(DEV).manual_seed(12)
+    x = torch.randn(R, D, device=DEV, generator=g, dtype=BF16)
+    weight = (torch.randn(V, D, device=DEV, generator=g) / 32).to(BF16)
+    targets, w = torch.randint(V, (R,), device=DEV, generator=g), torch.rand(R, device=DEV, generator=g) / R
+    loss, dx, dw = linear_cross_entropy_grad(x, weight, targets, w)
+    total = torch.zeros(V, D, device=DEV, dtype=torch.float64)
+    for rows in torch.arange(R, device=DEV).tensor_split(N):
+        a, b = int(rows[0]), int(rows[-1]) + 1
+        part = linear_cross_entropy_grad(x[a:b], weight, targets[a:b], w[a:b])
+        # (the same products in the same order, but for dx where its k may be cut)
+        assert torch.equal(loss[a:b], part[0])
+        assert (dx[a:b].float() - part[1].float()).norm() <= HALF[BF16] * part[1].float().norm()
+        total += part[2].double()
+    assert (dw - total).norm() <= 2 * HALF[BF16] * total.norm()
+
+
 def test_values():
     """Logits far apart, certain and hopeless predictions, soft-capped ones past the cap; infinite and NaN rows stay theirs."""
     from noise_amd.vocab import linear_cross_entropy, linear_cross_entropy_grad
