@@ -3,15 +3,26 @@
 //   loss_r = lse_r - z_{r,t_r},  dZ_rv = w_r (exp(z_rv - lse_r) - [v = t_r]) cap'(z_rv),  dx = dZ W,  dW = dZ^T x,
 // cap(z) = softcap tanh(z / softcap), cap' = 1 - (cap / softcap)^2. (The head is utils/model.py:204-206 and train/val/run.py:89-94.)
 //
-// Rows without a target take no part: the others are packed one after the other (which also zeroes what stands between them and
-// the end of a tile), and all counts of rows are read on the device. Rows are worked on in pieces, so that dZ never takes more
-// than kPieceBytes. Per piece, four products of R V D multiply-adds (two for the loss alone):
-//   loss_kernel     a tile of logits in registers, its rows' maxima and sums of exponentials left per 128 vocabulary entries;
-//                   lse_join_kernel adds those up
-//   dz_kernel       the logits once more, and dZ from them in 16 bits
-//   dx_kernel, dw_kernel  the gradients; k is split over workgroups where there are few tiles, with fp32 sums joined in order
+// Rows without a target take no part: live_kernel numbers the others and pack_kernel packs them one after the other (and zeroes what
+// stands between them and the end of a tile); all counts of rows are read on the device. Rows are worked on in pieces, so that dZ
+// takes at most kPieceBytes (but no fewer than kPad rows). Per piece:
+//   loss_kernel    a tile of logits in registers, its rows' maxima and sums of exponentials left per 128 vocabulary entries, which
+//                  lse_kernel adds up. Where bf16 gradients are asked for in the same call, the exponentials stay as well, and
+//                  lse_dz_kernel makes dZ of them: a pass over 2 R V bytes instead of another product
+//   dz_kernel      otherwise: the logits once more, and dZ from them, in 16 bits or two times 16
+//   grad_kernel    dx and dW in one launch, k split over workgroups where there are few tiles; sum_kernel joins the splits' fp32 sums
 // fp32 operands are held as sums of two fp16 values, scaled by a power of two per tensor (hi carries 11 bits of a value, lo the next
-// 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term.
+// 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term, and 2^-38 of the tensors' largest values.
+// For few rows few_kernel forms the logits (few_rows says when), and z_dz_kernel makes dZ of them.
+//
+// Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2 PFLOP/s),
+// on an x of zeros 2.96; a plain large product on this card reaches 1.35. Alone on the GPU, in us:
+//                                  live   pack   loss   lse or lse_dz   dz    grad   sum
+//   16384 x 4096 x 512 bf16, cap     9     10    119         53          -     144     9    (in one call)
+//   8192 x 131072 x 2048 bf16       10     15   4075        955          -    7496     -    (in one call)
+//   16384 x 4096 x 512 fp32          9     19    221          7         260    376    11    (through autograd; largest values 14)
+//   3333 x 50021 x 776 bf16, 2/3     5     30    193          6         224    482     9    (through autograd, packed in both calls)
+// At widths like 512, 8 stages of k, a tile's epilogue shows: two exponentials, a reciprocal and some 12 other operations per capped logit.
 #include "vocab_gemm.hpp"
 
 #include <type_traits>
@@ -216,7 +227,7 @@ __device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
 // run in one launch. Of no shares, and shares of one, a half and a third of what all stages take on 256 CUs, those that come out best
 // by what was measured: a workgroup takes 2.2 us per stage (3.3 where operands are sums of two) and 3 us more, 256 run at a time, and
 // joining costs 5 us and 0.09 us of the whole chip's time per tile's share. At most kSplitTiles shares of tiles, at least 4 stages each. (At
-// 16384 x 4096 x 512 dx then has 1 share and dW 4, and both take 154 us with the join; in two launches, with 2 and 8, it was 195.)
+// 16384 x 4096 x 512 dx then has 1 share and dW 4, and both take 153 us with the join; in two launches, with 2 and 8, it was 195.)
 constexpr uint32_t kSplitTiles = 512;
 template <class T, bool SPLIT>
 __device__ uint2 shares_of(int64_t rows, int64_t vocab, uint32_t tiles_m, bool dx, bool dw) {
@@ -473,7 +484,7 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, float *loss,
     if (lse) lse[to] = l;
 }
 
-// A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left:
+// A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left, at the rate of a copy (134 MB read and written in 53 us):
 // dZ_v = weight exp(top - lse) 2^-15 stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
 __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *loss) {
     __shared__ float2 slots[4];
@@ -512,6 +523,8 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
 // each, straight from memory into v_mfma_f32_16x16x32_bf16's (fp32: v_mfma_f32_16x16x4_f32's, exact products) operands: 16 lanes on
 // 16 rows of the weight, and the rows of x from the caches. The waves' sums meet in LDS; wave v takes entries 16 v on from there.
 //
+// Bound by HBM: 4 rows of 65536 x 2048 in bf16, 268 MB, take 53 us (5.1 TB/s) with 8 loads of 16 B per lane and block under way; loads
+// that bypass the caches were slower.
 // With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel.
 struct FewArgs {
     const void *x, *w, *targets;
@@ -878,7 +891,8 @@ __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, u
     }
 }
 
-// Both gradients in one launch: neither waits for the other's last workgroups
+// Both gradients in one launch: neither waits for the other's last workgroups (16384 x 4096 x 512: 144 us, 0.95 PFLOP/s; 8192 x 131072 x
+// 2048: 7.5 ms, 1.17)
 template <class T, bool SPLIT>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a, GradArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
