@@ -712,7 +712,7 @@ int noise_distill(const void *x, int type, int64_t rows, int64_t vocab, int64_t 
  *   factor = min(1, max_norm / (norm + 1e-6)),  g <- factor g in place, rounded once (not written where the factor is 1).
  * max_norm infinite: the norm alone. A norm that is NaN makes every gradient NaN; an infinite one makes the finite ones 0 and
  * the infinite ones NaN. The table is read on the host, before the call returns; gradients that share memory are refused.
- * workspace: noise_clip_workspace_bytes(count) bytes, 8 B aligned. */
+ * count is 1 .. 2^24. workspace: noise_clip_workspace_bytes(count) bytes (negative: invalid), 8 B aligned. */
 typedef struct {
     void *ptr;      /* contiguous elements, aligned to their type */
     int64_t numel;  /* 0: left out */
@@ -741,7 +741,8 @@ int noise_residual_norm(const noise_residual_t *r, void *out, void *h, float eps
 /* Its gradients from dout and dh (contiguous; NULL: zeros), each optional (NULL), contiguous and of its tensor's type: dx, dy,
  * dx0 as the tensors, dscale, dx0_scale, dy_weight, dweight in fp32 and dgate in gate_type, summed over rows in fp32 (the two
  * scalars in fp64) in a fixed order. With rows 0 nothing is written. workspace (not needed for dx, dy, dx0 and the gradient of
- * a gate with gate_rows 1 alone): noise_residual_norm_bwd_workspace_bytes, 16 B aligned; gate_rows: rows without a gate. */
+ * a gate with gate_rows 1 alone): noise_residual_norm_bwd_workspace_bytes (negative: invalid), 16 B aligned; gate_rows: rows
+ * without a gate. */
 typedef struct {
     void *dx, *dy, *dx0;
     float *dscale, *dx0_scale;
@@ -759,7 +760,7 @@ int noise_residual_norm_bwd(const noise_residual_t *r, const void *dout, const v
  * A row with any other target has loss 0 and no gradient, and may hold anything. x and weight are of `type` (bf16, or fp32, whose
  * products keep 21 bits of each operand, and of each tensor 2^-38 of its largest value), with row strides in elements (0 or more);
  * rows 0 .. 2^30, dim 1 .. 65536, vocab 1 .. 2^22. targets: int32, or int64 with targets_wide. workspace:
- * noise_vocab_workspace_bytes (16 B aligned; -1 for arguments that would be refused). */
+ * noise_vocab_workspace_bytes (negative: invalid), 16 B aligned. */
 typedef struct {
     const void *x;
     int64_t x_stride;

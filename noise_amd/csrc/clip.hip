@@ -197,14 +197,16 @@ int64_t units_of(const noise_gradient_t &g) { return g.numel == 0 ? 0 : (bytes_o
 using namespace noise;
 
 extern "C" int64_t noise_clip_workspace_bytes(int64_t count) {
-    return count < 0 ? 0 : 8 * (int64_t)(kGroups + count / kTensors + 1);
+    clear_error();
+    NOISE_CHECK_ARG(count > 0 && count <= (1 << 24), "noise_clip_workspace_bytes: 1 .. 2^24 gradients required, got %lld", (long long)count);
+    return 8 * (int64_t)(kGroups + count / kTensors + 1);
 }
 
 extern "C" int noise_clip_gradients(const noise_gradient_t *gradients, int64_t count, float max_norm, float *norm,
                                     void *workspace, int64_t workspace_bytes, noise_stream_t stream) {
     clear_error();
     const char *fn = "noise_clip_gradients";
-    NOISE_CHECK_ARG(count >= 0 && count <= (1 << 24) && (gradients || count == 0), "%s: bad table of gradients", fn);
+    NOISE_CHECK_ARG(gradients && count > 0 && count <= (1 << 24), "%s: bad table of gradients", fn);
     NOISE_CHECK_ARG(max_norm >= 0.f, "%s: max_norm must not be negative", fn);
     NOISE_CHECK_ARG(norm && aligned(norm, 4), "%s: norm NULL or not 4 B aligned", fn);
     NOISE_CHECK_ARG(workspace && aligned(workspace, 8) && workspace_bytes >= noise_clip_workspace_bytes(count),

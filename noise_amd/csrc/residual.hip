@@ -548,7 +548,9 @@ extern "C" int noise_residual_norm(const noise_residual_t *r, void *out, void *h
 }
 
 extern "C" int64_t noise_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t gate_rows, int64_t dim) {
-    if (rows <= 0 || gate_rows <= 0 || dim <= 0 || dim > kMaxDim) return 0;
+    clear_error();
+    NOISE_CHECK_ARG(rows > 0 && rows <= INT64_MAX / 8 / kMaxDim && gate_rows > 0 && rows % gate_rows == 0 && dim > 0 && dim <= kMaxDim,
+                    "noise_residual_norm_bwd_workspace_bytes: rows a multiple of gate_rows and dim 1 .. %d required", kMaxDim);
     const Cut c = cut_of(rows, gate_rows, dim);
     return c.parts * (2 * 4 * dim + 16) + c.gates * c.parts_per_gate * 4 * dim;
 }

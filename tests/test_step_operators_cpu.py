@@ -291,6 +291,17 @@ def test_vocab_entry_points_refuse_negative_strides():
         assert lib.noise_vocab_workspace_bytes(at, 1) == -1
 
 
+def test_workspace_queries_refuse():
+    lib = _lib.lib()
+    for query, bad in ((lib.noise_clip_workspace_bytes, ((0,), (-1,), (2 ** 24 + 1,))),
+                       (lib.noise_residual_norm_bwd_workspace_bytes, ((0, 1, 8), (4, 0, 8), (4, 3, 8), (4, 4, 0), (4, 4, 8193), (-4, 4, 8))),
+                       (lib.noise_vocab_workspace_bytes, ((None, 1),))):
+        for args in bad:
+            assert query(*args) == -1 and lib.noise_last_error(), (query, args)
+    good = gradients((4096, 10, 1))
+    assert lib.noise_clip_gradients(good.buffer_info()[0], 0, 1.0, 16, 16, 1 << 20, None) == -1
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     """The tables of 64-bit words that the Python layer packs have the C structs' sizes and orders."""
     fields = {'noise_gradient_t': 'ptr numel type', 'noise_residual_grads_t': 'dx dy dx0 dscale dx0_scale dgate dy_weight dweight',
