@@ -37,6 +37,7 @@ constexpr int kSegment = 128;                // vocabulary entries per partial m
 constexpr int kPad = 256;                    // rows of the packed matrices and of dZ come in these
 
 using Tile = Tiling<256, 256, 2, 4, 64, 2>;
+using HalfTile = Tiling<128, 256, 2, 4, 64, 2>;
 
 // What the kernels share. Row indices are those of the packed rows.
 struct HeadArgs {
@@ -846,39 +847,32 @@ __device__ __forceinline__ Cut cut_of(const HeadArgs &a, const GradArgs &g, int6
     return c;
 }
 
-// n: packed rows (DX) or vocabulary entries; m: columns of dim
+// A tile from column m0 and row or entry n0 on, over the stages first .. last - 1 of k
 template <class T, bool DX, bool SPLIT>
-__device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, uint32_t group, char *lds) {
+__device__ __forceinline__ void gradient_tile(const HeadArgs &a, const GradArgs &g, const Cut &c, uint32_t split, int m0, int64_t n0, int first,
+                                              int last, char *lds) {
     const Result &res = DX ? g.dx : g.dw;
-    const int64_t rows = piece_rows(a);
-    const Cut c = cut_of<T, DX, SPLIT>(a, g, rows);
-    if (group >= c.tiles * c.splits) return;
-    const uint32_t split = group / c.tiles;
-    int tm, tn;
-    tile_of(group - split * c.tiles, g.tiles_m, c.tiles_n, tm, tn);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int first = (int)((int64_t)c.stages * split / c.splits), last = (int)((int64_t)c.stages * (split + 1) / c.splits);
     const int dim8 = (int)a.x.ld / 8;   // chunks of a packed row
     f32x16 acc[T::FB][T::NB];
     if (DX)
-        product<T, true, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
-                                              T::NT - 1, first, last, a.vocab, lds, acc);
+        product<T, true, false, SPLIT, SPLIT>(a.w, m0, dim8 - m0 / 8 - 1, a.dz, n0, T::NT - 1, first, last, a.vocab, lds, acc);
     else {
         Operand x = a.x;
         x.ptr += a.row0 * x.ld;
-        product<T, true, true, SPLIT, SPLIT>(x, (int64_t)tm * T::MT, dim8 - tm * (T::MT / 8) - 1, a.dz, (int64_t)tn * T::NT,
-                                             (int)(a.dz.ld - (int64_t)tn * T::NT) / 8 - 1, first, last, 1ll << 40, lds, acc);
+        product<T, true, true, SPLIT, SPLIT>(x, m0, dim8 - m0 / 8 - 1, a.dz, n0, (int)(a.dz.ld - n0) / 8 - 1, first, last, 1ll << 40, lds,
+                                             acc);
     }
     const float unit = SPLIT ? 1.f / a.scales[2] / a.scales[DX ? 1 : 0] : 1.f;
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
-        const int64_t n = (int64_t)tn * T::NT + T::wn(wave) + 32 * j + (lane & 31);
+        const int64_t n = n0 + T::wn(wave) + 32 * j + (lane & 31);
         if (n >= c.n_end) continue;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int m = tm * T::MT + T::wm(wave) + 32 * i + 16 * h + 8 * (lane >> 5);
+                const int m = m0 + T::wm(wave) + 32 * i + 16 * h + 8 * (lane >> 5);
                 if (m >= a.dim) continue;
                 float v[8];
 #pragma unroll
@@ -889,6 +883,22 @@ __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, u
                     finish<DX>(a, g, n, m, v);
             }
     }
+}
+
+// n: packed rows (DX) or vocabulary entries; m: columns of dim. What is left of dim in the last tile takes half a tile where that is enough.
+template <class T, bool DX, bool SPLIT>
+__device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, uint32_t group, char *lds) {
+    const Cut c = cut_of<T, DX, SPLIT>(a, g, piece_rows(a));
+    if (group >= c.tiles * c.splits) return;
+    const uint32_t split = group / c.tiles;
+    int tm, tn;
+    tile_of(group - split * c.tiles, g.tiles_m, c.tiles_n, tm, tn);
+    const int first = (int)((int64_t)c.stages * split / c.splits), last = (int)((int64_t)c.stages * (split + 1) / c.splits);
+    static_assert(HalfTile::NT == T::NT && HalfTile::BK == T::BK && HalfTile::kLds <= T::kLds, "the same stages and columns of tiles");
+    if (a.dim - tm * T::MT <= HalfTile::MT)
+        gradient_tile<HalfTile, DX, SPLIT>(a, g, c, split, tm * T::MT, (int64_t)tn * T::NT, first, last, lds);
+    else
+        gradient_tile<T, DX, SPLIT>(a, g, c, split, tm * T::MT, (int64_t)tn * T::NT, first, last, lds);
 }
 
 // Both gradients in one launch: neither waits for the other's last workgroups (16384 x 4096 x 512: 144 us, 0.95 PFLOP/s; 8192 x 131072 x
