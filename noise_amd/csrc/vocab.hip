@@ -13,6 +13,8 @@
 //   grad_kernel    dx and dW in one launch, k split over workgroups where there are few tiles; sum_kernel joins the splits' fp32 sums
 // fp32 operands are held as sums of two fp16 values, scaled by a power of two per tensor (hi carries 11 bits of a value, lo the next
 // 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term, and 2^-38 of the tensors' largest values.
+// A bf16 weight is read where it is if its rows are whole 16 B: what its last stage of k lacks comes from the zeros behind a row of x
+// (losses of 300 rows of 131072 x 1000: 243 -> 153 us).
 // For few rows few_kernel forms the logits (few_rows says when), and z_dz_kernel makes dZ of them.
 //
 // Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2 PFLOP/s),
@@ -52,6 +54,7 @@ struct HeadArgs {
     int64_t row0;                // the piece's first packed row
     int64_t piece;               // rows of the piece, at most
     int vocab, dim, nk, segments;  // nk: stages of k over dim
+    int64_t w_k;                 // columns that w has in memory, if fewer than the stages (x's are zeros from dim on)
     int tiles_m;
     float softcap;
 };
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
-                                           T::NT - 1, 0, a.nk, 1ll << 40, lds, acc);
+                                           T::NT - 1, 0, a.nk, a.w_k, a.x.ptr + a.dim, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
     if (m0 >= a.vocab) return;
     to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
@@ -759,7 +762,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x16 acc[T::FB][T::NB];
     product<T, false, false, SPLIT, SPLIT>(a.w, (int64_t)tm * T::MT, a.vocab - 1 - tm * T::MT, a.x, a.row0 + (int64_t)tn * T::NT,
-                                           T::NT - 1, 0, a.nk, 1ll << 40, lds, acc);
+                                           T::NT - 1, 0, a.nk, a.w_k, a.x.ptr + a.dim, lds, acc);
     const int m0 = tm * T::MT + T::wm(wave);
     to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
     uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr));
@@ -853,15 +856,15 @@ __device__ __forceinline__ void gradient_tile(const HeadArgs &a, const GradArgs 
                                               int last, char *lds) {
     const Result &res = DX ? g.dx : g.dw;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int dim8 = (int)a.x.ld / 8;   // chunks of a packed row
+    const int dim8 = (a.dim + 7) / 8;   // chunks of a row
     f32x16 acc[T::FB][T::NB];
     if (DX)
-        product<T, true, false, SPLIT, SPLIT>(a.w, m0, dim8 - m0 / 8 - 1, a.dz, n0, T::NT - 1, first, last, a.vocab, lds, acc);
+        product<T, true, false, SPLIT, SPLIT>(a.w, m0, dim8 - m0 / 8 - 1, a.dz, n0, T::NT - 1, first, last, a.vocab, nullptr, lds, acc);
     else {
         Operand x = a.x;
         x.ptr += a.row0 * x.ld;
-        product<T, true, true, SPLIT, SPLIT>(x, m0, dim8 - m0 / 8 - 1, a.dz, n0, (int)(a.dz.ld - n0) / 8 - 1, first, last, 1ll << 40, lds,
-                                             acc);
+        product<T, true, true, SPLIT, SPLIT>(x, m0, dim8 - m0 / 8 - 1, a.dz, n0, (int)(a.dz.ld - n0) / 8 - 1, first, last, 1ll << 40,
+                                             nullptr, lds, acc);
     }
     const float unit = SPLIT ? 1.f / a.scales[2] / a.scales[DX ? 1 : 0] : 1.f;
 #pragma unroll
@@ -1018,8 +1021,8 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     p.pieces = (p.rows + p.piece - 1) / p.piece;
     p.piece = up((p.rows + p.pieces - 1) / p.pieces, kPad);
     p.pieces = (p.rows + p.piece - 1) / p.piece;
-    // the weight is read where it is if its rows are whole stages of k at 16 B addresses
-    p.pack_w = p.split || v->dim % Tile::BK || v->weight_stride % 8 || !aligned(v->weight, 16) || v->weight_stride >= (1 << 23);
+    // the weight is read where it is if its rows are whole 16 B at 16 B addresses
+    p.pack_w = p.split || v->dim % 8 || v->weight_stride % 8 || !aligned(v->weight, 16) || v->weight_stride >= (1 << 23);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -1113,6 +1116,7 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     a.weight = weight ? packed_weight : nullptr;
     a.lse = packed_lse, a.zt = zt, a.partial = reinterpret_cast<float2 *>(ws + p.at_partial);
     a.segments = (int)p.segments, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
+    a.w_k = p.pack_w ? p.ld : v->dim;
     if (dw && width > v->vocab) {
         const int64_t n = (width - v->vocab) * v->dim * (p.split ? 2 : 1);
         hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,

@@ -36,6 +36,16 @@ __device__ __forceinline__ f32x16 mfma16bit(bf16x8 a, bf16x8 b, f32x16 c) {
     }
 }
 
+// As lds_dma16_at, with an address of its own for each lane
+__device__ __forceinline__ void lds_dma16_from(uint64_t at, unsigned la) {
+    const unsigned l = (unsigned)__builtin_amdgcn_readfirstlane((int)la);
+    unsigned save;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save)
+                 : "v"(at), "s"(l)
+                 : "memory");
+}
+
 // One operand's tile of ROWS x BK in LDS and its copies by NW waves
 template <int ROWS, int BK, int NW, bool CROSSED>
 struct Side {
@@ -51,7 +61,7 @@ struct Side {
 
     uint64_t base;       // of the tile's first element
     unsigned off[N];     // this lane's byte offset of each copy
-    int row, chunk;      // crossed: this lane's row of the first copy and its chunk
+    int row, chunk;      // this lane's row of the first copy and its chunk
     int64_t ld;
 
     // last: the last row that exists (plain), or the last chunk of 8 columns (crossed), from the tile's first
@@ -67,8 +77,9 @@ struct Side {
             off[i] = (unsigned)((CROSSED || r < last ? r : last) * (uint32_t)ld * 2 + chunk * 16);
         }
     }
-    // k: the stage's first; left: how many k from there on have rows in memory (crossed)
-    __device__ __forceinline__ void copy(int64_t k, int64_t lo, int left, unsigned to, int wave) const {
+    // k: the stage's first; left: how many k from there on are in memory. Crossed: rows past them repeat the last one (the other operand
+    // is zero there). Plain: chunks past them are read from `zeros`.
+    __device__ __forceinline__ void copy(int64_t k, int64_t lo, int left, const void *zeros, unsigned to, int wave) const {
         const __bf16 *p = reinterpret_cast<const __bf16 *>(base) + lo + (CROSSED ? k * ld : k);
         to += wave * 1024;
         if (CROSSED && left < BK) {
@@ -77,6 +88,11 @@ struct Side {
                 const int r = row + i * NW * RPC;
                 lds_dma16_at(p, (unsigned)((r < left ? r : left - 1) * (uint32_t)ld * 2 + chunk * 16), to + i * NW * 1024);
             }
+            return;
+        }
+        if (!CROSSED && left < BK) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds_dma16_from(8 * chunk < left ? (uint64_t)p + off[i] : (uint64_t)zeros, to + i * NW * 1024);
             return;
         }
 #pragma unroll
@@ -129,10 +145,10 @@ template <class T, bool SPLIT>
 constexpr int kStep = SPLIT ? T::BK / 2 : T::BK;
 
 // acc = the product over the stages first .. last - 1 of k. With SPLIT, operands are sums of two, multiplied hi hi + hi lo + lo hi
-// from one reading of each. k_rows: how many k a crossed A has rows for. Ends with a barrier.
+// from one reading of each. a_k: how many k A has in memory (plain: whole chunks of 8). Ends with a barrier.
 template <class T, bool CA, bool CB, bool F16, bool SPLIT>
 __device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last, const Operand &b, int64_t b0, int b_last, int first,
-                                        int last, int64_t k_rows, char *lds, f32x16 (&acc)[T::FB][T::NB]) {
+                                        int last, int64_t a_k, const void *zeros, char *lds, f32x16 (&acc)[T::FB][T::NB]) {
     constexpr int BK = kStep<T, SPLIT>, NS = T::NS, SPK = BK / 16, P = SPLIT ? 2 : 1;
     using SA = Side<T::MT, BK, T::NW, CA>;
     using SB = Side<T::NT, BK, T::NW, CB>;
@@ -159,8 +175,8 @@ __device__ __forceinline__ void product(const Operand &a, int64_t a0, int a_last
         const int64_t k = (int64_t)(first + p) * BK;
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-            sa.copy(k, q ? a.lo : 0, k_rows - k < BK ? (int)(k_rows - k) : BK, st + q * SA::kBytes, wave);
-            sb.copy(k, q ? b.lo : 0, BK, st + P * SA::kBytes + q * SB::kBytes, wave);
+            sa.copy(k, q ? a.lo : 0, a_k - k < BK ? (int)(a_k - k) : BK, zeros, st + q * SA::kBytes, wave);
+            sb.copy(k, q ? b.lo : 0, BK, nullptr, st + P * SA::kBytes + q * SB::kBytes, wave);
         }
     };
     bf16x8 va[2][P][T::FB], vb[2][P][T::NB];

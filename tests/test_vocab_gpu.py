@@ -279,6 +279,24 @@ def test_values():
     check(x * 1e12, weight * 1e-12, targets, w * 1e-20, 400)
 
 
+@pytest.mark.parametrize('D', [8, 40, 72, 200, 776])
+def test_what_stands_beside_the_weight(D):
+    """Rows that end inside a stage, with NaN between them and behind the last; a logit of -inf leaves its token's loss finite."""
+    from noise_amd.vocab import linear_cross_entropy, linear_cross_entropy_grad
+    for R in (30, 300):
+        x, weight, targets, w = make(R, 500, D, BF16, D)
+        wide = torch.full((500, D + 16), float('nan'), device=DEV, dtype=BF16)
+        wide[:, :D] = weight
+        base = check(x, weight, targets, w, 500)
+        for a, b in zip(base, linear_cross_entropy_grad(x, wide[:, :D], targets, w)):
+            assert torch.equal(a, b)
+        x, targets = x.abs() + 1, targets % 499
+        weight[499, D - 1] = -float('inf')
+        loss = linear_cross_entropy(x, weight, targets)
+        weight[499] = -1e4
+        assert torch.isfinite(loss).all() and torch.equal(loss, linear_cross_entropy(x, weight, targets))
+
+
 def test_repetition_and_streams():
     """The same bits every time and on another stream."""
     from noise_amd.vocab import linear_cross_entropy_grad
