@@ -15,7 +15,8 @@
 // 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term, and 2^-38 of the tensors' largest values.
 // A bf16 weight is read where it is if its rows are whole 16 B: what its last stage of k lacks comes from the zeros behind a row of x
 // (losses of 300 rows of 131072 x 1000: 243 -> 153 us).
-// For few rows few_kernel forms the logits (few_rows says when), and z_dz_kernel makes dZ of them.
+// For few rows few_kernel forms the logits (few_rows says when), and z_dz_kernel makes dZ of them; up to 64 rows have gradients of their own
+// too (few_grad_rows).
 //
 // Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2 PFLOP/s),
 // on an x of zeros 2.96; a plain large product on this card reaches 1.35. Alone on the GPU, in us:
@@ -25,6 +26,7 @@
 //   16384 x 4096 x 512 fp32          9     19    221          7         260    376    11    (through autograd; largest values 14)
 //   3333 x 50021 x 776 bf16, 2/3     5     30    193          6         224    482     9    (through autograd, packed in both calls)
 // At widths like 512, 8 stages of k, a tile's epilogue shows: two exponentials, a reciprocal and some 12 other operations per capped logit.
+#include "vocab_few.hpp"
 #include "vocab_gemm.hpp"
 
 #include <type_traits>
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
 //
 // Bound by HBM: 4 rows of 65536 x 2048 in bf16, 268 MB, take 53 us (5.1 TB/s) with 8 loads of 16 B per lane and block under way; loads
 // that bypass the caches were slower.
-// With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel.
+// With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel or vocab_few_dz_kernel (and partial may be NULL).
 struct FewArgs {
     const void *x, *w, *targets;
     int64_t x_ld, w_ld;
@@ -635,7 +637,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
             if constexpr (WRITE) {
                 // (rows of the logits are whole 16 entries)
                 if (row < a.rows) __builtin_memcpy(__builtin_assume_aligned(a.z + row * a.z_ld + v, 16), z, 16);
-                continue;
+                if (!a.partial) continue;
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -653,7 +655,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(FewArgs a) {
             }
         }
     }
-    if constexpr (WRITE) return;
+    if (WRITE && !a.partial) return;
     __syncthreads();
     for (int row = threadIdx.x; row < 16 * RB; row += 256) {
         if (r0 + row >= a.rows) continue;
@@ -680,6 +682,34 @@ __global__ __launch_bounds__(256) void vocab_few_join_kernel(FewArgs a, float *l
     const float l = top + logf(s);
     loss[row] = in ? l - a.zt[row] : 0.f;
     if (lse) lse[row] = in ? l : 0.f;
+}
+
+// dZ of up to 64 rows from their logits and lse: by rows (dz, which may be z's place) and by entries (dzt). A thread takes an entry of N rows;
+// zeros where there is no row, target or entry.
+template <class E>
+__global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const float *lse, const float *weight, E *dz, E *dzt, int dz_rows, int kp) {
+    constexpr int N = 16 / sizeof(E);
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int r0 = blockIdx.y * N;
+    if (v >= a.z_ld) return;
+    E o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int r = r0 + e;
+        float d = 0.f;
+        if (r < a.rows && v < a.vocab) {
+            const int64_t t = a.wide ? static_cast<const int64_t *>(a.targets)[r] : (int64_t)static_cast<const int32_t *>(a.targets)[r];
+            if (t >= 0 && t < a.vocab) {
+                const float z = a.z[r * a.z_ld + v], w = weight ? weight[r] : 1.f, u = a.softcap > 0.f ? z / a.softcap : 0.f;
+                d = exp2_fast((z - lse[r]) * kLog2e);
+                if (v == t) d -= 1.f;
+                d *= w * (1.f - u * u);
+            }
+        }
+        o[e] = (E)d;
+        if (r < dz_rows) dz[r * a.z_ld + v] = o[e];
+    }
+    __builtin_memcpy(__builtin_assume_aligned(dzt + v * kp + r0, 16), o, 16);
 }
 
 // lse and loss of a packed row from its logits, and dZ; zeros in the rows behind the last
@@ -991,6 +1021,11 @@ void (*dz_of(float softcap))(HeadArgs) {
                               : vocab_dz_kernel<Tile, SPLIT, 0>;
 }
 
+// Gradients of rows this few have kernels of their own (vocab_few.hpp), whose columns come in 16 B. Tiles waste 192 of 256 rows or more, store
+// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 406, 433 and 557 us against
+// 667, 692 and 660; fp32: 761, 816 and 1367 against 1665, 1717 and 1939; 4096 x 512 bf16: 18, 21 and 29 against 40, 40 and 44.
+bool few_grad_rows(const noise_vocab_t *v) { return v->rows <= 64 && v->dim >= 8; }
+
 struct FewPlan {
     int blocks;   // of 16 entries per workgroup
     int64_t segments, bytes;
@@ -1001,6 +1036,44 @@ FewPlan few_plan(const noise_vocab_t *v) {
     p.blocks = v->vocab >= 32 * 512 ? 2 : 1;
     p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
     p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
+    return p;
+}
+
+// The gradients of up to 64 rows: where their workspace's parts are, behind the losses' (few_plan)
+struct FewGradPlan {
+    int64_t z_ld, at_lse, at_z, at_dz, at_dzt, at_slabs, bytes;
+    int rb, kb, kp, dz_rows;   // blocks of 16 rows (dx) and of 4 N rows (dW), rows in those
+    int columns, dx_per, dx_splits, dw_per, dw_chunks;
+};
+FewGradPlan few_grad_plan(const noise_vocab_t *v) {
+    FewGradPlan p;
+    const int size = v->type == NOISE_FP32 ? 4 : 2, n = 16 / size;
+    p.z_ld = up(v->vocab, 32);
+    p.rb = v->rows <= 16 ? 1 : v->rows <= 32 ? 2 : 4;
+    p.dz_rows = 16 * p.rb;
+    p.kb = size == 4 ? p.rb : p.rb == 4 ? 2 : 1;
+    p.kp = p.kb * 4 * n;
+    p.columns = (int)((v->dim + 16 * n - 1) / (16 * n));
+    // workgroups: two per CU for dx, whose sums are then joined, and eight for dW, whose waves hold x
+    auto cut = [&](int64_t groups, int64_t step, int *per) {
+        const int64_t want = groups / p.columns > 1 ? groups / p.columns : 1;
+        *per = (int)up((p.z_ld + want - 1) / want, step);
+        return (int)((p.z_ld + *per - 1) / *per);
+    };
+    p.dx_splits = cut(512, 128, &p.dx_per);
+    p.dw_chunks = cut(2048, 64, &p.dw_per);
+    int64_t at = up(few_plan(v).bytes, 1024);
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += up(bytes, 1024);
+        return here;
+    };
+    p.at_lse = take(4 * kFewRows);
+    p.at_z = take(4 * p.dz_rows * p.z_ld);
+    p.at_dz = size == 4 ? p.at_z : take(size * p.dz_rows * p.z_ld);
+    p.at_dzt = take(size * p.z_ld * p.kp);
+    p.at_slabs = take(16ll * 64 * n * p.rb * p.columns * p.dx_splits);
+    p.bytes = at;
     return p;
 }
 
@@ -1081,6 +1154,64 @@ int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, 
     return launch_status(fn);
 }
 
+template <class E>
+void few_grad_kernels(const FewGradPlan &p, const FewArgs &f, const FewGradArgs &g, const float *lse, const float *weight, hipStream_t stream) {
+    constexpr int N = 16 / sizeof(E);
+    E *dz = static_cast<E *>(const_cast<void *>(g.dz)), *dzt = static_cast<E *>(const_cast<void *>(g.dzt));
+    hipLaunchKernelGGL(vocab_few_dz_kernel<E>, dim3((unsigned)((p.z_ld + 255) / 256), p.kp / N), dim3(256), 0, stream, f, lse, weight, dz, dzt,
+                       p.dz_rows, p.kp);
+    if (g.dx) {
+        FewGradArgs d = g;
+        d.per = p.dx_per;
+        auto kernel = p.rb == 1 ? vocab_few_dx_kernel<E, 1> : p.rb == 2 ? vocab_few_dx_kernel<E, 2> : vocab_few_dx_kernel<E, 4>;
+        auto join = p.rb == 1   ? vocab_few_dx_join_kernel<E, 1>
+                    : p.rb == 2 ? vocab_few_dx_join_kernel<E, 2>
+                                : vocab_few_dx_join_kernel<E, 4>;
+        hipLaunchKernelGGL(kernel, dim3(p.dx_splits, p.columns), dim3(256), 0, stream, d);
+        hipLaunchKernelGGL(join, dim3((p.columns * N * p.rb * 64 + 255) / 256), dim3(256), 0, stream, d);
+    }
+    if (g.dw) {
+        FewGradArgs d = g;
+        d.per = p.dw_per;
+        auto kernel = p.kb == 1 ? vocab_few_dw_kernel<E, 1> : p.kb == 2 ? vocab_few_dw_kernel<E, 2> : vocab_few_dw_kernel<E, 4>;
+        hipLaunchKernelGGL(kernel, dim3(p.dw_chunks, p.columns), dim3(256), 0, stream, d);
+    }
+}
+
+void fill_behind(const noise_vocab_t *v, void *dw, int64_t width, hipStream_t stream) {
+    if (!dw || width <= v->vocab) return;
+    const int64_t halves = v->type == NOISE_FP32 ? 2 : 1, n = (width - v->vocab) * v->dim * halves;
+    hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,
+                       static_cast<uint16_t *>(dw) + v->vocab * v->dim * halves, n);
+}
+
+int run_few_grad(const char *fn, const noise_vocab_t *v, float softcap, const float *weight, float *loss, const float *given, void *dx,
+                 void *dw, int64_t width, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    const FewPlan q = few_plan(v);
+    const FewGradPlan p = few_grad_plan(v);
+    NOISE_CHECK_ARG(workspace && aligned(workspace, 16) && workspace_bytes >= p.bytes,
+                    "%s: workspace of %lld bytes (16 B aligned) required", fn, (long long)p.bytes);
+    char *ws = static_cast<char *>(workspace);
+    FewArgs f = {};
+    f.x = v->x, f.w = v->weight, f.targets = v->targets, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
+    f.zt = reinterpret_cast<float *>(ws);
+    f.partial = given ? nullptr : reinterpret_cast<float2 *>(f.zt + kFewRows);
+    f.rows = (int)v->rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.segments = (int)q.segments, f.wide = (int)v->targets_wide;
+    f.softcap = softcap, f.z = reinterpret_cast<float *>(ws + p.at_z), f.z_ld = p.z_ld;
+    float *lse = reinterpret_cast<float *>(ws + p.at_lse);
+    auto kernel = few_of<true>(v->type, q.blocks, v->rows, softcap > 0.f);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)q.segments, few_blocks(v->rows)), dim3(256), 0, stream, f);
+    if (!given) hipLaunchKernelGGL(vocab_few_join_kernel, dim3((unsigned)v->rows), dim3(256), 0, stream, f, loss, lse);
+    FewGradArgs g = {};
+    g.x = v->x, g.w = v->weight, g.targets = v->targets, g.x_ld = v->x_stride, g.w_ld = v->weight_stride;
+    g.dz = ws + p.at_dz, g.dzt = ws + p.at_dzt, g.slabs = reinterpret_cast<float *>(ws + p.at_slabs), g.dx = dx, g.dw = dw;
+    g.z_ld = p.z_ld, g.rows = f.rows, g.vocab = f.vocab, g.dim = f.dim, g.wide = f.wide, g.blocks = p.columns, g.splits = p.dx_splits;
+    if (v->type == NOISE_FP32) few_grad_kernels<float>(p, f, g, given ? given : lse, weight, stream);
+    else few_grad_kernels<__bf16>(p, f, g, given ? given : lse, weight, stream);
+    fill_behind(v, dw, width, stream);
+    return launch_status(fn);
+}
+
 // loss and lse (out, or with `given` lse in); dx and dw where grad
 int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weight, float *loss, float *lse, const float *given,
         void *dx, void *dw, int64_t width, bool grad, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
@@ -1117,11 +1248,7 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
     a.lse = packed_lse, a.zt = zt, a.partial = reinterpret_cast<float2 *>(ws + p.at_partial);
     a.segments = (int)p.segments, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.nk = p.nk, a.softcap = softcap;
     a.w_k = p.pack_w ? p.ld : v->dim;
-    if (dw && width > v->vocab) {
-        const int64_t n = (width - v->vocab) * v->dim * (p.split ? 2 : 1);
-        hipLaunchKernelGGL(vocab_fill_kernel, dim3(n < 256 * 1024 ? (unsigned)((n + 255) / 256) : 1024), dim3(256), 0, stream,
-                           static_cast<uint16_t *>(dw) + v->vocab * v->dim * (p.split ? 2 : 1), n);
-    }
+    fill_behind(v, dw, width, stream);
     const int threads = 64 * Tile::NW;
     const bool cap = softcap > 0.f;
     for (int64_t i = 0; i < p.pieces; ++i) {
@@ -1187,7 +1314,8 @@ extern "C" int64_t noise_vocab_workspace_bytes(const noise_vocab_t *v, int with_
     clear_error();
     if (check("noise_vocab_workspace_bytes", v, 0.f)) return -1;
     if (v->rows == 0) return 0;
-    return !with_grad && few_rows(v, false) ? few_plan(v).bytes : plan_of(v, with_grad != 0).bytes;
+    if (with_grad) return few_grad_rows(v) ? few_grad_plan(v).bytes : plan_of(v, true).bytes;
+    return few_rows(v, false) ? few_plan(v).bytes : plan_of(v, false).bytes;
 }
 
 extern "C" int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *lse, void *workspace,
@@ -1212,5 +1340,7 @@ extern "C" int noise_vocab_grad(const noise_vocab_t *v, float softcap, const flo
                     "%s: a pointer is not aligned to its type", fn);
     NOISE_CHECK_ARG(!dweight || (width >= v->vocab && width <= (1 << 30)), "%s: dweight needs vocab <= width", fn);
     if (v->rows == 0) return NOISE_OK;
+    if (few_grad_rows(v))
+        return run_few_grad(fn, v, softcap, weight, loss, lse, dx, dweight, width, workspace, workspace_bytes, (hipStream_t)stream);
     return run(fn, v, softcap, weight, loss, nullptr, lse, dx, dweight, width, true, workspace, workspace_bytes, (hipStream_t)stream);
 }
