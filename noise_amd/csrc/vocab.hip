@@ -1022,8 +1022,8 @@ void (*dz_of(float softcap))(HeadArgs) {
 }
 
 // Gradients of rows this few have kernels of their own (vocab_few.hpp), whose columns come in 16 B. Tiles waste 192 of 256 rows or more, store
-// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 406, 433 and 557 us against
-// 667, 692 and 660; fp32: 761, 816 and 1367 against 1665, 1717 and 1939; 4096 x 512 bf16: 18, 21 and 29 against 40, 40 and 44.
+// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 316, 351 and 506 us against
+// 667, 692 and 660; fp32: 639, 701 and 1323 against 1665, 1717 and 1939; 4096 x 512 bf16: 19, 21 and 30 against 40, 40 and 44.
 bool few_grad_rows(const noise_vocab_t *v) { return v->rows <= 64 && v->dim >= 8; }
 
 struct FewPlan {
@@ -1043,7 +1043,7 @@ FewPlan few_plan(const noise_vocab_t *v) {
 struct FewGradPlan {
     int64_t z_ld, at_lse, at_z, at_dz, at_dzt, at_slabs, bytes;
     int rb, kb, kp, dz_rows;   // blocks of 16 rows (dx) and of 4 N rows (dW), rows in those
-    int columns, dx_per, dx_splits, dw_per, dw_chunks;
+    int columns, dx_per, dx_splits, dw_per, dw_chunks, across;
 };
 FewGradPlan few_grad_plan(const noise_vocab_t *v) {
     FewGradPlan p;
@@ -1054,14 +1054,16 @@ FewGradPlan few_grad_plan(const noise_vocab_t *v) {
     p.kb = size == 4 ? p.rb : p.rb == 4 ? 2 : 1;
     p.kp = p.kb * 4 * n;
     p.columns = (int)((v->dim + 16 * n - 1) / (16 * n));
-    // workgroups: two per CU for dx, whose sums are then joined, and eight for dW, whose waves hold x
-    auto cut = [&](int64_t groups, int64_t step, int *per) {
-        const int64_t want = groups / p.columns > 1 ? groups / p.columns : 1;
+    // workgroups: two per CU for dx, whose sums are then joined, and four for dW, whose waves hold x (half as many or
+    // twice as many: up to 10 % more)
+    auto cut = [&](int64_t groups, int64_t columns, int64_t step, int *per) {
+        const int64_t want = groups / columns > 1 ? groups / columns : 1;
         *per = (int)up((p.z_ld + want - 1) / want, step);
         return (int)((p.z_ld + *per - 1) / *per);
     };
-    p.dx_splits = cut(512, 128, &p.dx_per);
-    p.dw_chunks = cut(2048, 64, &p.dw_per);
+    p.dx_splits = cut(512, p.columns, 128, &p.dx_per);
+    p.across = p.columns % 4 == 0 || p.columns >= 12;
+    p.dw_chunks = cut(1024, p.across ? (p.columns + 3) / 4 : p.columns, p.across ? 16 : 64, &p.dw_per);
     int64_t at = up(few_plan(v).bytes, 1024);
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -1172,9 +1174,10 @@ void few_grad_kernels(const FewGradPlan &p, const FewArgs &f, const FewGradArgs 
     }
     if (g.dw) {
         FewGradArgs d = g;
-        d.per = p.dw_per;
+        d.per = p.dw_per, d.across = p.across;
+        d.stream = d.dim * sizeof(E) % 128 == 0 && aligned(d.dw, 16) && (int64_t)d.vocab * d.dim * (int64_t)sizeof(E) > 1 << 28;
         auto kernel = p.kb == 1 ? vocab_few_dw_kernel<E, 1> : p.kb == 2 ? vocab_few_dw_kernel<E, 2> : vocab_few_dw_kernel<E, 4>;
-        hipLaunchKernelGGL(kernel, dim3(p.dw_chunks, p.columns), dim3(256), 0, stream, d);
+        hipLaunchKernelGGL(kernel, dim3(p.dw_chunks, p.across ? (p.columns + 3) / 4 : p.columns), dim3(256), 0, stream, d);
     }
 }
 

@@ -2,8 +2,8 @@
 // dW is written once, straight from and to memory, through v_mfma_f32_16x16x32_bf16 or, exact products, v_mfma_f32_16x16x4_f32.
 // A lane holds N consecutive columns (16 B) of a matrix's rows; product e of N takes the e-th of each lane's columns, so that rows are
 // read and written in runs of 256 B. Every row of dZ takes part, with zeros in those without a target, whose x is taken as zeros too.
-// Bound by HBM: at 131072 x 2048 and 4 rows in bf16, dx takes 96 us (5.6 TB/s of weight read) and dW 180 (3.0 TB/s written), in fp32 223
-// and 297.
+// Bound by HBM: at 131072 x 2048 and 4 rows in bf16, dx takes 96 us (5.6 TB/s of weight read) and dW 105 to 113 (5 TB/s written), in fp32
+// 219 and 205.
 #pragma once
 #include "vocab_gemm.hpp"
 
@@ -21,6 +21,7 @@ struct FewGradArgs {
     void *dx, *dw;
     int64_t z_ld;
     int rows, vocab, dim, wide, blocks, splits, per;   // blocks: of 16 N columns; per: entries of a workgroup
+    int across, stream;    // dW: a workgroup's waves take 4 blocks of columns (else entries in turn); stores that pass the caches by
 };
 
 __device__ __forceinline__ bool has_target(const void *targets, int wide, int64_t vocab, int r) {
@@ -143,14 +144,17 @@ __global__ __launch_bounds__(256) void vocab_few_dx_join_kernel(FewGradArgs a) {
     }
 }
 
-// dW: the product's rows are entries, its columns columns. The operands of x stay in registers; the workgroup's entries go to its waves
-// in turn, 16 at a time.
+// dW: the product's rows are entries, its columns columns. The operands of x stay in registers; the workgroup's waves take four blocks of
+// columns, so that 1 KB of a row is written at a time, or where there are too few blocks its entries in turn, 16 at a time. Rows of whole 128 B
+// of a dW larger than the caches are stored past them. (131072 x 2048 bf16: 180 us without either, 147 with the latter.)
 template <class E, int KB>
 __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
     constexpr int N = FewOperand<E>::N, KP = KB * 4 * N;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int c = column_of<N>(blockIdx.y, i, a.dim);
-    const bool mine = (int)blockIdx.y * 16 * N + N * i < a.dim;
+    const int block = a.across ? 4 * blockIdx.y + wave : blockIdx.y;
+    const int c = column_of<N>(block, i, a.dim);
+    const bool mine = block * 16 * N + N * i < a.dim;
+    if (block >= a.blocks) return;
     FewOperand<E> op[KB];
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
         op[b].set(rows);
     }
     const int begin = blockIdx.x * a.per, end = (int)(begin + a.per < a.z_ld ? begin + a.per : a.z_ld);
-    for (int v0 = begin + 16 * wave; v0 < end; v0 += 64) {
+    for (int v0 = begin + (a.across ? 0 : 16 * wave); v0 < end; v0 += a.across ? 16 : 64) {
         const E *dz = static_cast<const E *>(a.dzt) + (int64_t)(v0 + i) * KP + N * g;
         u32x4 z[KB];
 #pragma unroll
@@ -181,7 +185,15 @@ __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
 #pragma unroll
             for (int e = 0; e < N; ++e) o[e] = (E)acc[e][j];
             const int v = v0 + 4 * g + j;
-            if (mine && v < a.vocab) __builtin_memcpy(static_cast<E *>(a.dw) + (int64_t)v * a.dim + c, o, 16);
+            if (!mine || v >= a.vocab) continue;
+            E *to = static_cast<E *>(a.dw) + (int64_t)v * a.dim + c;
+            if (a.stream) {
+                u32x4 bits;
+                __builtin_memcpy(&bits, o, 16);
+                __builtin_nontemporal_store(bits, reinterpret_cast<u32x4 *>(to));
+            } else {
+                __builtin_memcpy(to, o, 16);
+            }
         }
     }
 }

@@ -131,6 +131,13 @@ def test_few_rows(V, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
+def test_few_rows_of_a_large_weight(dtype):
+    """Gradients past the caches' size, of rows of whole lines and of others."""
+    for D in (1024, 1032, 1001):
+        check(*make(20, 140000, D, dtype, D, 140003, masked=True), 140000, 15.0)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
 @pytest.mark.parametrize('cap', [1e-6, 0.01, 1.0, 32.0, 33.0, 100.0, 1e3, 1e6])
 def test_caps(cap, dtype):
     """Of the whole range, for few rows and for many: far above the logits they leave these as they are."""
