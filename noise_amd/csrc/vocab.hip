@@ -712,33 +712,20 @@ __global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const floa
     __builtin_memcpy(__builtin_assume_aligned(dzt + v * kp + r0, 16), o, 16);
 }
 
-// lse and loss of a packed row from its logits, and dZ; zeros in the rows behind the last
+// dZ of packed rows from their logits and lse, which are by row; zeros in the rows behind the last. blockIdx.y: a share of the entries
+constexpr int kDzEntries = 4096;
 template <bool SPLIT>
-__global__ __launch_bounds__(256) void vocab_z_dz_kernel(HeadArgs a, const float *logits, int64_t z_ld, float *loss) {
-    __shared__ float2 slots[4];
+__global__ __launch_bounds__(256) void vocab_z_dz_kernel(HeadArgs a, const float *logits, int64_t z_ld, const float *lse) {
     const int64_t at = blockIdx.x;
     const bool there = at < *a.count;
     const int row = there ? a.live[at] : 0, t = there ? a.target[at] : 0;
     const float *z = logits + row * z_ld;
-    float top = kLowest, s = 0.f;
-    if (there)
-        for (int c = 4 * threadIdx.x; c < a.vocab; c += 1024) {   // (-inf past the vocabulary)
-            float v[4];
-            __builtin_memcpy(v, __builtin_assume_aligned(z + c, 16), 16);
-            const float m = fmaxf(top, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-            s *= exp2_fast((top - m) * kLog2e);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s += exp2_fast((v[e] - m) * kLog2e);
-            top = m;
-        }
-    join_sums(top, s, slots);
-    const float l = top + logf(s), zt = z[t];
-    if (there && loss && threadIdx.x == 0) loss[row] = l - zt;
-    const float w = (a.weight ? a.weight[at] : 1.f) * (SPLIT ? a.scales[2] : 1.f);
+    const float l = lse[row], w = (a.weight ? a.weight[at] : 1.f) * (SPLIT ? a.scales[2] : 1.f);
     const bool cap = a.softcap > 0.f;
     const float bend = cap ? -w / a.softcap / a.softcap : 0.f;   // of w cap'
     uint16_t *dz = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld;
-    for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
+    const int begin = blockIdx.y * kDzEntries, end = begin + kDzEntries < (int)a.dz.ld ? begin + kDzEntries : (int)a.dz.ld;
+    for (int c = begin + 8 * threadIdx.x; c < end; c += 2048) {
         uint16_t hi[8] = {}, lo[8] = {};
         if (there && c < a.vocab) {
             float v[8];
@@ -977,7 +964,7 @@ struct Plan {
     int nk;
     bool split, pack_w, few;   // few: the logits of all rows are kept (at most 1 GiB)
     int64_t dx_groups, dw_groups, dx_slabs, dw_slabs;
-    int64_t at_int, at_float, at_cuts, at_z, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
+    int64_t at_int, at_float, at_cuts, at_z, at_few, at_partial, at_x, at_w, at_dz, at_dx, at_dw, at_sum, bytes;
 };
 
 // For any number of rows up to the piece's: the most workgroups of a gradient's product, and the fp32 values of its splits' sums.
@@ -1111,7 +1098,10 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
         p.few = few_rows(v, true);
-        if (p.few) p.at_z = take(4 * v->rows * up(v->vocab, 32));
+        if (p.few) {
+            p.at_z = take(4 * v->rows * up(v->vocab, 32));
+            p.at_few = take(up(few_plan(v).bytes, 16) + 4 * kFewRows);
+        }
         p.at_cuts = take(8 * p.pieces);
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
         most_of(true, p.piece, (v->vocab + step - 1) / step, p.ld, &p.dx_groups, &p.dx_slabs);
@@ -1263,14 +1253,20 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
         if (few) {
             const FewPlan q = few_plan(v);
             FewArgs f = {};
-            f.x = v->x, f.w = v->weight, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
+            f.x = v->x, f.w = v->weight, f.targets = v->targets, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
             f.z = reinterpret_cast<float *>(ws + p.at_z), f.z_ld = up(v->vocab, 32);
-            f.rows = (int)rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.softcap = softcap;
+            f.zt = reinterpret_cast<float *>(ws + p.at_few);
+            f.partial = given ? nullptr : reinterpret_cast<float2 *>(f.zt + kFewRows);
+            float *own = reinterpret_cast<float *>(ws + p.at_few + up(q.bytes, 16));
+            f.rows = (int)rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.segments = (int)q.segments, f.softcap = softcap;
+            f.wide = (int)v->targets_wide;
             auto kernel = few_of<true>(v->type, q.blocks, rows, cap);
             hipLaunchKernelGGL(kernel, dim3((unsigned)q.segments, few_blocks(rows)), dim3(256), 0, stream, f);
+            if (!given) hipLaunchKernelGGL(vocab_few_join_kernel, dim3((unsigned)rows), dim3(256), 0, stream, f, loss, own);
             // (dW's product reads whole stages of rows)
-            hipLaunchKernelGGL((p.split ? vocab_z_dz_kernel<true> : vocab_z_dz_kernel<false>), dim3((unsigned)up(rows, Tile::BK)), dim3(256),
-                               0, stream, a, f.z, f.z_ld, loss);
+            hipLaunchKernelGGL((p.split ? vocab_z_dz_kernel<true> : vocab_z_dz_kernel<false>),
+                               dim3((unsigned)up(rows, Tile::BK), (unsigned)((p.vocab_ld + kDzEntries - 1) / kDzEntries)), dim3(256), 0, stream, a,
+                               f.z, f.z_ld, given ? given : own);
         } else if (!given) {
             auto kernel = p.split ? loss_of<true, false>(softcap) : store ? loss_of<false, true>(softcap) : loss_of<false, false>(softcap);
             hipLaunchKernelGGL(kernel, tiles, dim3(threads), 0, stream, a);
