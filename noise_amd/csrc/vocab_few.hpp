@@ -140,7 +140,8 @@ __global__ __launch_bounds__(256) void vocab_few_dx_join_kernel(FewGradArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int q = 4 * (lane >> 4) + j;
-        if (block * 16 * N + N * q < a.dim) static_cast<E *>(a.dx)[(int64_t)r * a.dim + column_of<N>(block, q, a.dim) + e] = (E)(in ? v[j] : 0.f);
+        const int c = block * 16 * N + N * q, at = column_of<N>(block, q, a.dim) + e;
+        if (c < a.dim && at >= c) static_cast<E *>(a.dx)[(int64_t)r * a.dim + at] = (E)(in ? v[j] : 0.f);
     }
 }
 

@@ -348,6 +348,40 @@ def test_graph(dtype):
             assert torch.equal(a, b.detach())
 
 
+@pytest.mark.parametrize('R', [1, 40, 100])
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_few_rows_captured_and_repeated(dtype, R):
+    """The same bits every time, on another stream, and from two graphs replayed in turn on other tokens with other masks."""
+    from noise_amd.vocab import linear_cross_entropy, linear_cross_entropy_grad
+    V, D = 1500, 203
+    sets, graphs = [make(R, V, D, dtype, seed) for seed in (1, 2)], []
+
+    def step(x, weight, targets, w):
+        leaves = x.detach().requires_grad_(), weight.detach().requires_grad_()
+        loss = linear_cross_entropy(*leaves, targets, softcap=15.0)
+        return (loss.detach(), *torch.autograd.grad(loss, leaves, w), *linear_cross_entropy_grad(x, weight, targets, w, softcap=15.0))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    for s, o in zip(sets, other):
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(o, step(*s)))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(*s)
+        graphs.append((graph, outs))
+    for seed in range(3):
+        for s, (graph, outs) in zip(sets, graphs):
+            for a, b in zip(s, make(R, V, D, dtype, 30 + seed, masked=seed > 0)):
+                a.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip([o.clone() for o in outs], step(*s)):
+                assert torch.equal(a, b)
+
+
 def test_gradients_asked_for_one_by_one():
     from noise_amd.vocab import linear_cross_entropy
     x, weight, targets, w = make(300, 900, 128, BF16, 11)
@@ -356,6 +390,18 @@ def test_gradients_asked_for_one_by_one():
     for i in range(2):
         leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, weight))]
         assert torch.equal(torch.autograd.grad(linear_cross_entropy(*leaves, targets), leaves[i], w)[0], every[i])
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
+def test_few_gradients_asked_for_one_by_one(dtype):
+    from noise_amd.vocab import linear_cross_entropy
+    for R in (1, 33, 70):
+        x, weight, targets, w = make(R, 900, 127, dtype, 11, masked=R > 1)
+        both = [x.detach().requires_grad_(), weight.detach().requires_grad_()]
+        every = torch.autograd.grad(linear_cross_entropy(*both, targets), both, w)
+        for i in range(2):
+            leaves = [t.detach().requires_grad_(i == j) for j, t in enumerate((x, weight))]
+            assert torch.equal(torch.autograd.grad(linear_cross_entropy(*leaves, targets), leaves[i], w)[0], every[i])
 
 
 def test_differences():
