@@ -21,10 +21,10 @@
 // Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2 PFLOP/s),
 // on an x of zeros 2.96; a plain large product on this card reaches 1.35. Alone on the GPU, in us:
 //                                  live   pack   loss   lse or lse_dz   dz    grad   sum
-//   16384 x 4096 x 512 bf16, cap     9     10    119         53          -     144     9    (in one call)
-//   8192 x 131072 x 2048 bf16       10     15   4075        955          -    7496     -    (in one call)
-//   16384 x 4096 x 512 fp32          9     19    221          7         260    376    11    (through autograd; largest values 14)
-//   3333 x 50021 x 776 bf16, 2/3     5     30    193          6         224    482     9    (through autograd, packed in both calls)
+//   16384 x 4096 x 512 bf16, cap     9     10    120         54          -     144     9    (in one call)
+//   8192 x 131072 x 2048 bf16        8     15   4007        953          -    7405     -    (in one call)
+//   16384 x 4096 x 512 fp32          9     18    223          7         262    376    11    (through autograd; largest values 14)
+//   3333 x 50021 x 776 bf16, 2/3     6      7    207          5         230    483     9    (through autograd)
 // At widths like 512, 8 stages of k, a tile's epilogue shows: two exponentials, a reciprocal and some 12 other operations per capped logit.
 #include "vocab_few.hpp"
 #include "vocab_gemm.hpp"
@@ -689,10 +689,11 @@ __global__ __launch_bounds__(256) void vocab_few_join_kernel(FewArgs a, float *l
 template <class E>
 __global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const float *lse, const float *weight, E *dz, E *dzt, int dz_rows, int kp) {
     constexpr int N = 16 / sizeof(E);
+    const int parts = parts_of<E>(kp);
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int r0 = blockIdx.y * N;
     if (v >= a.z_ld) return;
-    E o[N];
+    E o[N], rest[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         const int r = r0 + e;
@@ -707,9 +708,14 @@ __global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const floa
             }
         }
         o[e] = (E)d;
-        if (r < dz_rows) dz[r * a.z_ld + v] = o[e];
+        rest[e] = (E)(d - (float)o[e]);
+        if (r < dz_rows) {
+            dz[r * a.z_ld + v] = o[e];
+            if (parts > 1) dz[(dz_rows + r) * a.z_ld + v] = rest[e];
+        }
     }
     __builtin_memcpy(__builtin_assume_aligned(dzt + v * kp + r0, 16), o, 16);
+    if (parts > 1) __builtin_memcpy(__builtin_assume_aligned(dzt + (a.z_ld + v) * kp + r0, 16), rest, 16);
 }
 
 // dZ of packed rows from their logits and lse, which are by row; zeros in the rows behind the last. blockIdx.y: a share of the entries
@@ -747,8 +753,6 @@ __global__ __launch_bounds__(256) void vocab_z_dz_kernel(HeadArgs a, const float
         if constexpr (SPLIT) __builtin_memcpy(__builtin_assume_aligned(dz + a.dz.lo + c, 16), lo, 16);
     }
 }
-
-constexpr int kFewRows = 256;
 
 template <class E, int VB, bool WRITE>
 void (*few_of(int64_t rows, bool cap))(FewArgs) {
@@ -922,7 +926,7 @@ __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, u
 }
 
 // Both gradients in one launch: neither waits for the other's last workgroups (16384 x 4096 x 512: 144 us, 0.95 PFLOP/s; 8192 x 131072 x
-// 2048: 7.5 ms, 1.17)
+// 2048: 7.4 ms, 1.19)
 template <class T, bool SPLIT>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a, GradArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
@@ -980,18 +984,23 @@ void most_of(bool rows, int64_t n_end, int64_t stages, int64_t ld, int64_t *grou
 }
 
 // Whether the logits come from vocab_few_kernel, whose every workgroup forms its own, or from the tiles of vocab_loss_kernel and
-// vocab_dz_kernel, which share operands but are few and long where there are few entries. By what was measured, in ns: the former read
-// 5 TB/s of weight for each 64 rows and then multiply at 268 TFLOP/s (fp32: 119); a tile takes 1.5 us per stage of 64 of dim when it
-// is one of the only 256 and 2.3 otherwise (twice that in fp32, whose gradients have two such passes in one call and whose losses alone need the
-// weight packed, 12 B read and written per value), and 15 us in all. 131072 x 2048 bf16, losses of 16, 32 and 64 rows: 132, 157 and
-// 233 us against 165; 4096 x 512: 6, 7 and 9 against 27; 131072 x 2048 fp32: 257, 322 and 478 against 970.
+// vocab_dz_kernel, which share operands but are few and long where there are few entries or rows. By what was measured, in ns: the former
+// read 5 TB/s of weight for each 64 rows and then multiply at 268 TFLOP/s (fp32: 119); a tile takes 1.5 us per stage of 64 of dim when it
+// is one of the only 256 and 2.3 otherwise (twice that in fp32, whose gradients have two such passes in one call and whose losses
+// alone need x and the weight packed, 12 B read and written per value), and 15 us in all. 131072 x 2048 bf16, losses of 16, 32 and 64
+// rows: 132, 157 and 233 us against 165; 4096 x 512: 6, 7 and 9 against 27; 131072 x 2048 fp32: 257, 322 and 478 against 970. Many rows
+// of few entries are alike: 793 x 119 x 4096, loss and gradients, bf16 67 us against 125, fp32 103 against 499; past some thousand rows
+// the tiles are as fast (4000 x 300 x 2048 bf16: 122 against 130).
 bool few_rows(const noise_vocab_t *v, bool grad) {
-    if (v->rows > kFewRows || (grad && v->rows * v->vocab > 1 << 28)) return false;
+    if (v->rows > 1 << 20 || v->rows * v->vocab > 1 << 28) return false;
     const double R = (double)v->rows, VD = (double)v->vocab * (double)v->dim, size = v->type == NOISE_FP32 ? 4 : 2;
-    const double few = VD * size * (double)((v->rows + 63) / 64) / 5e3 + 2 * R * VD / (size == 4 ? 119e3 : 268e3);
-    const double rounds = (double)((v->vocab + 65535) / 65536), stages = (double)((v->dim + 63) / 64);
+    double few = VD * size * (double)((v->rows + 63) / 64) / 5e3 + 2 * R * VD / (size == 4 ? 119e3 : 268e3);
+    const double rounds = (double)(((v->vocab + 255) / 256 * ((v->rows + 255) / 256) + 255) / 256), stages = (double)((v->dim + 63) / 64);
     double tiles = 15e3 + rounds * stages * (rounds > 1 ? 2300 : 1500) * (size == 4 ? (grad ? 4 : 2) : 1);
-    if (size == 4 && !grad) tiles += VD * 12 / 5e3;
+    if (size == 4 && !grad) tiles += (VD + R * (double)v->dim) * 12 / 5e3;
+    // rows of x, read from far; the logits written and read, or their exponentials
+    few += R * (double)v->dim / 250;
+    if (grad) few += R * (double)v->vocab * 8 / 5e3, tiles += size == 4 ? 0 : R * (double)v->vocab * 6 / 5e3;
     return few < tiles;
 }
 
@@ -1009,20 +1018,21 @@ void (*dz_of(float softcap))(HeadArgs) {
 }
 
 // Gradients of rows this few have kernels of their own (vocab_few.hpp), whose columns come in 16 B. Tiles waste 192 of 256 rows or more, store
-// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 316, 351 and 506 us against
-// 667, 692 and 660; fp32: 639, 701 and 1323 against 1665, 1717 and 1939; 4096 x 512 bf16: 19, 21 and 30 against 40, 40 and 44.
+// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 336, 373 and 503 us against
+// 667, 692 and 660; fp32: 641, 696 and 1291 against 1665, 1717 and 1939; 4096 x 512 bf16: 20, 22 and 30 against 40, 40 and 44.
 bool few_grad_rows(const noise_vocab_t *v) { return v->rows <= 64 && v->dim >= 8; }
 
 struct FewPlan {
     int blocks;   // of 16 entries per workgroup
-    int64_t segments, bytes;
+    int64_t segments, at_partial, bytes;
 };
 FewPlan few_plan(const noise_vocab_t *v) {
     FewPlan p;
     // 32 entries per workgroup, or 16 where that leaves fewer than two workgroups per CU
     p.blocks = v->vocab >= 32 * 512 ? 2 : 1;
     p.segments = (v->vocab + 16 * p.blocks - 1) / (16 * p.blocks);
-    p.bytes = 8 * p.segments * v->rows + 4 * kFewRows;
+    p.at_partial = up(4 * v->rows, 1024);
+    p.bytes = p.at_partial + 8 * p.segments * v->rows;
     return p;
 }
 
@@ -1057,10 +1067,11 @@ FewGradPlan few_grad_plan(const noise_vocab_t *v) {
         at += up(bytes, 1024);
         return here;
     };
-    p.at_lse = take(4 * kFewRows);
+    p.at_lse = take(4 * v->rows);
     p.at_z = take(4 * p.dz_rows * p.z_ld);
-    p.at_dz = size == 4 ? p.at_z : take(size * p.dz_rows * p.z_ld);
-    p.at_dzt = take(size * p.z_ld * p.kp);
+    // (dZ in two bf16 parts, or one of fp32)
+    p.at_dz = size == 4 ? p.at_z : take(4 * p.dz_rows * p.z_ld);
+    p.at_dzt = take(4 * p.z_ld * p.kp);
     p.at_slabs = take(16ll * 64 * n * p.rb * p.columns * p.dx_splits);
     p.bytes = at;
     return p;
@@ -1097,10 +1108,10 @@ Plan plan_of(const noise_vocab_t *v, bool grad) {
     p.at_x = take(2 * parts * p.rows * p.ld);
     if (p.pack_w) p.at_w = take(2 * parts * v->vocab * p.ld);
     if (grad) {
-        p.few = few_rows(v, true);
+        p.few = few_rows(v, true) && p.pieces == 1;
         if (p.few) {
             p.at_z = take(4 * v->rows * up(v->vocab, 32));
-            p.at_few = take(up(few_plan(v).bytes, 16) + 4 * kFewRows);
+            p.at_few = take(up(few_plan(v).bytes, 16) + 4 * v->rows);
         }
         p.at_cuts = take(8 * p.pieces);
         p.at_dz = take(2 * parts * p.piece * p.vocab_ld);
@@ -1137,7 +1148,7 @@ int run_few(const char *fn, const noise_vocab_t *v, float softcap, float *loss, 
     FewArgs a;
     a.x = v->x, a.w = v->weight, a.targets = v->targets, a.x_ld = v->x_stride, a.w_ld = v->weight_stride;
     a.zt = static_cast<float *>(workspace);
-    a.partial = reinterpret_cast<float2 *>(a.zt + kFewRows);
+    a.partial = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + p.at_partial);
     a.rows = (int)v->rows, a.vocab = (int)v->vocab, a.dim = (int)v->dim, a.segments = (int)p.segments, a.wide = (int)v->targets_wide;
     a.softcap = softcap, a.z = nullptr, a.z_ld = 0;
     auto kernel = few_of<false>(v->type, p.blocks, v->rows, softcap > 0.f);
@@ -1188,7 +1199,7 @@ int run_few_grad(const char *fn, const noise_vocab_t *v, float softcap, const fl
     FewArgs f = {};
     f.x = v->x, f.w = v->weight, f.targets = v->targets, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
     f.zt = reinterpret_cast<float *>(ws);
-    f.partial = given ? nullptr : reinterpret_cast<float2 *>(f.zt + kFewRows);
+    f.partial = given ? nullptr : reinterpret_cast<float2 *>(ws + q.at_partial);
     f.rows = (int)v->rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.segments = (int)q.segments, f.wide = (int)v->targets_wide;
     f.softcap = softcap, f.z = reinterpret_cast<float *>(ws + p.at_z), f.z_ld = p.z_ld;
     float *lse = reinterpret_cast<float *>(ws + p.at_lse);
@@ -1256,7 +1267,7 @@ int run(const char *fn, const noise_vocab_t *v, float softcap, const float *weig
             f.x = v->x, f.w = v->weight, f.targets = v->targets, f.x_ld = v->x_stride, f.w_ld = v->weight_stride;
             f.z = reinterpret_cast<float *>(ws + p.at_z), f.z_ld = up(v->vocab, 32);
             f.zt = reinterpret_cast<float *>(ws + p.at_few);
-            f.partial = given ? nullptr : reinterpret_cast<float2 *>(f.zt + kFewRows);
+            f.partial = given ? nullptr : reinterpret_cast<float2 *>(ws + p.at_few + q.at_partial);
             float *own = reinterpret_cast<float *>(ws + p.at_few + up(q.bytes, 16));
             f.rows = (int)rows, f.vocab = (int)v->vocab, f.dim = (int)v->dim, f.segments = (int)q.segments, f.softcap = softcap;
             f.wide = (int)v->targets_wide;

@@ -2,8 +2,9 @@
 // dW is written once, straight from and to memory, through v_mfma_f32_16x16x32_bf16 or, exact products, v_mfma_f32_16x16x4_f32.
 // A lane holds N consecutive columns (16 B) of a matrix's rows; product e of N takes the e-th of each lane's columns, so that rows are
 // read and written in runs of 256 B. Every row of dZ takes part, with zeros in those without a target, whose x is taken as zeros too.
-// Bound by HBM: at 131072 x 2048 and 4 rows in bf16, dx takes 96 us (5.6 TB/s of weight read) and dW 105 to 113 (5 TB/s written), in fp32
-// 219 and 205.
+// Of up to 32 rows dZ is a sum of two bf16 values beside bf16 operands: so few rows' roundings would not average out, and the products are
+// free. (Of 64 rows it would take 20 % longer at 131072 x 2048.)
+// Bound by HBM: at 131072 x 2048 and 4 rows in bf16, dx takes 109 us (4.9 TB/s of weight read) and dW 109 (4.9 TB/s written).
 #pragma once
 #include "vocab_gemm.hpp"
 
@@ -15,14 +16,18 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 struct FewGradArgs {
     const void *x, *w, *targets;
     int64_t x_ld, w_ld;
-    const void *dz;        // [16 RB][z_ld], zeros where nothing stands
-    const void *dzt;       // [z_ld][rows, up to whole steps]
+    const void *dz;        // [parts][16 RB][z_ld], zeros where nothing stands
+    const void *dzt;       // [parts][z_ld][rows, up to whole steps]
     float *slabs;          // dx's sums of each workgroup (splits), as its lanes hold them
     void *dx, *dw;
     int64_t z_ld;
     int rows, vocab, dim, wide, blocks, splits, per;   // blocks: of 16 N columns; per: entries of a workgroup
     int across, stream;    // dW: a workgroup's waves take 4 blocks of columns (else entries in turn); stores that pass the caches by
 };
+
+// dZ's parts: the value in its type, and the rest of it
+template <class E>
+constexpr int parts_of(int rows) { return sizeof(E) == 2 && rows <= 32 ? 2 : 1; }
 
 __device__ __forceinline__ bool has_target(const void *targets, int wide, int64_t vocab, int r) {
     const int64_t t = wide ? static_cast<const int64_t *>(targets)[r] : (int64_t)static_cast<const int32_t *>(targets)[r];
@@ -84,7 +89,7 @@ __device__ __forceinline__ int column_of(int block, int i, int dim) {
 // turn, whose sums meet in LDS.
 template <class E, int RB>
 __global__ __launch_bounds__(256) void vocab_few_dx_kernel(FewGradArgs a) {
-    constexpr int N = FewOperand<E>::N, K = 4 * N;
+    constexpr int N = FewOperand<E>::N, K = 4 * N, PARTS = parts_of<E>(16 * RB);
     __shared__ f32x4 sums[4][4][RB][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const E *w = static_cast<const E *>(a.w) + column_of<N>(blockIdx.y, i, a.dim);
@@ -92,20 +97,24 @@ __global__ __launch_bounds__(256) void vocab_few_dx_kernel(FewGradArgs a) {
     const int begin = blockIdx.x * a.per, end = (int)(begin + a.per < a.z_ld ? begin + a.per : a.z_ld);
     f32x4 acc[N][RB] = {};
     for (int v0 = begin + K * wave; v0 < end; v0 += 4 * K) {
-        u32x4 rows[N], z[RB];
+        u32x4 rows[N], z[PARTS][RB];
 #pragma unroll
         for (int s = 0; s < N; ++s) {
             const int v = v0 + N * g + s;
             __builtin_memcpy(&rows[s], w + (int64_t)(v < a.vocab ? v : a.vocab - 1) * a.w_ld, 16);
         }
 #pragma unroll
-        for (int b = 0; b < RB; ++b) __builtin_memcpy(&z[b], __builtin_assume_aligned(dz + 16 * b * a.z_ld + v0, 16), 16);
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) __builtin_memcpy(&z[q][b], __builtin_assume_aligned(dz + 16 * (q * RB + b) * a.z_ld + v0, 16), 16);
         FewOperand<E> op;
         op.set(rows);
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
+        for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e][b] = op.template times<true>(e, z[b], acc[e][b]);
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e][b] = op.template times<true>(e, z[q][b], acc[e][b]);
     }
     f32x4 *slab = reinterpret_cast<f32x4 *>(a.slabs) + ((int64_t)blockIdx.x * a.blocks + blockIdx.y) * (N * RB * 64);
 #pragma unroll
@@ -150,7 +159,7 @@ __global__ __launch_bounds__(256) void vocab_few_dx_join_kernel(FewGradArgs a) {
 // of a dW larger than the caches are stored past them. (131072 x 2048 bf16: 180 us without either, 147 with the latter.)
 template <class E, int KB>
 __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
-    constexpr int N = FewOperand<E>::N, KP = KB * 4 * N;
+    constexpr int N = FewOperand<E>::N, KP = KB * 4 * N, PARTS = parts_of<E>(KP);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const int block = a.across ? 4 * blockIdx.y + wave : blockIdx.y;
     const int c = column_of<N>(block, i, a.dim);
@@ -172,14 +181,18 @@ __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
     const int begin = blockIdx.x * a.per, end = (int)(begin + a.per < a.z_ld ? begin + a.per : a.z_ld);
     for (int v0 = begin + (a.across ? 0 : 16 * wave); v0 < end; v0 += a.across ? 16 : 64) {
         const E *dz = static_cast<const E *>(a.dzt) + (int64_t)(v0 + i) * KP + N * g;
-        u32x4 z[KB];
+        u32x4 z[PARTS][KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) __builtin_memcpy(&z[b], __builtin_assume_aligned(dz + 4 * N * b, 16), 16);
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) __builtin_memcpy(&z[q][b], __builtin_assume_aligned(dz + q * a.z_ld * KP + 4 * N * b, 16), 16);
         f32x4 acc[N] = {};
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
+        for (int q = PARTS - 1; q >= 0; --q)
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] = op[b].template times<false>(e, z[b], acc[e]);
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] = op[b].template times<false>(e, z[q][b], acc[e]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             E o[N];

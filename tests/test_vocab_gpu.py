@@ -131,6 +131,13 @@ def test_few_rows(V, dtype):
 
 
 @pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('R,V,D', [(793, 119, 4096), (257, 2, 2000), (2000, 33, 1001), (5000, 1, 64), (70000, 3, 40), (400, 1500, 3000)])
+def test_many_rows_of_few_entries(R, V, D, dtype):
+    """Whose logits may be formed as those of few rows are."""
+    check(*make(R, V, D, dtype, R, V + 2, masked=R % 2 == 1), V, 15.0 if R % 4 == 0 else None)
+
+
+@pytest.mark.parametrize('dtype', [BF16, F32])
 def test_few_rows_of_a_large_weight(dtype):
     """Gradients past the caches' size, of rows of whole lines and of others."""
     for D in (1024, 1032, 1001):
