@@ -403,7 +403,6 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
                 for (int r = 0; r < 16; ++r) z = t == 32 * i + 16 * (r / 8) + r % 8 ? acc[i][j][r] : z;
             if (mine) a.zt[row] = z;
         }
-        const float shift = top * kLog2e;
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
@@ -413,7 +412,9 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float z = acc[i][j][8 * h + e];
-                    float p = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
+                    // (the difference first: the rounding of a product with log2(e) would stay in the exponent, 2^-24 of it, and
+                    // the lowest values' would be infinite; where all are -inf, top is finite and z - top is not)
+                    float p = exp2_fast((z - top) * kLog2e);
                     s += p;
                     if constexpr (STORE) {
                         p *= CAP ? __builtin_fmaf(z * bend, z, 32768.f) : 32768.f;
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
         const bool there = at < rows;
         const float w = there ? (a.weight ? a.weight[row] : 1.f) * (SPLIT ? a.scales[2] : 1.f) : 0.f;
         const float bend = CAP ? -w / a.softcap / a.softcap : 0.f;   // of w cap'
-        const float shift = there ? a.lse[row] * kLog2e : 0.f;
+        const float lse = there ? a.lse[row] : 0.f;
         const int t = there ? a.target[row] - m0 - 8 * (lane >> 5) : -1;
 #pragma unroll
         for (int i = 0; i < T::FB; ++i)
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_dz_kernel(HeadArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float z = acc[i][j][8 * h + e];
-                    float d = exp2_fast(__builtin_fmaf(z, kLog2e, -shift));
+                    float d = exp2_fast((z - lse) * kLog2e);
                     if (t == 32 * i + 16 * h + e) d -= 1.f;
                     d *= CAP ? __builtin_fmaf(z * bend, z, w) : w;
                     if (!there) d = 0.f;
