@@ -220,11 +220,12 @@ __device__ __forceinline__ float scale_of(float top) {
     return ldexpf(1.f, e);
 }
 
-// f as a sum of two fp16 values, as bits
+// f as a sum of two fp16 values, as bits. An infinity is the second one: it meets the first of the other operand's alone, whose sign is that
+// of the value (the second may be 0, which would make a NaN of it, or of the other sign).
 __device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
-    const _Float16 h = (_Float16)f;
-    const float rest = fabsf(f) < __builtin_inff() ? f - (float)h : 0.f;
-    const _Float16 l = (_Float16)rest;
+    const bool far = fabsf(f) == __builtin_inff();
+    const _Float16 h = far ? (_Float16)copysignf(65504.f, f) : (_Float16)f;
+    const _Float16 l = (_Float16)(far ? f : f - (float)h);
     __builtin_memcpy(&hi, &h, 2);
     __builtin_memcpy(&lo, &l, 2);
 }

@@ -84,3 +84,10 @@ def test_logits_with_a_large_common_part(dtype, shift):
             for got in (one, two):
                 for name, a, b, c in zip(('loss', 'dx', 'dweight'), got, want, limit):
                     off_bounds(name, a, b, c)
+
+
+@pytest.mark.parametrize('runs', RUNS)
+def test_infinite_weights_fp32(runs):
+    """Held as two values too: the infinity must meet one value of x alone, whose sign is x's."""
+    for size in SIZES:
+        check(*size, F32, -INF, runs)
