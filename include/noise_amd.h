@@ -708,10 +708,13 @@ int noise_distill(const void *x, int type, int64_t rows, int64_t vocab, int64_t 
                   noise_stream_t stream);
 
 /* Global norm of `count` gradients (fp32 and bf16, any sizes), and the gradients scaled to a bound on it:
- *   norm = sqrt(sum of all squares) (summed in fp64, stored in fp32),
- *   factor = min(1, max_norm / (norm + 1e-6)),  g <- factor g in place, rounded once (not written where the factor is 1).
- * max_norm infinite: the norm alone. A norm that is NaN makes every gradient NaN; an infinite one makes the finite ones 0 and
- * the infinite ones NaN. The table is read on the host, before the call returns; gradients that share memory are refused.
+ *   norm = sqrt(sum of all squares),  factor = min(1, max_norm / (norm + 1e-6)),  g <- factor g in place (not written where the
+ *   factor is 1).
+ * Norm and factor are formed in fp64. The norm is stored in fp32, as infinite past fp32's range, where the gradients are scaled as
+ * ever; the factor has 24 bits, its product with a value is rounded to fp32 and then to the gradient's type. max_norm infinite: the
+ * norm alone. A NaN among the gradients makes the norm and every gradient NaN; an infinity makes the norm infinite, the finite
+ * gradients 0 and the infinite ones NaN. The table is read on the host, before the call returns; gradients that share memory are
+ * refused.
  * count is 1 .. 2^24. workspace: noise_clip_workspace_bytes(count) bytes (negative: invalid), 8 B aligned. */
 typedef struct {
     void *ptr;      /* contiguous elements, aligned to their type */

@@ -48,9 +48,11 @@ def clip_gradients(gradients, max_norm):
         norm = sqrt(sum of all squares),  g <- g min(1, max_norm / (norm + 1e-6))
 
     `gradients` are bfloat16 and float32 tensors of any sizes on one device (None is left out), their elements in any order but
-    without gaps, no two of them in the same memory. Squares are summed in 64 bits, in a fixed order; results are rounded once. An infinite `max_norm`
-    leaves the gradients as they are; a norm that is NaN makes them all NaN, an infinite one makes the finite ones 0 and the
-    infinite ones NaN. Nothing waits for the device: the norm stays on it."""
+    without gaps, no two of them in the same memory. Squares are summed in 64 bits, in a fixed order. The norm is rounded to
+    float32 (infinite past its range, where the gradients are scaled as ever), the factor to 24 bits, its products to float32 and
+    then to the gradients' type. An infinite `max_norm` leaves the gradients as they are. A NaN among them makes the norm and all
+    of them NaN; an infinity makes the norm infinite, the finite ones 0 and the infinite ones NaN. Nothing waits for the device:
+    the norm stays on it."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.clip_gradients([g for g in gradients if g is not None], float(max_norm))
     return clip('clip_gradients', gradients, max_norm)

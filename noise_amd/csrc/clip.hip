@@ -3,7 +3,8 @@
 // Memory bound: everything is read once for the norm, then read and written once where the factor is below 1. Two launches per
 // table of 192 tensors: the first leaves one partial sum per workgroup, and every workgroup of the second adds those up itself, in
 // the same order, so that nothing waits for a launch in between and results do not depend on timing. Squares are summed in fp64:
-// no finite fp32 or bf16 value's square overflows or vanishes there.
+// no finite fp32 or bf16 value's square overflows or vanishes there; the factor, which may then be too small for fp32, is 24 bits and
+// a power of two.
 // A workgroup takes a contiguous range of the bytes, forwards for the norm and backwards for the scaling, which starts with what
 // was read last and is still in the caches. 37.75 M fp32 values in 60 tensors: 29 us for the norm (5.2 TB/s) and 53 for the scaling
 // (5.7 TB/s read and written); 1e9 values in 300 tensors, fp32 and bf16: 736 us (5.1) and 1630 (4.6).
@@ -84,8 +85,15 @@ __device__ __forceinline__ void add_unit(void *p, int64_t n, int64_t unit, doubl
         }
 }
 
+// factor = part 2^power with part of 24 bits in 1/2 .. 1: no factor is too small for fp32, and a value's product is rounded as with any other
+struct Factor {
+    float part;
+    int power;
+    __device__ __forceinline__ float times(float v) const { return ldexpf(v * part, power); }
+};
+
 template <class E>
-__device__ __forceinline__ void scale_unit(void *p, int64_t n, int64_t unit, float factor) {
+__device__ __forceinline__ void scale_unit(void *p, int64_t n, int64_t unit, const Factor &factor) {
     constexpr int N = 16 / sizeof(E);
     const Span<E> sp(p, n);
     const int64_t at = unit * (kThreads * kUnroll) + threadIdx.x;
@@ -98,7 +106,7 @@ __device__ __forceinline__ void scale_unit(void *p, int64_t n, int64_t unit, flo
         if (at + i * kThreads < sp.pieces) {
             E o[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] = (E)(element<E>(v[i], e) * factor);
+            for (int e = 0; e < N; ++e) o[e] = (E)factor.times(element<E>(v[i], e));
             __builtin_memcpy(&v[i], o, 16);
             sp.body[at + i * kThreads] = v[i];
         }
@@ -106,7 +114,7 @@ __device__ __forceinline__ void scale_unit(void *p, int64_t n, int64_t unit, flo
         E *x = (int)threadIdx.x < sp.heads ? sp.head + threadIdx.x
                : (int)threadIdx.x - N >= 0 && (int)threadIdx.x - N < sp.tails ? sp.tail + (threadIdx.x - N)
                                                                               : nullptr;
-        if (x) *x = (E)((float)*x * factor);
+        if (x) *x = (E)factor.times((float)*x);
     }
 }
 
@@ -161,8 +169,10 @@ __device__ __forceinline__ double total_norm(const ClipBound &b) {
 __global__ __launch_bounds__(kThreads) void clip_scale_kernel(ClipArgs a, ClipBound b) {
     const double norm = total_norm(b);
     if (a.first + blockIdx.x == 0 && threadIdx.x == 0) *b.norm = (float)norm;
-    const double factor = (double)b.max_norm / (norm + 1e-6);
-    if (factor >= 1.) return;   // (a NaN goes on, into every gradient)
+    const double quotient = (double)b.max_norm / (norm + 1e-6);
+    if (quotient >= 1.) return;   // (a NaN goes on, into every gradient)
+    Factor factor;
+    factor.part = (float)frexp(quotient, &factor.power);
     const uint32_t begin = (uint32_t)((uint64_t)a.units * blockIdx.x / a.groups);
     const uint32_t end = (uint32_t)((uint64_t)a.units * (blockIdx.x + 1) / a.groups);
     if (begin == end) return;
@@ -170,8 +180,8 @@ __global__ __launch_bounds__(kThreads) void clip_scale_kernel(ClipArgs a, ClipBo
     for (uint32_t u = end; u-- > begin;) {
         while (a.unit[t] > u) --t;
         const int64_t n = a.numel[t];
-        if (n < 0) scale_unit<__bf16>(a.ptr[t], -n, u - a.unit[t], (float)factor);
-        else scale_unit<float>(a.ptr[t], n, u - a.unit[t], (float)factor);
+        if (n < 0) scale_unit<__bf16>(a.ptr[t], -n, u - a.unit[t], factor);
+        else scale_unit<float>(a.ptr[t], n, u - a.unit[t], factor);
     }
 }
 

@@ -150,3 +150,20 @@ def test_eggroll_step_clips():
     assert norm > 1e-3
     for g, w in zip(seen[2], want):
         assert ((g.double() - w).abs() <= 4 * F * w.abs() + 1e-45).all()
+
+
+def test_factors_past_fp32():
+    """Norms so far above the bound that the factor has no normal fp32 value: the values are as near as with any other (the 64-bit
+    factor's parts, one rounding to 24 bits and the product's); the norm, past fp32's range, is stored as infinite."""
+    from noise_amd.clip import clip_gradients
+    g = torch.Generator(DEV).manual_seed(5)
+    for types, scale, max_norm in (((F32,), 1e38, 1.0), ((BF16, F32), 1e38, 3.0), ((F32,), 1e38, 1e-30), ((F32, BF16), 1e10, 1e-30),
+                                   ((F32,), 3e38, 1e-38)):
+        gradients = [((torch.rand(n, device=DEV, generator=g) + 0.1) * scale).to(types[i % len(types)]) for i, n in enumerate((1000, 70001, 3))]
+        want, clipped = oracle.clip(gradients, max_norm)
+        norm = clip_gradients(gradients, max_norm)
+        assert norm.item() == math.inf if want > 3.5e38 else abs(norm.item() - want) <= 2 * F * want
+        for a, b in zip(gradients, clipped):
+            step = F if a.dtype == F32 else 2.0 ** -8 * (1 + 2 ** -10)
+            least = 2.0 ** -150 if a.dtype == F32 else 2.0 ** -134   # half the smallest values' step
+            assert ((a.double() - b).abs() <= (step + 3 * F) * b.abs() + 2 * least).all(), (types, scale, max_norm)
