@@ -152,6 +152,8 @@ def linear_cross_entropy_grad(x, weight, targets, token_weight=None, vocab=None,
     ones). Rows of dweight from `vocab` on are zeros. The results are plain tensors, for operands that require a gradient too
     (x.backward(dx) goes on from there)."""
     if torch.compiler.is_compiling():
-        return torch.ops.noise_amd.linear_cross_entropy_grad(x, weight, targets, token_weight,
+        # (the operator has no backward pass, and its results would ask for one)
+        return torch.ops.noise_amd.linear_cross_entropy_grad(x.detach(), weight.detach(), targets,
+                                                             None if token_weight is None else token_weight.detach(),
                                                              weight.shape[0] if vocab is None else int(vocab), softcap)
     return gradients('linear_cross_entropy_grad', x, weight, targets, token_weight, None, vocab, softcap)

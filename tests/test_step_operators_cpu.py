@@ -340,3 +340,22 @@ def test_definitions():
         assert abs((f(1e-6 * e) - f(-1e-6 * e)) / 2e-6 - (d * e).sum()) < 1e-8
     norm, clipped = oracle.clip([torch.tensor([3.0]), torch.tensor([4.0])], 1.0)
     assert norm == 5.0 and abs(clipped[0].item() - 3 / (5 + 1e-6)) < 1e-12
+
+
+def test_compiled_gradients_in_one_call_of_leaves(launches):
+    """linear_cross_entropy_grad's results are plain tensors for operands that require a gradient, compiled as well, and the steps
+    around it go on from them."""
+    def step(t):
+        loss, dx, dw = vocab.linear_cross_entropy_grad(t['x'], t['head'], t['targets'], t['token_weight'])
+        return loss, dx, dw, clip.clip_gradients([dw], 1.0)
+    made = []
+    for f in (step, torch.compile(step, backend='aot_eager', fullgraph=True)):
+        t = operands()
+        hidden = t['x'].requires_grad_() * 2
+        outs = f({**t, 'x': hidden, 'head': t['head'].requires_grad_(), 'token_weight': t['token_weight'].requires_grad_()})
+        assert not any(o.requires_grad for o in outs)
+        hidden.backward(outs[1])
+        assert torch.equal(t['x'].grad, 2 * outs[1]) or torch.isnan(outs[1]).any()
+        made.append([n for n, _ in launches])
+        launches.clear()
+    assert made[0] == made[1] == ['noise_vocab_grad', 'noise_clip_gradients']
