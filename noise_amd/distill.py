@@ -102,7 +102,9 @@ def distill_loss_grad(logits, teacher_logits, teacher_index, weight=None, vocab=
     Columns from `vocab` on get zeros. Both results are plain tensors, for logits that require a gradient too
     (logits.backward(gradient) goes on from there)."""
     if torch.compiler.is_compiling():
-        return torch.ops.noise_amd.distill_loss_grad(logits, teacher_logits, teacher_index, weight,
+        # (the operator has no backward pass, and its results would ask for one)
+        return torch.ops.noise_amd.distill_loss_grad(logits.detach(), teacher_logits.detach(), teacher_index,
+                                                     None if weight is None else weight.detach(),
                                                      logits.shape[-1] if vocab is None else int(vocab), float(temperature),
                                                      softcap)
     return distill('distill_loss_grad', logits, teacher_logits, teacher_index, weight, vocab, temperature, softcap, True)

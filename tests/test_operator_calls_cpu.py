@@ -317,3 +317,19 @@ def test_compiled_callers_may_give_whole_numbers(launches):
     torch.compile(lambda t: sinks.qk_norm_rotary(t['q'], t['k'], t['cos'], t['sin'], eps=1), backend='aot_eager',
                   fullgraph=True)(t)
     assert len(launches) == 4
+
+
+def test_compiled_gradients_in_one_call_of_leaves(launches):
+    """distill_loss_grad's results are plain tensors for logits that require a gradient, compiled as well, and logits.backward goes
+    on from them."""
+    step = lambda t, logits: distill.distill_loss_grad(logits, t['teacher'], t['index'], t['weight'])
+    for f in (step, torch.compile(step, backend='aot_eager', fullgraph=True)):
+        t = operands()
+        leaf = t['logits'].requires_grad_()
+        hidden = leaf * 2
+        loss, grad = f({**t, 'teacher': t['teacher'].requires_grad_(), 'weight': t['weight'].requires_grad_()}, hidden)
+        assert not loss.requires_grad and not grad.requires_grad
+        hidden.backward(torch.ones_like(grad))
+        assert torch.equal(leaf.grad, torch.full_like(leaf, 2))
+        assert [n for n, _ in launches] == ['noise_distill']
+        launches.clear()
