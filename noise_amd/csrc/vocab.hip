@@ -1071,9 +1071,10 @@ FewGradPlan few_grad_plan(const noise_vocab_t *v) {
     };
     p.at_lse = take(4 * v->rows);
     p.at_z = take(4 * p.dz_rows * p.z_ld);
-    // (dZ in two bf16 parts, or one of fp32)
-    p.at_dz = size == 4 ? p.at_z : take(4 * p.dz_rows * p.z_ld);
-    p.at_dzt = take(4 * p.z_ld * p.kp);
+    // (dZ in one or two bf16 parts, or one of fp32)
+    const int64_t each = size == 4 ? 4 : 2 * parts_of<__bf16>(p.kp);
+    p.at_dz = size == 4 ? p.at_z : take(each * p.dz_rows * p.z_ld);
+    p.at_dzt = take(each * p.z_ld * p.kp);
     p.at_slabs = take(16ll * 64 * n * p.rb * p.columns * p.dx_splits);
     p.bytes = at;
     return p;

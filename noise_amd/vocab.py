@@ -135,9 +135,11 @@ def linear_cross_entropy(x, weight, targets, vocab=None, softcap=None):
     A token whose target lies outside 0 .. vocab - 1 has loss 0 and no gradient, whatever its x holds. The logits are formed a
     tile at a time and never stored; their products, sums and softmax are in fp32, float32 operands with 21 bits in the products.
     Differentiable in x and weight (once): the backward pass forms the logits again, and holds their gradients in 16 bits (two
-    times 16 for float32) for at most 2 GiB of tokens and vocabulary at a time (few tokens, or many of a small vocabulary, may have
-    their logits in float32 beside it, 1 GiB at most). float32 values below 2^-38 of their tensor's largest, the tokens' weights among those tensors, count
-    as 0. Rows may lie at any distance from each other."""
+    times 16 for float32) for at most 2 GiB of tokens and vocabulary at a time, or for 256 tokens where those take more (float32
+    of more than 2^21 entries: up to 4 GiB). Up to 64 tokens have logits in float32 and their gradients twice instead, 2 GiB at
+    most together; many tokens of a small vocabulary may have logits in float32 besides, 1 GiB at most. float32 values below
+    2^-38 of their tensor's largest, the tokens' weights among those tensors, count as 0. Rows may lie at any distance from each
+    other."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.linear_cross_entropy(x, weight, targets, weight.shape[0] if vocab is None else int(vocab),
                                                         softcap)[0]

@@ -359,3 +359,30 @@ def test_compiled_gradients_in_one_call_of_leaves(launches):
         made.append([n for n, _ in launches])
         launches.clear()
     assert made[0] == made[1] == ['noise_vocab_grad', 'noise_clip_gradients']
+
+
+def test_vocab_workspaces_of_the_largest_vocabularies():
+    """What the documents bound: dZ by 2 GiB, or by 256 tokens' (fp32 of more than 2^21 entries: 4 GiB); few tokens' logits in fp32, and
+    their dZ twice, by rows and by entries, in as many parts as it has (of up to 32 bf16 tokens two, of 64 one; fp32 by rows takes the
+    logits' place)."""
+    lib = _lib.lib()
+
+    def need(rows, V, kind, grad=1, dim=64):
+        t = array('q', (4096, dim, 4096, dim, 4096, 1, rows, dim, V, kind))
+        return lib.noise_vocab_workspace_bytes(t.buffer_info()[0], grad)
+    for V in (2 ** 22, 2 ** 21 + 1, 2 ** 20, 131072):
+        up = (V + 255) // 256 * 256
+        for kind, size in ((0, 2), (1, 4)):
+            for rows in (65, 200, 257, 1000, 5000):
+                operands = size * (rows + 256 + V) * 128 + 40 * (rows + 256)
+                partial = 8 * (V + 127) // 128 * (rows + 256)
+                few = 4 * rows * (V + 32) + 8 * rows * (V // 16 + 1) if rows * V <= 2 ** 28 else 0
+                dz = max(2 ** 31, 256 * up * size)
+                assert 0 < need(rows, V, kind) <= operands + partial + few + dz + 2 ** 29 + 4 * V * 64 + 2 ** 22, (rows, V, kind)
+            for rows in (1, 16, 17, 32, 33, 64):
+                held, entries = (16, 32) if rows <= 16 else (32, 32) if rows <= 32 else (64, 64)
+                parts = 2 if kind == 0 and rows <= 32 else 1
+                if kind == 1:
+                    entries = held
+                logits, dz, dzt = 4 * held * (V + 32), 0 if kind else 2 * parts * held * (V + 32), size * parts * entries * (V + 32)
+                assert 0 < need(rows, V, kind) <= logits + dz + dzt + 8 * rows * (V // 16 + 1) + 2 ** 24, (rows, V, kind)
