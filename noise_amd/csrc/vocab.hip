@@ -365,8 +365,19 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
     }
 }
 
-// STORE: exp(z - the segment's maximum) cap'(z) 2^15 as fp16 in dZ's place, which vocab_lse_dz_kernel turns into dZ. (Its rounding, 2^-11,
-// comes before dZ's own, 2^-8; below 2^-29 of the segment's largest it has fewer bits, below 2^-39 none.)
+// u of 0 .. 2^kUnits in 16 bits, two to a word: the 6 bits of its exponent that may be set and 10 of its mantissa. Off by 2^-11, before dZ's
+// own 2^-8, and 0 below 2^-62 of the largest: fp16 has as many bits down to 2^-29 only, and none below 2^-39, where an improbable
+// entry's gradients (logits 27 below the largest of its 128) would be 0 beside those that backward() gives.
+constexpr int kUnits = -64;
+__device__ __forceinline__ uint32_t two_units(float a, float b) {
+    return __builtin_amdgcn_perm((__float_as_uint(b) << 3) + 0x8000u, (__float_as_uint(a) << 3) + 0x8000u, 0x07060302);
+}
+// 2^-kUnits u
+__device__ __forceinline__ float unit_of(uint32_t word, int i) {
+    return __uint_as_float(i ? word >> 3 & 0x1fffe000u : (word & 0xffffu) << 13) * 0x1p64f;
+}
+
+// STORE: 2^kUnits exp(z - the segment's maximum) cap'(z) as two_units in dZ's place, which vocab_lse_dz_kernel turns into dZ
 template <class T, bool SPLIT, int CAP, bool STORE>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
@@ -382,7 +393,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
     const int m0 = tm * T::MT + T::wm(wave);
     if (m0 >= a.vocab) return;
     to_logits<T, SPLIT, CAP>(a, m0, lane, acc);
-    const float bend = CAP ? -32768.f / a.softcap / a.softcap : 0.f;   // of cap' 2^15
+    const float bend = CAP ? -1.f / a.softcap / a.softcap : 0.f;   // of cap'
     static_assert(T::FB * 32 == kSegment, "a wave's entries are a segment");
 #pragma unroll
     for (int j = 0; j < T::NB; ++j) {
@@ -409,30 +420,28 @@ __global__ __launch_bounds__(64 * T::NW, 2) void vocab_loss_kernel(HeadArgs a) {
         for (int i = 0; i < T::FB; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                _Float16 v[8];
+                float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float z = acc[i][j][8 * h + e];
                     // (the difference first: the rounding of a product with log2(e) would stay in the exponent, 2^-24 of it, and
                     // the lowest values' would be infinite; where all are -inf, top is finite and z - top is not)
-                    float p = exp2_fast((z - top) * kLog2e);
-                    s += p;
-                    if constexpr (STORE) {
-                        p *= CAP ? __builtin_fmaf(z * bend, z, 32768.f) : 32768.f;
-                        v[e] = (_Float16)p;
-                    }
+                    v[e] = STORE ? exp2_fast(__builtin_fmaf(z - top, kLog2e, (float)kUnits)) : exp2_fast((z - top) * kLog2e);
+                    s += v[e];
+                    if (STORE && CAP) v[e] *= fmaxf(__builtin_fmaf(z * bend, z, 1.f), 0.f);
                 }
                 if constexpr (STORE) {
                     uint16_t *to = reinterpret_cast<uint16_t *>(const_cast<__bf16 *>(a.dz.ptr)) + at * a.dz.ld + m0 + 32 * i +
                                    16 * h + 8 * (lane >> 5);
+                    uint32_t words[4];
                     // (rows behind the last one are multiplied by zeros)
-                    if (!there)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = (_Float16)0.f;
-                    __builtin_memcpy(__builtin_assume_aligned(to, 16), v, 16);
+                    for (int e = 0; e < 4; ++e) words[e] = there ? two_units(v[2 * e], v[2 * e + 1]) : 0;
+                    __builtin_memcpy(__builtin_assume_aligned(to, 16), words, 16);
                 }
             }
         s += swap_halves(s);
+        if (STORE) s *= 0x1p64f;
         if (lane < 32 && there) a.partial[at * a.segments + m0 / kSegment] = float2{top, s};
     }
 }
@@ -493,7 +502,7 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, float *loss,
 }
 
 // A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left, at the rate of a copy (134 MB read and written in 53 us):
-// dZ_v = weight exp(top - lse) 2^-15 stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
+// dZ_v = weight exp(top - lse) stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
 __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *loss) {
     __shared__ float2 slots[4];
     const int64_t at = blockIdx.x, row = a.row0 + at;
@@ -512,11 +521,11 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
     for (int c = 8 * threadIdx.x; c < (int)a.dz.ld; c += 2048) {
         __bf16 o[8];
         if (c < end) {
-            _Float16 v[8];
+            uint32_t v[4];
             __builtin_memcpy(v, __builtin_assume_aligned(dz + c, 16), 16);
-            const float f = w * exp2_fast(__builtin_fmaf(part[c / kSegment].x - l, kLog2e, -15.f));
+            const float f = w * exp2_fast((part[c / kSegment].x - l) * kLog2e);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = (__bf16)(c + e == t ? own : (float)v[e] * f);
+            for (int e = 0; e < 8; ++e) o[e] = (__bf16)(c + e == t ? own : unit_of(v[e / 2], e % 2) * f);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = (__bf16)0.f;

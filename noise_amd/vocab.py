@@ -151,8 +151,9 @@ def linear_cross_entropy(x, weight, targets, vocab=None, softcap=None):
 def linear_cross_entropy_grad(x, weight, targets, token_weight=None, vocab=None, softcap=None):
     """(losses, dx, dweight) of linear_cross_entropy in one call, for a training step that knows its tokens' weights before the
     losses: the gradients, of x's and weight's shapes and type, are those of sum(token_weight * loss), token_weight [...] (None:
-    ones). Rows of dweight from `vocab` on are zeros. The results are plain tensors, for operands that require a gradient too
-    (x.backward(dx) goes on from there)."""
+    ones). Rows of dweight from `vocab` on are zeros. (Of many bfloat16 tokens, entries whose exponentials are below 2^-62 of the
+    largest of their 128 have no part in a token's gradients; backward() keeps those too.) The results are plain tensors, for
+    operands that require a gradient too (x.backward(dx) goes on from there)."""
     if torch.compiler.is_compiling():
         # (the operator has no backward pass, and its results would ask for one)
         return torch.ops.noise_amd.linear_cross_entropy_grad(x.detach(), weight.detach(), targets,

@@ -91,3 +91,24 @@ def test_infinite_weights_fp32(runs):
     """Held as two values too: the infinity must meet one value of x alone, whose sign is x's."""
     for size in SIZES:
         check(*size, F32, -INF, runs)
+
+
+@pytest.mark.parametrize('cap', [None, 80.0])
+@pytest.mark.parametrize('R,V,D', [(75, 35534, 391), (168, 37229, 772), (259, 30247, 200), (3000, 9001, 64)])
+def test_improbable_entries(R, V, D, cap):
+    """Logits some 80 apart: an improbable entry's gradients are as near as another's, in the call that keeps the exponentials as well,
+    whose 2^-11 is counted beside the bounds' 2^-8. That call may leave out exponentials below 2^-62 of the largest of 128 entries."""
+    from noise_amd.vocab import linear_cross_entropy, linear_cross_entropy_grad
+    x, weight, targets, w = make(R, V, D, BF16, R, V + 5, scale=10.0)
+    want = oracle.linear_cross_entropy(x, weight, targets, V, cap, w)
+    limit = [1.125 * b for b in bounds(x, weight, targets, w, V, cap, *want)]
+    leaves = x.detach().requires_grad_(), weight.detach().requires_grad_()
+    loss = linear_cross_entropy(*leaves, targets, vocab=V, softcap=cap)
+    most = 2.0 ** -62 * w.double()
+    left = 0.0, 128 * most[:, None] * weight[:V].double().abs().max(), most @ x.double().abs()
+    for how, got in (('backward', (loss.detach(), *torch.autograd.grad(loss, leaves, w))),
+                     ('one call', linear_cross_entropy_grad(x, weight, targets, w, vocab=V, softcap=cap))):
+        for name, a, b, c, d in zip(('loss', 'dx', 'dweight'), got, want, limit, left):
+            off = (a.double() - b).abs()
+            c = c + d if how == 'one call' else c
+            assert (off <= c).all(), (how, name, (off - c).max(), off.max(), int((off > c).sum()), b.numel())
