@@ -143,11 +143,6 @@ class Heads(ctypes.Structure):
                 ('heads', ctypes.c_int64)]
 
 
-class Gradient(ctypes.Structure):
-    """noise_gradient_t: a contiguous tensor of noise_clip_gradients."""
-    _fields_ = [('ptr', ctypes.c_void_p), ('numel', ctypes.c_int64), ('type', ctypes.c_int64)]
-
-
 SLICE_GROUPS_MAX = 64  # NOISE_SLICE_GROUPS_MAX
 
 

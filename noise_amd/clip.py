@@ -34,7 +34,7 @@ def clip(fn, gradients, max_norm):
     need = _lib.lib().noise_clip_workspace_bytes(len(gradients))
     norm = torch.empty((), dtype=F32, device=device)
     work = torch.empty(need, dtype=torch.uint8, device=device)
-    _call('noise_clip_gradients', device, table.buffer_info()[0], len(gradients), min(float(max_norm), float('inf')),
+    _call('noise_clip_gradients', device, table.buffer_info()[0], len(gradients), float(max_norm),
           norm.data_ptr(), work.data_ptr(), need)
     if max_norm != float('inf'):
         torch.autograd.graph.increment_version(gradients)

@@ -85,7 +85,7 @@ __device__ __forceinline__ void add_unit(void *p, int64_t n, int64_t unit, doubl
         }
 }
 
-// factor = part 2^power with part of 24 bits in 1/2 .. 1: no factor is too small for fp32, and a value's product is rounded as with any other
+// factor = part 2^power with part of 24 bits in 1/2 .. 1: no factor is too small for fp32, and its products are rounded as any
 struct Factor {
     float part;
     int power;

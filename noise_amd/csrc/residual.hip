@@ -7,17 +7,21 @@
 // The backward pass forms x' again from x, y and x0 in fp32, so that n carries none of x's rounding to its stored type (and
 // reads what ds, ds0 and dg need anyway).
 //
-// Memory bound. TEAM lanes hold a row, 8 consecutive elements each, as raw 16 B words that are unpacked where used (single bf16 values
-// take a register each, and the backward pass 1.6 times as long); sums over a row are lane swaps for teams of up to a wave, and one
-// exchange through LDS per sum for larger ones, which are a workgroup. Workgroups of the backward pass take a run of rows of one
-// gate each, hold the weights and the sums over rows in registers, and leave one row of partial sums; a second kernel adds those up in a fixed
-// order. Measured, in us (and TB/s of what has to be read and written):
+// Memory bound. TEAM lanes hold a row, 8 consecutive elements each, as raw 16 B words that are unpacked where used (single bf16
+// values take a register each, and the backward pass 1.6 times as long); sums over a row are lane swaps for teams of up to a wave,
+// and one exchange through LDS per sum for larger ones, which are a workgroup. Workgroups of the backward pass take a run of rows
+// of one gate each, hold the weights and the sums over rows in registers, and leave one row of partial sums; a second kernel adds
+// those up in a fixed order. Measured, in us (and TB/s of what has to be read and written):
 //                                                                        forward      backward     join
 //   16384 x 512, fp32 stream, bf16 branch, x0                            30 (4.4)     37 (5.9)       4
 //   3333 x 1001, fp32, both norms, weights, a gate per sequence          18 (3.0)     25 (3.2)       6
 //   8192 x 4096, bf16, both norms, weights, a gate per channel           54 (5.0)     98 (4.1)       4
-// (of one call after another; the first two are in the caches in part). The backward pass of 4096 holds 200 registers per lane, so one workgroup of 8 waves per CU: the
-// loads of a row wait for the sums of the one before. Loading a row ahead, or 128 registers, costs more (spills).
+//   2048 x 8192, fp32, both norms, weights, a gate per channel           63 (4.3)     90 (4.5)       6
+// (of one call after another; the first two are in the caches in part). Rows that are not whole 8 elements have tail code and, in
+// fp32, 4 B alignment: 3333 x 1000 takes 12, 19 and 5. The backward pass of 4096 holds 200 registers per lane, so one workgroup of
+// 8 waves per CU: the loads of a row wait for the sums of the one before. Loading a row ahead, or 128 registers, costs more
+// (spills). Past 4096 a row has 16 waves and 128 registers are all there are: with y's norm and x0, or with y's norm and tail code,
+// 6 to 32 of them go to memory (2048 x 8192 fp32 with x0: 119 us, 4.5 TB/s as without; 8191 wide, both: 168 us, 3.2).
 #include "common.hpp"
 #include "mfma.hpp"
 
@@ -88,8 +92,8 @@ __device__ __forceinline__ float add_dpp(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true));
 }
 
-// N sums over a team of TEAM lanes. Within a wave by DPP (lanes 1, 2, 4 and 8 apart: pairs and halves of four swapped, halves of 8 and
-// 16 lanes mirrored) and lane swaps: a sixth of the time of shuffles, which go through LDS. Teams larger than a wave are the
+// N sums over a team of TEAM lanes. Within a wave by DPP (lanes 1, 2, 4 and 8 apart: pairs and halves of four swapped, halves of 8
+// and 16 lanes mirrored) and lane swaps: a sixth of the time of shuffles, which go through LDS. Teams larger than a wave are the
 // workgroup: their waves' sums go through LDS, in two alternating sets of slots, so that one barrier per call is enough.
 template <int TEAM, int N>
 __device__ __forceinline__ void team_sum(float (&v)[N], float *slots, int &turn) {
@@ -199,7 +203,8 @@ __global__ __launch_bounds__(group_threads<TEAM>()) void residual_kernel(ResArgs
     put8<FULL>(static_cast<EY *>(a.h) + row * D + c, n, t);
 }
 
-// MIX: with x0. (Loading the next row before working on the present one was slower, by 5 to 10 %: it takes registers from other rows.)
+// MIX: with x0. (Loading the next row before working on the present one was slower, by 5 to 10 %: it takes registers from other
+// rows.)
 template <class EX, class EY, int TEAM, bool POST, bool MIX, bool FULL>
 __global__ __launch_bounds__(group_threads<TEAM>()) void residual_bwd_kernel(ResArgs a) {
     constexpr int NT = group_threads<TEAM>(), TEAMS = NT / TEAM;

@@ -9,23 +9,27 @@
 //   loss_kernel    a tile of logits in registers, its rows' maxima and sums of exponentials left per 128 vocabulary entries, which
 //                  lse_kernel adds up. Where bf16 gradients are asked for in the same call, the exponentials stay as well, and
 //                  lse_dz_kernel makes dZ of them: a pass over 2 R V bytes instead of another product
-//   dz_kernel      otherwise: the logits once more, and dZ from them, in 16 bits or two times 16
+//   dz_kernel      otherwise: the logits once more, and dZ from them, in bf16 or, beside fp32 operands, two times fp16
 //   grad_kernel    dx and dW in one launch, k split over workgroups where there are few tiles; sum_kernel joins the splits' fp32 sums
 // fp32 operands are held as sums of two fp16 values, scaled by a power of two per tensor (hi carries 11 bits of a value, lo the next
 // 11), and each product is hi hi + hi lo + lo hi: what is left out is 2^-22 of a term, and 2^-38 of the tensors' largest values.
 // A bf16 weight is read where it is if its rows are whole 16 B: what its last stage of k lacks comes from the zeros behind a row of x
 // (losses of 300 rows of 131072 x 1000: 243 -> 153 us).
-// For few rows few_kernel forms the logits (few_rows says when), and z_dz_kernel makes dZ of them; up to 64 rows have gradients of their own
-// too (few_grad_rows).
+// dZ beside bf16 operands is rounded to bf16, 2^-8 of each term, so that the gradients' products run at bf16's rate: at 16384 x
+// 4096 x 512 the results are off by 2.3e-3 of themselves, where fp32 inside and their own rounding leave 1.7e-3. A second part,
+// which up to 32 rows have, would double the gradients' products, 144 of that call's 290 us. For few rows few_kernel forms the
+// logits (few_rows says when), and z_dz_kernel makes dZ of them; up to 64 rows have gradients of their own too (few_grad_rows).
 //
-// Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2 PFLOP/s),
-// on an x of zeros 2.96; a plain large product on this card reaches 1.35. Alone on the GPU, in us:
+// Bound by the matrix units, and there by power at large sizes: the loss pass of 8192 x 131072 x 2048 in bf16 takes 3.65 ms (1.2
+// PFLOP/s), on an x of zeros 2.96; a plain large product on this card reaches 1.35. Alone on the GPU, in us:
 //                                  live   pack   loss   lse or lse_dz   dz    grad   sum
-//   16384 x 4096 x 512 bf16, cap     9     10    120         54          -     144     9    (in one call)
-//   8192 x 131072 x 2048 bf16        8     15   4007        953          -    7405     -    (in one call)
-//   16384 x 4096 x 512 fp32          9     18    223          7         262    376    11    (through autograd; largest values 14)
-//   3333 x 50021 x 776 bf16, 2/3     6      7    207          5         230    483     9    (through autograd)
-// At widths like 512, 8 stages of k, a tile's epilogue shows: two exponentials, a reciprocal and some 12 other operations per capped logit.
+//   16384 x 4096 x 512 bf16, cap     10     9    124         45          -     144     9    (in one call)
+//   8192 x 131072 x 2048 bf16        8     15   4025        922          -    7305     -    (in one call)
+//   16384 x 4096 x 512 fp32          9     19    224          7         265    374    11    (through autograd; largest values 14)
+//   the same in one call             10    19    224          7         262    377    11    (the logits twice as well; 15)
+//   3333 x 50021 x 776 bf16, 2/3     6      7    209          5         234    487     9    (through autograd)
+// At widths like 512, 8 stages of k, a tile's epilogue shows: two exponentials, a reciprocal and some 12 other operations per
+// capped logit.
 #include "vocab_few.hpp"
 #include "vocab_gemm.hpp"
 
@@ -80,9 +84,9 @@ __device__ __forceinline__ int64_t piece_rows(const HeadArgs &a) {
     return n < 0 ? 0 : n < a.piece ? n : a.piece;
 }
 
-// softcap tanh(z / softcap), k = 2 log2(e) / softcap, with an error of 2^-22 softcap: what enters exp(z) is absolute. Past kWideCap, where
-// that would be more than 2^-17, WIDE: below 0.35 of the cap tanh's odd series up to the 11th power (the next term is 1.2e-8 of the value
-// there), which leaves an error relative to the logit.
+// softcap tanh(z / softcap), k = 2 log2(e) / softcap, with an error of 2^-22 softcap: what enters exp(z) is absolute. Past
+// kWideCap, where that would be more than 2^-17, WIDE: below 0.35 of the cap tanh's odd series up to the 11th power (the next term
+// is 1.2e-8 of the value there), which leaves an error relative to the logit.
 constexpr float kWideCap = 32.f;
 template <bool WIDE>
 __device__ __forceinline__ float cap_of(float z, float cap, float k) {
@@ -220,8 +224,8 @@ __device__ __forceinline__ float scale_of(float top) {
     return ldexpf(1.f, e);
 }
 
-// f as a sum of two fp16 values, as bits. An infinity is the second one: it meets the first of the other operand's alone, whose sign is that
-// of the value (the second may be 0, which would make a NaN of it, or of the other sign).
+// f as a sum of two fp16 values, as bits. An infinity is the second one: it meets the first of the other operand's alone, whose
+// sign is that of the value (the second may be 0, which would make a NaN of it, or of the other sign).
 __device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
     const bool far = fabsf(f) == __builtin_inff();
     const _Float16 h = far ? (_Float16)copysignf(65504.f, f) : (_Float16)f;
@@ -230,11 +234,12 @@ __device__ __forceinline__ void halves(float f, uint16_t &hi, uint16_t &lo) {
     __builtin_memcpy(&lo, &l, 2);
 }
 
-// In how many shares workgroups take the stages of k of a tile of dx (x) and of dW (y), whose fp32 sums are then joined. Both products
-// run in one launch. Of no shares, and shares of one, a half and a third of what all stages take on 256 CUs, those that come out best
-// by what was measured: a workgroup takes 2.2 us per stage (3.3 where operands are sums of two) and 3 us more, 256 run at a time, and
-// joining costs 5 us and 0.09 us of the whole chip's time per tile's share. At most kSplitTiles shares of tiles, at least 4 stages each. (At
-// 16384 x 4096 x 512 dx then has 1 share and dW 4, and both take 153 us with the join; in two launches, with 2 and 8, it was 195.)
+// In how many shares workgroups take the stages of k of a tile of dx (x) and of dW (y), whose fp32 sums are then joined. Both
+// products run in one launch. Of no shares, and shares of one, a half and a third of what all stages take on 256 CUs, those that
+// come out best by what was measured: a workgroup takes 2.2 us per stage (3.3 where operands are sums of two) and 3 us more, 256
+// run at a time, and joining costs 5 us and 0.09 us of the whole chip's time per tile's share. At most kSplitTiles shares of tiles,
+// at least 4 stages each. (At 16384 x 4096 x 512 dx then has 1 share and dW 4, and both take 153 us with the join; in two launches,
+// with 2 and 8, it was 195.)
 constexpr uint32_t kSplitTiles = 512;
 template <class T, bool SPLIT>
 __device__ uint2 shares_of(int64_t rows, int64_t vocab, uint32_t tiles_m, bool dx, bool dw) {
@@ -338,8 +343,8 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(PackArgs a) {
 
 // --- logits ---
 
-// The tile's logits, unscaled and capped. Past the vocabulary: -inf, or under the cap (where they are multiplied by cap') a value whose
-// exponential vanishes beside any other's. CAP: 0 none, 2 past kWideCap.
+// The tile's logits, unscaled and capped. Past the vocabulary: -inf, or under the cap (where they are multiplied by cap') a value
+// whose exponential vanishes beside any other's. CAP: 0 none, 2 past kWideCap.
 template <class T, bool SPLIT, int CAP>
 __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f32x16 (&acc)[T::FB][T::NB]) {
     const float unit = SPLIT ? 1.f / a.scales[0] / a.scales[1] : 1.f, k = CAP ? 2.f * kLog2e / a.softcap : 0.f;
@@ -365,9 +370,9 @@ __device__ __forceinline__ void to_logits(const HeadArgs &a, int m0, int lane, f
     }
 }
 
-// u of 0 .. 2^kUnits in 16 bits, two to a word: the 6 bits of its exponent that may be set and 10 of its mantissa. Off by 2^-11, before dZ's
-// own 2^-8, and 0 below 2^-62 of the largest: fp16 has as many bits down to 2^-29 only, and none below 2^-39, where an improbable
-// entry's gradients (logits 27 below the largest of its 128) would be 0 beside those that backward() gives.
+// u of 0 .. 2^kUnits in 16 bits, two to a word: the 6 bits of its exponent that may be set and 10 of its mantissa. Off by 2^-11,
+// before dZ's own 2^-8, and 0 below 2^-62 of the largest: fp16 has as many bits down to 2^-29 only, and none below 2^-39, where an
+// improbable entry's gradients (logits 27 below the largest of its 128) would be 0 beside those that backward() gives.
 constexpr int kUnits = -64;
 __device__ __forceinline__ uint32_t two_units(float a, float b) {
     return __builtin_amdgcn_perm((__float_as_uint(b) << 3) + 0x8000u, (__float_as_uint(a) << 3) + 0x8000u, 0x07060302);
@@ -501,8 +506,8 @@ __global__ __launch_bounds__(256) void vocab_lse_kernel(HeadArgs a, float *loss,
     if (lse) lse[to] = l;
 }
 
-// A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left, at the rate of a copy (134 MB read and written in 53 us):
-// dZ_v = weight exp(top - lse) stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
+// A row's lse and loss from its segments, and dZ from what vocab_loss_kernel left, at the rate of a copy (134 MB read and written
+// in 45 us): dZ_v = weight exp(top - lse) stored_v, and at the target weight (exp(z - lse) - 1) cap'(z) from its logit
 __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *loss) {
     __shared__ float2 slots[4];
     const int64_t at = blockIdx.x, row = a.row0 + at;
@@ -536,13 +541,14 @@ __global__ __launch_bounds__(256) void vocab_lse_dz_kernel(HeadArgs a, float *lo
 
 // --- the losses of a few rows ---
 
-// What is read is the weight: a workgroup takes 16 VB vocabulary entries for 16 RB rows (blockIdx.y counts those), its four waves a quarter of dim
-// each, straight from memory into v_mfma_f32_16x16x32_bf16's (fp32: v_mfma_f32_16x16x4_f32's, exact products) operands: 16 lanes on
-// 16 rows of the weight, and the rows of x from the caches. The waves' sums meet in LDS; wave v takes entries 16 v on from there.
+// What is read is the weight: a workgroup takes 16 VB vocabulary entries for 16 RB rows (blockIdx.y counts those), its four waves a
+// quarter of dim each, straight from memory into v_mfma_f32_16x16x32_bf16's (fp32: v_mfma_f32_16x16x4_f32's, exact products)
+// operands: 16 lanes on 16 rows of the weight, and the rows of x from the caches. The waves' sums meet in LDS; wave v takes entries
+// 16 v on from there.
 //
-// Bound by HBM: 4 rows of 65536 x 2048 in bf16, 268 MB, take 53 us (5.1 TB/s) with 8 loads of 16 B per lane and block under way; loads
-// that bypass the caches were slower.
-// With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel or vocab_few_dz_kernel (and partial may be NULL).
+// Bound by HBM: 4 rows of 65536 x 2048 in bf16, 268 MB, take 53 us (5.1 TB/s) with 8 loads of 16 B per lane and block under way;
+// loads that bypass the caches were slower. With WRITE the logits themselves are left, fp32, for vocab_z_dz_kernel or
+// vocab_few_dz_kernel (and partial may be NULL).
 struct FewArgs {
     const void *x, *w, *targets;
     int64_t x_ld, w_ld;
@@ -695,8 +701,8 @@ __global__ __launch_bounds__(256) void vocab_few_join_kernel(FewArgs a, float *l
     if (lse) lse[row] = in ? l : 0.f;
 }
 
-// dZ of up to 64 rows from their logits and lse: by rows (dz, which may be z's place) and by entries (dzt). A thread takes an entry of N rows;
-// zeros where there is no row, target or entry.
+// dZ of up to 64 rows from their logits and lse: by rows (dz, which may be z's place) and by entries (dzt). A thread takes an entry
+// of N rows; zeros where there is no row, target or entry.
 template <class E>
 __global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const float *lse, const float *weight, E *dz, E *dzt, int dz_rows, int kp) {
     constexpr int N = 16 / sizeof(E);
@@ -729,7 +735,8 @@ __global__ __launch_bounds__(256) void vocab_few_dz_kernel(FewArgs a, const floa
     if (parts > 1) __builtin_memcpy(__builtin_assume_aligned(dzt + (a.z_ld + v) * kp + r0, 16), rest, 16);
 }
 
-// dZ of packed rows from their logits and lse, which are by row; zeros in the rows behind the last. blockIdx.y: a share of the entries
+// dZ of packed rows from their logits and lse, which are by row; zeros in the rows behind the last. blockIdx.y: a share of the
+// entries
 constexpr int kDzEntries = 4096;
 template <bool SPLIT>
 __global__ __launch_bounds__(256) void vocab_z_dz_kernel(HeadArgs a, const float *logits, int64_t z_ld, const float *lse) {
@@ -920,7 +927,8 @@ __device__ __forceinline__ void gradient_tile(const HeadArgs &a, const GradArgs 
     }
 }
 
-// n: packed rows (DX) or vocabulary entries; m: columns of dim. What is left of dim in the last tile takes half a tile where that is enough.
+// n: packed rows (DX) or vocabulary entries; m: columns of dim. What is left of dim in the last tile takes half a tile where that
+// is enough.
 template <class T, bool DX, bool SPLIT>
 __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, uint32_t group, char *lds) {
     const Cut c = cut_of<T, DX, SPLIT>(a, g, piece_rows(a));
@@ -936,8 +944,8 @@ __device__ __forceinline__ void gradient(const HeadArgs &a, const GradArgs &g, u
         gradient_tile<T, DX, SPLIT>(a, g, c, split, tm * T::MT, (int64_t)tn * T::NT, first, last, lds);
 }
 
-// Both gradients in one launch: neither waits for the other's last workgroups (16384 x 4096 x 512: 144 us, 0.95 PFLOP/s; 8192 x 131072 x
-// 2048: 7.4 ms, 1.19)
+// Both gradients in one launch: neither waits for the other's last workgroups (16384 x 4096 x 512: 144 us, 0.95 PFLOP/s; 8192 x
+// 131072 x 2048: 7.4 ms, 1.19)
 template <class T, bool SPLIT>
 __global__ __launch_bounds__(64 * T::NW, 2) void vocab_grad_kernel(HeadArgs a, GradArgs g) {
     __shared__ __attribute__((aligned(1024))) char lds[T::kLds];
@@ -995,13 +1003,13 @@ void most_of(bool rows, int64_t n_end, int64_t stages, int64_t ld, int64_t *grou
 }
 
 // Whether the logits come from vocab_few_kernel, whose every workgroup forms its own, or from the tiles of vocab_loss_kernel and
-// vocab_dz_kernel, which share operands but are few and long where there are few entries or rows. By what was measured, in ns: the former
-// read 5 TB/s of weight for each 64 rows and then multiply at 268 TFLOP/s (fp32: 119); a tile takes 1.5 us per stage of 64 of dim when it
-// is one of the only 256 and 2.3 otherwise (twice that in fp32, whose gradients have two such passes in one call and whose losses
-// alone need x and the weight packed, 12 B read and written per value), and 15 us in all. 131072 x 2048 bf16, losses of 16, 32 and 64
-// rows: 132, 157 and 233 us against 165; 4096 x 512: 6, 7 and 9 against 27; 131072 x 2048 fp32: 257, 322 and 478 against 970. Many rows
-// of few entries are alike: 793 x 119 x 4096, loss and gradients, bf16 67 us against 125, fp32 103 against 499; past some thousand rows
-// the tiles are as fast (4000 x 300 x 2048 bf16: 122 against 130).
+// vocab_dz_kernel, which share operands but are few and long where there are few entries or rows. By what was measured, in ns: the
+// former read 5 TB/s of weight for each 64 rows and then multiply at 268 TFLOP/s (fp32: 119); a tile takes 1.5 us per stage of 64
+// of dim when it is one of the only 256 and 2.3 otherwise (twice that in fp32, whose gradients have two such passes in one call and
+// whose losses alone need x and the weight packed, 12 B read and written per value), and 15 us in all. 131072 x 2048 bf16, losses
+// of 16, 32 and 64 rows: 132, 157 and 233 us against 165; 4096 x 512: 6, 7 and 9 against 27; 131072 x 2048 fp32: 257, 322 and 478
+// against 970. Many rows of few entries are alike: 793 x 119 x 4096, loss and gradients, bf16 67 us against 125, fp32 103 against
+// 499; past some thousand rows the tiles are as fast (4000 x 300 x 2048 bf16: 122 against 130).
 bool few_rows(const noise_vocab_t *v, bool grad) {
     if (v->rows > 1 << 20 || v->rows * v->vocab > 1 << 28) return false;
     const double R = (double)v->rows, VD = (double)v->vocab * (double)v->dim, size = v->type == NOISE_FP32 ? 4 : 2;
@@ -1028,9 +1036,10 @@ void (*dz_of(float softcap))(HeadArgs) {
                               : vocab_dz_kernel<Tile, SPLIT, 0>;
 }
 
-// Gradients of rows this few have kernels of their own (vocab_few.hpp), whose columns come in 16 B. Tiles waste 192 of 256 rows or more, store
-// dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 336, 373 and 503 us against
-// 667, 692 and 660; fp32: 641, 696 and 1291 against 1665, 1717 and 1939; 4096 x 512 bf16: 20, 22 and 30 against 40, 40 and 44.
+// Gradients of rows this few have kernels of their own (vocab_few.hpp), whose columns come in 16 B. Tiles waste 192 of 256 rows or
+// more, store dW in short runs, and need fp32 weights split: 131072 x 2048 bf16, loss and gradients of 4, 16 and 64 rows: 336, 373
+// and 503 us against 667, 692 and 660; fp32: 641, 696 and 1291 against 1665, 1717 and 1939; 4096 x 512 bf16: 20, 22 and 30 against
+// 40, 40 and 44.
 bool few_grad_rows(const noise_vocab_t *v) { return v->rows <= 64 && v->dim >= 8; }
 
 struct FewPlan {

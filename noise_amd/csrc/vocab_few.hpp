@@ -1,10 +1,10 @@
 // The gradients of the vocabulary's cross entropy for few rows (up to 64), where the weight's bytes count: it is read once for dx and
 // dW is written once, straight from and to memory, through v_mfma_f32_16x16x32_bf16 or, exact products, v_mfma_f32_16x16x4_f32.
-// A lane holds N consecutive columns (16 B) of a matrix's rows; product e of N takes the e-th of each lane's columns, so that rows are
-// read and written in runs of 256 B. Every row of dZ takes part, with zeros in those without a target, whose x is taken as zeros too.
-// Of up to 32 rows dZ is a sum of two bf16 values beside bf16 operands: so few rows' roundings would not average out, and the products are
-// free. (Of 64 rows it would take 20 % longer at 131072 x 2048.)
-// Bound by HBM: at 131072 x 2048 and 4 rows in bf16, dx takes 109 us (4.9 TB/s of weight read) and dW 109 (4.9 TB/s written).
+// A lane holds N consecutive columns (16 B) of a matrix's rows; product e of N takes the e-th of each lane's columns, so that rows
+// are read and written in runs of 256 B. Every row of dZ takes part, with zeros in those without a target, whose x is taken as
+// zeros too. Of up to 32 rows dZ is a sum of two bf16 values beside bf16 operands: so few rows' roundings would not average out,
+// and the products are free. (Of 64 rows it would take 20 % longer at 131072 x 2048.) Bound by HBM: at 131072 x 2048 and 4 rows in
+// bf16, dx takes 109 us (4.9 TB/s of weight read) and dW 109 (4.9 TB/s written).
 #pragma once
 #include "vocab_gemm.hpp"
 
@@ -154,9 +154,10 @@ __global__ __launch_bounds__(256) void vocab_few_dx_join_kernel(FewGradArgs a) {
     }
 }
 
-// dW: the product's rows are entries, its columns columns. The operands of x stay in registers; the workgroup's waves take four blocks of
-// columns, so that 1 KB of a row is written at a time, or where there are too few blocks its entries in turn, 16 at a time. Rows of whole 128 B
-// of a dW larger than the caches are stored past them. (131072 x 2048 bf16: 180 us without either, 147 with the latter.)
+// dW: the product's rows are entries, its columns columns. The operands of x stay in registers; the workgroup's waves take four
+// blocks of columns, so that 1 KB of a row is written at a time, or where there are too few blocks its entries in turn, 16 at a
+// time. Rows of whole 128 B of a dW larger than the caches are stored past them. (131072 x 2048 bf16: 180 us without either, 147
+// with the latter.)
 template <class E, int KB>
 __global__ __launch_bounds__(256) void vocab_few_dw_kernel(FewGradArgs a) {
     constexpr int N = FewOperand<E>::N, KP = KB * 4 * N, PARTS = parts_of<E>(KP);

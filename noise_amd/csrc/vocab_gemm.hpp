@@ -7,10 +7,12 @@
 // The rows of a 32-row block of A are taken in the order sigma (bits 2 and 3 of the index swapped), which makes register r of a
 // lane's block stand for m = 16 (r / 8) + 8 (lane / 32) + r % 8, n = lane % 32: eight consecutive m, 16 B of 16-bit results.
 //
-// The tile is 256 x 256 with 8 waves of 128 x 64, 64 of k per stage and two stages (128 KB of LDS): 12 fragments read per 32 products of
-// 32 x 32 x 16, two waves per SIMD. It reaches 1.05 to 1.27 PFLOP/s, a library's product 1.35. Measured and slower: 4 waves of 128 x 128
-// (by 8 to 12 %); 256 x 128 with stages of 32 and two workgroups per CU (the same at k = 512, 15 % slower at 2048); the same: wave
-// priorities, persistent workgroups whose next tile begins under the epilogue (1 to 2 % faster, which is not worth its code).
+// The tile is 256 x 256 with 8 waves of 128 x 64, 64 of k per stage and two stages (128 KB of LDS): 12 fragments read per 32
+// products of 32 x 32 x 16, two waves per SIMD. It reaches 1.1 to 1.27 PFLOP/s in large products (2048 wide), a library's product
+// 1.35; where k is short the start and end of a tile show: 0.95 in the gradients of 16384 x 4096 x 512, 0.72 and 0.58 in the losses
+// of 776 and 512 columns, with their exponentials. Measured and slower: 4 waves of 128 x 128 (by 8 to 12 %); 256 x 128 with stages
+// of 32 and two workgroups per CU (the same at k = 512, 15 % slower at 2048); the same: wave priorities, persistent workgroups
+// whose next tile begins under the epilogue (1 to 2 % faster, which is not worth its code).
 #pragma once
 #include "common.hpp"
 #include "mfma.hpp"
@@ -77,8 +79,8 @@ struct Side {
             off[i] = (unsigned)((CROSSED || r < last ? r : last) * (uint32_t)ld * 2 + chunk * 16);
         }
     }
-    // k: the stage's first; left: how many k from there on are in memory. Crossed: rows past them repeat the last one (the other operand
-    // is zero there). Plain: chunks past them are read from `zeros`.
+    // k: the stage's first; left: how many k from there on are in memory. Crossed: rows past them repeat the last one (the other
+    // operand is zero there). Plain: chunks past them are read from `zeros`.
     __device__ __forceinline__ void copy(int64_t k, int64_t lo, int left, const void *zeros, unsigned to, int wave) const {
         const __bf16 *p = reinterpret_cast<const __bf16 *>(base) + lo + (CROSSED ? k * ld : k);
         to += wave * 1024;

@@ -1,8 +1,9 @@
-"""The cross entropy of a linear head over a vocabulary of any size, without its logits in memory, beside noise_amd.dust's forward-only
-head_loss of the fixed model.
+"""The cross entropy of a linear head over a vocabulary of any size, without its logits in memory, beside noise_amd.dust's
+forward-only head_loss of the fixed model.
 
-  linear_cross_entropy(x, weight, targets, vocab, softcap)                      per-token losses; differentiable in x and weight
-  linear_cross_entropy_grad(x, weight, targets, token_weight, vocab, softcap)   losses and the weighted sum's gradients in one call
+  linear_cross_entropy(x, weight, targets, vocab, softcap)       per-token losses; differentiable in x and weight
+  linear_cross_entropy_grad(x, weight, targets, token_weight, vocab, softcap)
+                                                                 losses and the weighted sum's gradients in one call
 
 The head is utils/model.py:204-206's with its soft cap as an option, the loss that of train/val/run.py:89-94. The calls are
 torch.ops.noise_amd operators too. Derivatives are taken backwards and once, as in noise_amd.sinks.
@@ -134,12 +135,17 @@ def linear_cross_entropy(x, weight, targets, vocab=None, softcap=None):
 
     A token whose target lies outside 0 .. vocab - 1 has loss 0 and no gradient, whatever its x holds. The logits are formed a
     tile at a time and never stored; their products, sums and softmax are in fp32, float32 operands with 21 bits in the products.
-    Differentiable in x and weight (once): the backward pass forms the logits again, and holds their gradients in 16 bits (two
-    times 16 for float32) for at most 2 GiB of tokens and vocabulary at a time, or for 256 tokens where those take more (float32
-    of more than 2^21 entries: up to 4 GiB). Up to 64 tokens have logits in float32 and their gradients twice instead, 2 GiB at
-    most together; many tokens of a small vocabulary may have logits in float32 besides, 1 GiB at most. float32 values below
-    2^-38 of their tensor's largest, the tokens' weights among those tensors, count as 0. Rows may lie at any distance from each
-    other."""
+    Rows may lie at any distance from each other. Differentiable in x and weight (once): the backward pass forms the logits again.
+
+    Their gradients are held in 16 bits, as bfloat16 beside bfloat16 operands (up to 32 tokens: as a sum of two, 16 bits of a
+    value) and two times 16 beside float32 ones, for at most 2 GiB of tokens and vocabulary at a time, or for 256 tokens where
+    those take more (float32 of more than 2^21 entries: up to 4 GiB). Up to 64 tokens have logits in float32 and their gradients
+    twice instead, 2 GiB at most together; many tokens of a small vocabulary may have logits in float32 besides, 1 GiB at most.
+
+    float32 values below 2^-38 of their tensor's largest, the tokens' weights among those tensors, count as 0. So a column that
+    takes entries out of the vocabulary, beside a column of ones in x, should hold values like -1e4 or, for losses, -inf in
+    float32, not the type's lowest, beside which all other weights are 0; bfloat16 weights may hold either. (An infinite weight
+    makes its column of dx NaN, as 0 times infinity.) A token's probabilities are off by 2^-24 of its largest logit's size."""
     if torch.compiler.is_compiling():
         return torch.ops.noise_amd.linear_cross_entropy(x, weight, targets, weight.shape[0] if vocab is None else int(vocab),
                                                         softcap)[0]
