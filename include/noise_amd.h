@@ -778,7 +778,9 @@ int noise_vocab_loss(const noise_vocab_t *v, float softcap, float *loss, float *
                      noise_stream_t stream);
 /* The gradients of sum_r weight[r] loss[r] (weight fp32 [rows], NULL: ones), each optional (NULL): dx [rows][dim] and dweight
  * [width][dim], contiguous, of `type`; rows of dweight from vocab on are zeros. Either lse of the loss call comes in, or the
- * losses come out in the same call. With rows 0 nothing is written. */
+ * losses come out in the same call (where, of many bf16 rows, entries whose exponentials are below 2^-62 of the largest of their
+ * 128 have no part in a row's gradients). The logits' gradients are rounded to bf16 beside bf16 operands (up to 32 rows: to a sum
+ * of two), to two fp16 values beside fp32 ones. With rows 0 nothing is written. */
 int noise_vocab_grad(const noise_vocab_t *v, float softcap, const float *weight, const float *lse, float *loss, void *dx,
                      void *dweight, int64_t width, void *workspace, int64_t workspace_bytes, noise_stream_t stream);
 
